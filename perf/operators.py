@@ -271,17 +271,18 @@ def _to_e4m3(x):
 
 
 def _filled_cache(gen, blocks, block, hkv, dim):
-    """A pool of written blocks: values of normal keys and values, in steps of the block's own magnitude."""
-    data = torch.empty(2, blocks, block, hkv, dim, dtype=torch.float8_e4m3fn, device="cuda")
+    """A pool of written blocks [2, blocks, heads, tokens, dim]: normal keys and values, in steps of the
+    block's own magnitude."""
+    data = torch.empty(2, blocks, hkv, block, dim, dtype=torch.float8_e4m3fn, device="cuda")
     scales = torch.empty(2, blocks, hkv, dtype=torch.float32, device="cuda")
     step = max(1, (1 << 27) // (block * hkv * dim))
     for part in range(2):
         for i in range(0, blocks, step):
             n = min(step, blocks - i)
-            x = _normal(gen, n, block, hkv, dim, dtype=torch.float32)
-            x *= torch.exp2(torch.randint(-2, 3, (n, 1, hkv, 1), device="cuda", generator=gen).float() / 2)
-            s = _need(x.abs().amax(dim=(1, 3)))
-            data[part, i:i + n] = _to_e4m3(x / s[:, None, :, None])
+            x = _normal(gen, n, hkv, block, dim, dtype=torch.float32)
+            x *= torch.exp2(torch.randint(-2, 3, (n, hkv, 1, 1), device="cuda", generator=gen).float() / 2)
+            s = _need(x.abs().amax(dim=(2, 3)))
+            data[part, i:i + n] = _to_e4m3(x / s[..., None, None])
             scales[part, i:i + n] = s
     return data, scales
 
@@ -452,17 +453,17 @@ def _plain_append(st):
     keep = torch.where(nth == 0, past[who] % block, torch.zeros_like(nth))      # rows written by earlier calls
     row = torch.arange(block, device=dev)
     for part, x in enumerate((st["k"], st["v"])):
-        fresh = torch.zeros(pages.numel(), block, c["hkv"], c["dim"], dtype=torch.float32, device=dev)
-        fresh[pair, slot] = x.float()
+        fresh = torch.zeros(pages.numel(), c["hkv"], block, c["dim"], dtype=torch.float32, device=dev)
+        fresh[pair, :, slot] = x.float()
         before = st["scales"][part][pages]
-        scale = _need(fresh.abs().amax(dim=(1, 3)))
+        scale = _need(fresh.abs().amax(dim=(2, 3)))
         scale = torch.where((keep > 0)[:, None], torch.maximum(scale, before), scale)
         held = st["data"][part][pages]
-        old = _to_e4m3(held.float() * (before / scale)[:, None, :, None])
-        code = _to_e4m3(fresh / scale[:, None, :, None])
-        code = torch.where((row < keep[:, None])[..., None, None], old.view(torch.uint8), code.view(torch.uint8))
+        old = _to_e4m3(held.float() * (before / scale)[..., None, None])
+        code = _to_e4m3(fresh / scale[..., None, None])
+        code = torch.where((row < keep[:, None])[:, None, :, None], old.view(torch.uint8), code.view(torch.uint8))
         last = torch.minimum(past[who] + new[who] - (first[who] + nth) * block, torch.full_like(nth, block))
-        code = torch.where((row < last[:, None])[..., None, None], code, held.view(torch.uint8))
+        code = torch.where((row < last[:, None])[:, None, :, None], code, held.view(torch.uint8))
         st["data"][part].view(torch.uint8)[pages] = code
         st["scales"][part][pages] = scale
     return st["data"], st["scales"]
@@ -474,8 +475,8 @@ def _plain_decode(st):
     outs, lses = [], []
     for b, n in enumerate(st["lens"]):
         pages = st["table"][b, :-(-n // block)].long()
-        k, v = (st["data"][p][pages].float().mul_(st["scales"][p][pages][:, None, :, None])
-                .view(-1, c["hkv"], c["dim"])[:n] for p in range(2))
+        k, v = (st["data"][p][pages].float().mul_(st["scales"][p][pages][..., None, None])
+                .transpose(1, 2).reshape(-1, c["hkv"], c["dim"])[:n] for p in range(2))
         o, ls = _plain_attend(st["q"][b].float(), k, v, n - c["queries"], c, st["prefix"][b], st["slopes"])
         outs.append(o.to(st["q"].dtype))
         lses.append(ls)
@@ -567,10 +568,10 @@ def _exact_append(st):
                 s = torch.where(top > s, s * 2, torch.where((top <= s / 2) & (s > 2.0 ** -100), s / 2, s))
                 if off:
                     s = torch.maximum(s, scales[part, page])
-                    old = data[part, page, :off] * (scales[part, page] / s)[None, :, None]
-                    data[part, page, :off] = old.float().to(torch.float8_e4m3fn).double()
-                data[part, page, off:off + m] = (rows / s[None, :, None]).clamp(-448, 448).float() \
-                    .to(torch.float8_e4m3fn).double()
+                    old = data[part, page, :, :off] * (scales[part, page] / s)[:, None, None]
+                    data[part, page, :, :off] = old.float().to(torch.float8_e4m3fn).double()
+                data[part, page, :, off:off + m] = (rows / s[None, :, None]).clamp(-448, 448).float() \
+                    .to(torch.float8_e4m3fn).double().transpose(0, 1)
                 scales[part, page] = s
                 at += m
     return data, scales
@@ -610,8 +611,8 @@ def exact(case, seed):
     outs, lses = [], []
     for b, n in enumerate(st["lens"]):
         pages = st["table"][b, :-(-n // case["block"])].long()
-        k, v = ((st["data"][p][pages].double() * st["scales"][p][pages].double()[:, None, :, None])
-                .view(-1, case["hkv"], case["dim"])[:n] for p in range(2))
+        k, v = ((st["data"][p][pages].double() * st["scales"][p][pages].double()[..., None, None])
+                .transpose(1, 2).reshape(-1, case["hkv"], case["dim"])[:n] for p in range(2))
         o, ls = _exact_document(st["q"][b], k, v, n - case["queries"], case, st["prefix"][b], st["slopes"])
         outs.append(o)
         lses.append(ls)
