@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-enum { SEMBLO_BF16 = 0, SEMBLO_F32 = 1 };
+enum { SEMBLO_BF16 = 0, SEMBLO_F32 = 1, SEMBLO_F16 = 2 };
 
 int semblo_version(void);
 const char* semblo_last_error(void);
@@ -319,6 +319,36 @@ int semblo_paged_posting_attention(const void* q, const void* q_position, int po
 int semblo_merge_attention_states(const void* out_a, const float* lse_a, const void* out_b,
                                   const float* lse_b, int64_t rows, int head_dim, void* out,
                                   float* lse, void* stream);
+
+/* ---- dense requests: rotary positions and the 8-bit K/V cache ----------------------- */
+
+/* Rotary positions: q_out / k_out = q / k [tokens, heads, head_dim] (bf16, fp16 or fp32; strides in
+ * elements) with the first rotary_dim dimensions of token t turned by positions[t] * inv_freq[i]
+ * (inv_freq [rotary_dim / 2], double), cos and sin times attention_scale; pair i is (i, i + R/2), or
+ * (2i, 2i + 1) with interleaved; inverse turns back.  The other dimensions are copied.  An output may be
+ * its input (same pointer and strides).  k may be NULL.  The reference receives both tensors from the
+ * engine (semblo/vllm_plugin/model.py:1130-1167). */
+int semblo_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
+                  int64_t qo_token_stride, int64_t qo_head_stride, int num_q_heads, const void* k,
+                  int64_t k_token_stride, int64_t k_head_stride, void* k_out, int64_t ko_token_stride,
+                  int64_t ko_head_stride, int num_kv_heads, int64_t tokens, int head_dim, int rotary_dim,
+                  int dtype, const void* positions, int pos_is_int64, const double* inv_freq,
+                  float attention_scale, int interleaved, int inverse, void* stream);
+
+/* Append to the 8-bit paged cache: cache [2, cache_blocks, Hkv, block_size, D] e4m3 codes, scales
+ * [2, cache_blocks, Hkv] fp32; block_size a power of two in [16, 256], D 64, 128 or 256.  k, v [tokens,
+ * Hkv, D] bf16 or fp16 (strides in elements, multiples of 8); rows cu_seqlens[b] ... of request b are its
+ * positions start_positions[b] ... and go through block_table [batch, table_len] (row stride
+ * table_stride).  A block's scale is the smallest power of two in [2^-100, 2^120] that holds its largest
+ * finite magnitude within 448; a continued block keeps a sufficient scale, otherwise its earlier rows are
+ * re-rounded to the new one.  Status 201: a block outside the pool or the table, or a negative start (that
+ * block is skipped).  No reference counterpart. */
+int semblo_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                      int64_t v_token_stride, int64_t v_head_stride, int64_t tokens, int dtype, void* cache,
+                      float* scales, int64_t cache_blocks, int block_size, int num_kv_heads, int head_dim,
+                      const int32_t* block_table, int64_t table_stride, int table_len,
+                      const int32_t* cu_seqlens, const int32_t* start_positions, int batch, int32_t* status,
+                      void* stream);
 
 #ifdef __cplusplus
 }

@@ -5,6 +5,7 @@ module does not load it; the first call of :func:`lib` does, and raises if the
 shared object has not been built."""
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
 from pathlib import Path
@@ -71,6 +72,8 @@ _SIGNATURES = {
     "semblo_decode_step": (c_int, [c_void_p] * 6 + [c_int] + [c_void_p] * 5 + [c_int64] + [c_void_p] * 3 + [c_int] * 3 + [c_void_p] + [c_int] * 4 + [c_float, c_float, c_int, c_int, c_int, c_float, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p]),
     "semblo_paged_attention_workspace_bytes": (c_int64, [c_int, c_int, c_int, c_int]),
     "semblo_paged_posting_attention": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "semblo_rotary": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int] * 2 + [c_int64, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_float, c_int, c_int, c_void_p]),
+    "semblo_kv8_append": (c_int, [c_void_p, c_int64, c_int64] * 2 + [c_int64, c_int, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     "semblo_merge_attention_states": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
 }
 
@@ -121,6 +124,36 @@ def require_cuda(*tensors: torch.Tensor | None) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError("semblo_b200 runs on CUDA tensors only; there is no CPU path")
+
+
+def require_same_device(*tensors: torch.Tensor | None) -> None:
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"the tensors of a call must be on one device (got {sorted(map(str, devices))})")
+
+
+def refuse_gradients(*tensors: torch.Tensor | None) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("this operator serves inference and has no gradient: call it under torch.no_grad() or on "
+                           "tensors that require none")
+
+
+def device_scope(device: torch.device):
+    """Make ``device`` current for a call, so that its launches and stream are that device's."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _NO_SCOPE
+    return torch.cuda.device(device)
+
+
+_NO_SCOPE = contextlib.nullcontext()
+_DTYPE_CODES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+
+
+def dtype_code(dtype: torch.dtype, what: str) -> int:
+    try:
+        return _DTYPE_CODES[dtype]
+    except KeyError:
+        raise ValueError(f"{what}: unsupported dtype {dtype}") from None
 
 
 STATUS_TEXT = {0: "ok", 101: "load wait timed out", 102: "mma wait timed out", 103: "softmax wait timed out",

@@ -1,0 +1,110 @@
+"""A paged K/V cache held in 8 bits with a scale for each block of tokens and KV head: the store, the
+append that quantises into it, and the attention of generated tokens over it.
+
+The bf16 stores of the sparse path (the cluster-ordered copy, the suffix store) hold what the index
+selects from; this cache holds every token of a dense request in half the bytes.  Codes are e4m3
+[2, blocks, Hkv, block, D]: the tokens of one (block, head) lie side by side, so the attention of a head
+reads whole kilobytes where the token-major layout of the bf16 stores would give it pieces of D bytes.
+The reference has no 8-bit store."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._lib import (check, device_scope, dtype_code, lib, ptr, refuse_gradients, require_cuda, require_same_device,
+                   stream_ptr)
+
+BLOCK_SIZES = (16, 32, 64, 128, 256)
+HEAD_DIMS = (64, 128, 256)
+
+
+class Kv8Cache:
+    """``data`` [2, blocks, Hkv, block, D] float8_e4m3fn (K, V) and ``scales`` [2, blocks, Hkv] fp32: a stored value
+    is code * scale.  Any positive scales may be read; :func:`kv8_append` writes powers of two."""
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor) -> None:
+        if data.ndim != 5 or data.shape[0] != 2 or data.dtype != torch.float8_e4m3fn or not data.is_contiguous():
+            raise ValueError("the 8-bit cache is a contiguous float8_e4m3fn tensor [2, blocks, Hkv, block, D]")
+        _, self.num_blocks, self.num_kv_heads, self.block_size, self.head_dim = (int(n) for n in data.shape)
+        if scales.shape != (2, self.num_blocks, self.num_kv_heads) or scales.dtype != torch.float32 \
+                or not scales.is_contiguous():
+            raise ValueError("scales must be contiguous fp32 [2, blocks, Hkv]")
+        if self.block_size not in BLOCK_SIZES:
+            raise ValueError(f"the block size must be one of {BLOCK_SIZES} (got {self.block_size})")
+        if self.head_dim not in HEAD_DIMS:
+            raise ValueError(f"the head dimension must be one of {HEAD_DIMS} (got {self.head_dim})")
+        if scales.device != data.device:
+            raise ValueError("codes and scales must be on one device")
+        self.data = data
+        self.scales = scales
+
+    @classmethod
+    def allocate(cls, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int, device="cuda") -> "Kv8Cache":
+        """An empty pool (a block's scale is set by the first call that writes it)."""
+        shape = (2, int(num_blocks), int(num_kv_heads), int(block_size), int(head_dim))
+        data = torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+        return cls(data, torch.ones(shape[:3], dtype=torch.float32, device=device))
+
+    def gather(self, pages: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """K and V of the listed blocks as fp32 [len(pages) * block, Hkv, D] (for inspection)."""
+        pages = pages.long()
+        out = []
+        for part in range(2):
+            x = self.data[part][pages].float() * self.scales[part][pages][..., None, None]
+            out.append(x.transpose(1, 2).reshape(-1, self.num_kv_heads, self.head_dim))
+        return out[0], out[1]
+
+
+def _block_table(table: torch.Tensor, batch: int) -> torch.Tensor:
+    if table.ndim != 2 or int(table.shape[0]) != batch:
+        raise ValueError(f"the block table must have shape [{batch}, blocks per request] (got {tuple(table.shape)})")
+    if table.dtype != torch.int32:
+        table = table.to(torch.int32)
+    return table if table.stride(1) == 1 or table.shape[1] <= 1 else table.contiguous()
+
+
+def _per_request(name: str, x: torch.Tensor, n: int) -> torch.Tensor:
+    if x.shape != (n,) or x.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be {n} int32 or int64 values (got {x.dtype} {tuple(x.shape)})")
+    return (x if x.dtype == torch.int32 else x.to(torch.int32)).contiguous()
+
+
+def _token_rows(name: str, x: torch.Tensor) -> torch.Tensor:
+    """x [T, H, D] as the kernels read it: contiguous heads of a 16-byte aligned start and step."""
+    if x.stride(2) == 1 and x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0:
+        return x
+    return x.contiguous()
+
+
+def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
+               start_positions: torch.Tensor) -> None:
+    """Write ``k``, ``v`` [T, Hkv, D] (bf16 or fp16) into the cache.
+
+    Tokens cu_seqlens[b] ... cu_seqlens[b + 1] - 1 are positions start_positions[b], start_positions[b] + 1, ... of
+    request b and go to block ``block_table[b, position // block]``.  A block that starts with this call takes the
+    smallest power-of-two scale that holds its largest finite magnitude; one that is continued keeps its scale
+    unless a new value needs a larger one, and then the rows already there follow.  Infinities saturate, NaN stay
+    NaN.  Rows of ``k`` / ``v`` behind the last request and rows of a block behind the last token are left as they
+    are.  Two requests of one call must not share a block they write.  A table entry outside the pool, a position
+    outside the table or a negative start sets status 201, and what it names is not written."""
+    require_cuda(cache.data, k, v, block_table, cu_seqlens, start_positions)
+    refuse_gradients(k, v)
+    shape = tuple(k.shape)
+    if len(shape) != 3 or shape[1:] != (cache.num_kv_heads, cache.head_dim) or tuple(v.shape) != shape:
+        raise ValueError(f"k and v must have shape [T, {cache.num_kv_heads}, {cache.head_dim}] "
+                         f"(got {shape} and {tuple(v.shape)})")
+    if k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("k and v must both be bf16 or both fp16")
+    if cu_seqlens.ndim != 1 or cu_seqlens.shape[0] < 1:
+        raise ValueError("cu_seqlens must hold one more value than there are requests")
+    batch = int(cu_seqlens.shape[0]) - 1
+    require_same_device(cache.data, k, v, block_table, cu_seqlens, start_positions)
+    table = _block_table(block_table, batch)
+    cu, start = _per_request("cu_seqlens", cu_seqlens, batch + 1), _per_request("start_positions", start_positions, batch)
+    k, v = _token_rows("k", k), _token_rows("v", v)
+    with device_scope(k.device):
+        check(lib().semblo_kv8_append(
+            ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1), shape[0], dtype_code(k.dtype, "append"),
+            ptr(cache.data), ptr(cache.scales), cache.num_blocks, cache.block_size, cache.num_kv_heads, cache.head_dim,
+            ptr(table), table.stride(0), int(table.shape[1]), ptr(cu), ptr(start), batch,
+            ptr(_lib.status_for(k.device).word), stream_ptr()))
