@@ -9,9 +9,10 @@
 // turn in double: a float product is off by half a radian at position 1e6 * f = 1, which no later step
 // can repair.  sincospi of the reduced fraction is then as accurate as a float can be.
 //
-// Bound: HBM, one read and one write of every element.  A cos/sin costs ~40 instructions against the 8
-// bytes that a bf16 pair moves, so a thread keeps the cos/sin of its 8 (or 4) pairs in registers and takes
-// them through all heads of its head group: 4 loads of 2 x 16 bytes are requested before the first is used.
+// Bound: HBM, one read and one write of every element.  A cos/sin costs ~50 instructions and serves all
+// heads of a token, so a block takes whole tokens and computes each cos/sin once, while the rows that its
+// threads have requested (2 x 16 bytes each, 2 rows) travel; after one barrier a thread takes the cos/sin of
+// its column's 8 pairs from shared memory and turns its rows with them.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -24,13 +25,16 @@ using semblo::ceil_div;
 
 namespace {
 
+constexpr int THREADS = 256;
+constexpr int MAX_HEAD_DIM = 512;           // a block holds the columns of one row at least
+
 struct RotaryArgs {
   const void* in[2];            // q, k
   void* out[2];
   int64_t in_token[2], in_head[2], out_token[2], out_head[2];   // strides in elements
   int heads0, heads;            // query heads, query + key heads
-  int heads_per_group;
   int64_t tokens;
+  int tokens_per_block, head_lanes;     // threads per block: tokens x head lanes x columns
   int head_dim, rotary_dim;
   int cols;                     // threads per (token, head): rotating columns, then copying ones
   int rot_cols;
@@ -41,101 +45,127 @@ struct RotaryArgs {
   float sin_sign;
 };
 
-template <typename T> struct Conv;
-template <> struct Conv<__nv_bfloat16> {
-  static __device__ __forceinline__ float to(__nv_bfloat16 x) { return __bfloat162float(x); }
-  static __device__ __forceinline__ __nv_bfloat16 from(float x) { return __float2bfloat16_rn(x); }
-};
-template <> struct Conv<__half> {
-  static __device__ __forceinline__ float to(__half x) { return __half2float(x); }
-  static __device__ __forceinline__ __half from(float x) { return __float2half_rn(x); }
-};
-template <> struct Conv<float> {
-  static __device__ __forceinline__ float to(float x) { return x; }
-  static __device__ __forceinline__ float from(float x) { return x; }
-};
+// A pack is NP elements held as 32-bit words (16-bit elements two to a word), or one element (NP = 1).
+template <typename T, int NP>
+struct alignas(NP * sizeof(T) >= 16 ? 16 : NP * sizeof(T)) Pack { uint32_t w[NP * sizeof(T) / 4]; };
+template <typename T> struct Pack<T, 1> { T v; };
 
-// N elements moved as the widest aligned words (N * sizeof(T) is a multiple of 8, or N is 1).
-template <typename T, int N>
-struct alignas(N * sizeof(T) >= 16 ? 16 : N * sizeof(T)) Pack { T v[N]; };
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
+  const __half2 v = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
 
-// NP: pairs per thread and head.  A rotating column c covers the pairs [NP c, NP (c + 1)): two packs of NP
+// (x1, x2) <- (x1 c - x2 s, x2 c + x1 s) for the NP pairs of two packs; t(i) is pair i's (c, s).
+template <typename T, int NP, bool INTERLEAVED, typename F>
+__device__ __forceinline__ void turn_packs(Pack<T, NP>& p0, Pack<T, NP>& p1, F t) {
+  if constexpr (NP == 1) {
+    const float x = static_cast<float>(p0.v), y = static_cast<float>(p1.v);
+    const float2 cs = t(0);
+    p0.v = static_cast<T>(x * cs.x - y * cs.y);
+    p1.v = static_cast<T>(y * cs.x + x * cs.y);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      uint32_t& a = INTERLEAVED ? (i < NP / 2 ? p0.w[2 * i] : p1.w[2 * i - NP]) : p0.w[i];
+      uint32_t& b = INTERLEAVED ? (i < NP / 2 ? p0.w[2 * i + 1] : p1.w[2 * i + 1 - NP]) : p1.w[i];
+      const float x = __uint_as_float(a), y = __uint_as_float(b);
+      const float2 cs = t(i);
+      a = __float_as_uint(x * cs.x - y * cs.y);
+      b = __float_as_uint(y * cs.x + x * cs.y);
+    }
+  } else if constexpr (INTERLEAVED) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      uint32_t& a = i < NP / 2 ? p0.w[i] : p1.w[i - NP / 2];
+      const float2 x = unpack2<T>(a), cs = t(i);
+      a = pack2<T>(x.x * cs.x - x.y * cs.y, x.y * cs.x + x.x * cs.y);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NP; i += 2) {
+      const float2 x = unpack2<T>(p0.w[i / 2]), y = unpack2<T>(p1.w[i / 2]);
+      const float2 c0 = t(i), c1 = t(i + 1);
+      p0.w[i / 2] = pack2<T>(x.x * c0.x - y.x * c0.y, x.y * c1.x - y.y * c1.y);
+      p1.w[i / 2] = pack2<T>(y.x * c0.x + x.x * c0.y, y.y * c1.x + x.y * c1.y);
+    }
+  }
+}
+
+constexpr int AHEAD = 2;        // rows whose loads a thread keeps in flight
+
+// NP: pairs per thread and row.  A rotating column c covers the pairs [NP c, NP (c + 1)): two packs of NP
 // elements, R/2 apart (half) or adjacent (interleaved).  A copying column covers 2 NP elements from R on
 // (NP = 1: two single elements, the second may lie past the head).
 template <typename T, int NP, bool INTERLEAVED>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
-  constexpr int AHEAD = NP * (int)sizeof(T) > 16 ? 2 : 4;      // heads whose loads are in flight
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t token = idx / a.cols;
-  if (token >= a.tokens) return;
-  const int col = (int)(idx - token * a.cols);
-  const bool rotating = col < a.rot_cols;
-  int e0, e1;                                                  // element offsets of the two packs
-  if (rotating) {
-    e0 = INTERLEAVED ? 2 * NP * col : NP * col;
-    e1 = INTERLEAVED ? e0 + NP : e0 + a.rotary_dim / 2;
-  } else {
-    e0 = a.rotary_dim + 2 * NP * (col - a.rot_cols);
-    e1 = e0 + NP;
-  }
-  const bool second = e1 + NP <= a.head_dim;                   // false only for the odd end of a copied tail
-  float c[NP], s[NP];
-  if (rotating) {
-    const double pos = a.pos64 ? (double)static_cast<const int64_t*>(a.positions)[token]
-                               : (double)static_cast<const int32_t*>(a.positions)[token];
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      double turns = pos * a.inv_freq[NP * col + i] * 0.15915494309189535;      // 1 / (2 pi)
-      turns -= rint(turns);
-      float sn, cs;
-      sincospif((float)(2.0 * turns), &sn, &cs);
-      c[i] = cs * a.scale;
-      s[i] = sn * a.scale * a.sin_sign;
-    }
-  }
-  const int h_begin = blockIdx.y * a.heads_per_group;
-  const int h_end = min(a.heads, h_begin + a.heads_per_group);
-  for (int h0 = h_begin; h0 < h_end; h0 += AHEAD) {
-    Pack<T, NP> x0[AHEAD], x1[AHEAD];
+__global__ void __launch_bounds__(THREADS) rotary_kernel(const RotaryArgs a) {
+  extern __shared__ float2 turn[];        // cos, sin: [token][i][column] for pair NP column + i, so that a warp's reads do not collide
+  const int64_t token0 = (int64_t)blockIdx.x * a.tokens_per_block;
+  const int nt = (int)min((int64_t)a.tokens_per_block, a.tokens - token0);
+  const int pairs = a.rotary_dim >> 1;
+  const int row = threadIdx.x / a.cols, col = threadIdx.x - row * a.cols;
+  const int tk = row / a.head_lanes, lane = row - tk * a.head_lanes;
+  const bool mine = tk < nt, rotating = col < a.rot_cols;
+  const int e0 = rotating ? (INTERLEAVED ? 2 * NP * col : NP * col) : a.rotary_dim + 2 * NP * (col - a.rot_cols);
+  int step = rotating && !INTERLEAVED ? pairs : NP;            // to the second pack; 0 at the odd end of a tail
+  if (e0 + step + NP > a.head_dim) step = 0;
+  const int64_t token = token0 + tk;
+  Pack<T, NP> x0[AHEAD], x1[AHEAD];
+  auto load = [&](int h0) {
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int h = h0 + u;
-      if (h < h_end) {
-        const int which = h >= a.heads0;
-        const T* src = static_cast<const T*>(a.in[which]) + token * a.in_token[which] +
-                       (int64_t)(which ? h - a.heads0 : h) * a.in_head[which];
-        x0[u] = *reinterpret_cast<const Pack<T, NP>*>(src + e0);
-        if (second) x1[u] = *reinterpret_cast<const Pack<T, NP>*>(src + e1);
+      const int h = h0 + u * a.head_lanes;
+      if (h < a.heads) {
+        const bool key = h >= a.heads0;
+        const T* src = static_cast<const T*>(key ? a.in[1] : a.in[0]) +
+                       token * (key ? a.in_token[1] : a.in_token[0]) +
+                       (key ? h - a.heads0 : h) * (key ? a.in_head[1] : a.in_head[0]) + e0;
+        x0[u] = *reinterpret_cast<const Pack<T, NP>*>(src);
+        x1[u] = *reinterpret_cast<const Pack<T, NP>*>(src + step);
       }
     }
+  };
+  if (mine) load(lane);
+  for (int i = threadIdx.x; i < nt * pairs; i += THREADS) {
+    const int t = i / pairs, p = i - t * pairs;
+    const double pos = a.pos64 ? (double)static_cast<const int64_t*>(a.positions)[token0 + t]
+                               : (double)static_cast<const int32_t*>(a.positions)[token0 + t];
+    double turns = pos * a.inv_freq[p] * 0.15915494309189535;      // 1 / (2 pi)
+    turns -= rint(turns);
+    float sn, cs;
+    sincospif((float)(2.0 * turns), &sn, &cs);
+    turn[t * pairs + (p % NP) * a.rot_cols + p / NP] = make_float2(cs * a.scale, sn * a.scale * a.sin_sign);
+  }
+  __syncthreads();
+  if (!mine) return;
+  float2 cs[NP];
+  if (rotating) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) cs[i] = turn[tk * pairs + i * a.rot_cols + col];
+  }
+  for (int h0 = lane; h0 < a.heads; h0 += AHEAD * a.head_lanes) {
+    if (h0 != lane) load(h0);
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int h = h0 + u;
-      if (h >= h_end) break;
-      if (rotating) {
-        if constexpr (INTERLEAVED && NP > 1) {
-          // pairs sit next to each other inside the packs
-#pragma unroll
-          for (int i = 0; i < NP; ++i) {
-            T* p = i < NP / 2 ? &x0[u].v[2 * i] : &x1[u].v[2 * i - NP];
-            const float p1 = Conv<T>::to(p[0]), p2 = Conv<T>::to(p[1]);
-            p[0] = Conv<T>::from(p1 * c[i] - p2 * s[i]);
-            p[1] = Conv<T>::from(p2 * c[i] + p1 * s[i]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < NP; ++i) {
-            const float p1 = Conv<T>::to(x0[u].v[i]), p2 = Conv<T>::to(x1[u].v[i]);
-            x0[u].v[i] = Conv<T>::from(p1 * c[i] - p2 * s[i]);
-            x1[u].v[i] = Conv<T>::from(p2 * c[i] + p1 * s[i]);
-          }
-        }
-      }
-      const int which = h >= a.heads0;
-      T* dst = static_cast<T*>(a.out[which]) + token * a.out_token[which] +
-               (int64_t)(which ? h - a.heads0 : h) * a.out_head[which];
-      *reinterpret_cast<Pack<T, NP>*>(dst + e0) = x0[u];
-      if (second) *reinterpret_cast<Pack<T, NP>*>(dst + e1) = x1[u];
+      const int h = h0 + u * a.head_lanes;
+      if (h >= a.heads) break;
+      if (rotating) turn_packs<T, NP, INTERLEAVED>(x0[u], x1[u], [&](int i) { return cs[i]; });
+      const bool key = h >= a.heads0;
+      T* dst = static_cast<T*>(key ? a.out[1] : a.out[0]) + token * (key ? a.out_token[1] : a.out_token[0]) +
+               (key ? h - a.heads0 : h) * (key ? a.out_head[1] : a.out_head[0]) + e0;
+      *reinterpret_cast<Pack<T, NP>*>(dst) = x0[u];
+      if (step) *reinterpret_cast<Pack<T, NP>*>(dst + step) = x1[u];
     }
   }
 }
@@ -144,15 +174,22 @@ template <typename T, int NP>
 int launch(RotaryArgs& a, bool interleaved, cudaStream_t st) {
   a.rot_cols = a.rotary_dim / (2 * NP);
   a.cols = a.rot_cols + (int)ceil_div(a.head_dim - a.rotary_dim, 2 * NP);
-  // all heads in one thread once there are enough (token, column) threads to fill the part, else the heads
-  // are spread over threads, which recompute the cos/sin: 1 token of 20 heads takes one wave of one head each
-  const int64_t threads = a.tokens * a.cols;
-  const int64_t want = (int64_t)semblo::sm_count() * 2048;
-  const int64_t groups = std::min<int64_t>(a.heads, std::max<int64_t>(1, want / std::max<int64_t>(threads, 1)));
-  a.heads_per_group = (int)ceil_div(a.heads, groups);
-  dim3 grid((unsigned)ceil_div(threads, 256), (unsigned)ceil_div(a.heads, a.heads_per_group));
-  if (interleaved) rotary_kernel<T, NP, true><<<grid, 256, 0, st>>>(a);
-  else rotary_kernel<T, NP, false><<<grid, 256, 0, st>>>(a);
+  // each thread takes the heads of one batch of loads and the block as many tokens as then fit; while there
+  // are fewer tokens than two blocks per multiprocessor would take, one token per block and every thread
+  const int rows = THREADS / a.cols;
+  int lanes = (int)std::min<int64_t>(rows, ceil_div(a.heads, AHEAD));
+  int tb = rows / lanes;
+  if (a.tokens < (int64_t)tb * 2 * semblo::sm_count()) {
+    lanes = std::min(rows, a.heads);
+    tb = 1;
+  }
+  tb = std::min(tb, std::max(1, 4096 / std::max(1, a.rotary_dim / 2)));      // 32 KB of cos/sin
+  a.tokens_per_block = tb;
+  a.head_lanes = lanes;
+  const unsigned grid = (unsigned)ceil_div(a.tokens, tb);
+  const size_t smem = (size_t)tb * (a.rotary_dim / 2) * sizeof(float2);
+  if (interleaved) rotary_kernel<T, NP, true><<<grid, THREADS, smem, st>>>(a);
+  else rotary_kernel<T, NP, false><<<grid, THREADS, smem, st>>>(a);
   SEMBLO_LAUNCH_CHECK();
   return 0;
 }
@@ -187,11 +224,12 @@ extern "C" int semblo_rotary(const void* q, int64_t q_token_stride, int64_t q_he
   SEMBLO_REQUIRE(tokens >= 0 && num_q_heads > 0 && num_kv_heads >= 0, "bad token or head count");
   SEMBLO_REQUIRE(rotary_dim >= 0 && rotary_dim % 2 == 0 && rotary_dim <= head_dim,
                  "rotary_dim must be even and at most head_dim (got %d of %d)", rotary_dim, head_dim);
+  SEMBLO_REQUIRE(head_dim > 0 && head_dim <= MAX_HEAD_DIM, "head_dim must be at most %d (got %d)", MAX_HEAD_DIM, head_dim);
   SEMBLO_REQUIRE((k == nullptr) == (k_out == nullptr), "k and k_out come together");
   if (tokens == 0) return 0;
   SEMBLO_REQUIRE(q != nullptr && q_out != nullptr && positions != nullptr, "q, q_out and positions are required");
   SEMBLO_REQUIRE(rotary_dim == 0 || inv_freq != nullptr, "inv_freq is required");
-  SEMBLO_REQUIRE(tokens <= (int64_t)1 << 31, "too many tokens");
+  SEMBLO_REQUIRE(tokens < (int64_t)1 << 31, "too many tokens");
   RotaryArgs a{};
   a.in[0] = q; a.out[0] = q_out; a.in[1] = k; a.out[1] = k_out;
   a.in_token[0] = q_token_stride; a.in_head[0] = q_head_stride;

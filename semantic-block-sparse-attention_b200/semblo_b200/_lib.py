@@ -138,6 +138,11 @@ def refuse_gradients(*tensors: torch.Tensor | None) -> None:
                            "tensors that require none")
 
 
+def raw_stream(index: int) -> int:
+    """The current stream of device ``index`` as the C entries take it."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def device_scope(device: torch.device):
     """Make ``device`` current for a call, so that its launches and stream are that device's."""
     if device.index is None or device.index == torch.cuda.current_device():

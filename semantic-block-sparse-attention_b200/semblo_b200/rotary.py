@@ -12,8 +12,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import (check, device_scope, dtype_code, lib, ptr, refuse_gradients, require_cuda, require_same_device,
-                   stream_ptr)
+from ._lib import check, device_scope, dtype_code, lib, raw_stream, refuse_gradients, require_cuda
 
 _SCALING_KEYS = {"linear": {"factor"}, "ntk": {"factor"},
                  "yarn": {"factor", "original_max_position", "beta_fast", "beta_slow", "attention_factor"},
@@ -96,12 +95,15 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: dict 
     return RotaryFrequencies(inv.to(device), scale)
 
 
-def _rows(name: str, x: torch.Tensor, tokens: int, dim: int | None) -> None:
-    if x.ndim != 3 or x.shape[0] != tokens or (dim is not None and x.shape[2] != dim):
-        raise ValueError(f"{name} must have shape [T, heads, D] with T = {tokens}" +
-                         (f" and D = {dim}" if dim is not None else "") + f" (got {tuple(x.shape)})")
-    if x.shape[2] > 1 and x.stride(2) != 1:
+def _check_rows(name: str, x: torch.Tensor, tokens: int, dim: int, dtype, device) -> None:
+    if x.ndim != 3 or x.shape[0] != tokens or x.shape[2] != dim:
+        raise ValueError(f"{name} must have shape [{tokens}, heads, {dim}] (got {tuple(x.shape)})")
+    if x.stride(2) != 1 and dim > 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
+    if x.dtype != dtype:
+        raise ValueError("q_pre, k_pre and the outputs must have one dtype")
+    if x.device != device:
+        raise ValueError(f"the tensors of a call must be on one device ({name} is on {x.device}, q_pre on {device})")
 
 
 def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -114,6 +116,15 @@ def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
+def _check_output(name: str, y: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+    _check_rows(name, y, x.shape[0], x.shape[2], x.dtype, x.device)
+    if y.shape != x.shape:
+        raise ValueError(f"{name} must have the shape of its input")
+    if _overlaps(x, y) and (x.data_ptr() != y.data_ptr() or x.stride() != y.stride()):
+        raise ValueError(f"{name} overlaps its input without being it")
+    return y
+
+
 def apply_rotary(q_pre: torch.Tensor, k_pre: torch.Tensor | None, positions: torch.Tensor,
                  frequencies: RotaryFrequencies, *, interleaved: bool = False, inverse: bool = False,
                  q_out: torch.Tensor | None = None,
@@ -124,47 +135,42 @@ def apply_rotary(q_pre: torch.Tensor, k_pre: torch.Tensor | None, positions: tor
     The first ``frequencies.rotary_dim`` dimensions are rotated: pair i is (x_i, x_{i + R/2}), or (x_2i, x_2i+1)
     with ``interleaved``; the others are copied.  ``inverse`` rotates back (the transpose).  ``q_out`` / ``k_out``
     receive the result; either may be its input itself (in place).  Angles are formed in 64 bits."""
-    require_cuda(q_pre, k_pre, positions, frequencies.inv_freq, q_out, k_out)
+    require_cuda(q_pre, k_pre, positions, q_out, k_out)
     refuse_gradients(q_pre, k_pre)
     if q_pre.ndim != 3:
         raise ValueError("q_pre must have shape [T, Hq, D]")
-    tokens, hq, dim = (int(n) for n in q_pre.shape)
-    code = dtype_code(q_pre.dtype, "rotary")
+    tokens, hq, dim = q_pre.shape
+    dtype, device = q_pre.dtype, q_pre.device
+    code = dtype_code(dtype, "rotary")
+    _check_rows("q_pre", q_pre, tokens, dim, dtype, device)
     if positions.ndim != 1 or positions.shape[0] != tokens or positions.dtype not in (torch.int32, torch.int64):
         raise ValueError("positions must be one int32 or int64 per token")
-    if frequencies.rotary_dim > dim:
-        raise ValueError(f"rotary_dim {frequencies.rotary_dim} exceeds the head dimension {dim}")
-    _rows("q_pre", q_pre, tokens, dim)
-    if q_out is None:
-        q_out = torch.empty((tokens, hq, dim), dtype=q_pre.dtype, device=q_pre.device)
-    pairs = [("q_out", q_pre, q_out)]
+    inv_freq = frequencies.inv_freq
+    rotary_dim = 2 * inv_freq.shape[0]
+    if rotary_dim > dim:
+        raise ValueError(f"rotary_dim {rotary_dim} exceeds the head dimension {dim}")
+    if positions.device != device or inv_freq.device != device:
+        raise ValueError(f"the positions ({positions.device}) and frequencies ({inv_freq.device}) must be on the "
+                         f"device of q_pre ({device})")
+    q_out = torch.empty((tokens, hq, dim), dtype=dtype, device=device) if q_out is None else \
+        _check_output("q_out", q_out, q_pre)
+    hkv, k_args = 0, (None, 0, 0, None, 0, 0, 0)
     if k_pre is None:
         if k_out is not None:
             raise ValueError("k_out is given without k_pre")
     else:
-        _rows("k_pre", k_pre, tokens, dim)
-        if k_out is None:
-            k_out = torch.empty(tuple(k_pre.shape), dtype=k_pre.dtype, device=k_pre.device)
-        pairs.append(("k_out", k_pre, k_out))
-    for name, x, y in pairs:
-        if x.dtype != q_pre.dtype or y.dtype != q_pre.dtype:
-            raise ValueError("q_pre, k_pre and the outputs must have one dtype")
-        if y.shape != x.shape:
-            raise ValueError(f"{name} must have the shape of its input")
-        _rows(name, y, tokens, dim)
-        if _overlaps(x, y) and (x.data_ptr() != y.data_ptr() or x.stride() != y.stride()):
-            raise ValueError(f"{name} overlaps its input without being it")
-    require_same_device(q_pre, k_pre, positions, frequencies.inv_freq, q_out, k_out)
-    positions = positions.contiguous()
-    k_in, hkv = (k_pre, int(k_pre.shape[1])) if k_pre is not None else (None, 0)
-    ks = (k_pre.stride(0), k_pre.stride(1)) if k_pre is not None else (0, 0)
-    kos = (k_out.stride(0), k_out.stride(1)) if k_pre is not None else (0, 0)
-    if hkv == 0:
-        k_in = None
-    with device_scope(q_pre.device):
+        _check_rows("k_pre", k_pre, tokens, dim, dtype, device)
+        hkv = k_pre.shape[1]
+        k_out = torch.empty((tokens, hkv, dim), dtype=dtype, device=device) if k_out is None else \
+            _check_output("k_out", k_out, k_pre)
+        if hkv:
+            k_args = (k_pre.data_ptr(), k_pre.stride(0), k_pre.stride(1), k_out.data_ptr(), k_out.stride(0),
+                      k_out.stride(1), hkv)
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    with device_scope(device):
         check(lib().semblo_rotary(
-            ptr(q_pre), q_pre.stride(0), q_pre.stride(1), ptr(q_out), q_out.stride(0), q_out.stride(1), hq, ptr(k_in),
-            *ks, ptr(k_out) if k_in is not None else None, *kos, hkv, tokens, dim, frequencies.rotary_dim, code,
-            ptr(positions), 1 if positions.dtype == torch.int64 else 0, ptr(frequencies.inv_freq),
-            float(frequencies.attention_scale), 1 if interleaved else 0, 1 if inverse else 0, stream_ptr()))
+            q_pre.data_ptr(), q_pre.stride(0), q_pre.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1), hq,
+            *k_args, tokens, dim, rotary_dim, code, positions.data_ptr(), positions.dtype == torch.int64,
+            inv_freq.data_ptr(), frequencies.attention_scale, interleaved, inverse, raw_stream(device.index)))
     return q_out, k_out
