@@ -10,9 +10,10 @@
 // can repair.  sincospi of the reduced fraction is then as accurate as a float can be.
 //
 // Bound: HBM, one read and one write of every element.  A cos/sin costs ~50 instructions and serves all
-// heads of a token, so a block takes whole tokens and computes each cos/sin once, while the rows that its
-// threads have requested (2 x 16 bytes each, 2 rows) travel; after one barrier a thread takes the cos/sin of
-// its column's 8 pairs from shared memory and turns its rows with them.
+// heads of a token, so a block walks over tiles of whole tokens and keeps two of everything: while a thread
+// turns the rows it holds, its next rows (2 x 16 bytes each, 2 rows) travel and the next tile's cos/sin go
+// to the other half of shared memory; one barrier per tile.  A block per token instead of a walk spent a
+// third of its time waiting at that barrier for a chain of divisions, position loads and sines.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -103,26 +104,28 @@ __device__ __forceinline__ void turn_packs(Pack<T, NP>& p0, Pack<T, NP>& p1, F t
   }
 }
 
-constexpr int AHEAD = 2;        // rows whose loads a thread keeps in flight
+constexpr int AHEAD = 2;        // rows of a thread that travel together
 
 // NP: pairs per thread and row.  A rotating column c covers the pairs [NP c, NP (c + 1)): two packs of NP
 // elements, R/2 apart (half) or adjacent (interleaved).  A copying column covers 2 NP elements from R on
 // (NP = 1: two single elements, the second may lie past the head).
 template <typename T, int NP, bool INTERLEAVED>
 __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotaryArgs a) {
-  extern __shared__ float2 turn[];        // cos, sin: [token][i][column] for pair NP column + i, so that a warp's reads do not collide
-  const int64_t token0 = (int64_t)blockIdx.x * a.tokens_per_block;
-  const int nt = (int)min((int64_t)a.tokens_per_block, a.tokens - token0);
+  // cos, sin: [buffer][token][i][column] for pair NP column + i, so that a warp's reads do not collide
+  extern __shared__ float2 turn[];
   const int pairs = a.rotary_dim >> 1;
+  const int tile_pairs = a.tokens_per_block * pairs;
   const int row = threadIdx.x / a.cols, col = threadIdx.x - row * a.cols;
   const int tk = row / a.head_lanes, lane = row - tk * a.head_lanes;
-  const bool mine = tk < nt, rotating = col < a.rot_cols;
+  const bool mine = tk < a.tokens_per_block, rotating = col < a.rot_cols;
   const int e0 = rotating ? (INTERLEAVED ? 2 * NP * col : NP * col) : a.rotary_dim + 2 * NP * (col - a.rot_cols);
   int step = rotating && !INTERLEAVED ? pairs : NP;            // to the second pack; 0 at the odd end of a tail
   if (e0 + step + NP > a.head_dim) step = 0;
-  const int64_t token = token0 + tk;
-  Pack<T, NP> x0[AHEAD], x1[AHEAD];
-  auto load = [&](int h0) {
+  const int span = AHEAD * a.head_lanes;                       // heads of one batch
+  const int64_t advance = (int64_t)gridDim.x * a.tokens_per_block;
+
+  struct Batch { Pack<T, NP> x0[AHEAD], x1[AHEAD]; };
+  auto load = [&](Batch& b, int64_t token, int h0) {
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       const int h = h0 + u * a.head_lanes;
@@ -131,42 +134,64 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotaryArgs a) {
         const T* src = static_cast<const T*>(key ? a.in[1] : a.in[0]) +
                        token * (key ? a.in_token[1] : a.in_token[0]) +
                        (key ? h - a.heads0 : h) * (key ? a.in_head[1] : a.in_head[0]) + e0;
-        x0[u] = *reinterpret_cast<const Pack<T, NP>*>(src);
-        x1[u] = *reinterpret_cast<const Pack<T, NP>*>(src + step);
+        b.x0[u] = *reinterpret_cast<const Pack<T, NP>*>(src);
+        b.x1[u] = *reinterpret_cast<const Pack<T, NP>*>(src + step);
       }
     }
   };
-  if (mine) load(lane);
-  for (int i = threadIdx.x; i < nt * pairs; i += THREADS) {
-    const int t = i / pairs, p = i - t * pairs;
-    const double pos = a.pos64 ? (double)static_cast<const int64_t*>(a.positions)[token0 + t]
-                               : (double)static_cast<const int32_t*>(a.positions)[token0 + t];
-    double turns = pos * a.inv_freq[p] * 0.15915494309189535;      // 1 / (2 pi)
-    turns -= rint(turns);
-    float sn, cs;
-    sincospif((float)(2.0 * turns), &sn, &cs);
-    turn[t * pairs + (p % NP) * a.rot_cols + p / NP] = make_float2(cs * a.scale, sn * a.scale * a.sin_sign);
-  }
-  __syncthreads();
-  if (!mine) return;
-  float2 cs[NP];
-  if (rotating) {
-#pragma unroll
-    for (int i = 0; i < NP; ++i) cs[i] = turn[tk * pairs + i * a.rot_cols + col];
-  }
-  for (int h0 = lane; h0 < a.heads; h0 += AHEAD * a.head_lanes) {
-    if (h0 != lane) load(h0);
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      const int h = h0 + u * a.head_lanes;
-      if (h >= a.heads) break;
-      if (rotating) turn_packs<T, NP, INTERLEAVED>(x0[u], x1[u], [&](int i) { return cs[i]; });
-      const bool key = h >= a.heads0;
-      T* dst = static_cast<T*>(key ? a.out[1] : a.out[0]) + token * (key ? a.out_token[1] : a.out_token[0]) +
-               (key ? h - a.heads0 : h) * (key ? a.out_head[1] : a.out_head[0]) + e0;
-      *reinterpret_cast<Pack<T, NP>*>(dst) = x0[u];
-      if (step) *reinterpret_cast<Pack<T, NP>*>(dst + step) = x1[u];
+  auto angles = [&](float2* buf, int64_t token0) {
+    for (int i = threadIdx.x; i < tile_pairs; i += THREADS) {
+      const int t = a.tokens_per_block == 1 ? 0 : i / pairs, p = i - t * pairs;
+      if (token0 + t >= a.tokens) break;
+      const double pos = a.pos64 ? (double)static_cast<const int64_t*>(a.positions)[token0 + t]
+                                 : (double)static_cast<const int32_t*>(a.positions)[token0 + t];
+      double turns = pos * a.inv_freq[p] * 0.15915494309189535;      // 1 / (2 pi)
+      turns -= rint(turns);
+      float sn, cs;
+      sincospif((float)(2.0 * turns), &sn, &cs);
+      buf[t * pairs + (p % NP) * a.rot_cols + p / NP] = make_float2(cs * a.scale, sn * a.scale * a.sin_sign);
     }
+  };
+
+  int64_t token0 = (int64_t)blockIdx.x * a.tokens_per_block;
+  Batch now, next;
+  if (mine && token0 + tk < a.tokens) load(now, token0 + tk, lane);
+  angles(turn, token0);
+  __syncthreads();
+  for (int half = 0; token0 < a.tokens; token0 += advance, half ^= 1) {
+    const int64_t token = token0 + tk;
+    const bool have = mine && token < a.tokens;
+    const bool more = mine && token + advance < a.tokens;
+    float2 cs[NP];
+    if (rotating) {
+      const float2* c = turn + half * tile_pairs + (mine ? tk : 0) * pairs + col;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) cs[i] = c[i * a.rot_cols];
+    }
+    for (int h0 = lane; h0 < a.heads; h0 += span) {
+      if (h0 + span < a.heads) {
+        if (have) load(next, token, h0 + span);
+      } else if (more) {
+        load(next, token + advance, lane);
+      }
+      if (have) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          const int h = h0 + u * a.head_lanes;
+          if (h < a.heads) {
+            if (rotating) turn_packs<T, NP, INTERLEAVED>(now.x0[u], now.x1[u], [&](int i) { return cs[i]; });
+            const bool key = h >= a.heads0;
+            T* dst = static_cast<T*>(key ? a.out[1] : a.out[0]) + token * (key ? a.out_token[1] : a.out_token[0]) +
+                     (key ? h - a.heads0 : h) * (key ? a.out_head[1] : a.out_head[0]) + e0;
+            *reinterpret_cast<Pack<T, NP>*>(dst) = now.x0[u];
+            if (step) *reinterpret_cast<Pack<T, NP>*>(dst + step) = now.x1[u];
+          }
+        }
+      }
+      now = next;
+    }
+    if (token0 + advance < a.tokens) angles(turn + (half ^ 1) * tile_pairs, token0 + advance);
+    __syncthreads();
   }
 }
 
@@ -174,20 +199,23 @@ template <typename T, int NP>
 int launch(RotaryArgs& a, bool interleaved, cudaStream_t st) {
   a.rot_cols = a.rotary_dim / (2 * NP);
   a.cols = a.rot_cols + (int)ceil_div(a.head_dim - a.rotary_dim, 2 * NP);
-  // each thread takes the heads of one batch of loads and the block as many tokens as then fit; while there
-  // are fewer tokens than two blocks per multiprocessor would take, one token per block and every thread
+  // a block's threads are tokens x head lanes x columns: the split that leaves the fewest of them idle.  While
+  // there are fewer tokens than two blocks per multiprocessor would take, one token per block and every thread
   const int rows = THREADS / a.cols;
-  int lanes = (int)std::min<int64_t>(rows, ceil_div(a.heads, AHEAD));
-  int tb = rows / lanes;
-  if (a.tokens < (int64_t)tb * 2 * semblo::sm_count()) {
-    lanes = std::min(rows, a.heads);
-    tb = 1;
+  const int most_tokens = std::max(1, 1024 / std::max(1, a.rotary_dim / 2));          // 2 x 8 KB of cos/sin
+  int tb = 1, lanes = std::min(rows, a.heads);
+  double best = 0;
+  for (int l = 1; l <= std::min(rows, a.heads); ++l) {
+    const int t = std::min(rows / l, most_tokens);
+    if (a.tokens < (int64_t)t * 2 * semblo::sm_count()) continue;
+    const int64_t slots = ceil_div(ceil_div(a.heads, l), AHEAD) * AHEAD;
+    const double used = (double)t * a.heads / ((double)rows * slots);
+    if (used >= best) { best = used; tb = t; lanes = l; }
   }
-  tb = std::min(tb, std::max(1, 4096 / std::max(1, a.rotary_dim / 2)));      // 32 KB of cos/sin
   a.tokens_per_block = tb;
   a.head_lanes = lanes;
-  const unsigned grid = (unsigned)ceil_div(a.tokens, tb);
-  const size_t smem = (size_t)tb * (a.rotary_dim / 2) * sizeof(float2);
+  const size_t smem = 2 * (size_t)tb * (a.rotary_dim / 2) * sizeof(float2);
+  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(a.tokens, tb), (int64_t)semblo::sm_count() * 4);
   if (interleaved) rotary_kernel<T, NP, true><<<grid, THREADS, smem, st>>>(a);
   else rotary_kernel<T, NP, false><<<grid, THREADS, smem, st>>>(a);
   SEMBLO_LAUNCH_CHECK();
