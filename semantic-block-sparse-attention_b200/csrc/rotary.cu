@@ -30,9 +30,12 @@ constexpr int THREADS = 256;
 constexpr int MAX_HEAD_DIM = 512;           // a block holds the columns of one row at least
 
 struct RotaryArgs {
-  const void* in[2];            // q, k
-  void* out[2];
-  int64_t in_token[2], in_head[2], out_token[2], out_head[2];   // strides in elements
+  // scalars, not arrays of two: a select between array elements becomes a constant-bank load with an index
+  // that differs in the warp, and those serialise (half of all issue slots of an earlier form)
+  const void *q_in, *k_in;
+  void *q_out, *k_out;
+  int64_t q_in_token, q_in_head, q_out_token, q_out_head;       // strides in elements
+  int64_t k_in_token, k_in_head, k_out_token, k_out_head;
   int heads0, heads;            // query heads, query + key heads
   int64_t tokens;
   int tokens_per_block, head_lanes;     // threads per block: tokens x head lanes x columns
@@ -110,7 +113,7 @@ constexpr int AHEAD = 2;        // rows of a thread that travel together
 // elements, R/2 apart (half) or adjacent (interleaved).  A copying column covers 2 NP elements from R on
 // (NP = 1: two single elements, the second may lie past the head).
 template <typename T, int NP, bool INTERLEAVED>
-__global__ void __launch_bounds__(THREADS) rotary_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(THREADS, NP * sizeof(T) > 16 ? 2 : 3) rotary_kernel(const RotaryArgs a) {
   // cos, sin: [buffer][token][i][column] for pair NP column + i, so that a warp's reads do not collide
   extern __shared__ float2 turn[];
   const int pairs = a.rotary_dim >> 1;
@@ -131,9 +134,8 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotaryArgs a) {
       const int h = h0 + u * a.head_lanes;
       if (h < a.heads) {
         const bool key = h >= a.heads0;
-        const T* src = static_cast<const T*>(key ? a.in[1] : a.in[0]) +
-                       token * (key ? a.in_token[1] : a.in_token[0]) +
-                       (key ? h - a.heads0 : h) * (key ? a.in_head[1] : a.in_head[0]) + e0;
+        const T* src = (key ? static_cast<const T*>(a.k_in) + token * a.k_in_token + (h - a.heads0) * a.k_in_head
+                            : static_cast<const T*>(a.q_in) + token * a.q_in_token + h * a.q_in_head) + e0;
         b.x0[u] = *reinterpret_cast<const Pack<T, NP>*>(src);
         b.x1[u] = *reinterpret_cast<const Pack<T, NP>*>(src + step);
       }
@@ -181,8 +183,8 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotaryArgs a) {
           if (h < a.heads) {
             if (rotating) turn_packs<T, NP, INTERLEAVED>(now.x0[u], now.x1[u], [&](int i) { return cs[i]; });
             const bool key = h >= a.heads0;
-            T* dst = static_cast<T*>(key ? a.out[1] : a.out[0]) + token * (key ? a.out_token[1] : a.out_token[0]) +
-                     (key ? h - a.heads0 : h) * (key ? a.out_head[1] : a.out_head[0]) + e0;
+            T* dst = (key ? static_cast<T*>(a.k_out) + token * a.k_out_token + (h - a.heads0) * a.k_out_head
+                          : static_cast<T*>(a.q_out) + token * a.q_out_token + h * a.q_out_head) + e0;
             *reinterpret_cast<Pack<T, NP>*>(dst) = now.x0[u];
             if (step) *reinterpret_cast<Pack<T, NP>*>(dst + step) = now.x1[u];
           }
@@ -215,7 +217,10 @@ int launch(RotaryArgs& a, bool interleaved, cudaStream_t st) {
   a.tokens_per_block = tb;
   a.head_lanes = lanes;
   const size_t smem = 2 * (size_t)tb * (a.rotary_dim / 2) * sizeof(float2);
-  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(a.tokens, tb), (int64_t)semblo::sm_count() * 4);
+  // many more blocks than fit at once, each with a handful of tiles: with one resident wave the blocks step
+  // through memory in lockstep (131072 tokens x 20 heads x 256: 398 us at 64 per multiprocessor, 415 at 16, 500
+  // at 3; 8192 x 40 x 128: 30.8, 30.9 and 30.3)
+  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(a.tokens, tb), (int64_t)semblo::sm_count() * 64);
   if (interleaved) rotary_kernel<T, NP, true><<<grid, THREADS, smem, st>>>(a);
   else rotary_kernel<T, NP, false><<<grid, THREADS, smem, st>>>(a);
   SEMBLO_LAUNCH_CHECK();
@@ -226,11 +231,10 @@ int launch(RotaryArgs& a, bool interleaved, cudaStream_t st) {
 template <typename T>
 int dispatch(RotaryArgs& a, bool interleaved, cudaStream_t st) {
   uint64_t bits = 0;                                 // of every byte offset that a row can start at
-  for (int w = 0; w < 2; ++w) {
-    if (!a.in[w]) continue;
-    bits |= (uint64_t)(uintptr_t)a.in[w] | (uint64_t)(uintptr_t)a.out[w];
-    bits |= (uint64_t)(a.in_token[w] | a.in_head[w] | a.out_token[w] | a.out_head[w]) * sizeof(T);
-  }
+  bits |= (uint64_t)(uintptr_t)a.q_in | (uint64_t)(uintptr_t)a.q_out | (uint64_t)(uintptr_t)a.k_in |
+          (uint64_t)(uintptr_t)a.k_out;
+  bits |= (uint64_t)(a.q_in_token | a.q_in_head | a.q_out_token | a.q_out_head) * sizeof(T);
+  if (a.k_in) bits |= (uint64_t)(a.k_in_token | a.k_in_head | a.k_out_token | a.k_out_head) * sizeof(T);
   auto fits = [&](int np) {
     const uint64_t align = std::min<uint64_t>(16, np * sizeof(T));
     return a.rotary_dim % (2 * np) == 0 && a.head_dim % (2 * np) == 0 && bits % align == 0;
@@ -259,11 +263,11 @@ extern "C" int semblo_rotary(const void* q, int64_t q_token_stride, int64_t q_he
   SEMBLO_REQUIRE(rotary_dim == 0 || inv_freq != nullptr, "inv_freq is required");
   SEMBLO_REQUIRE(tokens < (int64_t)1 << 31, "too many tokens");
   RotaryArgs a{};
-  a.in[0] = q; a.out[0] = q_out; a.in[1] = k; a.out[1] = k_out;
-  a.in_token[0] = q_token_stride; a.in_head[0] = q_head_stride;
-  a.out_token[0] = qo_token_stride; a.out_head[0] = qo_head_stride;
-  a.in_token[1] = k_token_stride; a.in_head[1] = k_head_stride;
-  a.out_token[1] = ko_token_stride; a.out_head[1] = ko_head_stride;
+  a.q_in = q; a.q_out = q_out; a.k_in = k; a.k_out = k_out;
+  a.q_in_token = q_token_stride; a.q_in_head = q_head_stride;
+  a.q_out_token = qo_token_stride; a.q_out_head = qo_head_stride;
+  a.k_in_token = k_token_stride; a.k_in_head = k_head_stride;
+  a.k_out_token = ko_token_stride; a.k_out_head = ko_head_stride;
   a.heads0 = num_q_heads;
   a.heads = num_q_heads + (k ? num_kv_heads : 0);
   a.tokens = tokens;
