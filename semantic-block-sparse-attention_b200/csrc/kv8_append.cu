@@ -8,8 +8,8 @@
 //
 // e4m3 keeps three mantissa bits at every magnitude, so a power of two costs no accuracy against max / 448,
 // a new maximum inside the same octave changes nothing, and the codes of rows already written move by whole
-// exponents: they are rounded a second time only where they fall below 2^-6.  One thread block owns one (cache block, head,
-// K or V): no atomics, the same bytes on every run.
+// exponents: they are rounded a second time only where they fall below 2^-6.  One thread block owns one
+// (cache block, head, K or V): no atomics, the same bytes on every run.
 //
 // Bound: HBM, 2 bytes read and 1 written per value.  The maximum is needed before the first code, so a
 // thread holds its share of the block in registers between the two steps and the input is read once.
@@ -63,9 +63,18 @@ __device__ __forceinline__ uint32_t code4(float2 a, float2 b) {
   return lo | (hi << 16);
 }
 
+__device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
+  const __half2_raw r0 = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+  const __half2_raw r1 = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+  float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&r0));
+  float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&r1));
+  f0.x *= ratio; f0.y *= ratio; f1.x *= ratio; f1.y *= ratio;
+  return code4(f0, f1);
+}
+
 // Maximum over the thread block of a non-negative value (compared as bits).
 __device__ __forceinline__ float block_max(float v, uint32_t* slots) {
-  uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
+  const uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
   if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = b;
   __syncthreads();
   uint32_t m = 0;
@@ -80,6 +89,7 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs a) {
   __shared__ uint32_t slots[16];
   const int lane = threadIdx.x & 31;
   const int block = 1 << a.block_log2;
+  const int piece0 = threadIdx.x, piece_step = blockDim.x;
   // ---- which request and cache block: every warp walks the requests, 32 at a time
   int want = (int)blockIdx.x, seq = -1, n = 0, start = 0, nth = 0;
   int64_t row0 = 0;
@@ -123,13 +133,7 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs a) {
   const int64_t pos0 = ((int64_t)slot << a.block_log2) + off;
   const int m = (int)min((int64_t)(block - off), (int64_t)start + n - pos0);
   const int64_t page = slot < a.table_len ? a.table[seq * a.table_stride + slot] : -1;
-  if (page < 0 || page >= a.cache_blocks) {
-    if (threadIdx.x == 0) atomicCAS(a.status, 0, sm100::STATUS_OVERFLOW);
-    return;
-  }
   const int h = blockIdx.y, part = blockIdx.z;
-  const int64_t cell = ((int64_t)part * a.cache_blocks + page) * a.num_kv_heads + h;
-  uint8_t* dst = a.data + (cell << a.block_log2) * a.head_dim;
   const uint16_t* src = static_cast<const uint16_t*>(a.src[part]) + (row0 + pos0 - start) * a.src_token[part] +
                         (int64_t)h * a.src_head[part];
   // ---- the new rows into registers, their largest magnitude
@@ -137,7 +141,7 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs a) {
   uint4 x[NL][2];
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
-    const int p = i * blockDim.x + threadIdx.x;
+    const int p = i * piece_step + piece0;
     x[i][0] = x[i][1] = make_uint4(0u, 0u, 0u, 0u);
     if (p < pieces) {
       const uint4* s = reinterpret_cast<const uint4*>(src + (int64_t)(p >> a.col_log2) * a.src_token[part] +
@@ -146,6 +150,12 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs a) {
       x[i][1] = __ldg(s + 1);
     }
   }
+  if (page < 0 || page >= a.cache_blocks) {
+    if (threadIdx.x == 0) atomicCAS(a.status, 0, sm100::STATUS_OVERFLOW);
+    return;
+  }
+  const int64_t cell = ((int64_t)part * a.cache_blocks + page) * a.num_kv_heads + h;
+  uint8_t* dst = a.data + (cell << a.block_log2) * a.head_dim;
   const float before = off ? a.scales[cell] : 0.f;
   T2 top2;
   *reinterpret_cast<uint32_t*>(&top2) = 0u;
@@ -185,19 +195,18 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs a) {
       // the rows of earlier calls follow the new scale
       const float ratio = before / scale;
       uint4* rows = reinterpret_cast<uint4*>(dst);
-      for (int p = threadIdx.x; p < off << a.col_log2; p += blockDim.x) {
-        uint4 v = rows[p];
-        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+      const int held = off << a.col_log2;
+      for (int p = piece0; p < held; p += 4 * piece_step) {
+        uint4 v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const __half2_raw r0 = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i] & 0xffffu), __NV_E4M3);
-          const __half2_raw r1 = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i] >> 16), __NV_E4M3);
-          float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&r0));
-          float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&r1));
-          f0.x *= ratio; f0.y *= ratio; f1.x *= ratio; f1.y *= ratio;
-          w[i] = code4(f0, f1);
+        for (int u = 0; u < 4; ++u)
+          if (p + u * piece_step < held) v[u] = rows[p + u * piece_step];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (p + u * piece_step >= held) break;
+          rows[p + u * piece_step] = make_uint4(recode4(v[u].x, ratio), recode4(v[u].y, ratio),
+                                                recode4(v[u].z, ratio), recode4(v[u].w, ratio));
         }
-        rows[p] = v;
       }
     }
   }
@@ -207,7 +216,7 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs a) {
   const float inv = exact_inverse ? __int_as_float((254 << 23) - __float_as_int(scale)) : 0.f;
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
-    const int p = i * blockDim.x + threadIdx.x;
+    const int p = i * piece_step + piece0;
     if (p >= pieces) break;
     uint32_t out[4];
 #pragma unroll
@@ -226,17 +235,21 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs a) {
 }
 
 template <typename T2>
-int launch(const AppendArgs& a, cudaStream_t st) {
+int launch(AppendArgs& a, cudaStream_t st) {
   const int64_t block = (int64_t)1 << a.block_log2;
   const int64_t most = std::min<int64_t>(a.tokens, a.tokens / block + 2 * (int64_t)a.batch);
   const int64_t rows = std::min<int64_t>(block, a.tokens);        // new rows that a block can hold
-  const int64_t pieces = rows << a.col_log2;
+  const int64_t pieces = rows << a.col_log2, held = block << a.col_log2;
+  // 256 threads where the new rows fill them, or a continued block may have to be rounded again; 512 of 8
+  // pieces for the largest blocks (128 KB of input)
+  int64_t threads = std::min<int64_t>(256, std::max<int64_t>(64, held));
+  if (pieces > 2048) threads = 512;
+  const int64_t per_thread = ceil_div(pieces, threads);
   dim3 grid((unsigned)most, (unsigned)a.num_kv_heads, 2);
-  auto threads = [&](int nl) { return (unsigned)std::max<int64_t>(64, ceil_div(ceil_div(pieces, nl), 32) * 32); };
-  if (pieces <= 512) kv8_append_kernel<T2, 1><<<grid, threads(1), 0, st>>>(a);
-  else if (pieces <= 1024) kv8_append_kernel<T2, 2><<<grid, threads(2), 0, st>>>(a);
-  else if (pieces <= 2048) kv8_append_kernel<T2, 4><<<grid, threads(4), 0, st>>>(a);
-  else kv8_append_kernel<T2, 8><<<grid, threads(8), 0, st>>>(a);
+  if (per_thread <= 1) kv8_append_kernel<T2, 1><<<grid, (unsigned)threads, 0, st>>>(a);
+  else if (per_thread <= 2) kv8_append_kernel<T2, 2><<<grid, (unsigned)threads, 0, st>>>(a);
+  else if (per_thread <= 4) kv8_append_kernel<T2, 4><<<grid, (unsigned)threads, 0, st>>>(a);
+  else kv8_append_kernel<T2, 8><<<grid, (unsigned)threads, 0, st>>>(a);
   SEMBLO_LAUNCH_CHECK();
   return 0;
 }

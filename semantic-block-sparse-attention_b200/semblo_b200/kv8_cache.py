@@ -11,8 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import (check, device_scope, dtype_code, lib, ptr, refuse_gradients, require_cuda, require_same_device,
-                   stream_ptr)
+from ._lib import check, device_scope, dtype_code, lib, raw_stream, refuse_gradients, require_cuda, require_same_device
 
 BLOCK_SIZES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128, 256)
@@ -104,7 +103,8 @@ def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, block_table: t
     k, v = _token_rows("k", k), _token_rows("v", v)
     with device_scope(k.device):
         check(lib().semblo_kv8_append(
-            ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1), shape[0], dtype_code(k.dtype, "append"),
-            ptr(cache.data), ptr(cache.scales), cache.num_blocks, cache.block_size, cache.num_kv_heads, cache.head_dim,
-            ptr(table), table.stride(0), int(table.shape[1]), ptr(cu), ptr(start), batch,
-            ptr(_lib.status_for(k.device).word), stream_ptr()))
+            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), shape[0],
+            dtype_code(k.dtype, "append"), cache.data.data_ptr(), cache.scales.data_ptr(), cache.num_blocks,
+            cache.block_size, cache.num_kv_heads, cache.head_dim, table.data_ptr(), table.stride(0), table.shape[1],
+            cu.data_ptr(), start.data_ptr(), batch, _lib.status_for(k.device).word.data_ptr(),
+            raw_stream(k.device.index)))
