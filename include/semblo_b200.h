@@ -350,6 +350,24 @@ int semblo_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stri
                       const int32_t* cu_seqlens, const int32_t* start_positions, int batch, int32_t* status,
                       void* stream);
 
+/* Attention of the last `queries` (1 to 16) tokens of each request over the 8-bit paged cache: q, out
+ * [batch, queries, Hq, D] bf16 or fp16 (contiguous), D 64, 128 or 256; query i of request b is at position
+ * lengths[b] - queries + i and sees key j < lengths[b] when (j <= p and (window == 0 or p - j < window)) or
+ * j < prefix_lens[b] (NULL: none).  softcap > 0: scores become softcap tanh(score / softcap); alibi_slopes
+ * [Hq] fp32 (NULL: none): minus slope |p - j|.  lse [batch, queries, Hq] natural log, -inf for a row that
+ * sees nothing (its output is 0), may be NULL.  The workspace needs no initialisation; its size is 0 where
+ * every request's keys fit one block's share.  Status 201: a table entry outside the pool (its keys are
+ * taken as absent) or a length beyond the table. */
+int64_t semblo_kv8_decode_workspace_bytes(int batch, int queries, int num_q_heads, int num_kv_heads,
+                                          int head_dim, int block_size, int table_len, int window,
+                                          int has_prefix);
+int semblo_kv8_decode(const void* q, int dtype, int batch, int queries, int num_q_heads, int num_kv_heads,
+                      int head_dim, const void* cache, const float* scales, int64_t cache_blocks,
+                      int block_size, const int32_t* block_table, int64_t table_stride, int table_len,
+                      const int32_t* lengths, const int32_t* prefix_lens, int window, float sm_scale,
+                      float softcap, const float* alibi_slopes, void* out, float* lse, void* workspace,
+                      int64_t workspace_bytes, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

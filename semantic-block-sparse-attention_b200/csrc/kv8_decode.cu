@@ -1,0 +1,765 @@
+// Attention of generated tokens over the 8-bit paged K/V cache (one query, or a few, per request).
+//
+//   s_j = cap tanh(q . k_j sm / cap)  (or q . k_j sm) - slope |p - j|,  k_j = code_j * k_scale(block of j)
+//   o   = sum_j 2^(s_j log2e - m) v_j / sum_j 2^(s_j log2e - m),          p = length - queries + query index
+//   key j is seen when j < length and ((j <= p and p - j < window) or j < prefix).
+//
+// Bound: HBM, 2 D bytes per key and KV head.  What has to keep up with 24 bytes per clock and
+// multiprocessor is the way of a byte through it:
+//   * a warp takes 16 keys at a time through a private ring in shared memory; every lane copies (cp.async)
+//     exactly the bytes that it reads back, so the ring needs no barrier and no padding;
+//   * e4m3 becomes fp16 by the hardware's pair conversion and is exact there, as is the query after a power
+//     of two per row is taken out, so the products S^T = K Q^T of m16n8k16 are exact up to the fp32 sums.
+//     The order of the 16 values inside a k-step is free as long as K and Q agree: a lane's 16 consecutive
+//     bytes are its elements of four k-steps.  The same freedom over the rows of O^T = V^T P^T turns 16
+//     consecutive bytes of four keys into eight A fragments with two byte permutes per four values;
+//   * P^T is S^T's accumulator transposed by movmatrix; heads are the n dimension of both products, so that
+//     up to 8 rows (queries x heads of a KV head) cost one n-tile, up to 16 two.
+// V's scale changes from block to block, so P carries it: P' = 2^(s + log2 scale - M + 11) in fp16 with its own
+// running reference M next to the softmax's m (a block of large values with little weight must not push the
+// others under fp16's range).  Both move only when a score passes them by 2^4: P' stays below 2^15, and what
+// fp16 drops at its lower end is below 2^-36 of the largest term.
+//
+// Work is split evenly whatever the lengths: the 16-key groups of all (request, KV head, row tile) segments
+// form one line, every block takes an equal piece of it, writes the segments that lie inside its piece and
+// leaves partials of those that do not; a second launch (a programmatic dependent) merges them.  Where no
+// segment can be longer than 64 groups, a block takes one segment and there is nothing to merge.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "../../include/semblo_b200.h"
+#include "host_common.h"
+#include "sm100.cuh"
+
+using semblo::ceil_div;
+
+namespace {
+
+constexpr int WARPS = 8;
+constexpr int THREADS = WARPS * 32;
+constexpr int GROUP = 16;                 // keys per step of a warp
+constexpr int DIRECT_GROUPS = 64;         // longest segment that one block takes whole
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr float GAP = 4.f;                // log2 units by which a score may pass a reference
+constexpr float P_BIAS = 11.f;            // P' reaches 2^(P_BIAS + GAP) = 2^15
+
+struct DecodeArgs {
+  const void* q;                          // [B, n, Hq, D]
+  int q_f16;
+  void* out;                              // as q
+  float* lse;                             // [B, n, Hq] or null
+  const uint8_t* data;                    // [2, blocks, Hkv, block, D]
+  const float* scales;                    // [2, blocks, Hkv]
+  int64_t cache_blocks;
+  int block_log2;
+  const int32_t* table;
+  int64_t table_stride;
+  int table_len;
+  const int32_t* lengths;                 // [B]
+  const int32_t* prefix;                  // [B] or null
+  const float* slopes;                    // [Hq] or null
+  int batch, queries, num_q_heads, num_kv_heads, group;     // group: query heads per KV head
+  int rows, row_tiles;                    // queries * group, tiles of 8 NT rows
+  int window;                             // 0: none
+  float sm_scale, softcap;
+  int direct;
+  float* partial;                         // [grid][2][record]
+  int* status;
+};
+
+// ---------------------------------------------------------------- pieces
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp8(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Two e4m3 codes (low byte first) to two fp16.
+__device__ __forceinline__ uint32_t widen_lo(uint32_t w) {
+  uint32_t d;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(d) : "r"(w));
+  return d;
+}
+__device__ __forceinline__ uint32_t widen_hi(uint32_t w) {
+  uint32_t d;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(d) : "r"(w));
+  return d;
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ uint32_t half2_bits(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 2^(a - b) where equal references (both -inf among them) give 1.
+__device__ __forceinline__ float ratio2(float a, float b) { return a == b ? 1.f : sm100::fast_exp2(a - b); }
+
+// The groups of one request: prefix groups [0, gp), then [glo, ...).
+struct Span {
+  int length, first, lo, prefix;          // keys, position of the first query, first key of the window, prefix keys
+  int gp, glo, groups;
+  __device__ __forceinline__ int group_of(int i) const { return i < gp ? i : i - gp + glo; }
+};
+
+__device__ __forceinline__ Span span_of(const DecodeArgs& a, int b) {
+  Span s;
+  const int64_t room = (int64_t)a.table_len << a.block_log2;
+  const int given = a.lengths[b];
+  s.length = (int)min((int64_t)max(given, 0), room);
+  s.first = given - a.queries;
+  s.prefix = a.prefix ? min(max(a.prefix[b], 0), s.length) : 0;
+  s.lo = a.window > 0 ? max(0, s.first - a.window + 1) : 0;
+  s.gp = (s.prefix + GROUP - 1) / GROUP;
+  const int end = (s.length + GROUP - 1) / GROUP;
+  s.glo = min(max(s.gp, s.lo / GROUP), end);
+  s.groups = s.gp + end - s.glo;
+  return s;
+}
+
+template <int D, int NT>
+struct Cfg {
+  static constexpr int STAGES = D == 256 ? 3 : D == 128 ? 3 : 4;
+  static constexpr int KV_BYTES = GROUP * D;                    // K or V of a group
+  static constexpr int RING = STAGES * 2 * KV_BYTES;            // per warp
+  static constexpr int KC = D / 32;                             // 16-byte pieces of K per lane
+  static constexpr int VI = D == 256 ? 2 : 1;                   // pieces of V per lane and key (16 bytes, 8 for D = 64)
+  static constexpr int KSTEPS = D / 16;
+  static constexpr int ROWS = 8 * NT;
+  static constexpr bool Q_SMEM = D * NT > 256;                  // the query's fragments do not fit in registers
+  static constexpr int ACC = KSTEPS * NT * 4;                   // accumulators of O^T per lane
+  static constexpr int RECORD = ACC * 32 + 3 * ROWS;            // floats: O fragments, then m, M, l of each row
+  static constexpr int META_OFF = WARPS * RING;                 // float [WARPS][STAGES][2]: the group's scales
+  static constexpr int ML_OFF = META_OFF + WARPS * STAGES * 8;  // float [3][WARPS][ROWS]
+  static constexpr int FAC_OFF = ML_OFF + 3 * WARPS * ROWS * 4; // float [WARPS][ROWS] factors, [3][ROWS] totals
+  static constexpr int Q_OFF = FAC_OFF + (WARPS + 3) * ROWS * 4;
+  static constexpr int SUM_OFF = Q_OFF + (Q_SMEM ? KSTEPS * NT * 32 * 8 : 0);   // int [batch + 1], then [WARPS]
+  static_assert(ACC * 32 * 4 <= RING, "a warp's O must fit its ring");
+};
+
+// Inclusive sums of groups * segments-per-request over the batch into sums[1 ...]; sums[0] = 0.
+__device__ __forceinline__ void line_sums(const DecodeArgs& a, int segs, int* sums, int* scratch) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  int carry = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += blockDim.x) {
+    const int b = b0 + threadIdx.x;
+    int v = b < a.batch ? span_of(a, b).groups * segs : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += t;
+    }
+    if (lane == 31) scratch[warp] = v;
+    __syncthreads();
+    int before = carry;
+    for (int w = 0; w < warps; ++w) {
+      const int t = scratch[w];
+      if (w < warp) before += t;
+      carry += t;
+    }
+    if (b < a.batch) sums[b + 1] = before + v;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) sums[0] = 0;
+  __syncthreads();
+}
+
+__device__ __forceinline__ int quota_of(int total, int blocks) {
+  return max(WARPS, (total + blocks - 1) / blocks);
+}
+
+// Element e of a record in fragment order -> row of the tile and dimension.
+template <int D, int NT>
+__device__ __forceinline__ void element_of(int e, int& row, int& dim) {
+  const int lane = e & 31, c = (e >> 5) & 3, j = (e >> 7) % (D / 16), nt = (e >> 7) / (D / 16);
+  const int g = lane >> 2, t = lane & 3;
+  row = nt * 8 + 2 * t + (c & 1);
+  const int x = 2 * j + (c >> 1);                               // which of the lane's values of V
+  if constexpr (D == 64) dim = 8 * g + x;
+  else dim = 16 * g + (x & 15) + 128 * (x >> 4);
+}
+
+__device__ __forceinline__ void store_value(const DecodeArgs& a, int64_t at, float v) {
+  if (a.q_f16) static_cast<__half*>(a.out)[at] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
+}
+
+// One output value (and, with dimension 0, the row's log-sum-exp) from the sum of P' codes and the references.
+template <int D>
+__device__ __forceinline__ void finish(const DecodeArgs& a, int b, int h, int row, int dim, float acc, float m, float mv,
+                                       float l) {
+  const int qi = row / a.group;
+  const int64_t at = ((int64_t)b * a.queries + qi) * a.num_q_heads + h * a.group + row - qi * a.group;
+  store_value(a, at * D + dim, l == 0.f ? 0.f : acc * (sm100::fast_exp2(mv - m - P_BIAS) / l));
+  if (dim == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2;
+}
+
+// ---------------------------------------------------------------- attention
+template <int D, int NT, bool CAP>
+__global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_decode_kernel(const DecodeArgs a) {
+  using C = Cfg<D, NT>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  int* sums = reinterpret_cast<int*>(smem + C::SUM_OFF);
+  int* scratch = sums + a.batch + 1;
+  float* meta = reinterpret_cast<float*>(smem + C::META_OFF) + warp * C::STAGES * 2;
+  float* ml = reinterpret_cast<float*>(smem + C::ML_OFF);
+  float* factors = reinterpret_cast<float*>(smem + C::FAC_OFF);
+  float* totals = factors + WARPS * C::ROWS;
+  uint2* q_frag = reinterpret_cast<uint2*>(smem + C::Q_OFF);
+  uint8_t* ring = smem + warp * C::RING;
+  const uint32_t ring_u32 = sm100::smem_u32(ring), meta_u32 = sm100::smem_u32(meta);
+  const int segs = a.num_kv_heads * a.row_tiles;
+
+  int pos, end, quota = 0;
+  if (a.direct) {
+    pos = 0; end = 1;
+  } else {
+    line_sums(a, segs, sums, scratch);
+    const int total = sums[a.batch];
+    quota = quota_of(total, gridDim.x);
+    pos = (int)min((int64_t)total, (int64_t)blockIdx.x * quota);
+    end = min(total, pos + quota);
+  }
+
+  while (pos < end) {
+    // ---- the segment at pos
+    int b, seg, i0, i1;
+    Span sp;
+    if (a.direct) {
+      b = blockIdx.x / segs; seg = blockIdx.x - b * segs;
+      sp = span_of(a, b);
+      i0 = 0; i1 = sp.groups;
+      pos = end;
+    } else {
+      int lo = 0, hi = a.batch;                                 // the last request that starts at or before pos
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (sums[mid] <= pos) lo = mid; else hi = mid;
+      }
+      b = lo;
+      sp = span_of(a, b);
+      const int off = pos - sums[b];
+      seg = off / sp.groups;
+      i0 = off - seg * sp.groups;
+      i1 = min(sp.groups, i0 + end - pos);
+      pos += i1 - i0;
+    }
+    const int h = seg / a.row_tiles, row0 = (seg - h * a.row_tiles) * C::ROWS;
+    if (a.lengths[b] > sp.length && threadIdx.x == 0) atomicCAS(a.status, 0, sm100::STATUS_OVERFLOW);
+
+    // ---- pipeline over this warp's groups
+    const int count = max(0, (i1 - i0 - warp + WARPS - 1) / WARPS);
+    const int64_t table_row = (int64_t)b * a.table_stride;
+    auto page_for = [&](int it) -> int {                        // lane's look at the table for one iteration
+      if (it >= count) return -1;
+      const int slot = (sp.group_of(i0 + warp + it * WARPS) * GROUP) >> a.block_log2;
+      return a.table[table_row + slot];
+    };
+    int pages = page_for(lane), pages_next = 0;
+    uint32_t bad = 0;                                           // per stage: its block does not exist
+    auto issue = [&](int it) {
+      if ((it & 31) == 16) pages_next = page_for(it - 16 + 32 + lane);
+      if ((it & 31) == 0 && it > 0) pages = pages_next;
+      const int page = __shfl_sync(0xffffffffu, pages, it & 31);
+      if (it < count) {
+        const int st = it % C::STAGES;
+        const int key0 = sp.group_of(i0 + warp + it * WARPS) * GROUP;
+        if (page < 0 || page >= a.cache_blocks) {
+          bad |= 1u << st;
+          if (lane == 0) atomicCAS(a.status, 0, sm100::STATUS_OVERFLOW);
+        } else {
+          bad &= ~(1u << st);
+          const int64_t cell = (int64_t)page * a.num_kv_heads + h;
+          const int64_t part = a.cache_blocks * a.num_kv_heads;
+          const uint8_t* k = a.data + ((cell << a.block_log2) + (key0 & ((1 << a.block_log2) - 1))) * D;
+          const uint8_t* v = k + (part << a.block_log2) * D;
+          const uint32_t dst = ring_u32 + st * 2 * C::KV_BYTES;
+          // rows that no query sees are not read: zeros, since 0 * NaN would not vanish in P V
+          const bool whole = key0 + GROUP <= sp.length && (key0 >= sp.lo || key0 + GROUP <= sp.prefix);
+          auto bytes_of = [&](int r, int n) -> uint32_t {
+            const int key = key0 + r;
+            return whole || (key < sp.length && (key >= sp.lo || key < sp.prefix)) ? n : 0;
+          };
+#pragma unroll
+          for (int i = 0; i < C::KC / 2; ++i) {
+            cp16(dst + (2 * i * 32 + lane) * 16, k + g * D + 16 * t + 64 * i, bytes_of(g, 16));
+            cp16(dst + ((2 * i + 1) * 32 + lane) * 16, k + (g + 8) * D + 16 * t + 64 * i, bytes_of(g + 8, 16));
+          }
+          const uint32_t vdst = dst + C::KV_BYTES;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int key = 2 * t + (r & 1) + 8 * (r >> 1);
+            if constexpr (D == 64) {
+              cp8(vdst + (r * 32 + lane) * 8, v + key * D + 8 * g, bytes_of(key, 8));
+            } else {
+#pragma unroll
+              for (int i = 0; i < C::VI; ++i)
+                cp16(vdst + ((r * C::VI + i) * 32 + lane) * 16, v + key * D + 16 * g + 128 * i, bytes_of(key, 16));
+            }
+          }
+          if (lane < 2) cp4(meta_u32 + (st * 2 + lane) * 4, a.scales + cell + lane * part);
+        }
+      }
+      cp_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < C::STAGES - 1; ++s) issue(s);
+
+    // ---- the query: a power of two taken out of each row, fragments of fp16
+    uint2 qf[C::Q_SMEM ? 1 : C::KSTEPS * NT];
+    float coef[NT][2];
+    int qpos[NT][2];
+    float slope[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = row0 + nt * 8 + g;
+      const bool have = r < a.rows;
+      const int qi = have ? r / a.group : 0;
+      const int64_t qrow = ((int64_t)b * a.queries + qi) * a.num_q_heads + h * a.group + (have ? r - qi * a.group : 0);
+      uint2 raw[C::KSTEPS];
+      float top = 0.f;
+      auto pair = [&](uint32_t w) -> float2 {
+        if (a.q_f16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+      };
+#pragma unroll
+      for (int s = 0; s < C::KSTEPS; ++s) {
+        raw[s] = make_uint2(0u, 0u);
+        if (have) raw[s] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.q) + qrow * D + 64 * (s >> 2) +
+                                                                16 * t + 4 * (s & 3)));
+        const float2 x = pair(raw[s].x), y = pair(raw[s].y);
+        top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      int e = (int)(__float_as_uint(top) >> 23) - 126;          // top < 2^e
+      if (e == 129 || top == 0.f) e = 0;                        // infinities pass as they are
+      e = max(e, -100);
+      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+      for (int s = 0; s < C::KSTEPS; ++s) {
+        const float2 x = pair(raw[s].x), y = pair(raw[s].y);
+        const uint2 f = make_uint2(half2_bits(x.x * down, x.y * down), half2_bits(y.x * down, y.y * down));
+        if constexpr (C::Q_SMEM) {
+          if (warp == 0) q_frag[(s * NT + nt) * 32 + lane] = f;
+        } else {
+          qf[s * NT + nt] = f;
+        }
+      }
+      const float up = a.sm_scale * __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {                             // the rows of this lane's accumulator columns
+        const float u = __shfl_sync(0xffffffffu, up, (2 * t + c) * 4);
+        coef[nt][c] = CAP ? u / a.softcap : u * LOG2E;
+        const int rr = row0 + nt * 8 + 2 * t + c;
+        const int qq = rr < a.rows ? rr / a.group : 0;
+        qpos[nt][c] = sp.first + qq;
+        slope[nt][c] = a.slopes && rr < a.rows ? a.slopes[h * a.group + rr - qq * a.group] * LOG2E : 0.f;
+      }
+    }
+    if constexpr (C::Q_SMEM) __syncthreads();
+
+    float o[NT][C::KSTEPS][4];
+    float m[NT][2], mv[NT][2], l[NT][2];                        // mv: the reference of P'
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int j = 0; j < C::KSTEPS; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[nt][j][c] = 0.f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) { m[nt][c] = mv[nt][c] = -INFINITY; l[nt][c] = 0.f; }
+    }
+
+    for (int it = 0; it < count; ++it) {
+      issue(it + C::STAGES - 1);
+      cp_wait<C::STAGES - 1>();
+      __syncwarp();
+      const int st = it % C::STAGES;
+      if (bad >> st & 1) continue;
+      const int key0 = sp.group_of(i0 + warp + it * WARPS) * GROUP;
+      const uint8_t* kp = ring + st * 2 * C::KV_BYTES;
+      const float ks = meta[st * 2], vs = meta[st * 2 + 1];
+      // ---- S^T = K Q^T
+      float s[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+      for (int i = 0; i < C::KC / 2; ++i) {
+        const uint4 k0 = *reinterpret_cast<const uint4*>(kp + (2 * i * 32 + lane) * 16);
+        const uint4 k8 = *reinterpret_cast<const uint4*>(kp + ((2 * i + 1) * 32 + lane) * 16);
+        const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w8[4] = {k8.x, k8.y, k8.z, k8.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint32_t a0 = widen_lo(w0[u]), a1 = widen_lo(w8[u]), a2 = widen_hi(w0[u]), a3 = widen_hi(w8[u]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            uint2 q;
+            if constexpr (C::Q_SMEM) q = q_frag[((4 * i + u) * NT + nt) * 32 + lane];
+            else q = qf[(4 * i + u) * NT + nt];
+            mma16816(s[nt], a0, a1, a2, a3, q.x, q.y);
+          }
+        }
+      }
+      // ---- scores in log2 units; accumulator c: key g + 8 (c >> 1), row 2 t + (c & 1)
+      const float lv = __log2f(vs);
+      const bool all_seen = key0 + GROUP - 1 <= sp.first &&
+                            (a.window == 0 || key0 >= sp.first + a.queries - a.window || key0 + GROUP <= sp.prefix) &&
+                            key0 + GROUP <= sp.length;
+      bool need = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float x = s[nt][c] * (ks * coef[nt][c & 1]);
+          if constexpr (CAP) {
+            // tanh(x) = 1 - 2 / (1 + e^2x): exact at both ends, absolute error a few 2^-24
+            const float ex = sm100::fast_exp2(x * (2.f * LOG2E));
+            x = a.softcap * LOG2E * (1.f - __fdividef(2.f, 1.f + ex));
+          }
+          const int key = key0 + g + 8 * (c >> 1);
+          if (a.slopes) x -= slope[nt][c & 1] * fabsf((float)(qpos[nt][c & 1] - key));
+          if (!all_seen) {
+            const int d = qpos[nt][c & 1] - key;
+            const bool seen = key < sp.length && ((d >= 0 && (a.window == 0 || d < a.window)) || key < sp.prefix);
+            if (!seen) x = -INFINITY;
+          }
+          s[nt][c] = x;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float x = fmaxf(s[nt][c], s[nt][c + 2]);
+          need |= x > m[nt][c] + GAP || x + lv > mv[nt][c] + GAP;
+        }
+      }
+      if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float x = fmaxf(s[nt][c], s[nt][c + 2]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+            const float m1 = fmaxf(m[nt][c], x), mv1 = fmaxf(mv[nt][c], x + lv);
+            l[nt][c] *= ratio2(m[nt][c], m1);
+            const float f = ratio2(mv[nt][c], mv1);
+            m[nt][c] = m1;
+            mv[nt][c] = mv1;
+#pragma unroll
+            for (int j = 0; j < C::KSTEPS; ++j) { o[nt][j][c] *= f; o[nt][j][c + 2] *= f; }
+          }
+        }
+      }
+      uint32_t p[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float w[4];                                             // P', by an exponential of its own: it cannot overflow
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float ref = m[nt][c & 1], refv = mv[nt][c & 1];
+          l[nt][c & 1] += sm100::fast_exp2(s[nt][c] - (ref == -INFINITY ? 0.f : ref));
+          w[c] = sm100::fast_exp2(s[nt][c] + (refv == -INFINITY ? -INFINITY : lv - refv + P_BIAS));
+        }
+        p[nt][0] = transpose8x8(half2_bits(w[0], w[1]));
+        p[nt][1] = transpose8x8(half2_bits(w[2], w[3]));
+      }
+      // ---- O^T += V^T P^T
+      const uint8_t* vp = kp + C::KV_BYTES;
+#pragma unroll
+      for (int i = 0; i < C::VI; ++i) {
+        uint32_t w[4][4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (D == 64) {
+            const uint2 x = *reinterpret_cast<const uint2*>(vp + (r * 32 + lane) * 8);
+            w[r][0] = x.x; w[r][1] = x.y; w[r][2] = w[r][3] = 0u;
+          } else {
+            const uint4 x = *reinterpret_cast<const uint4*>(vp + ((r * C::VI + i) * 32 + lane) * 16);
+            w[r][0] = x.x; w[r][1] = x.y; w[r][2] = x.z; w[r][3] = x.w;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < (D == 64 ? 2 : 4); ++u) {
+          const uint32_t x01 = __byte_perm(w[0][u], w[1][u], 0x5140), y01 = __byte_perm(w[0][u], w[1][u], 0x7362);
+          const uint32_t x23 = __byte_perm(w[2][u], w[3][u], 0x5140), y23 = __byte_perm(w[2][u], w[3][u], 0x7362);
+          const uint32_t ax[4] = {widen_lo(x01), widen_hi(x01), widen_lo(x23), widen_hi(x23)};
+          const uint32_t ay[4] = {widen_lo(y01), widen_hi(y01), widen_lo(y23), widen_hi(y23)};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816(o[nt][8 * i + 2 * u], ax[0], ax[1], ax[2], ax[3], p[nt][0], p[nt][1]);
+            mma16816(o[nt][8 * i + 2 * u + 1], ay[0], ay[1], ay[2], ay[3], p[nt][0], p[nt][1]);
+          }
+        }
+      }
+      __syncwarp();
+    }
+    cp_wait<0>();
+
+    // ---- the warps' states into one
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], d);
+        if (g == 0) {
+          const int r = nt * 8 + 2 * t + c;
+          ml[warp * C::ROWS + r] = m[nt][c];
+          ml[(WARPS + warp) * C::ROWS + r] = mv[nt][c];
+          ml[(2 * WARPS + warp) * C::ROWS + r] = l[nt][c];
+        }
+      }
+    __syncwarp();
+    float* frag = reinterpret_cast<float*>(ring);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < C::KSTEPS; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) frag[((nt * C::KSTEPS + j) * 4 + c) * 32 + lane] = o[nt][j][c];
+    __syncthreads();
+    if (threadIdx.x < C::ROWS) {
+      const int r = threadIdx.x;
+      float mt = -INFINITY, mvt = -INFINITY, lt = 0.f;
+      for (int w = 0; w < WARPS; ++w) {
+        mt = fmaxf(mt, ml[w * C::ROWS + r]);
+        mvt = fmaxf(mvt, ml[(WARPS + w) * C::ROWS + r]);
+      }
+      for (int w = 0; w < WARPS; ++w) {
+        lt += ml[(2 * WARPS + w) * C::ROWS + r] * ratio2(ml[w * C::ROWS + r], mt);
+        factors[w * C::ROWS + r] = ratio2(ml[(WARPS + w) * C::ROWS + r], mvt);
+      }
+      totals[r] = mt; totals[C::ROWS + r] = mvt; totals[2 * C::ROWS + r] = lt;
+    }
+    __syncthreads();
+    const bool complete = i0 == 0 && i1 == sp.groups;
+    float* record = complete ? nullptr : a.partial + ((int64_t)blockIdx.x * 2 + (i0 == 0 ? 1 : 0)) * C::RECORD;
+    for (int e = threadIdx.x; e < C::ACC * 32; e += THREADS) {
+      int r, dim;
+      element_of<D, NT>(e, r, dim);
+      float acc = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w)
+        acc += reinterpret_cast<const float*>(smem + w * C::RING)[e] * factors[w * C::ROWS + r];
+      if (!complete) {
+        record[e] = acc;
+      } else if (row0 + r < a.rows) {
+        finish<D>(a, b, h, row0 + r, dim, acc, totals[r], totals[C::ROWS + r], totals[2 * C::ROWS + r]);
+      }
+    }
+    if (!complete && threadIdx.x < 3 * C::ROWS) record[C::ACC * 32 + threadIdx.x] = totals[threadIdx.x];
+    __syncthreads();
+  }
+  sm100::pdl_launch_dependents();
+}
+
+// ---------------------------------------------------------------- segments that more than one block worked on
+// blockIdx.x: segment; blockIdx.y: 256 of its record's elements.
+template <int D, int NT>
+__global__ void __launch_bounds__(THREADS) kv8_merge_kernel(const DecodeArgs a, int blocks) {
+  using C = Cfg<D, NT>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* factors = reinterpret_cast<float*>(smem);              // [blocks][ROWS]
+  float* totals = factors + blocks * C::ROWS;                   // [3][ROWS]
+  int* sums = reinterpret_cast<int*>(totals + 3 * C::ROWS);
+  int* scratch = sums + a.batch + 1;
+  const int segs = a.num_kv_heads * a.row_tiles;
+  const int b = blockIdx.x / segs, seg = blockIdx.x - b * segs;
+  line_sums(a, segs, sums, scratch);
+  const Span sp = span_of(a, b);
+  const int quota = quota_of(sums[a.batch], blocks);
+  const int s0 = sums[b] + seg * sp.groups, s1 = s0 + sp.groups;
+  const int c0 = s0 / quota, c1 = sp.groups ? (s1 - 1) / quota : c0;
+  sm100::pdl_wait();                                  // every block waits: this launch must not end before the other
+  if (sp.groups > 0 && c0 == c1) return;              // one block had it whole
+  const int parts = sp.groups ? c1 - c0 + 1 : 0;
+  // the block where the segment starts left it in its slot 1, the others in their slot 0
+  auto record = [&](int i) { return a.partial + ((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * C::RECORD; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int r = warp; r < C::ROWS; r += WARPS) {
+    float mt = -INFINITY, mvt = -INFINITY, lt = 0.f;
+    for (int i = lane; i < parts; i += 32) {
+      const float* x = record(i) + C::ACC * 32;
+      mt = fmaxf(mt, x[r]);
+      mvt = fmaxf(mvt, x[C::ROWS + r]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
+      mvt = fmaxf(mvt, __shfl_xor_sync(0xffffffffu, mvt, o));
+    }
+    for (int i = lane; i < parts; i += 32) {
+      const float* x = record(i) + C::ACC * 32;
+      lt += x[2 * C::ROWS + r] * ratio2(x[r], mt);
+      factors[i * C::ROWS + r] = ratio2(x[C::ROWS + r], mvt);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) lt += __shfl_xor_sync(0xffffffffu, lt, o);
+    if (lane == 0) { totals[r] = mt; totals[C::ROWS + r] = mvt; totals[2 * C::ROWS + r] = lt; }
+  }
+  __syncthreads();
+  const int h = seg / a.row_tiles, row0 = (seg - h * a.row_tiles) * C::ROWS;
+  const int e = blockIdx.y * THREADS + threadIdx.x;
+  int r, dim;
+  element_of<D, NT>(e, r, dim);
+  if (row0 + r >= a.rows) return;
+  float acc = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < parts; ++i) acc += record(i)[e] * factors[i * C::ROWS + r];
+  finish<D>(a, b, h, row0 + r, dim, acc, totals[r], totals[C::ROWS + r], totals[2 * C::ROWS + r]);
+}
+
+struct Plan {
+  int blocks, direct;
+  int64_t bytes;
+};
+
+template <int D, int NT>
+Plan plan_for(int64_t segments, int64_t longest) {
+  using C = Cfg<D, NT>;
+  Plan p;
+  p.direct = longest <= DIRECT_GROUPS;
+  const int64_t per_sm = (D == 256 || NT == 2) ? 1 : 2;
+  // no more blocks than there can be pieces of WARPS groups
+  p.blocks = (int)(p.direct ? segments
+                            : std::min<int64_t>(semblo::sm_count() * per_sm, ceil_div(segments * longest, WARPS)));
+  p.bytes = p.direct ? 0 : (int64_t)p.blocks * 2 * C::RECORD * 4;
+  return p;
+}
+
+int64_t longest_segment(int queries, int window, int table_len, int block_size, bool prefix) {
+  int64_t keys = (int64_t)table_len * block_size;
+  if (window > 0 && !prefix) keys = std::min<int64_t>(keys, (int64_t)window + queries + GROUP);
+  return ceil_div(keys, GROUP);
+}
+
+template <int D, int NT, bool CAP>
+int launch(DecodeArgs& a, const Plan& plan, cudaStream_t st) {
+  using C = Cfg<D, NT>;
+  const int sums = (a.batch + 1 + WARPS) * 4;
+  const int smem = C::SUM_OFF + sums;
+  auto kern = kv8_decode_kernel<D, NT, CAP>;
+  SEMBLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  a.direct = plan.direct;
+  kern<<<plan.blocks, THREADS, smem, st>>>(a);
+  SEMBLO_LAUNCH_CHECK();
+  if (plan.direct) return 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(a.batch * a.num_kv_heads * a.row_tiles), C::ACC * 32 / THREADS);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = sums + (plan.blocks + 3) * C::ROWS * 4;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  SEMBLO_CUDA(cudaLaunchKernelEx(&cfg, kv8_merge_kernel<D, NT>, (const DecodeArgs)a, plan.blocks));
+  return 0;
+}
+
+int check_shape(int batch, int queries, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                int table_len, int window, int* rows, int* nt, int* tiles) {
+  SEMBLO_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, "head_dim must be 64, 128 or 256 (got %d)",
+                 head_dim);
+  SEMBLO_REQUIRE(num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0,
+                 "query heads must be a multiple of the KV heads");
+  SEMBLO_REQUIRE(block_size >= 16 && block_size <= 256 && (block_size & (block_size - 1)) == 0,
+                 "block_size must be 16, 32, 64, 128 or 256 (got %d)", block_size);
+  SEMBLO_REQUIRE(queries >= 1 && queries <= 16, "1 to 16 queries per request (got %d)", queries);
+  SEMBLO_REQUIRE(batch >= 0 && batch <= 4096, "at most 4096 requests (got %d)", batch);
+  SEMBLO_REQUIRE(table_len >= 0 && window >= 0, "negative table length or window");
+  *rows = queries * (num_q_heads / num_kv_heads);
+  *nt = *rows <= 8 ? 1 : 2;
+  *tiles = (int)ceil_div(*rows, 8 * *nt);
+  const int64_t groups = ceil_div((int64_t)table_len * block_size, 16);
+  SEMBLO_REQUIRE(groups * batch * num_kv_heads * *tiles < ((int64_t)1 << 31), "batch x context is too large for one call");
+  return 0;
+}
+
+Plan plan_of(int head_dim, int nt, int64_t segments, int64_t longest) {
+#define SEMBLO_PLAN(DD, NN) if (head_dim == DD && nt == NN) return plan_for<DD, NN>(segments, longest);
+  SEMBLO_PLAN(64, 1) SEMBLO_PLAN(64, 2) SEMBLO_PLAN(128, 1) SEMBLO_PLAN(128, 2) SEMBLO_PLAN(256, 1)
+#undef SEMBLO_PLAN
+  return plan_for<256, 2>(segments, longest);
+}
+
+}  // namespace
+
+extern "C" int64_t semblo_kv8_decode_workspace_bytes(int batch, int queries, int num_q_heads, int num_kv_heads,
+                                                     int head_dim, int block_size, int table_len, int window,
+                                                     int has_prefix) {
+  int rows, nt, tiles;
+  const int rc = check_shape(batch, queries, num_q_heads, num_kv_heads, head_dim, block_size, table_len, window,
+                             &rows, &nt, &tiles);
+  if (rc) return rc;
+  return plan_of(head_dim, nt, (int64_t)batch * num_kv_heads * tiles,
+                 longest_segment(queries, window, table_len, block_size, has_prefix)).bytes;
+}
+
+extern "C" int semblo_kv8_decode(const void* q, int dtype, int batch, int queries, int num_q_heads,
+                                 int num_kv_heads, int head_dim, const void* cache, const float* scales,
+                                 int64_t cache_blocks, int block_size, const int32_t* block_table,
+                                 int64_t table_stride, int table_len, const int32_t* lengths,
+                                 const int32_t* prefix_lens, int window, float sm_scale, float softcap,
+                                 const float* alibi_slopes, void* out, float* lse, void* workspace,
+                                 int64_t workspace_bytes, int32_t* status, void* stream) {
+  int rows, nt, tiles;
+  const int rc = check_shape(batch, queries, num_q_heads, num_kv_heads, head_dim, block_size, table_len, window,
+                             &rows, &nt, &tiles);
+  if (rc) return rc;
+  SEMBLO_REQUIRE(dtype == SEMBLO_BF16 || dtype == SEMBLO_F16, "queries are bf16 or fp16 (got dtype code %d)", dtype);
+  SEMBLO_REQUIRE(softcap >= 0.f, "the soft cap must not be negative");
+  if (batch == 0) return 0;
+  SEMBLO_REQUIRE(q && cache && scales && block_table && lengths && out && status, "null pointer");
+  SEMBLO_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache)) & 15) == 0,
+                 "q and the cache must be 16-byte aligned");
+  const Plan plan = plan_of(head_dim, nt, (int64_t)batch * num_kv_heads * tiles,
+                            longest_segment(queries, window, table_len, block_size, prefix_lens != nullptr));
+  if (plan.bytes > workspace_bytes || (plan.bytes && !workspace))
+    return semblo::fail(semblo::SEMBLO_ENOSPC, "workspace of %lld bytes needed, %lld given", (long long)plan.bytes,
+                        (long long)workspace_bytes);
+  DecodeArgs a{};
+  a.q = q; a.q_f16 = dtype == SEMBLO_F16;
+  a.out = out; a.lse = lse;
+  a.data = (const uint8_t*)cache; a.scales = scales; a.cache_blocks = cache_blocks;
+  while ((1 << a.block_log2) < block_size) ++a.block_log2;
+  a.table = block_table; a.table_stride = table_stride; a.table_len = table_len;
+  a.lengths = lengths; a.prefix = prefix_lens; a.slopes = alibi_slopes;
+  a.batch = batch; a.queries = queries; a.num_q_heads = num_q_heads; a.num_kv_heads = num_kv_heads;
+  a.group = num_q_heads / num_kv_heads;
+  a.rows = rows; a.row_tiles = tiles;
+  a.window = window; a.sm_scale = sm_scale; a.softcap = softcap;
+  a.partial = (float*)workspace;
+  a.status = status;
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool cap = softcap > 0.f;
+#define SEMBLO_DECODE(DD, NN)                                                                     \
+  if (head_dim == DD && nt == NN)                                                                 \
+    return cap ? launch<DD, NN, true>(a, plan, st) : launch<DD, NN, false>(a, plan, st);
+  SEMBLO_DECODE(64, 1) SEMBLO_DECODE(64, 2) SEMBLO_DECODE(128, 1) SEMBLO_DECODE(128, 2) SEMBLO_DECODE(256, 1)
+  SEMBLO_DECODE(256, 2)
+#undef SEMBLO_DECODE
+  return semblo::fail(semblo::SEMBLO_EINVAL, "unreachable");
+}

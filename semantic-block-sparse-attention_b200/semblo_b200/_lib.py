@@ -74,6 +74,8 @@ _SIGNATURES = {
     "semblo_paged_posting_attention": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
     "semblo_rotary": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int] * 2 + [c_int64, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_float, c_int, c_int, c_void_p]),
     "semblo_kv8_append": (c_int, [c_void_p, c_int64, c_int64] * 2 + [c_int64, c_int, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "semblo_kv8_decode_workspace_bytes": (c_int64, [c_int] * 9),
+    "semblo_kv8_decode": (c_int, [c_void_p] + [c_int] * 6 + [c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_float, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
     "semblo_merge_attention_states": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
 }
 

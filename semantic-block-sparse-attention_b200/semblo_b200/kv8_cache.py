@@ -12,6 +12,7 @@ import torch
 
 from . import _lib
 from ._lib import check, device_scope, dtype_code, lib, raw_stream, refuse_gradients, require_cuda, require_same_device
+from .paged_attention import PagedSparseAttentionResult
 
 BLOCK_SIZES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128, 256)
@@ -108,3 +109,85 @@ def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, block_table: t
             cache.block_size, cache.num_kv_heads, cache.head_dim, table.data_ptr(), table.stride(0), table.shape[1],
             cu.data_ptr(), start.data_ptr(), batch, _lib.status_for(k.device).word.data_ptr(),
             raw_stream(k.device.index)))
+
+
+MAX_QUERIES = 16
+
+
+def _mask_arguments(window, softcap, prefix_lens, alibi_slopes, batch: int, heads: int, device):
+    """The masks and caps that the dense operators share, checked: (window, softcap, prefix, slopes)."""
+    window = int(window or 0)
+    if window < 0:
+        raise ValueError(f"the window must not be negative (got {window}; 0 is none)")
+    softcap = float(softcap or 0.0)
+    if not 0.0 <= softcap < float("inf"):
+        raise ValueError(f"the soft cap must be finite and not negative (got {softcap}; 0 is none)")
+    if prefix_lens is not None:
+        prefix_lens = _per_request("prefix_lens", prefix_lens, batch)
+        if prefix_lens.device != device:
+            raise ValueError("prefix_lens must be on the device of the queries")
+    if alibi_slopes is not None:
+        if alibi_slopes.shape != (heads,) or alibi_slopes.dtype != torch.float32:
+            raise ValueError(f"alibi_slopes must be {heads} fp32 values, one for each query head")
+        if alibi_slopes.device != device:
+            raise ValueError("alibi_slopes must be on the device of the queries")
+        alibi_slopes = alibi_slopes.contiguous()
+    return window, softcap, prefix_lens, alibi_slopes
+
+
+def kv8_decode_attention(q: torch.Tensor, cache: Kv8Cache, block_table: torch.Tensor, lengths: torch.Tensor, *,
+                         sm_scale: float, softcap: float | None = None, window: int = 0,
+                         prefix_lens: torch.Tensor | None = None, alibi_slopes: torch.Tensor | None = None,
+                         out: torch.Tensor | None = None, return_logsumexp: bool = False) -> PagedSparseAttentionResult:
+    """Attention of the last tokens of each request over the 8-bit cache.
+
+    ``q`` [B, n, Hq, D] (bf16 or fp16; 1 to 16 queries per request): query i of request b stands at position
+    p = lengths[b] - n + i and sees key j < lengths[b] if j <= p (and p - j < ``window``, where one is given) or
+    j < prefix_lens[b].  Scores are q . k sm_scale, then ``softcap`` tanh(score / softcap), then minus
+    alibi_slopes[h] |p - j|.  A row that sees nothing (a length of 0, a position below 0) gives 0 and a log-sum-exp
+    of -inf.  The result [B, n, Hq, D] has the type of ``q``; log-sum-exps are natural, fp32 [B, n, Hq].  Table
+    entries outside the pool are taken as absent and set status 201, as does a length beyond the table."""
+    require_cuda(q, cache.data, block_table, lengths, prefix_lens, alibi_slopes, out)
+    refuse_gradients(q)
+    if q.ndim != 4:
+        raise ValueError("q must have shape [B, n, Hq, D]")
+    batch, queries, hq, dim = q.shape
+    dtype, device = q.dtype, q.device
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("q must be bf16 or fp16")
+    if dim != cache.head_dim:
+        raise ValueError(f"the head dimension of q ({dim}) differs from the cache's ({cache.head_dim})")
+    if hq == 0 or hq % cache.num_kv_heads:
+        raise ValueError(f"query heads ({hq}) must be a multiple of the KV heads ({cache.num_kv_heads})")
+    if not 1 <= queries <= MAX_QUERIES:
+        raise ValueError(f"1 to {MAX_QUERIES} queries per request (got {queries}); longer ones belong to the prompt's "
+                         "attention")
+    if cache.data.device != device or block_table.device != device or lengths.device != device:
+        raise ValueError("q, the cache, the block table and the lengths must be on one device")
+    table = _block_table(block_table, batch)
+    lengths = _per_request("lengths", lengths, batch)
+    window, softcap, prefix_lens, alibi_slopes = _mask_arguments(window, softcap, prefix_lens, alibi_slopes, batch, hq,
+                                                                 device)
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    if out is None:
+        out = torch.empty((batch, queries, hq, dim), dtype=dtype, device=device)
+    elif out.shape != q.shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
+        raise ValueError("out must be contiguous and have the shape, type and device of q")
+    lse = torch.empty((batch, queries, hq), dtype=torch.float32, device=device) if return_logsumexp else None
+    width = table.shape[1]
+    with device_scope(device):
+        nbytes = lib().semblo_kv8_decode_workspace_bytes(batch, queries, hq, cache.num_kv_heads, dim, cache.block_size,
+                                                         width, window, prefix_lens is not None)
+        if nbytes < 0:
+            check(int(nbytes))
+        # made for this call: a recorded graph keeps its own, and calls on two streams do not share one
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        check(lib().semblo_kv8_decode(
+            q.data_ptr(), dtype_code(dtype, "decode"), batch, queries, hq, cache.num_kv_heads, dim,
+            cache.data.data_ptr(), cache.scales.data_ptr(), cache.num_blocks, cache.block_size, table.data_ptr(),
+            table.stride(0), width, lengths.data_ptr(), None if prefix_lens is None else prefix_lens.data_ptr(), window,
+            sm_scale, softcap, None if alibi_slopes is None else alibi_slopes.data_ptr(), out.data_ptr(),
+            None if lse is None else lse.data_ptr(), None if workspace is None else workspace.data_ptr(), nbytes,
+            _lib.status_for(device).word.data_ptr(), raw_stream(device.index)))
+    return PagedSparseAttentionResult(out, lse)
