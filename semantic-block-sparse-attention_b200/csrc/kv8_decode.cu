@@ -96,8 +96,7 @@ __device__ __forceinline__ uint32_t widen_hi(uint32_t w) {
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -278,12 +277,19 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
     };
     int pages = page_for(lane), pages_next = 0;
     uint32_t bad = 0;                                           // per stage: its block does not exist
+    const int64_t part = a.cache_blocks * a.num_kv_heads;       // cells of K, then those of V
+    const int64_t v_off = (part << a.block_log2) * D;
+    const uint8_t* const k_lane = a.data + g * D + 16 * t;
+    const uint8_t* const v_lane = a.data + v_off + 2 * t * D + (D == 64 ? 8 : 16) * g;
+    const float* const scale_lane = a.scales + (lane & 1) * part;
+    const int in_block = (1 << a.block_log2) - 1;
+    int issue_stage = 0;
     auto issue = [&](int it) {
       if ((it & 31) == 16) pages_next = page_for(it - 16 + 32 + lane);
       if ((it & 31) == 0 && it > 0) pages = pages_next;
       const int page = __shfl_sync(0xffffffffu, pages, it & 31);
       if (it < count) {
-        const int st = it % C::STAGES;
+        const int st = issue_stage;
         const int key0 = sp.group_of(i0 + warp + it * WARPS) * GROUP;
         if (page < 0 || page >= a.cache_blocks) {
           bad |= 1u << st;
@@ -291,36 +297,43 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
         } else {
           bad &= ~(1u << st);
           const int64_t cell = (int64_t)page * a.num_kv_heads + h;
-          const int64_t part = a.cache_blocks * a.num_kv_heads;
-          const uint8_t* k = a.data + ((cell << a.block_log2) + (key0 & ((1 << a.block_log2) - 1))) * D;
-          const uint8_t* v = k + (part << a.block_log2) * D;
-          const uint32_t dst = ring_u32 + st * 2 * C::KV_BYTES;
-          // rows that no query sees are not read: zeros, since 0 * NaN would not vanish in P V
-          const bool whole = key0 + GROUP <= sp.length && (key0 >= sp.lo || key0 + GROUP <= sp.prefix);
-          auto bytes_of = [&](int r, int n) -> uint32_t {
-            const int key = key0 + r;
-            return whole || (key < sp.length && (key >= sp.lo || key < sp.prefix)) ? n : 0;
-          };
+          const int64_t at = ((cell << a.block_log2) + (key0 & in_block)) * D;
+          const uint8_t* k = k_lane + at;
+          const uint8_t* v = v_lane + at;
+          const uint32_t dst = ring_u32 + st * 2 * C::KV_BYTES + lane * 16;
+          const uint32_t vdst = ring_u32 + st * 2 * C::KV_BYTES + C::KV_BYTES + lane * (D == 64 ? 8 : 16);
+          // bytes(r): what to copy of the group's key r, the rest of the 16 is filled with zeros
+          auto copy = [&](auto bytes) {
 #pragma unroll
-          for (int i = 0; i < C::KC / 2; ++i) {
-            cp16(dst + (2 * i * 32 + lane) * 16, k + g * D + 16 * t + 64 * i, bytes_of(g, 16));
-            cp16(dst + ((2 * i + 1) * 32 + lane) * 16, k + (g + 8) * D + 16 * t + 64 * i, bytes_of(g + 8, 16));
-          }
-          const uint32_t vdst = dst + C::KV_BYTES;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int key = 2 * t + (r & 1) + 8 * (r >> 1);
-            if constexpr (D == 64) {
-              cp8(vdst + (r * 32 + lane) * 8, v + key * D + 8 * g, bytes_of(key, 8));
-            } else {
-#pragma unroll
-              for (int i = 0; i < C::VI; ++i)
-                cp16(vdst + ((r * C::VI + i) * 32 + lane) * 16, v + key * D + 16 * g + 128 * i, bytes_of(key, 16));
+            for (int i = 0; i < C::KC / 2; ++i) {
+              cp16(dst + 2 * i * 512, k + 64 * i, bytes(g, 16));
+              cp16(dst + (2 * i + 1) * 512, k + 8 * D + 64 * i, bytes(g + 8, 16));
             }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int key = (r & 1) + 8 * (r >> 1);
+              if constexpr (D == 64) {
+                cp8(vdst + r * 256, v + key * D, bytes(2 * t + key, 8));
+              } else {
+#pragma unroll
+                for (int i = 0; i < C::VI; ++i)
+                  cp16(vdst + (r * C::VI + i) * 512, v + key * D + 128 * i, bytes(2 * t + key, 16));
+              }
+            }
+          };
+          if (key0 + GROUP <= sp.length && (key0 >= sp.lo || key0 + GROUP <= sp.prefix)) {
+            copy([](int, int n) -> uint32_t { return n; });
+          } else {
+            // rows that no query sees are not read: zeros, since 0 * NaN would not vanish in P V
+            copy([&](int r, int n) -> uint32_t {
+              const int key = key0 + r;
+              return key < sp.length && (key >= sp.lo || key < sp.prefix) ? n : 0;
+            });
           }
-          if (lane < 2) cp4(meta_u32 + (st * 2 + lane) * 4, a.scales + cell + lane * part);
+          if (lane < 2) cp4(meta_u32 + (st * 2 + lane) * 4, scale_lane + cell);
         }
       }
+      issue_stage = issue_stage == C::STAGES - 1 ? 0 : issue_stage + 1;
       cp_commit();
     };
 #pragma unroll
@@ -392,19 +405,25 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
       for (int c = 0; c < 2; ++c) { m[nt][c] = mv[nt][c] = -INFINITY; l[nt][c] = 0.f; }
     }
 
+    int stage = 0;
     for (int it = 0; it < count; ++it) {
       issue(it + C::STAGES - 1);
       cp_wait<C::STAGES - 1>();
       __syncwarp();
-      const int st = it % C::STAGES;
+      const int st = stage;
+      stage = stage == C::STAGES - 1 ? 0 : stage + 1;
       if (bad >> st & 1) continue;
       const int key0 = sp.group_of(i0 + warp + it * WARPS) * GROUP;
       const uint8_t* kp = ring + st * 2 * C::KV_BYTES;
       const float ks = meta[st * 2], vs = meta[st * 2 + 1];
       // ---- S^T = K Q^T
-      float s[NT][4];
+      // independent chains of products: one would put D / 16 latencies of the tensor core in a row
+      constexpr int CHAINS = D / 64;
+      float sc[NT][CHAINS][4], s[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < CHAINS; ++i) sc[nt][i][0] = sc[nt][i][1] = sc[nt][i][2] = sc[nt][i][3] = 0.f;
 #pragma unroll
       for (int i = 0; i < C::KC / 2; ++i) {
         const uint4 k0 = *reinterpret_cast<const uint4*>(kp + (2 * i * 32 + lane) * 16);
@@ -418,18 +437,22 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
             uint2 q;
             if constexpr (C::Q_SMEM) q = q_frag[((4 * i + u) * NT + nt) * 32 + lane];
             else q = qf[(4 * i + u) * NT + nt];
-            mma16816(s[nt], a0, a1, a2, a3, q.x, q.y);
+            mma16816(sc[nt][i], a0, a1, a2, a3, q.x, q.y);
           }
         }
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if constexpr (CHAINS == 4) s[nt][c] = (sc[nt][0][c] + sc[nt][1][c]) + (sc[nt][2][c] + sc[nt][3][c]);
+          else if constexpr (CHAINS == 2) s[nt][c] = sc[nt][0][c] + sc[nt][1][c];
+          else s[nt][c] = sc[nt][0][c];
+        }
       // ---- scores in log2 units; accumulator c: key g + 8 (c >> 1), row 2 t + (c & 1)
       const float lv = __log2f(vs);
-      const bool all_seen = key0 + GROUP - 1 <= sp.first &&
-                            (a.window == 0 || key0 >= sp.first + a.queries - a.window || key0 + GROUP <= sp.prefix) &&
-                            key0 + GROUP <= sp.length;
-      bool need = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           float x = s[nt][c] * (ks * coef[nt][c & 1]);
@@ -438,21 +461,29 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
             const float ex = sm100::fast_exp2(x * (2.f * LOG2E));
             x = a.softcap * LOG2E * (1.f - __fdividef(2.f, 1.f + ex));
           }
-          const int key = key0 + g + 8 * (c >> 1);
-          if (a.slopes) x -= slope[nt][c & 1] * fabsf((float)(qpos[nt][c & 1] - key));
-          if (!all_seen) {
-            const int d = qpos[nt][c & 1] - key;
-            const bool seen = key < sp.length && ((d >= 0 && (a.window == 0 || d < a.window)) || key < sp.prefix);
-            if (!seen) x = -INFINITY;
-          }
           s[nt][c] = x;
         }
+      const bool all_seen = key0 + GROUP - 1 <= sp.first &&
+                            (a.window == 0 || key0 >= sp.first + a.queries - a.window || key0 + GROUP <= sp.prefix) &&
+                            key0 + GROUP <= sp.length;
+      if (!all_seen || a.slopes) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int key = key0 + g + 8 * (c >> 1), d = qpos[nt][c & 1] - key;
+            const bool seen = key < sp.length && ((d >= 0 && (a.window == 0 || d < a.window)) || key < sp.prefix);
+            s[nt][c] = seen ? s[nt][c] - slope[nt][c & 1] * fabsf((float)d) : -INFINITY;
+          }
+      }
+      bool need = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const float x = fmaxf(s[nt][c], s[nt][c + 2]);
           need |= x > m[nt][c] + GAP || x + lv > mv[nt][c] + GAP;
         }
-      }
       if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
