@@ -6,8 +6,10 @@
 //
 // Bound: HBM, 2 D bytes per key and KV head.  What has to keep up with 24 bytes per clock and
 // multiprocessor is the way of a byte through it:
-//   * a warp takes 16 keys at a time through a private ring in shared memory; every lane copies (cp.async)
-//     exactly the bytes that it reads back, so the ring needs no barrier and no padding;
+//   * a warp takes 16 keys at a time through a private ring in shared memory, copied (cp.async) in the order
+//     of memory, 512 consecutive bytes an instruction: the same copies with each lane fetching the pieces that
+//     it will need itself reached 4.7 TB/s, in memory order 6.2.  The 16-byte pieces are permuted inside their
+//     128-byte lines so that the fragments are read back without bank conflicts;
 //   * e4m3 becomes fp16 by the hardware's pair conversion and is exact there, as is the query after a power
 //     of two per row is taken out, so the products S^T = K Q^T of m16n8k16 are exact up to the fp32 sums.
 //     The order of the 16 values inside a k-step is free as long as K and Q agree: a lane's 16 consecutive
@@ -73,9 +75,6 @@ struct DecodeArgs {
 // ---------------------------------------------------------------- pieces
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp8(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
@@ -270,24 +269,29 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
     // ---- pipeline over this warp's groups
     const int count = max(0, (i1 - i0 - warp + WARPS - 1) / WARPS);
     const int64_t table_row = (int64_t)b * a.table_stride;
-    auto page_for = [&](int it) -> int {                        // lane's look at the table for one iteration
-      if (it >= count) return -1;
-      const int slot = (sp.group_of(i0 + warp + it * WARPS) * GROUP) >> a.block_log2;
-      return a.table[table_row + slot];
+    // the table entry of the group to be issued next is read while the one before it is issued
+    auto page_for = [&](int it) -> int {
+      if (it >= count) return 0;
+      return a.table[table_row + ((sp.group_of(i0 + warp + it * WARPS) * GROUP) >> a.block_log2)];
     };
-    int pages = page_for(lane), pages_next = 0;
+    int page_ahead = page_for(0);
     uint32_t bad = 0;                                           // per stage: its block does not exist
     const int64_t part = a.cache_blocks * a.num_kv_heads;       // cells of K, then those of V
     const int64_t v_off = (part << a.block_log2) * D;
-    const uint8_t* const k_lane = a.data + g * D + 16 * t;
-    const uint8_t* const v_lane = a.data + v_off + 2 * t * D + (D == 64 ? 8 : 16) * g;
-    const float* const scale_lane = a.scales + (lane & 1) * part;
+    // instruction i of a copy takes row i (512 / D) + lane / (D / 16), piece lane % (D / 16).  Where a piece goes
+    // in its line: K's reader has 2 rows x 4 pieces per quarter warp, V's 4 even or odd rows x 2 pieces
+    const uint8_t* const k_lane = a.data + ((int64_t)h << a.block_log2) * D + lane * 16;
+    const uint8_t* const v_lane = k_lane + v_off;
+    const uint32_t k_dst = ring_u32 + (lane * 16 ^ (D == 64 ? 0 : D == 128 ? (lane >> 3 & 1) * 64 : (lane >> 4) * 64));
+    const uint32_t v_dst = ring_u32 + C::KV_BYTES + (lane * 16 ^ (D == 64 ? (lane >> 3) * 32 : D == 128 ? (lane >> 4) * 32 : 0));
+    const int copy_row = lane / (D / 16);
+    const float* const scale_lane = a.scales + (lane & 1) * part + h;
+    const int64_t block_bytes = (int64_t)D << a.block_log2, page_bytes = a.num_kv_heads * block_bytes;
     const int in_block = (1 << a.block_log2) - 1;
     int issue_stage = 0;
     auto issue = [&](int it) {
-      if ((it & 31) == 16) pages_next = page_for(it - 16 + 32 + lane);
-      if ((it & 31) == 0 && it > 0) pages = pages_next;
-      const int page = __shfl_sync(0xffffffffu, pages, it & 31);
+      const int page = page_ahead;
+      page_ahead = page_for(it + 1);
       if (it < count) {
         const int st = issue_stage;
         const int key0 = sp.group_of(i0 + warp + it * WARPS) * GROUP;
@@ -296,41 +300,31 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
           if (lane == 0) atomicCAS(a.status, 0, sm100::STATUS_OVERFLOW);
         } else {
           bad &= ~(1u << st);
-          const int64_t cell = (int64_t)page * a.num_kv_heads + h;
-          const int64_t at = ((cell << a.block_log2) + (key0 & in_block)) * D;
+          const int64_t at = page * page_bytes + (key0 & in_block) * D;
           const uint8_t* k = k_lane + at;
           const uint8_t* v = v_lane + at;
-          const uint32_t dst = ring_u32 + st * 2 * C::KV_BYTES + lane * 16;
-          const uint32_t vdst = ring_u32 + st * 2 * C::KV_BYTES + C::KV_BYTES + lane * (D == 64 ? 8 : 16);
+          const uint32_t so = st * 2 * C::KV_BYTES;
           // bytes(r): what to copy of the group's key r, the rest of the 16 is filled with zeros
           auto copy = [&](auto bytes) {
 #pragma unroll
-            for (int i = 0; i < C::KC / 2; ++i) {
-              cp16(dst + 2 * i * 512, k + 64 * i, bytes(g, 16));
-              cp16(dst + (2 * i + 1) * 512, k + 8 * D + 64 * i, bytes(g + 8, 16));
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int key = (r & 1) + 8 * (r >> 1);
-              if constexpr (D == 64) {
-                cp8(vdst + r * 256, v + key * D, bytes(2 * t + key, 8));
-              } else {
-#pragma unroll
-                for (int i = 0; i < C::VI; ++i)
-                  cp16(vdst + (r * C::VI + i) * 512, v + key * D + 128 * i, bytes(2 * t + key, 16));
-              }
+            for (int i = 0; i < C::KC; ++i) {
+              const uint32_t n = bytes(copy_row + i * (512 / D));
+              // V's permutation depends on (row >> 1) & 3; what of it comes from i is a constant
+              const uint32_t turn = D == 128 ? (i & 1) * 64 : D == 256 ? (i & 3) * 32 : 0;
+              cp16(k_dst + so + i * 512, k + i * 512, n);
+              cp16((v_dst ^ turn) + so + i * 512, v + i * 512, n);
             }
           };
           if (key0 + GROUP <= sp.length && (key0 >= sp.lo || key0 + GROUP <= sp.prefix)) {
-            copy([](int, int n) -> uint32_t { return n; });
+            copy([](int) -> uint32_t { return 16; });
           } else {
             // rows that no query sees are not read: zeros, since 0 * NaN would not vanish in P V
-            copy([&](int r, int n) -> uint32_t {
+            copy([&](int r) -> uint32_t {
               const int key = key0 + r;
-              return key < sp.length && (key >= sp.lo || key < sp.prefix) ? n : 0;
+              return key < sp.length && (key >= sp.lo || key < sp.prefix) ? 16 : 0;
             });
           }
-          if (lane < 2) cp4(meta_u32 + (st * 2 + lane) * 4, scale_lane + cell);
+          if (lane < 2) cp4(meta_u32 + (st * 2 + lane) * 4, scale_lane + (int64_t)page * a.num_kv_heads);
         }
       }
       issue_stage = issue_stage == C::STAGES - 1 ? 0 : issue_stage + 1;
@@ -395,6 +389,7 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
 
     float o[NT][C::KSTEPS][4];
     float m[NT][2], mv[NT][2], l[NT][2];                        // mv: the reference of P'
+    float ms[NT][2], mvs[NT][2];                                // as subtracted: a row without keys has 0 and inf
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -402,7 +397,7 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[nt][j][c] = 0.f;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) { m[nt][c] = mv[nt][c] = -INFINITY; l[nt][c] = 0.f; }
+      for (int c = 0; c < 2; ++c) { m[nt][c] = mv[nt][c] = -INFINITY; l[nt][c] = 0.f; ms[nt][c] = 0.f; mvs[nt][c] = INFINITY; }
     }
 
     int stage = 0;
@@ -426,8 +421,9 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
         for (int i = 0; i < CHAINS; ++i) sc[nt][i][0] = sc[nt][i][1] = sc[nt][i][2] = sc[nt][i][3] = 0.f;
 #pragma unroll
       for (int i = 0; i < C::KC / 2; ++i) {
-        const uint4 k0 = *reinterpret_cast<const uint4*>(kp + (2 * i * 32 + lane) * 16);
-        const uint4 k8 = *reinterpret_cast<const uint4*>(kp + ((2 * i + 1) * 32 + lane) * 16);
+        const uint8_t* x = kp + (D == 64 ? g * D + 16 * t : g * D + 16 * t + (i >> 1) * 128 + ((i ^ g) & 1) * 64);
+        const uint4 k0 = *reinterpret_cast<const uint4*>(x);
+        const uint4 k8 = *reinterpret_cast<const uint4*>(x + 8 * D);
         const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w8[4] = {k8.x, k8.y, k8.z, k8.w};
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -482,7 +478,7 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const float x = fmaxf(s[nt][c], s[nt][c + 2]);
-          need |= x > m[nt][c] + GAP || x + lv > mv[nt][c] + GAP;
+          need |= x > fminf(m[nt][c] + GAP, mv[nt][c] + (GAP - lv));
         }
       if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
@@ -497,6 +493,8 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
             const float f = ratio2(mv[nt][c], mv1);
             m[nt][c] = m1;
             mv[nt][c] = mv1;
+            ms[nt][c] = m1 == -INFINITY ? 0.f : m1;
+            mvs[nt][c] = mv1 == -INFINITY ? INFINITY : mv1;
 #pragma unroll
             for (int j = 0; j < C::KSTEPS; ++j) { o[nt][j][c] *= f; o[nt][j][c + 2] *= f; }
           }
@@ -508,9 +506,8 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
         float w[4];                                             // P', by an exponential of its own: it cannot overflow
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const float ref = m[nt][c & 1], refv = mv[nt][c & 1];
-          l[nt][c & 1] += sm100::fast_exp2(s[nt][c] - (ref == -INFINITY ? 0.f : ref));
-          w[c] = sm100::fast_exp2(s[nt][c] + (refv == -INFINITY ? -INFINITY : lv - refv + P_BIAS));
+          l[nt][c & 1] += sm100::fast_exp2(s[nt][c] - ms[nt][c & 1]);
+          w[c] = sm100::fast_exp2(s[nt][c] + ((lv + P_BIAS) - mvs[nt][c & 1]));
         }
         p[nt][0] = transpose8x8(half2_bits(w[0], w[1]));
         p[nt][1] = transpose8x8(half2_bits(w[2], w[3]));
@@ -523,10 +520,12 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           if constexpr (D == 64) {
-            const uint2 x = *reinterpret_cast<const uint2*>(vp + (r * 32 + lane) * 8);
+            const uint2 x = *reinterpret_cast<const uint2*>(vp + (t + 4 * (r >> 1)) * 128 +
+                                                            16 * ((g >> 1) ^ (2 * t) ^ (4 * (r & 1))) + 8 * (g & 1));
             w[r][0] = x.x; w[r][1] = x.y; w[r][2] = w[r][3] = 0u;
           } else {
-            const uint4 x = *reinterpret_cast<const uint4*>(vp + ((r * C::VI + i) * 32 + lane) * 16);
+            const uint4 x = *reinterpret_cast<const uint4*>(vp + (2 * t + (r & 1) + 8 * (r >> 1)) * D + 16 * (g ^ (2 * t)) +
+                                                            128 * i);
             w[r][0] = x.x; w[r][1] = x.y; w[r][2] = x.z; w[r][3] = x.w;
           }
         }
