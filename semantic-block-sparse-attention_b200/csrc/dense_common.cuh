@@ -1,0 +1,169 @@
+// What the two prompt-attention kernels share: which document and query tile a block works on, which key
+// tiles that tile sees, the mask of a row, the scores' transformation, and the packing of P.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "sm100.cuh"
+
+namespace dense {
+
+using namespace sm100;
+
+constexpr float LN2F = 0.6931471805599453f;
+constexpr float LOG2EF = 1.4426950408889634f;
+constexpr float RESCALE_GAP = 8.0f;              // log2 units: rescale O only when the max moved by > 2^8
+
+struct Args {
+  const void* q;                  // [Tq, Hq, D], strides in elements
+  int64_t q_token, q_head;
+  void* out;                      // [Tq, Hq, D] contiguous
+  float* lse;                     // [Tq, Hq] or null
+  const int32_t* cu_q;            // [docs + 1]
+  const int32_t* cu_k;
+  const int32_t* prefix;          // [docs] or null
+  const float* slopes;            // [Hq] or null
+  int docs, group, num_q_heads;
+  int queries_per_tile;
+  int64_t tokens_q, tokens_k;
+  int causal, window;
+  int zero_tail;                  // write zeros to the rows behind the last document
+  float score_scale;              // raw product -> log2 units, or -> argument of the capping tanh
+  float cap_log2;                 // cap * log2(e)
+  int* status;
+};
+
+// The block's share: queries [q0, q0 + nq) of a document (token of query 0: tok0), keys k0 ... of length lk.
+struct Tile {
+  int doc;
+  int first;                      // index of the tile's first query in its document
+  int count;                      // its queries
+  int64_t token;                  // its first token
+  int k0, lk;                     // the document's first key row and its keys
+  int pos;                        // position of the tile's first query
+  int prefix;
+};
+
+// Tile number `want` (0 ...): documents in order, inside a document the last queries first (they see the most
+// keys).  doc = -1 behind the last one; then `first` counts the tiles behind it.  Warp-collective; every warp of
+// the block computes the same answer.
+__device__ __forceinline__ Tile find_tile(const Args& a, int want) {
+  const int lane = threadIdx.x & 31;
+  Tile t{};
+  t.doc = -1;
+  const int qt = a.queries_per_tile;
+  for (int d0 = 0; d0 < a.docs; d0 += 32) {
+    const int d = d0 + lane;
+    int64_t c0 = 0, c1 = 0;
+    int n = 0;
+    if (d < a.docs) {
+      c0 = min(max((int64_t)a.cu_q[d], (int64_t)0), a.tokens_q);
+      c1 = min(max((int64_t)a.cu_q[d + 1], c0), a.tokens_q);
+      n = (int)((c1 - c0 + qt - 1) / qt);
+    }
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const int total = __shfl_sync(0xffffffffu, upto, 31);
+    if (want < total) {
+      const int at = __ffs(__ballot_sync(0xffffffffu, upto > want)) - 1;
+      const int tiles = __shfl_sync(0xffffffffu, n, at);
+      const int nth = tiles - 1 - (want - (__shfl_sync(0xffffffffu, upto, at) - tiles));
+      const int64_t q0 = __shfl_sync(0xffffffffu, c0, at), q1 = __shfl_sync(0xffffffffu, c1, at);
+      t.doc = d0 + at;
+      t.first = nth * qt;
+      t.count = (int)min((int64_t)qt, q1 - q0 - t.first);
+      t.token = q0 + t.first;
+      const int64_t k0 = min(max((int64_t)a.cu_k[t.doc], (int64_t)0), a.tokens_k);
+      const int64_t k1 = min(max((int64_t)a.cu_k[t.doc + 1], k0), a.tokens_k);
+      t.k0 = (int)k0;
+      t.lk = (int)(k1 - k0);
+      t.pos = t.lk - (int)(q1 - q0) + t.first;
+      t.prefix = a.prefix ? min(max(a.prefix[t.doc], 0), t.lk) : 0;
+      return t;
+    }
+    want -= total;
+  }
+  t.first = want;
+  return t;
+}
+
+// Rows behind the last document, as zeros with a log-sum-exp of -inf: the spare blocks share them by tiles.
+template <int D>
+__device__ __forceinline__ void zero_tail(const Args& a, int nth, int kv_head, int threads) {
+  const int64_t last = min(max((int64_t)a.cu_q[a.docs], (int64_t)0), a.tokens_q);
+  const int64_t t0 = last + (int64_t)nth * a.queries_per_tile;
+  const int64_t t1 = min(a.tokens_q, t0 + a.queries_per_tile);
+  constexpr int CH = D / 8;
+  for (int64_t i = threadIdx.x; i < (t1 - t0) * a.group * CH; i += threads) {
+    const int64_t row = i / CH;
+    const int64_t at = (t0 + row / a.group) * a.num_q_heads + kv_head * a.group + row % a.group;
+    reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at * D)[i % CH] = make_uint4(0u, 0u, 0u, 0u);
+    if (a.lse && i % CH == 0) a.lse[at] = -INFINITY;
+  }
+}
+
+// Keys that a row at position p sees: [lo, hi) and [0, pre).
+struct Seen { int lo, hi, pre; };
+__device__ __forceinline__ Seen seen_by(const Args& a, const Tile& t, int p) {
+  Seen s;
+  s.hi = a.causal ? min(t.lk, max(p + 1, 0)) : t.lk;
+  s.lo = a.causal && a.window > 0 ? max(0, p - a.window + 1) : 0;
+  s.pre = a.causal ? t.prefix : 0;
+  return s;
+}
+
+// The key tiles of BN rows that any row of the block's tile sees: [0, gp) then [glo, ...), n in all.
+template <int BN>
+struct KeyTiles {
+  int gp, glo, n;
+  __device__ __forceinline__ KeyTiles(const Args& a, const Tile& t) {
+    const Seen lo = seen_by(a, t, t.pos), hi = seen_by(a, t, t.pos + t.count - 1);
+    gp = (lo.pre + BN - 1) / BN;
+    const int end = max(gp, (hi.hi + BN - 1) / BN);
+    glo = min(max(gp, lo.lo / BN), end);
+    n = gp + end - glo;
+  }
+  __device__ __forceinline__ int at(int j) const { return (j < gp ? j : j - gp + glo) * BN; }
+};
+
+// tanh(x) = 1 - 2 / (1 + e^2x): exact at both ends, absolute error a few 2^-24.
+__device__ __forceinline__ float tanh_exp(float x) {
+  return 1.f - __fdividef(2.f, 1.f + fast_exp2(x * (2.f * LOG2EF)));
+}
+
+template <bool F16> __device__ __forceinline__ uint32_t pack_pair(float x, float y) {
+  if constexpr (F16) {
+    const __half2 v = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// fp16 keeps P up to 2^(8 + 6): what underflows at its lower end is then below 2^-31 of the largest term.
+// bf16 has float's range and needs no shift.
+template <bool F16> __host__ __device__ constexpr float p_bias() { return F16 ? 6.f : 0.f; }
+
+// Instruction descriptor for kind::f16 with an fp32 accumulator.
+template <bool F16>
+__host__ __device__ constexpr uint32_t idesc_of(int m, int n, bool b_mn_major) {
+  const uint32_t d = make_idesc_bf16(m, n, false, b_mn_major);
+  return F16 ? d & ~((1u << 7) | (1u << 10)) : d;
+}
+
+// Zero rows [from, to) of a swizzled 128-byte-row tile of D columns (all of a row, so the permutation inside it
+// does not matter).  One warp; the caller fences before the tensor core reads.
+template <int D, int BN>
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int from, int to) {
+  const int lane = threadIdx.x & 31;
+  for (int i = lane; i < (to - from) * 8 * (D / 64); i += 32) {
+    const int slab = i / ((to - from) * 8), r = i % ((to - from) * 8);
+    reinterpret_cast<uint4*>(tile + slab * BN * 128 + (from + r / 8) * 128)[r % 8] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+}  // namespace dense

@@ -69,11 +69,12 @@ def _per_request(name: str, x: torch.Tensor, n: int) -> torch.Tensor:
     return (x if x.dtype == torch.int32 else x.to(torch.int32)).contiguous()
 
 
-def _token_rows(name: str, x: torch.Tensor) -> torch.Tensor:
+def _token_rows(x: torch.Tensor) -> torch.Tensor:
     """x [T, H, D] as the kernels read it: contiguous heads of a 16-byte aligned start and step."""
-    if x.stride(2) == 1 and x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0:
+    s0, s1, s2 = x.stride()
+    if s2 == 1 and x.data_ptr() % 16 == 0 and s0 % 8 == 0 and s1 % 8 == 0 and s0 > 0 and s1 > 0:
         return x
-    return x.contiguous()
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -101,7 +102,7 @@ def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, block_table: t
     require_same_device(cache.data, k, v, block_table, cu_seqlens, start_positions)
     table = _block_table(block_table, batch)
     cu, start = _per_request("cu_seqlens", cu_seqlens, batch + 1), _per_request("start_positions", start_positions, batch)
-    k, v = _token_rows("k", k), _token_rows("v", v)
+    k, v = _token_rows(k), _token_rows(v)
     with device_scope(k.device):
         check(lib().semblo_kv8_append(
             k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), shape[0],
