@@ -129,9 +129,94 @@ struct KeyTiles {
   __device__ __forceinline__ int at(int j) const { return (j < gp ? j : j - gp + glo) * BN; }
 };
 
-// tanh(x) = 1 - 2 / (1 + e^2x): exact at both ends, absolute error a few 2^-24.
+// ---- two floats in a 64-bit register: one instruction for both
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 join(float x, float y) {
+  f32x2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+  return d;
+}
+__device__ __forceinline__ void split(f32x2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// tanh(x) = 1 - 2 / (1 + e^2x): exact at both ends, absolute error a few 2^-24; two special-function operations.
 __device__ __forceinline__ float tanh_exp(float x) {
   return 1.f - __fdividef(2.f, 1.f + fast_exp2(x * (2.f * LOG2EF)));
+}
+
+// tanh on [-1.5, 1.5] as x P(x^2), P of degree 7 fitted for the smallest largest error (3.4e-7; 5.0e-7 as
+// evaluated in 32 bits), on the multiply-add pipe: the exponentials of the softmax already fill the
+// special-function unit.  Scores beyond 1.5 caps are rare and take tanh_exp.
+constexpr float TANH_POLY_RANGE = 1.5f;
+__device__ __forceinline__ constexpr float tanh_coefficient(int i) {
+  const float c[8] = {0.999996006f, -0.333240598f, 0.132696271f, -0.0519587733f,
+                      0.0183639843f, -0.00511101866f, 0.000926402514f, -7.81826457e-05f};
+  return c[i];
+}
+__device__ __forceinline__ f32x2 tanh_poly2(f32x2 x) {
+  const f32x2 u = mul2(x, x);
+  f32x2 r = join(tanh_coefficient(7), tanh_coefficient(7));
+#pragma unroll
+  for (int i = 6; i >= 0; --i) r = fma2(r, u, join(tanh_coefficient(i), tanh_coefficient(i)));
+  return mul2(r, x);
+}
+
+// What happens to a raw score: 0 scaled only, 1 capped, 2 biased by distance (and capped, if there is a cap).
+enum Mode { LINEAR = 0, CAPPED = 1, BIASED = 2 };
+
+// 32 raw scores in place -> what the exponential's scale multiplies.  All lanes of a warp take part.
+template <int MODE>
+__device__ __forceinline__ void transform32(uint32_t* x, const Args& a, float slope, int p, int key0) {
+  if constexpr (MODE == LINEAR) return;
+  if (MODE == CAPPED || a.cap_log2 > 0.f) {
+    const f32x2 sc = join(a.score_scale, a.score_scale);
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      float v0, v1;
+      split(mul2(join(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc), v0, v1);
+      x[i] = __float_as_uint(v0);
+      x[i + 1] = __float_as_uint(v1);
+      top = fmax3(top, fabsf(v0), fabsf(v1));
+    }
+    if (__all_sync(0xffffffffu, top <= TANH_POLY_RANGE)) {
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        float v0, v1;
+        split(tanh_poly2(join(__uint_as_float(x[i]), __uint_as_float(x[i + 1]))), v0, v1);
+        x[i] = __float_as_uint(v0);
+        x[i + 1] = __float_as_uint(v1);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(tanh_exp(__uint_as_float(x[i])));
+    }
+  }
+  if constexpr (MODE == BIASED) {
+    const float scale = a.cap_log2 > 0.f ? a.cap_log2 : a.score_scale;
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      x[i] = __float_as_uint(__uint_as_float(x[i]) * scale - slope * fabsf((float)(p - key0 - i)));
+  }
+}
+
+// The factor that turns transformed scores into log2 units (positive: the maximum commutes with it).
+template <int MODE> __device__ __forceinline__ float scale_of(const Args& a) {
+  return MODE == LINEAR ? a.score_scale : MODE == CAPPED ? a.cap_log2 : 1.f;
 }
 
 template <bool F16> __device__ __forceinline__ uint32_t pack_pair(float x, float y) {

@@ -1,0 +1,384 @@
+// Attention of packed prompts for head dimensions 64 and 128 (the mathematics is in dense_prefill.cu).
+//
+// One block owns two tiles of 128 rows (queries x the heads of a KV head) that take turns: while the tensor core
+// works on one tile (P V of a key tile, then S of the next), a warpgroup runs the softmax of the other, one
+// thread per row and 128 keys at a time.  At D = 128 the two S buffers and the two O accumulators are all of
+// tensor memory; P lies over the S it came from.  Q, K and V are in shared memory (64 KB of Q and a ring of
+// K, V tiles by TMA).  P is handed over in two halves, so that P V starts when half the exponentials are done.
+#include <algorithm>
+
+#include "dense_pair.h"
+#include "host_common.h"
+
+using namespace dense;
+using semblo::ceil_div;
+
+namespace {
+
+constexpr int BN = PAIR_BN;
+constexpr int PAGE = 16;
+
+template <int D>
+struct Cfg {
+  static constexpr int SLABS = D / 64;                         // 128-byte wide slabs of a 16-bit tile
+  static constexpr int TILE = BN * D * 2;                      // a tile of Q, K or V
+  static constexpr int SLOTS = D == 128 ? 5 : 8;
+  static constexpr int Q_OFF = 0;
+  static constexpr int KV_OFF = 2 * TILE;
+  static constexpr int BAR_OFF = KV_OFF + SLOTS * TILE;
+  static constexpr int TOTAL = BAR_OFF + 256;
+  static constexpr int S_COL = 0;                              // + 128 x: S and P of tile x
+  static constexpr int O_COL = 256;                            // + D x
+  static constexpr int TMEM_COLS = 512;
+};
+
+enum { B_Q = 0, B_S = 1, B_P = 3, B_O = 7, B_FULL = 9 };       // B_S + x, B_P + 2 x + half, B_O + x
+
+// Which key tiles the block walks over and which of its two row tiles sees each.
+struct Walk {
+  int gp, first, n;                       // prefix tiles, first tile of the main part, tiles in all
+  int glo[2], end[2];
+  bool any[2];
+  __device__ __forceinline__ Walk(const Args& a, const Tile& t) {
+    const int qt = a.queries_per_tile >> 1;
+    int last = 0;
+    first = 1 << 30;
+    gp = 0;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      Tile s = t;
+      s.pos += x * qt;
+      s.count = min(qt, t.count - x * qt);
+      any[x] = s.count > 0;
+      glo[x] = end[x] = 0;
+      if (!any[x]) continue;
+      const KeyTiles<BN> k(a, s);
+      gp = k.gp;
+      glo[x] = k.glo;
+      end[x] = k.glo + k.n - k.gp;
+      if (end[x] > glo[x]) {
+        first = min(first, glo[x]);
+        last = max(last, end[x]);
+      }
+    }
+    n = gp + max(0, last - first);
+  }
+  __device__ __forceinline__ int tile(int j) const { return j < gp ? j : j - gp + first; }
+  __device__ __forceinline__ bool sees(int x, int j) const {
+    const int i = tile(j);
+    return any[x] && j < n && (j < gp || (i >= glo[x] && i < end[x]));
+  }
+};
+
+template <int D, bool F16, int MODE>
+__global__ void __launch_bounds__(320, 1)
+dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                  const __grid_constant__ CUtensorMap tmap_v, const Args a) {
+  using C = Cfg<D>;
+  constexpr int SLOTS = C::SLOTS;
+  constexpr int B_EMPTY = B_FULL + SLOTS;
+  static_assert(8 * (B_EMPTY + SLOTS) + 8 <= 256, "barrier area");
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.y;
+  if (smem_u32(smem) & 1023u) {                    // the swizzled tiles need 1024-byte alignment
+    if (threadIdx.x == 0) atomicCAS(a.status, 0, STATUS_SMEM_ALIGN);
+    return;
+  }
+  const Tile tile = find_tile(a, blockIdx.x);
+  if (tile.doc < 0) {
+    if (a.zero_tail) zero_tail<D>(a, tile.first, h, blockDim.x);
+    return;
+  }
+  const Walk walk(a, tile);
+  const int qt = a.queries_per_tile >> 1;
+
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::TOTAL - 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  if (threadIdx.x == 0) {
+    mbar_init(bar(B_Q), 1);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(bar(B_S + x), 1);
+      mbar_init(bar(B_P + 2 * x), 4);              // the warps of the tile's softmax
+      mbar_init(bar(B_P + 2 * x + 1), 4);
+      mbar_init(bar(B_O + x), 1);
+    }
+    for (int s = 0; s < SLOTS; ++s) {
+      mbar_init(bar(B_FULL + s), 1);
+      mbar_init(bar(B_EMPTY + s), 1);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ producer: Q, then K(0), V(0), K(1), ...
+    if (lane == 0 && walk.n > 0) {
+      tma_prefetch_desc(&tmap_q);
+      tma_prefetch_desc(&tmap_k);
+      tma_prefetch_desc(&tmap_v);
+      const int tiles = walk.any[1] ? 2 : 1;
+      mbar_arrive_expect_tx(bar(B_Q), (uint32_t)(tiles * C::SLABS * qt * a.group * 128));
+      for (int x = 0; x < tiles; ++x)
+        for (int sl = 0; sl < C::SLABS; ++sl)
+          tma_load_3d(smem_u32(smem + C::Q_OFF + x * C::TILE + sl * BN * 128), &tmap_q, bar(B_Q), sl * 64, h * a.group,
+                      (int)tile.token + x * qt);
+      bool ok = true;
+      for (int i = 0; i < 2 * walk.n && ok; ++i) {
+        const int s = i % SLOTS;
+        ok = mbar_wait(bar(B_EMPTY + s), ((i / SLOTS) & 1) ^ 1, abort_flag, a.status, STATUS_TIMEOUT_LOAD);
+        if (!ok) break;
+        const int row = tile.k0 + walk.tile(i >> 1) * BN;
+        mbar_arrive_expect_tx(bar(B_FULL + s), (uint32_t)C::TILE);
+        for (int sl = 0; sl < C::SLABS; ++sl)
+          tma_load_3d(smem_u32(smem + C::KV_OFF + s * C::TILE + sl * BN * 128), (i & 1) ? &tmap_v : &tmap_k,
+                      bar(B_FULL + s), sl * 64, h, row);
+      }
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ UMMA issuer
+    // Lane 0 issues; the whole warp walks along, since it clears V's rows behind the document's end (their P is
+    // 0, but 0 * NaN would not vanish).  UMMAs of one thread execute in order: S(j + 1) may overwrite the P that
+    // the P V before it reads.
+    constexpr uint32_t idesc_pv = idesc_of<F16>(128, D, true);
+    bool ok = walk.n == 0 || mbar_wait_warp(bar(B_Q), 0, abort_flag, a.status, STATUS_TIMEOUT_MMA);
+    auto keys_of = [&](int j) { return min(BN, tile.lk - walk.tile(j) * BN); };
+    auto wait_slot = [&](int i) {
+      ok = ok && mbar_wait_warp(bar(B_FULL + i % SLOTS), (i / SLOTS) & 1, abort_flag, a.status, STATUS_TIMEOUT_MMA);
+      return ok;
+    };
+    auto issue_s = [&](int x, int j) {             // K(j) has arrived
+      if (lane == 0) {
+        tc_fence_after();
+        const uint32_t q_base = smem_u32(smem + C::Q_OFF + x * C::TILE);
+        const uint32_t k_base = smem_u32(smem + C::KV_OFF + (2 * j) % SLOTS * C::TILE);
+        const uint32_t idesc = idesc_of<F16>(128, (keys_of(j) + PAGE - 1) / PAGE * PAGE, false);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * BN * 128 + (kk & 3) * 32;
+          umma_ss(tmem_base + C::S_COL + x * 128, make_smem_desc(q_base + off, 16, 1024), make_smem_desc(k_base + off, 16, 1024),
+                  idesc, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(bar(B_S + x));
+      }
+      __syncwarp();
+    };
+    int done[2] = {0, 0};                          // P V products of each tile
+    auto issue_pv = [&](int x, int j) {            // V(j) has arrived
+      const int pages = (keys_of(j) + PAGE - 1) / PAGE;
+      const uint32_t v_base = smem_u32(smem + C::KV_OFF + (2 * j + 1) % SLOTS * C::TILE);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        ok = ok && mbar_wait_warp(bar(B_P + 2 * x + half), done[x] & 1, abort_flag, a.status, STATUS_TIMEOUT_MMA);
+        if (!ok) return;
+        if (lane == 0) {
+          tc_fence_after();
+#pragma unroll
+          for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+            if (kk < pages)
+              umma_ts(tmem_base + C::O_COL + x * D, tmem_base + C::S_COL + x * 128 + kk * 8,
+                      make_smem_desc(v_base + kk * PAGE * 128, BN * 128, 1024), idesc_pv, (done[x] > 0 || kk > 0) ? 1u : 0u);
+        }
+        __syncwarp();
+      }
+      ++done[x];
+    };
+    auto release = [&](int i) {
+      if (lane == 0) umma_commit(bar(B_EMPTY + i % SLOTS));
+      __syncwarp();
+    };
+    if (ok && walk.n > 0 && wait_slot(0)) {
+      for (int x = 0; x < 2; ++x)
+        if (walk.sees(x, 0)) issue_s(x, 0);
+      release(0);
+    }
+    for (int j = 0; ok && j < walk.n; ++j) {
+      if (!wait_slot(2 * j + 1)) break;
+      const int keys = keys_of(j);
+      if (keys & (PAGE - 1)) {
+        zero_rows<D, BN>(smem + C::KV_OFF + (2 * j + 1) % SLOTS * C::TILE, keys, (keys + PAGE - 1) / PAGE * PAGE);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      const bool more = j + 1 < walk.n;
+      for (int x = 0; x < 2 && ok; ++x) {
+        if (walk.sees(x, j)) issue_pv(x, j);
+        if (x == 1) release(2 * j + 1);
+        if (more && ok) {
+          if (x == 0 && !wait_slot(2 * j + 2)) break;
+          if (walk.sees(x, j + 1)) issue_s(x, j + 1);
+          if (x == 1) release(2 * j + 2);
+        }
+      }
+    }
+    if (ok && lane == 0) {
+      umma_commit(bar(B_O));
+      umma_commit(bar(B_O + 1));
+    }
+  } else {
+    // ------------------------------------------------------------ softmax + epilogue: thread = row
+    const int x = warp >> 2;
+    const int row = threadIdx.x & 127;
+    const int qi = row / a.group, hg = row - qi * a.group;
+    const bool valid = qi < qt && x * qt + qi < tile.count;
+    const int p = tile.pos + x * qt + qi;
+    const Seen seen = valid ? seen_by(a, tile, p) : Seen{0, 0, 0};
+    const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem_base + lane_addr + C::S_COL + x * 128;
+    const uint32_t o_addr = tmem_base + lane_addr + C::O_COL + x * D;
+    const int head = h * a.group + hg;
+    const float slope = a.slopes && valid ? a.slopes[head] * LOG2EF : 0.f;
+    const float scale = scale_of<MODE>(a);
+    float m_ref = -INFINITY, l = 0.f;
+    bool ok = true;
+    int count = 0;
+    for (int j = 0; j < walk.n; ++j) {
+      if (!walk.sees(x, j)) continue;
+      const int key0 = walk.tile(j) * BN;
+      ok = mbar_wait_warp(bar(B_S + x), (uint32_t)(count & 1), abort_flag, a.status, STATUS_TIMEOUT_SOFTMAX);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, s[c]);
+      tmem_ld_wait();
+      const int lo = seen.lo - key0, hi = seen.hi - key0, pre = seen.pre - key0;
+      const bool all = __all_sync(0xffffffffu, (lo <= 0 && hi >= BN) || pre >= BN);
+      float top[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        transform32<MODE>(s[c], a, slope, p, key0 + 32 * c);
+        if (!all) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!((32 * c + i >= lo && 32 * c + i < hi) || 32 * c + i < pre)) s[c][i] = 0xff800000u;
+        }
+        float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          t0 = fmax3(t0, __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+          t1 = fmax3(t1, __uint_as_float(s[c][i + 2]), __uint_as_float(s[c][i + 3]));
+        }
+        top[c] = fmaxf(t0, t1);
+      }
+      const float tmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+      // lazy rescale: only when the running reference falls more than 2^8 behind.  O is quiescent: S's barrier
+      // covers the P V issued before it
+      const bool need = m_ref != -INFINITY && tmax > m_ref + RESCALE_GAP;
+      float alpha = 1.f;
+      if (need) {
+        alpha = fast_exp2(m_ref - tmax);
+        m_ref = tmax;
+        l *= alpha;
+      } else if (m_ref == -INFINITY) {
+        m_ref = tmax;
+      }
+      if (__any_sync(0xffffffffu, need)) {
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(o_addr + c * 32, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st32(o_addr + c * 32, o);
+        }
+      }
+      const float neg_m = m_ref == -INFINITY ? 0.f : p_bias<F16>() - m_ref;
+      const f32x2 scale2 = join(scale, scale), neg2 = join(neg_m, neg_m);
+      f32x2 sum0 = join(0.f, 0.f), sum1 = sum0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float e0, e1;
+          split(fma2(join(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])), scale2, neg2), e0, e1);
+          e0 = fast_exp2(e0);
+          e1 = fast_exp2(e1);
+          packed[i] = pack_pair<F16>(e0, e1);
+          if (i & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
+        }
+        // keys 32 c + 2 i, + 1 of the row share column 16 c + i: P lies over logits that are in registers
+        tmem_st16(s_addr + c * 16, packed);
+        if (c & 1) {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(B_P + 2 * x + (c >> 1)));
+        }
+      }
+      float s0, s1;
+      split(add2(sum0, sum1), s0, s1);
+      l += s0 + s1;
+      ++count;
+    }
+    if (ok) ok = mbar_wait_warp(bar(B_O + x), 0, abort_flag, a.status, STATUS_TIMEOUT_EPILOGUE);
+    tc_fence_after();
+    if (ok && walk.any[x]) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int64_t at = (tile.token + x * qt + qi) * a.num_q_heads + head;
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at * D);
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (count > 0) {
+          tmem_ld32(o_addr + c * 32, o);
+          tmem_ld_wait();
+        }
+        if (valid) {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            w[i] = l == 0.f ? 0u : pack_pair<F16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dst[c * 4 + i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        }
+      }
+      if (valid && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m_ref + __log2f(l) - p_bias<F16>()) * LN2F;
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (*abort_flag) __nanosleep(50000);
+  if (warp == 0) tmem_dealloc(tmem_base, C::TMEM_COLS);
+}
+
+template <int D, bool F16, int MODE>
+int launch(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, const Args& a, int kv_heads, cudaStream_t st) {
+  using C = Cfg<D>;
+  auto kern = dense_pair_kernel<D, F16, MODE>;
+  SEMBLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TOTAL));
+  dim3 grid((unsigned)(ceil_div(a.tokens_q, a.queries_per_tile) + a.docs), (unsigned)kv_heads);
+  kern<<<grid, 320, C::TOTAL, st>>>(mq, mk, mv, a);
+  SEMBLO_LAUNCH_CHECK();
+  return 0;
+}
+
+}  // namespace
+
+namespace dense {
+
+int launch_pair(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, const Args& a, int head_dim,
+                bool f16, int mode, int kv_heads, cudaStream_t st) {
+#define SEMBLO_PAIR(DD, FF, MM) \
+  if (head_dim == DD && f16 == FF && mode == MM) return launch<DD, FF, MM>(mk, mv, mq, a, kv_heads, st);
+  SEMBLO_PAIR(64, false, LINEAR) SEMBLO_PAIR(64, false, CAPPED) SEMBLO_PAIR(64, false, BIASED)
+  SEMBLO_PAIR(64, true, LINEAR) SEMBLO_PAIR(64, true, CAPPED) SEMBLO_PAIR(64, true, BIASED)
+  SEMBLO_PAIR(128, false, LINEAR) SEMBLO_PAIR(128, false, CAPPED) SEMBLO_PAIR(128, false, BIASED)
+  SEMBLO_PAIR(128, true, LINEAR) SEMBLO_PAIR(128, true, CAPPED) SEMBLO_PAIR(128, true, BIASED)
+#undef SEMBLO_PAIR
+  return semblo::fail(semblo::SEMBLO_EINVAL, "unreachable");
+}
+
+}  // namespace dense

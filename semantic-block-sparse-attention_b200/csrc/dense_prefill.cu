@@ -5,13 +5,15 @@
 //   key j of the document is seen when (j <= p_i and p_i - j < window) or j < prefix   (causal; else always)
 //   o_i  = sum_j 2^(s_ij log2e - m_i) v_j / sum_j 2^(s_ij log2e - m_i), one pass with a running m_i
 //
-// One block owns 128 rows (queries x the heads of a KV head, heads adjacent) and walks over the 64-key tiles
-// that any of them sees.  Q, P, S (two buffers) and O live in tensor memory, K and V come by TMA.  Softmax: 8
-// warps, two threads per row; one thread issues the products in the fixed order S(0), S(1), then P V(t), S(t + 2).
+// This file: the entry point, and the kernel for D = 256.  One block owns 128 rows (queries x the heads of a KV
+// head, heads adjacent) and walks over the 64-key tiles that any of them sees.  Q, P, S (two buffers) and O
+// fill tensor memory, K and V come by TMA.  Softmax: 8 warps, two threads per row; one thread issues the
+// products in the fixed order S(0), S(1), then P V(t), S(t + 2).
 #include <algorithm>
 
 #include "../../include/semblo_b200.h"
 #include "dense_common.cuh"
+#include "dense_pair.h"
 #include "host_common.h"
 
 using namespace dense;
@@ -41,7 +43,7 @@ struct Cfg {
 
 enum { B_QFULL = 0, B_OREADY = 1, B_SFULL = 2, B_PFULL = 4, B_PVDONE = 6, B_EPI = 8, B_PAIR = 9, B_KVFULL = 13 };
 
-template <int D, bool F16, bool CAP>
+template <int D, bool F16, int MODE>
 __global__ void __launch_bounds__(320, 1)
 dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                      const Args a) {
@@ -192,6 +194,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       tc_fence_before();
       mbar_arrive(bar(B_QFULL));
     }
+    const float scale = scale_of<MODE>(a);
     float m_ref = -INFINITY, l_part = 0.f;
     bool ok = true;
     float* mx = reinterpret_cast<float*>(smem + C::MX_OFF);
@@ -207,17 +210,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       if (active) {
         tmem_ld32(s_addr, x);
         tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float v = __uint_as_float(x[i]) * a.score_scale;
-          if constexpr (CAP) v = a.cap_log2 * tanh_exp(v);
-          x[i] = __float_as_uint(v);
-        }
-        if (a.slopes) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            x[i] = __float_as_uint(__uint_as_float(x[i]) - slope * fabsf((float)(p - key0 - i)));
-        }
+        transform32<MODE>(x, a, slope, p, key0);
         const int lo = seen.lo - key0, hi = seen.hi - key0, pre = seen.pre - key0;
         if (!__all_sync(0xffffffffu, (lo <= 0 && hi >= 32) || pre >= 32)) {
 #pragma unroll
@@ -238,7 +231,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       if (lane == 0) mbar_arrive(bar(B_PAIR + (warp & 3)));
       ok = mbar_wait_warp(bar(B_PAIR + (warp & 3)), (uint32_t)(j & 1), abort_flag, a.status, STATUS_TIMEOUT_SOFTMAX);
       if (!ok) break;
-      const float tmax = fmaxf(hm, slot[(hf ^ 1) * 128 + row]);
+      const float tmax = fmaxf(hm, slot[(hf ^ 1) * 128 + row]) * scale;
       // lazy rescale: only when the running reference falls more than 2^8 behind
       const bool need = m_ref != -INFINITY && tmax > m_ref + RESCALE_GAP;
       float alpha = 1.f;
@@ -272,8 +265,8 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         float add0 = 0.f, add1 = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float e0 = fast_exp2(__uint_as_float(x[2 * i]) + neg_m);
-          const float e1 = fast_exp2(__uint_as_float(x[2 * i + 1]) + neg_m);
+          const float e0 = fast_exp2(fmaf(__uint_as_float(x[2 * i]), scale, neg_m));
+          const float e1 = fast_exp2(fmaf(__uint_as_float(x[2 * i + 1]), scale, neg_m));
           packed[i] = pack_pair<F16>(e0, e1);
           if (i & 1) add1 += e0 + e1; else add0 += e0 + e1;
         }
@@ -322,10 +315,10 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   if (warp == 0) tmem_dealloc(tmem_base, C::TMEM_COLS);
 }
 
-template <int D, bool F16, bool CAP>
+template <int D, bool F16, int MODE>
 int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int kv_heads, cudaStream_t st) {
   using C = Cfg<D>;
-  auto kern = dense_prefill_kernel<D, F16, CAP>;
+  auto kern = dense_prefill_kernel<D, F16, MODE>;
   SEMBLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TOTAL));
   dim3 grid((unsigned)(ceil_div(a.tokens_q, a.queries_per_tile) + a.docs), (unsigned)kv_heads);
   kern<<<grid, 320, C::TOTAL, st>>>(mk, mv, a);
@@ -354,6 +347,7 @@ extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64
   SEMBLO_REQUIRE(tokens_q >= 0 && tokens_k >= 0 && documents >= 0, "negative token or document count");
   SEMBLO_REQUIRE(tokens_q < ((int64_t)1 << 30) && tokens_k < ((int64_t)1 << 30) && documents < (1 << 30), "too many tokens");
   SEMBLO_REQUIRE(window >= 0 && softcap >= 0.f, "negative window or soft cap");
+  SEMBLO_REQUIRE(sm_scale > 0.f, "the score scale must be positive");
   SEMBLO_REQUIRE(causal || (window == 0 && prefix_lens == nullptr), "a window or a prefix needs the causal mask");
   if (tokens_q == 0 || (documents == 0 && !zero_tail)) return 0;
   SEMBLO_REQUIRE(q && out && status && cu_seqlens_q && cu_seqlens_k && (tokens_k == 0 || (k && v)), "null pointer");
@@ -366,7 +360,7 @@ extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64
   a.out = out; a.lse = lse;
   a.cu_q = cu_seqlens_q; a.cu_k = cu_seqlens_k; a.prefix = prefix_lens; a.slopes = alibi_slopes;
   a.docs = documents; a.group = group; a.num_q_heads = num_q_heads;
-  a.queries_per_tile = 128 / group;
+  a.queries_per_tile = (head_dim <= 128 ? 2 : 1) * (128 / group);
   a.tokens_q = tokens_q; a.tokens_k = tokens_k;
   a.causal = causal; a.window = window; a.zero_tail = zero_tail;
   a.score_scale = softcap > 0.f ? sm_scale / softcap : sm_scale * LOG2EF;
@@ -377,21 +371,26 @@ extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64
   const uint64_t dims[3] = {(uint64_t)head_dim, (uint64_t)num_kv_heads, (uint64_t)std::max<int64_t>(tokens_k, 1)};
   const uint64_t sk[2] = {(uint64_t)k_head_stride * 2, (uint64_t)k_token_stride * 2};
   const uint64_t sv[2] = {(uint64_t)v_head_stride * 2, (uint64_t)v_token_stride * 2};
-  const uint32_t box[3] = {64, 1, BN};
+  const int bn = head_dim <= 128 ? PAIR_BN : BN;
+  const uint32_t box[3] = {64, 1, (uint32_t)bn};
   const uint64_t dense_stride[2] = {(uint64_t)head_dim * 2, (uint64_t)head_dim * num_kv_heads * 2};
   int rc = semblo::make_tensor_map_bf16(&mk, tokens_k ? k : q, 3, dims, tokens_k ? sk : dense_stride, box);
   if (rc) return rc;
   rc = semblo::make_tensor_map_bf16(&mv, tokens_k ? v : q, 3, dims, tokens_k ? sv : dense_stride, box);
   if (rc) return rc;
+  CUtensorMap mq;
+  if (head_dim <= 128) {
+    const uint64_t qd[3] = {(uint64_t)head_dim, (uint64_t)num_q_heads, (uint64_t)tokens_q};
+    const uint64_t qs[2] = {(uint64_t)q_head_stride * 2, (uint64_t)q_token_stride * 2};
+    const uint32_t qbox[3] = {64, (uint32_t)group, (uint32_t)(128 / group)};
+    rc = semblo::make_tensor_map_bf16(&mq, q, 3, qd, qs, qbox);
+    if (rc) return rc;
+  }
   cudaStream_t st = (cudaStream_t)stream;
-  const bool f16 = dtype == SEMBLO_F16, cap = softcap > 0.f;
-#define SEMBLO_DENSE(DD)                                                                                        \
-  if (head_dim == DD)                                                                                           \
-    return f16 ? (cap ? launch<DD, true, true>(mk, mv, a, num_kv_heads, st)                                     \
-                      : launch<DD, true, false>(mk, mv, a, num_kv_heads, st))                                   \
-               : (cap ? launch<DD, false, true>(mk, mv, a, num_kv_heads, st)                                    \
-                      : launch<DD, false, false>(mk, mv, a, num_kv_heads, st));
-  SEMBLO_DENSE(64) SEMBLO_DENSE(128) SEMBLO_DENSE(256)
-#undef SEMBLO_DENSE
-  return semblo::fail(semblo::SEMBLO_EINVAL, "unreachable");
+  const bool f16 = dtype == SEMBLO_F16;
+  const int mode = alibi_slopes ? BIASED : softcap > 0.f ? CAPPED : LINEAR;
+  if (head_dim <= 128) return dense::launch_pair(mk, mv, mq, a, head_dim, f16, mode, num_kv_heads, st);
+  if (mode == LINEAR) return f16 ? launch<256, true, LINEAR>(mk, mv, a, num_kv_heads, st) : launch<256, false, LINEAR>(mk, mv, a, num_kv_heads, st);
+  if (mode == CAPPED) return f16 ? launch<256, true, CAPPED>(mk, mv, a, num_kv_heads, st) : launch<256, false, CAPPED>(mk, mv, a, num_kv_heads, st);
+  return f16 ? launch<256, true, BIASED>(mk, mv, a, num_kv_heads, st) : launch<256, false, BIASED>(mk, mv, a, num_kv_heads, st);
 }

@@ -65,6 +65,8 @@ def dense_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *
     if not causal and (window or prefix_lens is not None):
         raise ValueError("a window or a prefix needs the causal mask")
     q, k, v = _token_rows(q), _token_rows(k), _token_rows(v)
+    if not float(sm_scale) > 0.0:
+        raise ValueError(f"sm_scale must be positive (got {sm_scale})")
     given = out is not None
     if not given:
         out = torch.empty((tokens_q, hq, dim), dtype=dtype, device=device)
