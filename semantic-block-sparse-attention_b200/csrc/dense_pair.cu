@@ -147,18 +147,17 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------ UMMA issuer
-    // Lane 0 issues; the whole warp walks along, since it clears V's rows behind the document's end (their P is
-    // 0, but 0 * NaN would not vanish).  UMMAs of one thread execute in order: S(j + 1) may overwrite the P that
-    // the P V before it reads.
-    constexpr uint32_t idesc_pv = idesc_of<F16>(128, D, true);
-    bool ok = walk.n == 0 || mbar_wait_warp(bar(B_Q), 0, abort_flag, a.status, STATUS_TIMEOUT_MMA);
-    auto keys_of = [&](int j) { return min(BN, tile.lk - walk.tile(j) * BN); };
-    auto wait_slot = [&](int i) {
-      ok = ok && mbar_wait_warp(bar(B_FULL + i % SLOTS), (i / SLOTS) & 1, abort_flag, a.status, STATUS_TIMEOUT_MMA);
-      return ok;
-    };
-    auto issue_s = [&](int x, int j) {             // K(j) has arrived
-      if (lane == 0) {
+    // UMMAs of one thread execute in order: S(j + 1) may overwrite the P that the P V before it reads.
+    if (elect_one()) {
+      constexpr uint32_t idesc_pv = idesc_of<F16>(128, D, true);
+      const int n = walk.n;
+      bool ok = n == 0 || mbar_wait(bar(B_Q), 0, abort_flag, a.status, STATUS_TIMEOUT_MMA);
+      auto keys_of = [&](int j) { return min(BN, tile.lk - walk.tile(j) * BN); };
+      auto wait_slot = [&](int i) {
+        ok = ok && mbar_wait(bar(B_FULL + i % SLOTS), (i / SLOTS) & 1, abort_flag, a.status, STATUS_TIMEOUT_MMA);
+        return ok;
+      };
+      auto issue_s = [&](int x, int j) {           // K(j) has arrived
         tc_fence_after();
         const uint32_t q_base = smem_u32(smem + C::Q_OFF + x * C::TILE);
         const uint32_t k_base = smem_u32(smem + C::KV_OFF + (2 * j) % SLOTS * C::TILE);
@@ -170,18 +169,15 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                   idesc, kk > 0 ? 1u : 0u);
         }
         umma_commit(bar(B_S + x));
-      }
-      __syncwarp();
-    };
-    int done[2] = {0, 0};                          // P V products of each tile
-    auto issue_pv = [&](int x, int j) {            // V(j) has arrived
-      const int pages = (keys_of(j) + PAGE - 1) / PAGE;
-      const uint32_t v_base = smem_u32(smem + C::KV_OFF + (2 * j + 1) % SLOTS * C::TILE);
+      };
+      int done[2] = {0, 0};                        // P V products of each tile
+      auto issue_pv = [&](int x, int j) {          // V(j) has arrived
+        const int pages = (keys_of(j) + PAGE - 1) / PAGE;
+        const uint32_t v_base = smem_u32(smem + C::KV_OFF + (2 * j + 1) % SLOTS * C::TILE);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        ok = ok && mbar_wait_warp(bar(B_P + 2 * x + half), done[x] & 1, abort_flag, a.status, STATUS_TIMEOUT_MMA);
-        if (!ok) return;
-        if (lane == 0) {
+        for (int half = 0; half < 2; ++half) {
+          ok = ok && mbar_wait(bar(B_P + 2 * x + half), done[x] & 1, abort_flag, a.status, STATUS_TIMEOUT_MMA);
+          if (!ok) return;
           tc_fence_after();
 #pragma unroll
           for (int kk = half * 4; kk < half * 4 + 4; ++kk)
@@ -189,41 +185,32 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
               umma_ts(tmem_base + C::O_COL + x * D, tmem_base + C::S_COL + x * 128 + kk * 8,
                       make_smem_desc(v_base + kk * PAGE * 128, BN * 128, 1024), idesc_pv, (done[x] > 0 || kk > 0) ? 1u : 0u);
         }
-        __syncwarp();
+        ++done[x];
+      };
+      if (ok && n > 0 && wait_slot(0)) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (walk.sees(x, 0)) issue_s(x, 0);
+        umma_commit(bar(B_EMPTY));
       }
-      ++done[x];
-    };
-    auto release = [&](int i) {
-      if (lane == 0) umma_commit(bar(B_EMPTY + i % SLOTS));
-      __syncwarp();
-    };
-    if (ok && walk.n > 0 && wait_slot(0)) {
-      for (int x = 0; x < 2; ++x)
-        if (walk.sees(x, 0)) issue_s(x, 0);
-      release(0);
-    }
-    for (int j = 0; ok && j < walk.n; ++j) {
-      if (!wait_slot(2 * j + 1)) break;
-      const int keys = keys_of(j);
-      if (keys & (PAGE - 1)) {
-        zero_rows<D, BN>(smem + C::KV_OFF + (2 * j + 1) % SLOTS * C::TILE, keys, (keys + PAGE - 1) / PAGE * PAGE);
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-      const bool more = j + 1 < walk.n;
-      for (int x = 0; x < 2 && ok; ++x) {
-        if (walk.sees(x, j)) issue_pv(x, j);
-        if (x == 1) release(2 * j + 1);
-        if (more && ok) {
-          if (x == 0 && !wait_slot(2 * j + 2)) break;
-          if (walk.sees(x, j + 1)) issue_s(x, j + 1);
-          if (x == 1) release(2 * j + 2);
+      for (int j = 0; ok && j < n; ++j) {
+        if (!wait_slot(2 * j + 1)) break;
+        const bool more = j + 1 < n;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (ok && walk.sees(x, j)) issue_pv(x, j);
+          if (x == 1 && ok) umma_commit(bar(B_EMPTY + (2 * j + 1) % SLOTS));
+          if (more && ok) {
+            if (x == 0) wait_slot(2 * j + 2);
+            if (ok && walk.sees(x, j + 1)) issue_s(x, j + 1);
+            if (x == 1 && ok) umma_commit(bar(B_EMPTY + (2 * j + 2) % SLOTS));
+          }
         }
       }
-    }
-    if (ok && lane == 0) {
-      umma_commit(bar(B_O));
-      umma_commit(bar(B_O + 1));
+      if (ok) {
+        umma_commit(bar(B_O));
+        umma_commit(bar(B_O + 1));
+      }
     }
   } else {
     // ------------------------------------------------------------ softmax + epilogue: thread = row
@@ -311,6 +298,15 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         }
         // keys 32 c + 2 i, + 1 of the row share column 16 c + i: P lies over logits that are in registers
         tmem_st16(s_addr + c * 16, packed);
+        // V's rows behind the document's end (another document's, or anything) are cleared: their P is 0, but 0 * NaN
+        // would not vanish.  Both tiles' warps may do it; the stage stays until both have been multiplied
+        const int left = tile.lk - key0;
+        if (c == 1 && (warp & 3) == 0 && left < BN && (left & (PAGE - 1))) {
+          ok = mbar_wait_warp(bar(B_FULL + (2 * j + 1) % SLOTS), ((2 * j + 1) / SLOTS) & 1, abort_flag, a.status,
+                              STATUS_TIMEOUT_SOFTMAX);
+          if (ok) zero_rows<D, BN>(smem + C::KV_OFF + (2 * j + 1) % SLOTS * C::TILE, left, (left + PAGE - 1) / PAGE * PAGE);
+          fence_proxy_async_smem();
+        }
         if (c & 1) {
           tmem_st_wait();
           tc_fence_before();
