@@ -2,9 +2,11 @@
 //
 // One block owns two tiles of 128 rows (queries x the heads of a KV head) that take turns: while the tensor core
 // works on one tile (P V of a key tile, then S of the next), a warpgroup runs the softmax of the other, one
-// thread per row and 128 keys at a time.  At D = 128 the two S buffers and the two O accumulators are all of
+// thread per row and two times 64 keys.  At D = 128 the two S buffers and the two O accumulators are all of
 // tensor memory; P lies over the S it came from.  Q, K and V are in shared memory (64 KB of Q and a ring of
-// K, V tiles by TMA).  P is handed over in two halves, so that P V starts when half the exponentials are done.
+// K, V tiles by TMA).  P is handed over in halves, so that P V starts when half the exponentials are done; a
+// half is a step of the running maximum of its own, which keeps 64 scores in registers instead of 128 (those
+// spilled).
 #include <algorithm>
 
 #include "dense_pair.h"
@@ -32,7 +34,7 @@ struct Cfg {
   static constexpr int TMEM_COLS = 512;
 };
 
-enum { B_Q = 0, B_S = 1, B_P = 3, B_O = 7, B_FULL = 9 };       // B_S + x, B_P + 2 x + half, B_O + x
+enum { B_Q = 0, B_S = 1, B_P = 3, B_H = 7, B_O = 9, B_FULL = 11 };     // B_S + x, B_P + 2 x + half, B_H + x, B_O + x
 
 // Which key tiles the block walks over and which of its two row tiles sees each.
 struct Walk {
@@ -103,6 +105,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       mbar_init(bar(B_S + x), 1);
       mbar_init(bar(B_P + 2 * x), 4);              // the warps of the tile's softmax
       mbar_init(bar(B_P + 2 * x + 1), 4);
+      mbar_init(bar(B_H + x), 1);                  // P V of a first half is complete
       mbar_init(bar(B_O + x), 1);
     }
     for (int s = 0; s < SLOTS; ++s) {
@@ -184,6 +187,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             if (kk < pages)
               umma_ts(tmem_base + C::O_COL + x * D, tmem_base + C::S_COL + x * 128 + kk * 8,
                       make_smem_desc(v_base + kk * PAGE * 128, BN * 128, 1024), idesc_pv, (done[x] > 0 || kk > 0) ? 1u : 0u);
+          if (half == 0) umma_commit(bar(B_H + x));
         }
         ++done[x];
       };
@@ -235,88 +239,98 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       ok = mbar_wait_warp(bar(B_S + x), (uint32_t)(count & 1), abort_flag, a.status, STATUS_TIMEOUT_SOFTMAX);
       if (!ok) break;
       tc_fence_after();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, s[c]);
-      tmem_ld_wait();
-      const int lo = seen.lo - key0, hi = seen.hi - key0, pre = seen.pre - key0;
-      const bool all = __all_sync(0xffffffffu, (lo <= 0 && hi >= BN) || pre >= BN);
-      float top[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        transform32<MODE>(s[c], a, slope, p, key0 + 32 * c);
-        if (!all) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!((32 * c + i >= lo && 32 * c + i < hi) || 32 * c + i < pre)) s[c][i] = 0xff800000u;
-        }
-        float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          t0 = fmax3(t0, __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
-          t1 = fmax3(t1, __uint_as_float(s[c][i + 2]), __uint_as_float(s[c][i + 3]));
-        }
-        top[c] = fmaxf(t0, t1);
-      }
-      const float tmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
-      // lazy rescale: only when the running reference falls more than 2^8 behind.  O is quiescent: S's barrier
-      // covers the P V issued before it
-      const bool need = m_ref != -INFINITY && tmax > m_ref + RESCALE_GAP;
-      float alpha = 1.f;
-      if (need) {
-        alpha = fast_exp2(m_ref - tmax);
-        m_ref = tmax;
-        l *= alpha;
-      } else if (m_ref == -INFINITY) {
-        m_ref = tmax;
-      }
-      if (__any_sync(0xffffffffu, need)) {
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld32(o_addr + c * 32, o);
-          tmem_ld_wait();
+      for (int half = 0; half < 2; ++half) {
+        const int k0 = key0 + 64 * half;
+        uint32_t s[2][32];
+        tmem_ld32(s_addr + half * 64, s[0]);
+        tmem_ld32(s_addr + half * 64 + 32, s[1]);
+        tmem_ld_wait();
+        const int lo = seen.lo - k0, hi = seen.hi - k0, pre = seen.pre - k0;
+        const bool all = __all_sync(0xffffffffu, (lo <= 0 && hi >= 64) || pre >= 64);
+        float top[2];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_st32(o_addr + c * 32, o);
+        for (int c = 0; c < 2; ++c) {
+          transform32<MODE>(s[c], a, slope, p, k0 + 32 * c);
+          if (!all) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!((32 * c + i >= lo && 32 * c + i < hi) || 32 * c + i < pre)) s[c][i] = 0xff800000u;
+          }
+          float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            t0 = fmax3(t0, __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+            t1 = fmax3(t1, __uint_as_float(s[c][i + 2]), __uint_as_float(s[c][i + 3]));
+          }
+          top[c] = fmaxf(t0, t1);
         }
-      }
-      const float neg_m = m_ref == -INFINITY ? 0.f : p_bias<F16>() - m_ref;
-      const f32x2 scale2 = join(scale, scale), neg2 = join(neg_m, neg_m);
-      f32x2 sum0 = join(0.f, 0.f), sum1 = sum0;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t packed[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float e0, e1;
-          split(fma2(join(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])), scale2, neg2), e0, e1);
-          e0 = fast_exp2(e0);
-          e1 = fast_exp2(e1);
-          packed[i] = pack_pair<F16>(e0, e1);
-          if (i & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
+        const float tmax = fmaxf(top[0], top[1]) * scale;
+        // lazy rescale: only when the running reference falls more than 2^8 behind
+        const bool need = m_ref != -INFINITY && tmax > m_ref + RESCALE_GAP;
+        float alpha = 1.f;
+        if (need) {
+          alpha = fast_exp2(m_ref - tmax);
+          m_ref = tmax;
+          l *= alpha;
+        } else if (m_ref == -INFINITY) {
+          m_ref = tmax;
         }
-        // keys 32 c + 2 i, + 1 of the row share column 16 c + i: P lies over logits that are in registers
-        tmem_st16(s_addr + c * 16, packed);
+        if (__any_sync(0xffffffffu, need)) {
+          // O is quiescent in the first half (S's barrier covers the P V issued before it), in the second when
+          // the first half's P V has completed
+          if (half == 1) {
+            ok = mbar_wait_warp(bar(B_H + x), (uint32_t)(count & 1), abort_flag, a.status, STATUS_TIMEOUT_SOFTMAX);
+            if (!ok) break;
+            tc_fence_after();
+          }
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + c * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st32(o_addr + c * 32, o);
+          }
+        }
+        const float neg_m = m_ref == -INFINITY ? 0.f : p_bias<F16>() - m_ref;
+        const f32x2 scale2 = join(scale, scale), neg2 = join(neg_m, neg_m);
+        f32x2 sum0 = join(0.f, 0.f), sum1 = sum0;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float e0, e1;
+            split(fma2(join(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])), scale2, neg2), e0, e1);
+            e0 = fast_exp2(e0);
+            e1 = fast_exp2(e1);
+            packed[i] = pack_pair<F16>(e0, e1);
+            if (i & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
+          }
+          // keys 2 i, 2 i + 1 of the chunk share a column: P lies over logits that have been read
+          tmem_st16(s_addr + half * 32 + c * 16, packed);
+        }
         // V's rows behind the document's end (another document's, or anything) are cleared: their P is 0, but 0 * NaN
         // would not vanish.  Both tiles' warps may do it; the stage stays until both have been multiplied
         const int left = tile.lk - key0;
-        if (c == 1 && (warp & 3) == 0 && left < BN && (left & (PAGE - 1))) {
+        if (half == 0 && (warp & 3) == 0 && left < BN && (left & (PAGE - 1))) {
           ok = mbar_wait_warp(bar(B_FULL + (2 * j + 1) % SLOTS), ((2 * j + 1) / SLOTS) & 1, abort_flag, a.status,
                               STATUS_TIMEOUT_SOFTMAX);
-          if (ok) zero_rows<D, BN>(smem + C::KV_OFF + (2 * j + 1) % SLOTS * C::TILE, left, (left + PAGE - 1) / PAGE * PAGE);
+          if (!ok) break;
+          zero_rows<D, BN>(smem + C::KV_OFF + (2 * j + 1) % SLOTS * C::TILE, left, (left + PAGE - 1) / PAGE * PAGE);
           fence_proxy_async_smem();
         }
-        if (c & 1) {
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(B_P + 2 * x + (c >> 1)));
-        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_P + 2 * x + half));
+        float s0, s1;
+        split(add2(sum0, sum1), s0, s1);
+        l += s0 + s1;
       }
-      float s0, s1;
-      split(add2(sum0, sum1), s0, s1);
-      l += s0 + s1;
+      if (!ok) break;
       ++count;
     }
     if (ok) ok = mbar_wait_warp(bar(B_O + x), 0, abort_flag, a.status, STATUS_TIMEOUT_EPILOGUE);
