@@ -11,7 +11,6 @@ using namespace sm100;
 
 constexpr float LN2F = 0.6931471805599453f;
 constexpr float LOG2EF = 1.4426950408889634f;
-constexpr float RESCALE_GAP = 8.0f;              // log2 units: rescale O only when the max moved by > 2^8
 
 struct Args {
   const void* q;                  // [Tq, Hq, D], strides in elements
@@ -27,7 +26,7 @@ struct Args {
   int64_t tokens_q, tokens_k;
   int causal, window;
   int zero_tail;                  // write zeros to the rows behind the last document
-  float score_scale;              // raw product -> log2 units, or -> argument of the capping tanh
+  float score_scale;              // raw product -> log2 units, or -> 4/3 of the capping tanh's argument
   float cap_log2;                 // cap * log2(e)
   int* status;
 };
@@ -153,58 +152,53 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   return d;
 }
 
+__device__ __forceinline__ float fmin3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // tanh(x) = 1 - 2 / (1 + e^2x): exact at both ends, absolute error a few 2^-24; two special-function operations.
 __device__ __forceinline__ float tanh_exp(float x) {
   return 1.f - __fdividef(2.f, 1.f + fast_exp2(x * (2.f * LOG2EF)));
 }
 
-// tanh on [-1.5, 1.5] as x P(x^2), P of degree 7 fitted for the smallest largest error (3.4e-7; 5.0e-7 as
+// tanh(3/4 y) on (-2, 2) as y P(y^2), P of degree 7 fitted for the smallest largest error (3.4e-7; 5e-7 as
 // evaluated in 32 bits), on the multiply-add pipe: the exponentials of the softmax already fill the
 // special-function unit.  Scores beyond 1.5 caps are rare and take tanh_exp.
-constexpr float TANH_POLY_RANGE = 1.5f;
+constexpr float TANH_ARG = 4.f / 3.f, TANH_LIMIT = 2.f;
 __device__ __forceinline__ constexpr float tanh_coefficient(int i) {
-  const float c[8] = {0.999996006f, -0.333240598f, 0.132696271f, -0.0519587733f,
-                      0.0183639843f, -0.00511101866f, 0.000926402514f, -7.81826457e-05f};
+  const float c[8] = {0.74999702f, -0.140585884f, 0.0314894468f, -0.00693565886f,
+                      0.00137885404f, -0.000215864566f, 2.20087895e-05f, -1.04479068e-06f};
   return c[i];
 }
-__device__ __forceinline__ f32x2 tanh_poly2(f32x2 x) {
-  const f32x2 u = mul2(x, x);
-  f32x2 r = join(tanh_coefficient(7), tanh_coefficient(7));
+// factor * tanh(3/4 y) = y P(y^2) with the factor in the coefficients.
+struct TanhPoly {
+  f32x2 c[8];
+  __device__ __forceinline__ explicit TanhPoly(float factor) {
 #pragma unroll
-  for (int i = 6; i >= 0; --i) r = fma2(r, u, join(tanh_coefficient(i), tanh_coefficient(i)));
-  return mul2(r, x);
-}
+    for (int i = 0; i < 8; ++i) c[i] = join(factor * tanh_coefficient(i), factor * tanh_coefficient(i));
+  }
+  // y P(y^2) + add
+  __device__ __forceinline__ f32x2 operator()(f32x2 y, f32x2 add) const {
+    const f32x2 u = mul2(y, y);
+    f32x2 r = c[7];
+#pragma unroll
+    for (int i = 6; i >= 0; --i) r = fma2(r, u, c[i]);
+    return fma2(r, y, add);
+  }
+};
 
 // What happens to a raw score: 0 scaled only, 1 capped, 2 biased by distance (and capped, if there is a cap).
 enum Mode { LINEAR = 0, CAPPED = 1, BIASED = 2 };
 
-// 32 raw scores in place -> what the exponential's scale multiplies.  All lanes of a warp take part.
+// 32 raw scores in place -> what the exponential's scale multiplies.
 template <int MODE>
 __device__ __forceinline__ void transform32(uint32_t* x, const Args& a, float slope, int p, int key0) {
   if constexpr (MODE == LINEAR) return;
   if (MODE == CAPPED || a.cap_log2 > 0.f) {
-    const f32x2 sc = join(a.score_scale, a.score_scale);
-    float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      float v0, v1;
-      split(mul2(join(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc), v0, v1);
-      x[i] = __float_as_uint(v0);
-      x[i + 1] = __float_as_uint(v1);
-      top = fmax3(top, fabsf(v0), fabsf(v1));
-    }
-    if (__all_sync(0xffffffffu, top <= TANH_POLY_RANGE)) {
-#pragma unroll
-      for (int i = 0; i < 32; i += 2) {
-        float v0, v1;
-        split(tanh_poly2(join(__uint_as_float(x[i]), __uint_as_float(x[i + 1]))), v0, v1);
-        x[i] = __float_as_uint(v0);
-        x[i + 1] = __float_as_uint(v1);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(tanh_exp(__uint_as_float(x[i])));
-    }
+    for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(tanh_exp(__uint_as_float(x[i]) * (a.score_scale * (1.f / TANH_ARG))));
   }
   if constexpr (MODE == BIASED) {
     const float scale = a.cap_log2 > 0.f ? a.cap_log2 : a.score_scale;
@@ -219,6 +213,23 @@ template <int MODE> __device__ __forceinline__ float scale_of(const Args& a) {
   return MODE == LINEAR ? a.score_scale : MODE == CAPPED ? a.cap_log2 : 1.f;
 }
 
+// Largest and smallest of 32 values (the smallest only where it is asked for).
+template <bool LEAST>
+__device__ __forceinline__ void range32(const uint32_t* x, float& most, float& least) {
+  float t0 = most, t1 = -INFINITY, u0 = least, u1 = INFINITY;
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) {
+    t0 = fmax3(t0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+    t1 = fmax3(t1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+    if constexpr (LEAST) {
+      u0 = fmin3(u0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+      u1 = fmin3(u1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+    }
+  }
+  most = fmaxf(t0, t1);
+  if constexpr (LEAST) least = fminf(u0, u1);
+}
+
 template <bool F16> __device__ __forceinline__ uint32_t pack_pair(float x, float y) {
   if constexpr (F16) {
     const __half2 v = __floats2half2_rn(x, y);
@@ -229,9 +240,12 @@ template <bool F16> __device__ __forceinline__ uint32_t pack_pair(float x, float
   }
 }
 
-// fp16 keeps P up to 2^(8 + 6): what underflows at its lower end is then below 2^-31 of the largest term.
-// bf16 has float's range and needs no shift.
+// The running reference moves (and O is rescaled) only when a score passes it by more than this many log2 units.
+// fp16 holds P up to 2^(8 + 6): what underflows at its lower end is then below 2^-31 of the largest term.  bf16
+// has float's range, so 24 cost no accuracy, and P V up to 2^24 * keys * |v| stays far inside it; with 8, scores of
+// a spread of 9 units (6 nats) made some row of a warp rescale in every second tile.
 template <bool F16> __host__ __device__ constexpr float p_bias() { return F16 ? 6.f : 0.f; }
+template <bool F16> __host__ __device__ constexpr float rescale_gap() { return F16 ? 8.f : 24.f; }
 
 // Instruction descriptor for kind::f16 with an fp32 accumulator.
 template <bool F16>

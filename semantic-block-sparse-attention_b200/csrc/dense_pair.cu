@@ -2,11 +2,11 @@
 //
 // One block owns two tiles of 128 rows (queries x the heads of a KV head) that take turns: while the tensor core
 // works on one tile (P V of a key tile, then S of the next), a warpgroup runs the softmax of the other, one
-// thread per row and two times 64 keys.  At D = 128 the two S buffers and the two O accumulators are all of
+// thread per row.  At D = 128 the two S buffers and the two O accumulators are all of
 // tensor memory; P lies over the S it came from.  Q, K and V are in shared memory (64 KB of Q and a ring of
-// K, V tiles by TMA).  P is handed over in halves, so that P V starts when half the exponentials are done; a
-// half is a step of the running maximum of its own, which keeps 64 scores in registers instead of 128 (those
-// spilled).
+// K, V tiles by TMA).  P is handed over in halves, so that P V starts when half the exponentials are done.
+// Where scores are capped or biased, a half is a step of the running maximum of its own: the 128 scores of a
+// whole row, the polynomial's coefficients and its chains do not fit in registers together.
 #include <algorithm>
 
 #include "dense_pair.h"
@@ -230,44 +230,57 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     const int head = h * a.group + hg;
     const float slope = a.slopes && valid ? a.slopes[head] * LOG2EF : 0.f;
     const float scale = scale_of<MODE>(a);
+    const TanhPoly capped(a.cap_log2);
     float m_ref = -INFINITY, l = 0.f;
     bool ok = true;
     int count = 0;
-    for (int j = 0; j < walk.n; ++j) {
-      if (!walk.sees(x, j)) continue;
+    // this tile's walk: [0, gp), then [j0, j1)
+    const bool any = x ? walk.any[1] : walk.any[0];
+    const int glo = x ? walk.glo[1] : walk.glo[0], gend = x ? walk.end[1] : walk.end[0];
+    const int gp = any ? walk.gp : 0;
+    const int j0 = any && gend > glo ? walk.gp + glo - walk.first : gp;
+    const int j1 = any && gend > glo ? j0 + gend - glo : gp;
+    for (int j = gp > 0 ? 0 : j0; j < gp || (j >= j0 && j < j1); j = j + 1 == gp ? j0 : j + 1) {
       const int key0 = walk.tile(j) * BN;
       ok = mbar_wait_warp(bar(B_S + x), (uint32_t)(count & 1), abort_flag, a.status, STATUS_TIMEOUT_SOFTMAX);
       if (!ok) break;
       tc_fence_after();
+      constexpr int STEPS = MODE == LINEAR ? 1 : 2, CH = 4 / STEPS;       // chunks of 32 keys in a step
 #pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-        const int k0 = key0 + 64 * half;
-        uint32_t s[2][32];
-        tmem_ld32(s_addr + half * 64, s[0]);
-        tmem_ld32(s_addr + half * 64 + 32, s[1]);
+      for (int step = 0; step < STEPS; ++step) {
+        const int k0 = key0 + 64 * step;
+        uint32_t s[CH][32];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) tmem_ld32(s_addr + step * 64 + c * 32, s[c]);
         tmem_ld_wait();
         const int lo = seen.lo - k0, hi = seen.hi - k0, pre = seen.pre - k0;
-        const bool all = __all_sync(0xffffffffu, (lo <= 0 && hi >= 64) || pre >= 64);
-        float top[2];
+        const bool all = __all_sync(0xffffffffu, (lo <= 0 && hi >= 32 * CH) || pre >= 32 * CH);
+        float tmax = -INFINITY, least = INFINITY;
+        bool poly = false;                             // tanh by polynomial, in the exponential's pass
+        if constexpr (MODE != BIASED) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          transform32<MODE>(s[c], a, slope, p, k0 + 32 * c);
-          if (!all) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!((32 * c + i >= lo && 32 * c + i < hi) || 32 * c + i < pre)) s[c][i] = 0xff800000u;
-          }
-          float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            t0 = fmax3(t0, __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
-            t1 = fmax3(t1, __uint_as_float(s[c][i + 2]), __uint_as_float(s[c][i + 3]));
-          }
-          top[c] = fmaxf(t0, t1);
+          for (int c = 0; c < CH; ++c) range32<MODE == CAPPED>(s[c], tmax, least);
         }
-        const float tmax = fmaxf(top[0], top[1]) * scale;
-        // lazy rescale: only when the running reference falls more than 2^8 behind
-        const bool need = m_ref != -INFINITY && tmax > m_ref + RESCALE_GAP;
+        if constexpr (MODE == CAPPED) {
+          poly = all && __all_sync(0xffffffffu, fmaxf(tmax, -least) * a.score_scale < TANH_LIMIT);
+          if (poly) tmax = tanh_exp(tmax * (a.score_scale * (1.f / TANH_ARG)));
+        }
+        if (MODE == BIASED || (MODE == CAPPED && !poly) || (MODE == LINEAR && !all)) {
+          tmax = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < CH; ++c) {
+            transform32<MODE>(s[c], a, slope, p, k0 + 32 * c);
+            if (!all) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!((32 * c + i >= lo && 32 * c + i < hi) || 32 * c + i < pre)) s[c][i] = 0xff800000u;
+            }
+            range32<false>(s[c], tmax, least);
+          }
+        }
+        tmax *= scale;
+        // lazy rescale: only when the running reference falls far behind
+        const bool need = m_ref != -INFINITY && tmax > m_ref + rescale_gap<F16>();
         float alpha = 1.f;
         if (need) {
           alpha = fast_exp2(m_ref - tmax);
@@ -277,9 +290,9 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           m_ref = tmax;
         }
         if (__any_sync(0xffffffffu, need)) {
-          // O is quiescent in the first half (S's barrier covers the P V issued before it), in the second when
+          // O is quiescent in the first step (S's barrier covers the P V issued before it), in the second when
           // the first half's P V has completed
-          if (half == 1) {
+          if (step == 1) {
             ok = mbar_wait_warp(bar(B_H + x), (uint32_t)(count & 1), abort_flag, a.status, STATUS_TIMEOUT_SOFTMAX);
             if (!ok) break;
             tc_fence_after();
@@ -297,35 +310,45 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         const float neg_m = m_ref == -INFINITY ? 0.f : p_bias<F16>() - m_ref;
         const f32x2 scale2 = join(scale, scale), neg2 = join(neg_m, neg_m);
         f32x2 sum0 = join(0.f, 0.f), sum1 = sum0;
+        auto exponentials = [&](auto argument) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t packed[16];
+          for (int c = 0; c < CH; ++c) {
+            uint32_t packed[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float e0, e1;
-            split(fma2(join(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])), scale2, neg2), e0, e1);
-            e0 = fast_exp2(e0);
-            e1 = fast_exp2(e1);
-            packed[i] = pack_pair<F16>(e0, e1);
-            if (i & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
+            for (int i = 0; i < 16; ++i) {
+              float e0, e1;
+              split(argument(join(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1]))), e0, e1);
+              e0 = fast_exp2(e0);
+              e1 = fast_exp2(e1);
+              packed[i] = pack_pair<F16>(e0, e1);
+              if (i & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
+            }
+            // keys 2 i, 2 i + 1 of the chunk share a column: P lies over logits that have been read
+            tmem_st16(s_addr + step * 32 + c * 16, packed);
+            if (c & 1) {
+              const int half = step + (c >> 1);
+              // V's rows behind the document's end (another document's, or anything) are cleared: their P is 0, but
+              // 0 * NaN would not vanish.  Both tiles' warps may do it; the stage stays until both are multiplied
+              const int left = tile.lk - key0;
+              if (half == 0 && (warp & 3) == 0 && left < BN && (left & (PAGE - 1))) {
+                ok = mbar_wait_warp(bar(B_FULL + (2 * j + 1) % SLOTS), ((2 * j + 1) / SLOTS) & 1, abort_flag, a.status,
+                                    STATUS_TIMEOUT_SOFTMAX);
+                if (ok) zero_rows<D, BN>(smem + C::KV_OFF + (2 * j + 1) % SLOTS * C::TILE, left, (left + PAGE - 1) / PAGE * PAGE);
+                fence_proxy_async_smem();
+              }
+              tmem_st_wait();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(B_P + 2 * x + half));
+            }
           }
-          // keys 2 i, 2 i + 1 of the chunk share a column: P lies over logits that have been read
-          tmem_st16(s_addr + half * 32 + c * 16, packed);
+        };
+        if (MODE == CAPPED && poly) {
+          const f32x2 arg2 = join(a.score_scale, a.score_scale);
+          exponentials([&](f32x2 v) { return capped(mul2(v, arg2), neg2); });
+        } else {
+          exponentials([&](f32x2 v) { return fma2(v, scale2, neg2); });
         }
-        // V's rows behind the document's end (another document's, or anything) are cleared: their P is 0, but 0 * NaN
-        // would not vanish.  Both tiles' warps may do it; the stage stays until both have been multiplied
-        const int left = tile.lk - key0;
-        if (half == 0 && (warp & 3) == 0 && left < BN && (left & (PAGE - 1))) {
-          ok = mbar_wait_warp(bar(B_FULL + (2 * j + 1) % SLOTS), ((2 * j + 1) / SLOTS) & 1, abort_flag, a.status,
-                              STATUS_TIMEOUT_SOFTMAX);
-          if (!ok) break;
-          zero_rows<D, BN>(smem + C::KV_OFF + (2 * j + 1) % SLOTS * C::TILE, left, (left + PAGE - 1) / PAGE * PAGE);
-          fence_proxy_async_smem();
-        }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_P + 2 * x + half));
         float s0, s1;
         split(add2(sum0, sum1), s0, s1);
         l += s0 + s1;
@@ -335,7 +358,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
     if (ok) ok = mbar_wait_warp(bar(B_O + x), 0, abort_flag, a.status, STATUS_TIMEOUT_EPILOGUE);
     tc_fence_after();
-    if (ok && walk.any[x]) {
+    if (ok && any) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int64_t at = (tile.token + x * qt + qi) * a.num_q_heads + head;
       uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at * D);

@@ -190,6 +190,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       mbar_arrive(bar(B_QFULL));
     }
     const float scale = scale_of<MODE>(a);
+    const TanhPoly capped(a.cap_log2);
     float m_ref = -INFINITY, l_part = 0.f;
     bool ok = true;
     float* mx = reinterpret_cast<float*>(smem + C::MX_OFF);
@@ -201,24 +202,28 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       const uint32_t s_addr = tmem_base + lane_addr + b * BN + hf * 32;
       const bool active = tile.lk > key0;                // the product wrote at least one page of this half
       uint32_t x[32];
-      float hm = -INFINITY;
+      float hm = -INFINITY, least = INFINITY;
+      bool poly = MODE == CAPPED;                        // this half's tanh by polynomial, in the exponential's pass
       if (active) {
         tmem_ld32(s_addr, x);
         tmem_ld_wait();
-        transform32<MODE>(x, a, slope, p, key0);
         const int lo = seen.lo - key0, hi = seen.hi - key0, pre = seen.pre - key0;
-        if (!__all_sync(0xffffffffu, (lo <= 0 && hi >= 32) || pre >= 32)) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!((i >= lo && i < hi) || i < pre)) x[i] = 0xff800000u;
+        const bool all = __all_sync(0xffffffffu, (lo <= 0 && hi >= 32) || pre >= 32);
+        if constexpr (MODE == CAPPED) {
+          range32<true>(x, hm, least);
+          poly = all && __all_sync(0xffffffffu, fmaxf(hm, -least) * a.score_scale < TANH_LIMIT);
+          if (poly) hm = tanh_exp(hm * (a.score_scale * (1.f / TANH_ARG)));
         }
-        float tm[2] = {-INFINITY, -INFINITY};            // two short chains
+        if (!poly) {
+          transform32<MODE>(x, a, slope, p, key0);
+          if (!all) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          tm[0] = fmax3(tm[0], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-          tm[1] = fmax3(tm[1], __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+            for (int i = 0; i < 32; ++i)
+              if (!((i >= lo && i < hi) || i < pre)) x[i] = 0xff800000u;
+          }
+          hm = -INFINITY;
+          range32<false>(x, hm, least);
         }
-        hm = fmaxf(tm[0], tm[1]);
       }
       float* slot = mx + b * 256;
       slot[hf * 128 + row] = hm;
@@ -227,8 +232,8 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       ok = mbar_wait_warp(bar(B_PAIR + (warp & 3)), (uint32_t)(j & 1), abort_flag, a.status, STATUS_TIMEOUT_SOFTMAX);
       if (!ok) break;
       const float tmax = fmaxf(hm, slot[(hf ^ 1) * 128 + row]) * scale;
-      // lazy rescale: only when the running reference falls more than 2^8 behind
-      const bool need = m_ref != -INFINITY && tmax > m_ref + RESCALE_GAP;
+      // lazy rescale: only when the running reference falls far behind
+      const bool need = m_ref != -INFINITY && tmax > m_ref + rescale_gap<F16>();
       float alpha = 1.f;
       if (need) {
         alpha = fast_exp2(m_ref - tmax);
@@ -257,15 +262,28 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       if (active) {
         const float neg_m = m_ref == -INFINITY ? 0.f : p_bias<F16>() - m_ref;
         uint32_t packed[16];
-        float add0 = 0.f, add1 = 0.f;
+        f32x2 sum0 = join(0.f, 0.f), sum1 = sum0;
+        auto exponentials = [&](auto argument) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e0 = fast_exp2(fmaf(__uint_as_float(x[2 * i]), scale, neg_m));
-          const float e1 = fast_exp2(fmaf(__uint_as_float(x[2 * i + 1]), scale, neg_m));
-          packed[i] = pack_pair<F16>(e0, e1);
-          if (i & 1) add1 += e0 + e1; else add0 += e0 + e1;
+          for (int i = 0; i < 16; ++i) {
+            float e0, e1;
+            split(argument(join(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]))), e0, e1);
+            e0 = fast_exp2(e0);
+            e1 = fast_exp2(e1);
+            packed[i] = pack_pair<F16>(e0, e1);
+            if (i & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
+          }
+        };
+        const f32x2 neg2 = join(neg_m, neg_m), scale2 = join(scale, scale);
+        if (MODE == CAPPED && poly) {
+          const f32x2 arg2 = join(a.score_scale, a.score_scale);
+          exponentials([&](f32x2 v) { return capped(mul2(v, arg2), neg2); });
+        } else {
+          exponentials([&](f32x2 v) { return fma2(v, scale2, neg2); });
         }
-        l_part += add0 + add1;
+        float s0, s1;
+        split(add2(sum0, sum1), s0, s1);
+        l_part += s0 + s1;
         // P lies over this half's own logits; P V takes its 16-key slices from columns 0, 8, 32 and 40
         tmem_st16(s_addr, packed);
       }
@@ -365,7 +383,7 @@ extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64
   a.queries_per_tile = (head_dim <= 128 ? 2 : 1) * (128 / group);
   a.tokens_q = tokens_q; a.tokens_k = tokens_k;
   a.causal = causal; a.window = window; a.zero_tail = zero_tail;
-  a.score_scale = softcap > 0.f ? sm_scale / softcap : sm_scale * LOG2EF;
+  a.score_scale = softcap > 0.f ? sm_scale / softcap * TANH_ARG : sm_scale * LOG2EF;
   a.cap_log2 = softcap * LOG2EF;
   a.status = status;
   // no keys at all: the maps are not read, but have to describe something
