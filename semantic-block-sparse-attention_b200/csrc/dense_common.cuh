@@ -53,12 +53,17 @@ __device__ __forceinline__ Tile find_tile(const Args& a, int want) {
   for (int d0 = 0; d0 < a.docs; d0 += 32) {
     const int d = d0 + lane;
     int64_t c0 = 0, c1 = 0;
-    int n = 0;
-    if (d < a.docs) {
-      c0 = min(max((int64_t)a.cu_q[d], (int64_t)0), a.tokens_q);
-      c1 = min(max((int64_t)a.cu_q[d + 1], c0), a.tokens_q);
-      n = (int)((c1 - c0 + qt - 1) / qt);
+    int k0 = 0, k1 = 0, pre = 0;
+    if (d < a.docs) {                              // all that may be needed, in one round trip
+      c0 = a.cu_q[d];
+      c1 = a.cu_q[d + 1];
+      k0 = a.cu_k[d];
+      k1 = a.cu_k[d + 1];
+      if (a.prefix) pre = a.prefix[d];
     }
+    c0 = min(max(c0, (int64_t)0), a.tokens_q);
+    c1 = min(max(c1, c0), a.tokens_q);
+    const int n = (int)((c1 - c0 + qt - 1) / qt);
     int upto = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -71,16 +76,17 @@ __device__ __forceinline__ Tile find_tile(const Args& a, int want) {
       const int tiles = __shfl_sync(0xffffffffu, n, at);
       const int nth = tiles - 1 - (want - (__shfl_sync(0xffffffffu, upto, at) - tiles));
       const int64_t q0 = __shfl_sync(0xffffffffu, c0, at), q1 = __shfl_sync(0xffffffffu, c1, at);
+      k0 = __shfl_sync(0xffffffffu, k0, at);
+      k1 = __shfl_sync(0xffffffffu, k1, at);
+      pre = __shfl_sync(0xffffffffu, pre, at);
       t.doc = d0 + at;
       t.first = nth * qt;
       t.count = (int)min((int64_t)qt, q1 - q0 - t.first);
       t.token = q0 + t.first;
-      const int64_t k0 = min(max((int64_t)a.cu_k[t.doc], (int64_t)0), a.tokens_k);
-      const int64_t k1 = min(max((int64_t)a.cu_k[t.doc + 1], k0), a.tokens_k);
-      t.k0 = (int)k0;
-      t.lk = (int)(k1 - k0);
+      t.k0 = (int)min(max((int64_t)k0, (int64_t)0), a.tokens_k);
+      t.lk = (int)min(max((int64_t)k1, (int64_t)t.k0), a.tokens_k) - t.k0;
       t.pos = t.lk - (int)(q1 - q0) + t.first;
-      t.prefix = a.prefix ? min(max(a.prefix[t.doc], 0), t.lk) : 0;
+      t.prefix = min(max(pre, 0), t.lk);
       return t;
     }
     want -= total;
@@ -112,6 +118,15 @@ __device__ __forceinline__ Seen seen_by(const Args& a, const Tile& t, int p) {
   s.lo = a.causal && a.window > 0 ? max(0, p - a.window + 1) : 0;
   s.pre = a.causal ? t.prefix : 0;
   return s;
+}
+
+// Bit i: key i of 32 is seen, for limits relative to the first of them; and what is not seen becomes -inf.
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t seen_bits(int lo, int hi, int pre) { return (below(hi) & ~below(lo)) | below(pre); }
+__device__ __forceinline__ void hide32(uint32_t* x, uint32_t bits) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (!(bits & (1u << i))) x[i] = 0xff800000u;
 }
 
 // The key tiles of BN rows that any row of the block's tile sees: [0, gp) then [glo, ...), n in all.
@@ -202,9 +217,10 @@ __device__ __forceinline__ void transform32(uint32_t* x, const Args& a, float sl
   }
   if constexpr (MODE == BIASED) {
     const float scale = a.cap_log2 > 0.f ? a.cap_log2 : a.score_scale;
+    const float dist = (float)(p - key0);            // a conversion per key would cost as much as its exponential
 #pragma unroll
     for (int i = 0; i < 32; ++i)
-      x[i] = __float_as_uint(__uint_as_float(x[i]) * scale - slope * fabsf((float)(p - key0 - i)));
+      x[i] = __float_as_uint(fmaf(-slope, fabsf(dist - (float)i), __uint_as_float(x[i]) * scale));
   }
 }
 
@@ -252,6 +268,18 @@ template <bool F16>
 __host__ __device__ constexpr uint32_t idesc_of(int m, int n, bool b_mn_major) {
   const uint32_t d = make_idesc_bf16(m, n, false, b_mn_major);
   return F16 ? d & ~((1u << 7) | (1u << 10)) : d;
+}
+
+// A warp's share of the output: each lane holds 32 values of its row (16-byte pieces piece0 ... + 3 as packed
+// words) and has put them into `stage` (32 rows of PIECES 16-byte pieces, permuted so that neither side
+// collides); this writes `rows` rows of it, PIECES lanes to a row, so that whole lines leave at once.
+template <int PIECES>
+__device__ __forceinline__ void stage_pieces(uint8_t* stage, int piece0, const uint32_t (&w)[16]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    reinterpret_cast<uint4*>(stage)[lane * PIECES + ((piece0 + i) ^ (lane & (PIECES - 1)))] =
+        make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
 }
 
 // Zero rows [from, to) of a swizzled 128-byte-row tile of D columns (all of a row, so the permutation inside it

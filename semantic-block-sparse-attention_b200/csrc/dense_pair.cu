@@ -87,19 +87,13 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     if (threadIdx.x == 0) atomicCAS(a.status, 0, STATUS_SMEM_ALIGN);
     return;
   }
-  const Tile tile = find_tile(a, blockIdx.x);
-  if (tile.doc < 0) {
-    if (a.zero_tail) zero_tail<D>(a, tile.first, h, blockDim.x);
-    return;
-  }
-  const Walk walk(a, tile);
-  const int qt = a.queries_per_tile >> 1;
-
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::TOTAL - 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
-  if (threadIdx.x == 0) {
+  // barriers by the warp that loads, which need not wait for anybody with its first loads; tensor memory by the
+  // warp that issues, while the others look for their tile
+  if (warp == 8 && lane == 0) {
     mbar_init(bar(B_Q), 1);
     for (int x = 0; x < 2; ++x) {
       mbar_init(bar(B_S + x), 1);
@@ -114,8 +108,37 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
     *abort_flag = 0;
     mbar_fence_init();
+    fence_proxy_async_smem();
+    tma_prefetch_desc(&tmap_q);
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
   }
-  if (warp == 0) {
+  __syncwarp();
+  const Tile tile = find_tile(a, blockIdx.x);      // the same answer in every warp
+  if (tile.doc < 0) {
+    if (a.zero_tail) zero_tail<D>(a, tile.first, h, blockDim.x);
+    return;
+  }
+  const Walk walk(a, tile);
+  const int qt = a.queries_per_tile >> 1;
+  auto load_kv = [&](int i) {                      // K(i / 2) or V(i / 2) into its slot, which is free
+    const int s = i % SLOTS, row = tile.k0 + walk.tile(i >> 1) * BN;
+    mbar_arrive_expect_tx(bar(B_FULL + s), (uint32_t)C::TILE);
+    for (int sl = 0; sl < C::SLABS; ++sl)
+      tma_load_3d(smem_u32(smem + C::KV_OFF + s * C::TILE + sl * BN * 128), (i & 1) ? &tmap_v : &tmap_k, bar(B_FULL + s),
+                  sl * 64, h, row);
+  };
+  if (warp == 8 && lane == 0 && walk.n > 0) {
+    const int tiles = walk.any[1] ? 2 : 1;
+    mbar_arrive_expect_tx(bar(B_Q), (uint32_t)(tiles * C::SLABS * qt * a.group * 128));
+    for (int x = 0; x < tiles; ++x)
+      for (int sl = 0; sl < C::SLABS; ++sl)
+        tma_load_3d(smem_u32(smem + C::Q_OFF + x * C::TILE + sl * BN * 128), &tmap_q, bar(B_Q), sl * 64, h * a.group,
+                    (int)tile.token + x * qt);
+    load_kv(0);
+    load_kv(1);
+  }
+  if (warp == 9) {
     tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
     tmem_relinquish();
   }
@@ -125,27 +148,11 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp == 8) {
-    // ------------------------------------------------------------ producer: Q, then K(0), V(0), K(1), ...
-    if (lane == 0 && walk.n > 0) {
-      tma_prefetch_desc(&tmap_q);
-      tma_prefetch_desc(&tmap_k);
-      tma_prefetch_desc(&tmap_v);
-      const int tiles = walk.any[1] ? 2 : 1;
-      mbar_arrive_expect_tx(bar(B_Q), (uint32_t)(tiles * C::SLABS * qt * a.group * 128));
-      for (int x = 0; x < tiles; ++x)
-        for (int sl = 0; sl < C::SLABS; ++sl)
-          tma_load_3d(smem_u32(smem + C::Q_OFF + x * C::TILE + sl * BN * 128), &tmap_q, bar(B_Q), sl * 64, h * a.group,
-                      (int)tile.token + x * qt);
-      bool ok = true;
-      for (int i = 0; i < 2 * walk.n && ok; ++i) {
-        const int s = i % SLOTS;
-        ok = mbar_wait(bar(B_EMPTY + s), ((i / SLOTS) & 1) ^ 1, abort_flag, a.status, STATUS_TIMEOUT_LOAD);
-        if (!ok) break;
-        const int row = tile.k0 + walk.tile(i >> 1) * BN;
-        mbar_arrive_expect_tx(bar(B_FULL + s), (uint32_t)C::TILE);
-        for (int sl = 0; sl < C::SLABS; ++sl)
-          tma_load_3d(smem_u32(smem + C::KV_OFF + s * C::TILE + sl * BN * 128), (i & 1) ? &tmap_v : &tmap_k,
-                      bar(B_FULL + s), sl * 64, h, row);
+    // ------------------------------------------------------------ producer: after Q, K(0), V(0): K(1), V(1), ...
+    if (lane == 0) {
+      for (int i = 2; i < 2 * walk.n; ++i) {
+        if (!mbar_wait(bar(B_EMPTY + i % SLOTS), ((i / SLOTS) & 1) ^ 1, abort_flag, a.status, STATUS_TIMEOUT_LOAD)) break;
+        load_kv(i);
       }
     }
   } else if (warp == 9) {
@@ -271,9 +278,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           for (int c = 0; c < CH; ++c) {
             transform32<MODE>(s[c], a, slope, p, k0 + 32 * c);
             if (!all) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!((32 * c + i >= lo && 32 * c + i < hi) || 32 * c + i < pre)) s[c][i] = 0xff800000u;
+              hide32(s[c], seen_bits(lo - 32 * c, hi - 32 * c, pre - 32 * c));
             }
             range32<false>(s[c], tmax, least);
           }
@@ -361,7 +366,9 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     if (ok && any) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int64_t at = (tile.token + x * qt + qi) * a.num_q_heads + head;
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at * D);
+      // through Q's shared memory (no product is in flight any more), 8 KB of it per warp
+      constexpr int PIECES = D / 8;
+      uint8_t* stage = smem + C::Q_OFF + warp * 32 * D * 2;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -369,14 +376,21 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           tmem_ld32(o_addr + c * 32, o);
           tmem_ld_wait();
         }
-        if (valid) {
-          uint32_t w[16];
+        uint32_t w[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            w[i] = l == 0.f ? 0u : pack_pair<F16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dst[c * 4 + i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-        }
+        for (int i = 0; i < 16; ++i)
+          w[i] = l == 0.f ? 0u : pack_pair<F16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+        stage_pieces<PIECES>(stage, c * 4, w);
+      }
+      __syncwarp();
+#pragma unroll 4
+      for (int i = lane; i < 32 * PIECES; i += 32) {
+        const int r = i / PIECES, piece = i % PIECES, rr = (warp & 3) * 32 + r;
+        const int q = rr / a.group;
+        if (q < qt && x * qt + q < tile.count)
+          reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) +
+                                   ((tile.token + x * qt + q) * a.num_q_heads + h * a.group + rr - q * a.group) * D)[piece] =
+              reinterpret_cast<const uint4*>(stage)[r * PIECES + (piece ^ (r & (PIECES - 1)))];
       }
       if (valid && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m_ref + __log2f(l) - p_bias<F16>()) * LN2F;
     }
@@ -384,7 +398,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   }
   __syncthreads();
   if (*abort_flag) __nanosleep(50000);
-  if (warp == 0) tmem_dealloc(tmem_base, C::TMEM_COLS);
+  if (warp == 9) tmem_dealloc(tmem_base, C::TMEM_COLS);
 }
 
 template <int D, bool F16, int MODE>

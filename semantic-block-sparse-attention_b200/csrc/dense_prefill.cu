@@ -217,9 +217,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         if (!poly) {
           transform32<MODE>(x, a, slope, p, key0);
           if (!all) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!((i >= lo && i < hi) || i < pre)) x[i] = 0xff800000u;
+            hide32(x, seen_bits(lo, hi, pre));
           }
           hm = -INFINITY;
           range32<false>(x, hm, least);
