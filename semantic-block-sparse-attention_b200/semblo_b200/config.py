@@ -69,6 +69,7 @@ class SembloVllmConfig:
     runtime_weights_file: str | None = None   # the routing maps' side-car (runtime_weights.py)
     runtime_manifest_file: str | None = None
     runtime_allow_unused_layers: bool = False
+    dense_cache_bits: int = 0                 # 8: dense requests and layers are served here, K/V held in 8 bits
 
     @classmethod
     def from_hf_config(cls, config: Any, *, identity_router: bool = False) -> "SembloVllmConfig":
@@ -136,6 +137,7 @@ class SembloVllmConfig:
             runtime_weights_file=weights_file,
             runtime_manifest_file=str(_get(text, "semblo_runtime_manifest_file", "")) or None,
             runtime_allow_unused_layers=bool(_get(text, "semblo_runtime_allow_unused_layers", False)),
+            dense_cache_bits=int(_get(text, "semblo_dense_cache_bits", 0)),
         )
         cfg.validate()
         return cfg
@@ -162,5 +164,7 @@ class SembloVllmConfig:
             if not 0 < budget <= self.token_capacity:
                 raise ValueError(f"the target_tokens of layer {layer} ({budget}) must lie in (0, token_capacity "
                                  f"{self.token_capacity}]")
+        if self.dense_cache_bits not in (0, 8):
+            raise ValueError(f"dense_cache_bits must be 0 or 8 (got {self.dense_cache_bits})")
         if self.selection_temperature <= 0 or self.query_chunk_size <= 0 or self.prefill_chunk < 0:
             raise ValueError("selection_temperature and query_chunk_size must be positive, prefill_chunk not negative")

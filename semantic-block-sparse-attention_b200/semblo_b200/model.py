@@ -9,7 +9,8 @@ Mirror of the hot-path half of semblo/vllm_plugin/model.py (SembloAttention):
 ``begin_streamed_prefill`` / ``begin_token_outer_prefill`` 1271-1287, ``_ingest_prompt_kv`` 1301-1382
 and ``StreamedPrefillSession`` 1431-1529, for the configuration the kernels serve: flat partition,
 identity routing map with whole-vector normalisation, the layer's own cluster-ordered prompt
-copy (own_prompt_cache); generated tokens go through the fused decode step over the decode arena
+copy (own_prompt_cache); dense requests and layers, which the reference leaves to the engine, are served with
+``dense_cache_bits = 8`` (exact attention of the prompt, generated tokens over an 8-bit K/V cache); generated tokens go through the fused decode step over the decode arena
 (SEMBLO_FULL_GRAPH_DECODE=1) or, without an arena, through the decode kernels over the request's own
 index plus the layer's store of generated K/V, recorded once per request as a CUDA graph
 (decode_graph.DecodeStepGraph).  The model-specific
@@ -33,7 +34,10 @@ from . import fused_prefill as _fused_prefill
 from .attention_op import register_layer, sparse_attention_op
 from .config import SembloVllmConfig
 from .decode_graph import DecodeStepGraph, tensor_signature
+from .dense_prefill import dense_prefill_attention
+from .kv8_cache import kv8_append, kv8_decode_attention
 from .paged_attention import PostingTiles, merge_paged_attention_results, paged_posting_attention
+from .rotary import RotaryFrequencies, apply_rotary
 from .routing_map import SembloKeyRouter
 from .flat_index import routing_normalize
 from .state import ProductPostingIndex, SembloRuntimeState
@@ -46,11 +50,17 @@ class SembloAttention(nn.Module):
     def _init_semblo_runtime(self, *, runtime_config: SembloVllmConfig, runtime_state: SembloRuntimeState,
                              layer_idx: int, source_layer_idx: int, uses_sparse_attention: bool = True,
                              builds_product_index: bool = True,
-                             attention_logits_soft_cap: float | None = None) -> None:
-        """Requires ``num_heads / num_kv_heads / head_dim / scaling`` to be set already."""
+                             attention_logits_soft_cap: float | None = None, attention_window: int = 0,
+                             rotary: RotaryFrequencies | None = None, rotary_interleaved: bool = False) -> None:
+        """Requires ``num_heads / num_kv_heads / head_dim / scaling`` to be set already.  ``attention_window`` (0: none)
+        is the local window of a layer that is not sparse; ``rotary`` are the frequencies of :meth:`_rotate`."""
         runtime_config.validate()
-        if attention_logits_soft_cap:
+        serves_dense_only = not uses_sparse_attention and bool(runtime_config.dense_cache_bits)
+        if attention_logits_soft_cap and not serves_dense_only:
             raise RuntimeError("the fused sparse path has no logit soft cap")
+        if attention_window and not serves_dense_only:
+            raise RuntimeError("a local window is served in dense layers only (uses_sparse_attention=False with "
+                               "dense_cache_bits=8)")
         if int(runtime_config.index_dim) > int(self.head_dim):
             raise RuntimeError("the kernels route in a space of the head dimension: index_dim must not exceed "
                                "head_dim (the identity map, a loaded square map, or a map into fewer dimensions, "
@@ -62,6 +72,9 @@ class SembloAttention(nn.Module):
         self.runtime_config = runtime_config
         self.runtime_state = runtime_state
         self.attention_logits_soft_cap = attention_logits_soft_cap
+        self.attention_window = int(attention_window)
+        self.rotary = rotary
+        self.rotary_interleaved = bool(rotary_interleaved)
         self.layer_target_tokens = runtime_config.layer_target_tokens.get(self.layer_idx, runtime_config.target_tokens)
         self.layer_decode_target_tokens = (
             self.layer_target_tokens
@@ -84,6 +97,16 @@ class SembloAttention(nn.Module):
     # ---- the traced side -----------------------------------------------------------------
     def _positions_for_runtime(self, positions: torch.Tensor):
         return positions, positions
+
+    def _rotate(self, rope_positions: torch.Tensor, q_pre: torch.Tensor, k_pre: torch.Tensor | None):
+        """q_post, k_post of ``_project_qkv`` from the projections (any leading token dimension, heads flattened or
+        not): routing keeps reading the vectors before the rotation."""
+        if self.rotary is None:
+            raise RuntimeError("the layer was initialised without rotary frequencies")
+        q3 = q_pre.view(-1, self.num_heads, self.head_dim)
+        k3 = None if k_pre is None else k_pre.view(-1, self.num_kv_heads, self.head_dim)
+        q_post, k_post = apply_rotary(q3, k3, rope_positions.view(-1), self.rotary, interleaved=self.rotary_interleaved)
+        return q_post.view(q_pre.shape), None if k_post is None else k_post.view(k_pre.shape)
 
     def _sparse_layer_forward(self, positions: torch.Tensor, hidden_states: torch.Tensor) -> torch.Tensor:
         rope_positions, positions = self._positions_for_runtime(positions)
@@ -360,13 +383,62 @@ class SembloAttention(nn.Module):
         _lib.status_for(q.device).poll()
         return output.flatten(-2, -1)
 
+    # ---- dense requests and layers -------------------------------------------------------
+    def _dense_attention(self, positions, q_post, k_post, v_states, output) -> None:
+        """Exact attention: a prompt over its own K/V, a generated token over the layer's 8-bit cache, which both
+        write.  A layer that shares another layer's K/V reads what that layer left."""
+        state = self.runtime_state
+        device = q_post.device
+        tokens = positions.numel()
+        q = q_post.view(tokens, self.num_heads, self.head_dim)
+        out = output.view(tokens, self.num_heads, self.head_dim)
+        cache, table = state.dense_cache(self.source_layer_idx, num_kv_heads=self.num_kv_heads, head_dim=self.head_dim,
+                                         device=device)
+        if not self.is_kv_shared_layer and (k_post is None or v_states is None):
+            raise RuntimeError("physical layers must produce K/V")
+        first = positions[:1].to(torch.int32)
+        starts = torch.arange(0, 2 * tokens, tokens, dtype=torch.int32, device=device)           # 0, tokens
+        if not self.is_kv_shared_layer:
+            k = k_post.view(tokens, self.num_kv_heads, self.head_dim)
+            v = v_states.view(tokens, self.num_kv_heads, self.head_dim)
+            kv8_append(cache, k, v, table, starts, first)
+        if tokens == 1:
+            state.dense_prompt_kv.pop(self.source_layer_idx, None)
+            kv8_decode_attention(q.view(1, 1, self.num_heads, self.head_dim), cache, table, first + 1,
+                                 sm_scale=self.scaling, softcap=self.attention_logits_soft_cap,
+                                 window=self.attention_window, out=out.view(1, 1, self.num_heads, self.head_dim))
+        else:
+            if int(positions[0].item()) != 0:
+                raise RuntimeError("the full prompt of a dense request must arrive in one call")
+            if self.is_kv_shared_layer:
+                if self.source_layer_idx not in state.dense_prompt_kv:
+                    raise RuntimeError(f"layer {self.layer_idx} shares the K/V of layer {self.source_layer_idx}, which "
+                                       "has not seen this prompt")
+                k, v = state.dense_prompt_kv[self.source_layer_idx]
+            else:
+                state.dense_prompt_kv[self.source_layer_idx] = (k, v)
+            dense_prefill_attention(q, k, v, cu_seqlens_q=starts, sm_scale=self.scaling,
+                                    softcap=self.attention_logits_soft_cap, window=self.attention_window, out=out)
+        _lib.status_for(device).poll()
+
     def attention_forward(self, positions, hidden_states, q_post, k_post, v_states, q_pre, k_pre, output) -> None:
         """The attention core, reached only through the operator; the result goes into ``output``."""
+        serves_dense = bool(self.runtime_config.dense_cache_bits)
+        if serves_dense and not self.uses_sparse_attention:
+            # the bookkeeping of a dense layer needs no host state, so that a caller may be capturing
+            if not torch.cuda.is_current_stream_capturing():
+                self.runtime_state.maybe_begin_prompt(self.layer_idx, positions,
+                                                      engage_above_tokens=self.runtime_config.engage_above_tokens)
+            self._dense_attention(positions, q_post, k_post, v_states, output)
+            return
         if _arena.full_graph_decode_enabled() and positions.numel() == 1:
             self._full_graph_decode_step(positions, q_post, k_post, v_states, q_pre, output, k_pre=k_pre)
             return
         self.runtime_state.maybe_begin_prompt(self.layer_idx, positions,
                                               engage_above_tokens=self.runtime_config.engage_above_tokens)
+        if self.runtime_state.dense_request and serves_dense:
+            self._dense_attention(positions, q_post, k_post, v_states, output)
+            return
         if self.runtime_state.dense_request or not self.uses_sparse_attention:
             raise RuntimeError("this layer serves the sparse path only: the stock attention of a dense request "
                                "stays with the model's own attention layer")

@@ -12,8 +12,10 @@ import torch
 
 from . import flat_index
 from ._lib import check, lib, ptr, require_cuda, stream_ptr
+from .kv8_cache import Kv8Cache
 
 _PACK_ALIGN = 256          # state.py:17
+DENSE_BLOCK = 256          # tokens per block of the dense requests' 8-bit cache
 HEAD_SEED_STRIDE = 1000003
 
 
@@ -287,6 +289,20 @@ class SembloRuntimeState:
         self.step_suffix_key = None
         self.step_suffix_tiles = None
         self.step_recorded_key = None
+        self.dense_prompt_kv: dict = {}          # of the running prompt, by source layer (for layers that share it)
+
+    # ---- 8-bit cache of the dense requests and layers ------------------------------------------
+    def dense_cache(self, layer_idx: int, *, num_kv_heads: int, head_dim: int, device):
+        """(cache, block table [1, blocks]) of one source layer for every position of a request: made on first
+        use and kept (the blocks of a new request are written anew, block by block)."""
+        blocks = -(-self.max_model_len // DENSE_BLOCK)
+        key, signature = ("dense", int(layer_idx)), (blocks, num_kv_heads, head_dim, torch.device(device))
+        held = self.index_buffers.get(key)
+        if held is None or held[0] != signature:
+            table = torch.arange(blocks, dtype=torch.int32, device=device).view(1, -1)
+            held = (signature, Kv8Cache.allocate(blocks, DENSE_BLOCK, num_kv_heads, head_dim, device), table)
+            self.index_buffers[key] = held
+        return held[1], held[2]
 
     # ---- the layers' own store of generated K/V (state.py:1239-1284 of the reference) ----------
     def ensure_suffix_store(self, layer_idx, *, prompt_length, max_model_len, num_kv_heads, head_dim, dtype,
