@@ -21,12 +21,12 @@ def _lib():
 @pytest.fixture
 def hostside(monkeypatch):
     """The operators' modules with the CUDA check removed and the library replaced: reaching it is a failure."""
-    from semblo_b200 import kv8_cache, rotary
+    from semblo_b200 import dense_prefill, kv8_cache, rotary
 
     def reached(*_):
         raise AssertionError("the call was not refused")
 
-    for m in (rotary, kv8_cache):
+    for m in (rotary, kv8_cache, dense_prefill):
         monkeypatch.setattr(m, "require_cuda", lambda *_: None)
         monkeypatch.setattr(m, "lib", reached)
     return rotary, kv8_cache
@@ -155,6 +155,90 @@ def test_kv8_cache_and_append_refusals(hostside):
     no(ValueError, x, x, table.to("meta"), cu, start)
 
 
+def test_decode_refusals(hostside):
+    _, kv8 = hostside
+    cache = kv8.Kv8Cache.allocate(4, 16, 2, 64, "cpu")
+    q = torch.zeros(3, 1, 4, 64, dtype=torch.bfloat16)
+    table, lens = torch.zeros(3, 2, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+
+    def no(exc, q=q, table=table, lens=lens, **kw):
+        with pytest.raises(exc):
+            kv8.kv8_decode_attention(q, cache, table, lens, **{"sm_scale": 0.1, **kw})
+
+    no(ValueError, q=q[0])
+    no(ValueError, q=q.float())
+    no(ValueError, q=torch.zeros(3, 1, 4, 128, dtype=torch.bfloat16))
+    no(ValueError, q=torch.zeros(3, 1, 3, 64, dtype=torch.bfloat16))
+    no(ValueError, q=torch.zeros(3, 1, 0, 64, dtype=torch.bfloat16))
+    no(ValueError, q=torch.zeros(3, 17, 4, 64, dtype=torch.bfloat16))
+    no(ValueError, q=torch.zeros(3, 0, 4, 64, dtype=torch.bfloat16))
+    no(ValueError, table=table[:2])
+    no(ValueError, table=table[0])
+    no(ValueError, lens=lens[:2])
+    no(ValueError, lens=lens.float())
+    no(ValueError, lens=lens.to("meta"))
+    no(ValueError, window=-1)
+    no(ValueError, softcap=-1.0)
+    no(ValueError, softcap=math.inf)
+    no(ValueError, softcap=math.nan)
+    no(ValueError, prefix_lens=lens[:2])
+    no(ValueError, prefix_lens=lens.to("meta"))
+    no(ValueError, alibi_slopes=torch.zeros(3))
+    no(ValueError, alibi_slopes=torch.zeros(4, dtype=torch.float64))
+    no(ValueError, out=torch.zeros(3, 1, 4, 64))
+    no(ValueError, out=torch.zeros(3, 1, 64, 4, dtype=torch.bfloat16).transpose(2, 3))
+    no(RuntimeError, q=q.clone().requires_grad_())
+
+
+def test_dense_prefill_refusals(hostside):
+    from semblo_b200 import dense_prefill
+    q, k = torch.zeros(5, 4, 64, dtype=torch.float16), torch.zeros(7, 2, 64, dtype=torch.float16)
+    cu = torch.tensor([0, 5], dtype=torch.int32)
+
+    def no(exc, q=q, k=k, v=None, **kw):
+        with pytest.raises(exc):
+            dense_prefill.dense_prefill_attention(q, k, k if v is None else v,
+                                                  **{"cu_seqlens_q": cu, "sm_scale": 0.1, **kw})
+
+    no(ValueError, q=q[0])
+    no(ValueError, v=k[:6])
+    no(ValueError, q=q.float())
+    no(ValueError, k=k.bfloat16())
+    no(ValueError, v=k.bfloat16())
+    no(ValueError, q=torch.zeros(5, 4, 128, dtype=torch.float16))
+    no(ValueError, q=torch.zeros(5, 4, 96, dtype=torch.float16), k=torch.zeros(7, 2, 96, dtype=torch.float16))
+    no(ValueError, q=torch.zeros(5, 3, 64, dtype=torch.float16))
+    no(ValueError, q=torch.zeros(5, 258, 64, dtype=torch.float16))
+    no(ValueError, cu_seqlens_q=cu[None])
+    no(ValueError, cu_seqlens_q=cu.float())
+    no(ValueError, cu_seqlens_q=cu[:0])
+    no(ValueError, cu_seqlens_q=cu.to("meta"))
+    no(ValueError, cu_seqlens_k=torch.tensor([0, 5, 7]))
+    no(ValueError, cu_seqlens_k=cu.to("meta"))
+    no(ValueError, sm_scale=0.0)
+    no(ValueError, sm_scale=-1.0)
+    no(ValueError, sm_scale=math.nan)
+    no(ValueError, window=-2)
+    no(ValueError, softcap=-2.0)
+    no(ValueError, causal=False, window=3)
+    no(ValueError, causal=False, prefix_lens=torch.tensor([1]))
+    no(ValueError, prefix_lens=torch.tensor([1, 2]))
+    no(ValueError, alibi_slopes=torch.zeros(2))
+    no(ValueError, out=torch.zeros(5, 4, 64))
+    no(ValueError, out=torch.zeros(6, 4, 64, dtype=torch.float16)[:5, :, ::1].transpose(0, 1))
+    no(RuntimeError, k=k.clone().requires_grad_())
+
+
+def test_token_rows_are_copied_where_a_kernel_cannot_read_them():
+    from semblo_b200.kv8_cache import _token_rows
+    x = torch.zeros(6, 4, 64, dtype=torch.bfloat16)
+    assert _token_rows(x) is x and _token_rows(x[:, 1:3]).data_ptr() == x[:, 1:3].data_ptr()
+    for y in (torch.zeros(6, 4, 65, dtype=torch.bfloat16)[..., 1:], x.transpose(1, 2).contiguous().transpose(1, 2),
+              x[:1].expand(6, 4, 64), x[:, :1].expand(6, 4, 64)):
+        z = _token_rows(y)
+        assert z.is_contiguous() and z.shape == y.shape and z.data_ptr() != y.data_ptr()
+
+
 def test_c_entries_refuse():
     lib = _lib()
     p = ctypes.c_void_p(256)
@@ -177,3 +261,31 @@ def test_c_entries_refuse():
                dict(k=ctypes.c_void_p(264)), dict(stride=60), dict(table=None), dict(status=None), dict(code=1),
                dict(tokens=-1)):
         assert append(**kw) == -1, kw
+
+    def decode(dtype=0, batch=1, queries=1, hq=2, hkv=1, dim=64, block=16, width=4, q=p, cache=p, softcap=0.0, window=0,
+               ws=None, nbytes=0):
+        return lib.semblo_kv8_decode(q, dtype, batch, queries, hq, hkv, dim, cache, p, 4, block, p, width, width, p, None,
+                                     window, 0.1, softcap, None, p, None, ws, nbytes, p, None)
+
+    assert decode(batch=0) == 0
+    for kw in (dict(dtype=1), dict(queries=0), dict(queries=17), dict(hq=3, hkv=2), dict(hq=0), dict(dim=96), dict(block=8),
+               dict(q=None), dict(cache=None), dict(q=ctypes.c_void_p(264)), dict(softcap=-1.0), dict(window=-1),
+               dict(batch=5000), dict(batch=-1), dict(batch=4096, hkv=8, hq=8, width=1 << 20)):
+        assert decode(**kw) == -1, kw
+    long_table = dict(width=4096)                                # a workspace is needed, and none is given
+    assert lib.semblo_kv8_decode_workspace_bytes(1, 1, 2, 1, 64, 16, 4096, 0, 0) > 0
+    assert decode(**long_table) == -3
+    assert lib.semblo_kv8_decode_workspace_bytes(1, 1, 2, 1, 64, 16, 4, 0, 0) == 0
+    assert lib.semblo_kv8_decode_workspace_bytes(1, 1, 2, 1, 64, 16, 4096, 100, 0) == 0       # a window bounds the work
+    assert lib.semblo_kv8_decode_workspace_bytes(1, 1, 3, 2, 64, 16, 4096, 0, 0) == -1
+
+    def prefill(q=p, k=p, v=p, tq=4, tk=4, hq=2, hkv=1, dim=64, dtype=0, cu=p, docs=1, causal=1, window=0, prefix=None,
+                sm=0.1, cap=0.0, out=p, stride=64, status=p):
+        return lib.semblo_dense_prefill(q, stride, 64, k, 64, 64, v, 64, 64, tq, tk, hq, hkv, dim, dtype, cu, cu, docs, causal,
+                                        window, prefix, sm, cap, None, out, 0, None, status, None)
+
+    assert prefill(tq=0) == 0 and prefill(docs=0) == 0
+    for kw in (dict(dim=80), dict(hq=3, hkv=2), dict(hq=129), dict(dtype=1), dict(tq=-1), dict(window=-1), dict(cap=-1.0),
+               dict(sm=0.0), dict(causal=0, window=4), dict(causal=0, prefix=p), dict(q=None), dict(k=None), dict(out=None),
+               dict(cu=None), dict(status=None), dict(q=ctypes.c_void_p(264)), dict(stride=60)):
+        assert prefill(**kw) == -1, kw
