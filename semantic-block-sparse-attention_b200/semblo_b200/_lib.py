@@ -136,9 +136,11 @@ def require_same_device(*tensors: torch.Tensor | None) -> None:
 
 
 def refuse_gradients(*tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("this operator serves inference and has no gradient: call it under torch.no_grad() or on "
-                           "tensors that require none")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("this operator serves inference and has no gradient: call it under torch.no_grad() "
+                                   "or on tensors that require none")
 
 
 def raw_stream(index: int) -> int:
@@ -148,7 +150,7 @@ def raw_stream(index: int) -> int:
 
 def device_scope(device: torch.device):
     """Make ``device`` current for a call, so that its launches and stream are that device's."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index == torch._C._cuda_getDevice():
         return _NO_SCOPE
     return torch.cuda.device(device)
 

@@ -105,7 +105,7 @@ def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, block_table: t
     k, v = _token_rows(k), _token_rows(v)
     with device_scope(k.device):
         check(lib().semblo_kv8_append(
-            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), shape[0],
+            k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2], shape[0],
             dtype_code(k.dtype, "append"), cache.data.data_ptr(), cache.scales.data_ptr(), cache.num_blocks,
             cache.block_size, cache.num_kv_heads, cache.head_dim, table.data_ptr(), table.stride(0), table.shape[1],
             cu.data_ptr(), start.data_ptr(), batch, _lib.status_for(k.device).word.data_ptr(),

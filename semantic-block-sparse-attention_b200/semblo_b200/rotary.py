@@ -95,15 +95,18 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: dict 
     return RotaryFrequencies(inv.to(device), scale)
 
 
-def _check_rows(name: str, x: torch.Tensor, tokens: int, dim: int, dtype, device) -> None:
-    if x.ndim != 3 or x.shape[0] != tokens or x.shape[2] != dim:
-        raise ValueError(f"{name} must have shape [{tokens}, heads, {dim}] (got {tuple(x.shape)})")
-    if x.stride(2) != 1 and dim > 1:
+def _check_rows(name: str, x: torch.Tensor, tokens: int, dim: int, dtype, device) -> tuple:
+    """The strides of x [tokens, heads, dim]."""
+    shape, strides = x.shape, x.stride()
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != dim:
+        raise ValueError(f"{name} must have shape [{tokens}, heads, {dim}] (got {tuple(shape)})")
+    if strides[2] != 1 and dim > 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
     if x.dtype != dtype:
         raise ValueError("q_pre, k_pre and the outputs must have one dtype")
     if x.device != device:
         raise ValueError(f"the tensors of a call must be on one device ({name} is on {x.device}, q_pre on {device})")
+    return strides
 
 
 def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -116,13 +119,13 @@ def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
-def _check_output(name: str, y: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
-    _check_rows(name, y, x.shape[0], x.shape[2], x.dtype, x.device)
+def _check_output(name: str, y: torch.Tensor, x: torch.Tensor) -> tuple:
+    strides = _check_rows(name, y, x.shape[0], x.shape[2], x.dtype, x.device)
     if y.shape != x.shape:
         raise ValueError(f"{name} must have the shape of its input")
     if _overlaps(x, y) and (x.data_ptr() != y.data_ptr() or x.stride() != y.stride()):
         raise ValueError(f"{name} overlaps its input without being it")
-    return y
+    return strides
 
 
 def apply_rotary(q_pre: torch.Tensor, k_pre: torch.Tensor | None, positions: torch.Tensor,
@@ -142,7 +145,7 @@ def apply_rotary(q_pre: torch.Tensor, k_pre: torch.Tensor | None, positions: tor
     tokens, hq, dim = q_pre.shape
     dtype, device = q_pre.dtype, q_pre.device
     code = dtype_code(dtype, "rotary")
-    _check_rows("q_pre", q_pre, tokens, dim, dtype, device)
+    qs = _check_rows("q_pre", q_pre, tokens, dim, dtype, device)
     if positions.ndim != 1 or positions.shape[0] != tokens or positions.dtype not in (torch.int32, torch.int64):
         raise ValueError("positions must be one int32 or int64 per token")
     inv_freq = frequencies.inv_freq
@@ -152,25 +155,28 @@ def apply_rotary(q_pre: torch.Tensor, k_pre: torch.Tensor | None, positions: tor
     if positions.device != device or inv_freq.device != device:
         raise ValueError(f"the positions ({positions.device}) and frequencies ({inv_freq.device}) must be on the "
                          f"device of q_pre ({device})")
-    q_out = torch.empty((tokens, hq, dim), dtype=dtype, device=device) if q_out is None else \
-        _check_output("q_out", q_out, q_pre)
+    if q_out is None:
+        q_out, qos = torch.empty((tokens, hq, dim), dtype=dtype, device=device), (hq * dim, dim)
+    else:
+        qos = _check_output("q_out", q_out, q_pre)
     hkv, k_args = 0, (None, 0, 0, None, 0, 0, 0)
     if k_pre is None:
         if k_out is not None:
             raise ValueError("k_out is given without k_pre")
     else:
-        _check_rows("k_pre", k_pre, tokens, dim, dtype, device)
+        ks = _check_rows("k_pre", k_pre, tokens, dim, dtype, device)
         hkv = k_pre.shape[1]
-        k_out = torch.empty((tokens, hkv, dim), dtype=dtype, device=device) if k_out is None else \
-            _check_output("k_out", k_out, k_pre)
+        if k_out is None:
+            k_out, kos = torch.empty((tokens, hkv, dim), dtype=dtype, device=device), (hkv * dim, dim)
+        else:
+            kos = _check_output("k_out", k_out, k_pre)
         if hkv:
-            k_args = (k_pre.data_ptr(), k_pre.stride(0), k_pre.stride(1), k_out.data_ptr(), k_out.stride(0),
-                      k_out.stride(1), hkv)
+            k_args = (k_pre.data_ptr(), ks[0], ks[1], k_out.data_ptr(), kos[0], kos[1], hkv)
     if not positions.is_contiguous():
         positions = positions.contiguous()
     with device_scope(device):
         check(lib().semblo_rotary(
-            q_pre.data_ptr(), q_pre.stride(0), q_pre.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1), hq,
+            q_pre.data_ptr(), qs[0], qs[1], q_out.data_ptr(), qos[0], qos[1], hq,
             *k_args, tokens, dim, rotary_dim, code, positions.data_ptr(), positions.dtype == torch.int64,
             inv_freq.data_ptr(), frequencies.attention_scale, interleaved, inverse, raw_stream(device.index)))
     return q_out, k_out
