@@ -12,7 +12,10 @@
 // (cache block, head, K or V): no atomics, the same bytes on every run.
 //
 // Bound: HBM, 2 bytes read and 1 written per value.  The maximum is needed before the first code, so a
-// thread holds its share of the block in registers between the two steps and the input is read once.
+// thread holds its share of the block in registers between the two steps and the input is read once.  A few
+// tokens take one thread block per cache block (kv8_append_kernel); a prompt's blocks are a stream
+// (kv8_stream_kernel): while a group of threads works on one block from registers, the next one's rows travel
+// into shared memory (131072 tokens x 4 heads x 256: 166 us without that overlap).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -35,7 +38,7 @@ struct AppendArgs {
   float* scales;
   int64_t cache_blocks;
   int block_log2;
-  int num_kv_heads, head_dim, col_log2; // 16-value columns of a row, a power of two
+  int num_kv_heads, head_dim, col_log2; // 8-value columns of a row, a power of two
   const int32_t* table;
   int64_t table_stride;
   int table_len;
@@ -83,17 +86,23 @@ __device__ __forceinline__ float block_max(float v, uint32_t* slots) {
   return __uint_as_float(m);
 }
 
-// T2: the packed pair type of the input.  NL: 16-value pieces of the cache block per thread.
-template <typename T2, int NL>
-__global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs a) {
-  __shared__ uint32_t slots[16];
+// One cache block of one head that a call writes: rows [off, off + m) of it, from token row `row`.
+struct Unit {
+  bool have;
+  int off, m;
+  int64_t row;
+  int64_t page;                          // -1: not in the pool or the table
+};
+
+// Cache block number `want` (0 ...) of the call, requests in order; warp-collective.  A caller that asks with
+// rising numbers passes the same Cursor again.
+struct Cursor { int request, before; };  // before: cache blocks of the requests in front of it
+__device__ __forceinline__ Unit find_unit(const AppendArgs& a, int64_t want, Cursor& from) {
   const int lane = threadIdx.x & 31;
   const int block = 1 << a.block_log2;
-  const int piece0 = threadIdx.x, piece_step = blockDim.x;
-  // ---- which request and cache block: every warp walks the requests, 32 at a time
-  int want = (int)blockIdx.x, seq = -1, n = 0, start = 0, nth = 0;
-  int64_t row0 = 0;
-  for (int b0 = 0; b0 < a.batch && seq < 0; b0 += 32) {
+  Unit u{};
+  int64_t rest = want - from.before;
+  for (int b0 = from.request; b0 < a.batch; b0 += 32) {
     const int b = b0 + lane;
     int bn = 0, bs = 0, blocks = 0;
     int64_t c0 = 0;
@@ -103,7 +112,7 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs a) {
       bs = a.start[b];
       bn = c0 < 0 ? 0 : (int)max((int64_t)0, c1 - c0);
       if (bn > 0 && bs < 0) {
-        if (blockIdx.x == 0 && threadIdx.x == lane) atomicCAS(a.status, 0, sm100::STATUS_OVERFLOW);
+        atomicCAS(a.status, 0, sm100::STATUS_OVERFLOW);
         bn = 0;
       }
       if (bn > 0) blocks = (int)(((int64_t)bs + bn - 1) >> a.block_log2) - (bs >> a.block_log2) + 1;
@@ -115,114 +124,110 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs a) {
       if (lane >= o) upto += t;
     }
     const int total = __shfl_sync(0xffffffffu, upto, 31);
-    if (want < total) {
-      const uint32_t above = __ballot_sync(0xffffffffu, upto > want);
-      const int at = __ffs(above) - 1;
-      seq = b0 + at;
-      nth = want - __shfl_sync(0xffffffffu, upto - blocks, at);
-      n = __shfl_sync(0xffffffffu, bn, at);
-      start = __shfl_sync(0xffffffffu, bs, at);
-      row0 = __shfl_sync(0xffffffffu, c0, at);
-    } else {
-      want -= total;
+    if (rest < total) {
+      const int at = __ffs(__ballot_sync(0xffffffffu, upto > rest)) - 1;
+      const int ahead = __shfl_sync(0xffffffffu, upto - blocks, at);
+      const int nth = (int)rest - ahead;
+      const int n = __shfl_sync(0xffffffffu, bn, at), start = __shfl_sync(0xffffffffu, bs, at);
+      const int64_t row0 = __shfl_sync(0xffffffffu, c0, at);
+      const int slot = (start >> a.block_log2) + nth;
+      u.have = true;
+      u.off = nth == 0 ? start & (block - 1) : 0;
+      const int64_t pos0 = ((int64_t)slot << a.block_log2) + u.off;
+      u.m = (int)min((int64_t)(block - u.off), (int64_t)start + n - pos0);
+      u.row = row0 + pos0 - start;
+      u.page = slot < a.table_len ? a.table[(int64_t)(b0 + at) * a.table_stride + slot] : -1;
+      if (u.page >= a.cache_blocks) u.page = -1;
+      from.before = (int)(want - nth);
+      from.request = b0 + at;
+      return u;
     }
+    rest -= total;
   }
-  if (seq < 0) return;                                // the grid covers the largest possible number of blocks
-  const int slot = (start >> a.block_log2) + nth;
-  const int off = nth == 0 ? start & (block - 1) : 0;
-  const int64_t pos0 = ((int64_t)slot << a.block_log2) + off;
-  const int m = (int)min((int64_t)(block - off), (int64_t)start + n - pos0);
-  const int64_t page = slot < a.table_len ? a.table[seq * a.table_stride + slot] : -1;
-  const int h = blockIdx.y, part = blockIdx.z;
-  const uint16_t* src = static_cast<const uint16_t*>(a.src[part]) + (row0 + pos0 - start) * a.src_token[part] +
-                        (int64_t)h * a.src_head[part];
-  // ---- the new rows into registers, their largest magnitude
-  const int pieces = m << a.col_log2, colmask = (1 << a.col_log2) - 1;
-  uint4 x[NL][2];
-#pragma unroll
-  for (int i = 0; i < NL; ++i) {
-    const int p = i * piece_step + piece0;
-    x[i][0] = x[i][1] = make_uint4(0u, 0u, 0u, 0u);
-    if (p < pieces) {
-      const uint4* s = reinterpret_cast<const uint4*>(src + (int64_t)(p >> a.col_log2) * a.src_token[part] +
-                                                      (p & colmask) * 16);
-      x[i][0] = __ldg(s);
-      x[i][1] = __ldg(s + 1);
-    }
-  }
-  if (page < 0 || page >= a.cache_blocks) {
-    if (threadIdx.x == 0) atomicCAS(a.status, 0, sm100::STATUS_OVERFLOW);
-    return;
-  }
-  const int64_t cell = ((int64_t)part * a.cache_blocks + page) * a.num_kv_heads + h;
-  uint8_t* dst = a.data + (cell << a.block_log2) * a.head_dim;
-  const float before = off ? a.scales[cell] : 0.f;
+  return u;                              // behind the last one
+}
+
+// 2^e * 256 <= largest < 2^e * 512 with 448 as the limit: the exponent of the scale a block needs.
+__device__ __forceinline__ int exponent_for(float largest) {
+  const uint32_t bits = __float_as_uint(largest);
+  int e = (int)(bits >> 23) - 127 - 8;
+  if (__uint_as_float((bits & 0x7fffffu) | 0x3f800000u) > E4M3_MAX_MANTISSA) ++e;
+  return min(max(e, -100), 120);
+}
+
+template <typename T2, int NL>
+__device__ __forceinline__ float largest_of(const uint4 (&x)[NL]) {
   T2 top2;
   *reinterpret_cast<uint32_t*>(&top2) = 0u;
 #pragma unroll
   for (int i = 0; i < NL; ++i)
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      const uint4& q = x[i][w >> 2];
-      uint32_t u = (w & 3) == 0 ? q.x : (w & 3) == 1 ? q.y : (w & 3) == 2 ? q.z : q.w;
+    for (int w = 0; w < 4; ++w) {
+      const uint4& q = x[i];
+      uint32_t u = w == 0 ? q.x : w == 1 ? q.y : w == 2 ? q.z : q.w;
       top2 = __hmax2(top2, __habs2(*reinterpret_cast<T2*>(&u)));
     }
   const float2 t2 = widen<T2>(*reinterpret_cast<uint32_t*>(&top2));
-  float amax = block_max(fmaxf(t2.x, t2.y), slots);
-  if (!(amax <= 3.4e38f)) {
-    // infinities saturate and NaN stay NaN, but neither sets the scale of the others
-    float f = 0.f;
+  return fmaxf(t2.x, t2.y);
+}
+
+// The same without infinities and NaN: they saturate and stay, but do not set the scale of the others.
+template <typename T2, int NL>
+__device__ __forceinline__ float largest_finite_of(const uint4 (&x)[NL]) {
+  float f = 0.f;
 #pragma unroll
-    for (int i = 0; i < NL; ++i)
+  for (int i = 0; i < NL; ++i)
 #pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        const uint4& q = x[i][w >> 2];
-        const float2 v = widen<T2>((w & 3) == 0 ? q.x : (w & 3) == 1 ? q.y : (w & 3) == 2 ? q.z : q.w);
-        if (fabsf(v.x) <= 3.4e38f) f = fmaxf(f, fabsf(v.x));
-        if (fabsf(v.y) <= 3.4e38f) f = fmaxf(f, fabsf(v.y));
-      }
-    amax = block_max(f, slots);
-  }
-  const uint32_t bits = __float_as_uint(amax);
-  int e = (int)(bits >> 23) - 127 - 8;                // 2^e * 256 <= max < 2^e * 512
-  if (__uint_as_float((bits & 0x7fffffu) | 0x3f800000u) > E4M3_MAX_MANTISSA) ++e;
-  e = min(max(e, -100), 120);
-  float scale = pow2(e);
-  if (off) {
+    for (int w = 0; w < 4; ++w) {
+      const uint4& q = x[i];
+      const float2 v = widen<T2>(w == 0 ? q.x : w == 1 ? q.y : w == 2 ? q.z : q.w);
+      if (fabsf(v.x) <= 3.4e38f) f = fmaxf(f, fabsf(v.x));
+      if (fabsf(v.y) <= 3.4e38f) f = fmaxf(f, fabsf(v.y));
+    }
+  return f;
+}
+
+// Scale, earlier rows and codes of one unit, by `threads` threads of which this is number `tid`; x are its
+// pieces tid, tid + threads, ... of the new rows and `largest` their largest magnitude over the unit.
+template <typename T2, int NL>
+__device__ __forceinline__ void write_unit(const AppendArgs& a, const Unit& u, int64_t cell, float before, float largest,
+                                           const uint4 (&x)[NL], int tid, int threads) {
+  uint8_t* dst = a.data + (cell << a.block_log2) * a.head_dim;
+  float scale = pow2(exponent_for(largest));
+  if (u.off) {
     if (before >= scale) {
       scale = before;
     } else {
       // the rows of earlier calls follow the new scale
       const float ratio = before / scale;
       uint4* rows = reinterpret_cast<uint4*>(dst);
-      const int held = off << a.col_log2;
-      for (int p = piece0; p < held; p += 4 * piece_step) {
+      const int held = u.off << (a.col_log2 - 1);
+      for (int p = tid; p < held; p += 4 * threads) {
         uint4 v[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (p + u * piece_step < held) v[u] = rows[p + u * piece_step];
+        for (int i = 0; i < 4; ++i)
+          if (p + i * threads < held) v[i] = rows[p + i * threads];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (p + u * piece_step >= held) break;
-          rows[p + u * piece_step] = make_uint4(recode4(v[u].x, ratio), recode4(v[u].y, ratio),
-                                                recode4(v[u].z, ratio), recode4(v[u].w, ratio));
+        for (int i = 0; i < 4; ++i) {
+          if (p + i * threads >= held) break;
+          rows[p + i * threads] = make_uint4(recode4(v[i].x, ratio), recode4(v[i].y, ratio), recode4(v[i].z, ratio),
+                                             recode4(v[i].w, ratio));
         }
       }
     }
   }
-  if (threadIdx.x == 0) a.scales[cell] = scale;
-  // ---- the codes
+  if (tid == 0) a.scales[cell] = scale;
+  const int pieces = u.m << a.col_log2;
   const bool exact_inverse = (__float_as_uint(scale) & 0x7fffffu) == 0 && scale >= pow2(-126) && scale <= pow2(126);
   const float inv = exact_inverse ? __int_as_float((254 << 23) - __float_as_int(scale)) : 0.f;
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
-    const int p = i * piece_step + piece0;
+    const int p = i * threads + tid;
     if (p >= pieces) break;
-    uint32_t out[4];
+    uint32_t out[2];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const uint4& q = x[i][w >> 1];
-      float2 f0 = widen<T2>((w & 1) ? q.z : q.x), f1 = widen<T2>((w & 1) ? q.w : q.y);
+    for (int w = 0; w < 2; ++w) {
+      float2 f0 = widen<T2>(w ? x[i].z : x[i].x), f1 = widen<T2>(w ? x[i].w : x[i].y);
       if (exact_inverse) {
         f0.x *= inv; f0.y *= inv; f1.x *= inv; f1.y *= inv;
       } else {                                        // a scale set by the caller: divided as written
@@ -230,8 +235,123 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs a) {
       }
       out[w] = code4(f0, f1);
     }
-    reinterpret_cast<uint4*>(dst)[(off << a.col_log2) + p] = make_uint4(out[0], out[1], out[2], out[3]);
+    reinterpret_cast<uint2*>(dst)[(u.off << a.col_log2) + p] = make_uint2(out[0], out[1]);
   }
+}
+
+// T2: the packed pair type of the input.  NL: 8-value pieces of the cache block per thread.
+template <typename T2, int NL>
+__global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs a) {
+  __shared__ uint32_t slots[16];
+  const int h = blockIdx.y, part = blockIdx.z;
+  Cursor cursor{0, 0};
+  const Unit u = find_unit(a, blockIdx.x, cursor);
+  if (!u.have) return;                                // the grid covers the largest possible number of blocks
+  const uint16_t* src = static_cast<const uint16_t*>(a.src[part]) + u.row * a.src_token[part] + (int64_t)h * a.src_head[part];
+  // ---- the new rows into registers, their largest magnitude
+  const int pieces = u.m << a.col_log2, colmask = (1 << a.col_log2) - 1;
+  uint4 x[NL];
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int p = i * blockDim.x + threadIdx.x;
+    x[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (p < pieces)
+      x[i] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)(p >> a.col_log2) * a.src_token[part] + (p & colmask) * 8));
+  }
+  if (u.page < 0) {
+    if (threadIdx.x == 0) atomicCAS(a.status, 0, sm100::STATUS_OVERFLOW);
+    return;
+  }
+  const int64_t cell = ((int64_t)part * a.cache_blocks + u.page) * a.num_kv_heads + h;
+  const float before = u.off ? a.scales[cell] : 0.f;
+  float largest = block_max(largest_of<T2, NL>(x), slots);
+  if (!(largest <= 3.4e38f)) largest = block_max(largest_finite_of<T2, NL>(x), slots);
+  write_unit<T2, NL>(a, u, cell, before, largest, x, threadIdx.x, blockDim.x);
+}
+
+// A stream of cache blocks: GROUP threads take one (cache block, head, part) after the other, NL pieces a thread.
+// A thread copies (cp.async) exactly the pieces that it reads back, so the shared memory needs no barrier.
+constexpr int STREAM_THREADS = 512;
+template <typename T2, int NL, int GROUP>
+__global__ void __launch_bounds__(STREAM_THREADS, NL == 4 ? 2 : 1) kv8_stream_kernel(const AppendArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];    // [NL][STREAM_THREADS] 16-byte pieces, then the maxima
+  constexpr int GROUPS = STREAM_THREADS / GROUP;
+  uint32_t* slots = reinterpret_cast<uint32_t*>(smem + NL * STREAM_THREADS * 16);
+  const int group = threadIdx.x / GROUP, tid = threadIdx.x % GROUP;
+  const int colmask = (1 << a.col_log2) - 1;
+  const uint32_t mine = sm100::smem_u32(smem) + threadIdx.x * 16;
+  const int heads2 = 2 * a.num_kv_heads;
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+
+  auto group_max = [&](float v) {
+    uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
+    if constexpr (GROUP > 32) {
+      if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = b;
+      asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(GROUP) : "memory");
+      b = 0;
+#pragma unroll
+      for (int i = 0; i < GROUP / 32; ++i) b = max(b, slots[group * (GROUP / 32) + i]);
+      asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(GROUP) : "memory");
+    }
+    return __uint_as_float(b);
+  };
+  auto request = [&](const Unit& u, int h, int part) {        // the new rows of a unit on their way
+    if (u.have && u.page >= 0) {
+      const uint16_t* src = static_cast<const uint16_t*>(a.src[part]) + u.row * a.src_token[part] + (int64_t)h * a.src_head[part];
+      const int pieces = u.m << a.col_log2;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int p = i * GROUP + tid;
+        const bool in = p < pieces;
+        const uint16_t* s = in ? src + (int64_t)(p >> a.col_log2) * a.src_token[part] + (p & colmask) * 8 : src;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mine + i * STREAM_THREADS * 16), "l"(s),
+                     "r"(in ? 16 : 0)
+                     : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+
+  Cursor cursor{0, 0};
+  int64_t n = (int64_t)blockIdx.x * GROUPS + group;
+  auto look = [&](int64_t i) { return find_unit(a, i / heads2, cursor); };
+  Unit next = look(n);
+  int h = (int)(n % heads2) >> 1, part = (int)(n & 1);
+  request(next, h, part);
+  while (next.have) {
+    const Unit u = next;
+    const int64_t cell = ((int64_t)part * a.cache_blocks + max(u.page, (int64_t)0)) * a.num_kv_heads + h;
+    const float before = u.off && u.page >= 0 ? a.scales[cell] : 0.f;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    uint4 x[NL];
+#pragma unroll
+    for (int i = 0; i < NL; ++i) x[i] = *reinterpret_cast<const uint4*>(smem + i * STREAM_THREADS * 16 + threadIdx.x * 16);
+    const float own = largest_of<T2, NL>(x);          // every piece is in its register before its place is reused
+    n += step;
+    next = look(n);
+    h = (int)(n % heads2) >> 1;
+    part = (int)(n & 1);
+    request(next, h, part);
+    float largest = group_max(own);
+    if (u.page < 0) {
+      if (tid == 0) atomicCAS(a.status, 0, sm100::STATUS_OVERFLOW);
+      continue;
+    }
+    if (!(largest <= 3.4e38f)) largest = group_max(largest_finite_of<T2, NL>(x));
+    write_unit<T2, NL>(a, u, cell, before, largest, x, tid, GROUP);
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+template <typename T2, int NL, int GROUP>
+int launch_stream(const AppendArgs& a, int64_t units, cudaStream_t st) {
+  auto kern = kv8_stream_kernel<T2, NL, GROUP>;
+  const int smem = NL * STREAM_THREADS * 16 + STREAM_THREADS / 32 * 4;
+  SEMBLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int64_t blocks = std::min<int64_t>(ceil_div(units, STREAM_THREADS / GROUP), (int64_t)semblo::sm_count() * (NL == 4 ? 2 : 1));
+  kern<<<(unsigned)blocks, STREAM_THREADS, smem, st>>>(a);
+  SEMBLO_LAUNCH_CHECK();
+  return 0;
 }
 
 template <typename T2>
@@ -240,16 +360,30 @@ int launch(AppendArgs& a, cudaStream_t st) {
   const int64_t most = std::min<int64_t>(a.tokens, a.tokens / block + 2 * (int64_t)a.batch);
   const int64_t rows = std::min<int64_t>(block, a.tokens);        // new rows that a block can hold
   const int64_t pieces = rows << a.col_log2, held = block << a.col_log2;
-  // 256 threads where the new rows fill them, or a continued block may have to be rounded again; 512 of 8
-  // pieces for the largest blocks (128 KB of input)
-  int64_t threads = std::min<int64_t>(256, std::max<int64_t>(64, held));
-  if (pieces > 2048) threads = 512;
-  const int64_t per_thread = ceil_div(pieces, threads);
+  // enough new rows for every group of threads to overlap one cache block with the next: a stream
+  const int64_t units = ceil_div(a.tokens, block) * a.num_kv_heads * 2;
+  const int64_t per_thread = held <= 128 ? 4 : held <= 256 ? 8 : 16;
+  const int64_t groups = (int64_t)semblo::sm_count() * STREAM_THREADS * (per_thread == 4 ? 2 : 1) / std::max<int64_t>(32, held / 16);
+  if (units >= 2 * groups) {
+    if (held <= 128) return launch_stream<T2, 4, 32>(a, units, st);
+    if (held <= 256) return launch_stream<T2, 8, 32>(a, units, st);
+    if (held <= 512) return launch_stream<T2, 16, 32>(a, units, st);
+    if (held <= 1024) return launch_stream<T2, 16, 64>(a, units, st);
+    if (held <= 2048) return launch_stream<T2, 16, 128>(a, units, st);
+    if (held <= 4096) return launch_stream<T2, 16, 256>(a, units, st);
+    return launch_stream<T2, 16, 512>(a, units, st);
+  }
+  // 256 threads where the new rows fill them, or a continued block may have to be rounded again; 512 for the
+  // largest blocks (128 KB of input)
+  int64_t threads = std::min<int64_t>(256, std::max<int64_t>(64, held / 2));
+  if (pieces > 4096) threads = 512;
+  const int64_t nl = ceil_div(pieces, threads);
   dim3 grid((unsigned)most, (unsigned)a.num_kv_heads, 2);
-  if (per_thread <= 1) kv8_append_kernel<T2, 1><<<grid, (unsigned)threads, 0, st>>>(a);
-  else if (per_thread <= 2) kv8_append_kernel<T2, 2><<<grid, (unsigned)threads, 0, st>>>(a);
-  else if (per_thread <= 4) kv8_append_kernel<T2, 4><<<grid, (unsigned)threads, 0, st>>>(a);
-  else kv8_append_kernel<T2, 8><<<grid, (unsigned)threads, 0, st>>>(a);
+  if (nl <= 1) kv8_append_kernel<T2, 1><<<grid, (unsigned)threads, 0, st>>>(a);
+  else if (nl <= 2) kv8_append_kernel<T2, 2><<<grid, (unsigned)threads, 0, st>>>(a);
+  else if (nl <= 4) kv8_append_kernel<T2, 4><<<grid, (unsigned)threads, 0, st>>>(a);
+  else if (nl <= 8) kv8_append_kernel<T2, 8><<<grid, (unsigned)threads, 0, st>>>(a);
+  else kv8_append_kernel<T2, 16><<<grid, (unsigned)threads, 0, st>>>(a);
   SEMBLO_LAUNCH_CHECK();
   return 0;
 }
@@ -284,7 +418,7 @@ extern "C" int semblo_kv8_append(const void* k, int64_t k_token_stride, int64_t 
   a.scales = scales;
   a.cache_blocks = cache_blocks;
   while ((1 << a.block_log2) < block_size) ++a.block_log2;
-  while ((16 << a.col_log2) < head_dim) ++a.col_log2;
+  while ((8 << a.col_log2) < head_dim) ++a.col_log2;
   a.num_kv_heads = num_kv_heads; a.head_dim = head_dim;
   a.table = block_table; a.table_stride = table_stride; a.table_len = table_len;
   a.cu = cu_seqlens; a.start = start_positions; a.batch = batch;

@@ -107,6 +107,74 @@ def test_many_requests(dev):
     _run_and_compare(*_case(dev, 5, 32, 1, 64, torch.bfloat16, new, past), 32)
 
 
+@pytest.mark.parametrize("block,dim,tokens", [(16, 64, 60000), (16, 128, 40000), (32, 128, 40000), (64, 128, 40000),
+                                              (128, 128, 60000), (128, 256, 90000), (256, 256, 90000)])
+def test_a_prompt_as_a_stream(dev, block, dim, tokens):
+    """Enough blocks that every group of threads takes several: odd ends, continued blocks, special values, bad pages."""
+    from semblo_b200 import _lib
+    from semblo_b200.kv8_cache import Kv8Cache, kv8_append
+    heads = 4
+    new, past = [tokens - 777 - 40, 0, 777, 40], [3, 0, block - 1, 1]
+    gen = torch.Generator(device=dev).manual_seed(block + dim)
+    need = [-(-(n + p) // block) for n, p in zip(new, past)]
+    blocks = sum(need) + 5
+    order = torch.randperm(blocks, device=dev, generator=gen).to(torch.int32)
+    table = torch.full((4, max(need)), -1, dtype=torch.int32, device=dev)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at:at + n]
+        at += n
+    table[0, 7] = blocks                                       # one block of the long request is not in the pool
+    k = torch.randn(tokens, heads, dim, device=dev, generator=gen).to(torch.bfloat16)
+    v = (k.float() * 3).to(torch.bfloat16)
+    k[100, 1, 3], v[5000, 2, 7] = math.inf, math.nan
+    cu = torch.tensor([0, new[0], new[0], new[0] + new[2], tokens], device=dev, dtype=torch.int32)
+    start = torch.tensor(past, device=dev, dtype=torch.int32)
+    base = Kv8Cache.allocate(blocks, block, heads, dim, dev)
+    base.data.view(torch.uint8).random_(0, 120, generator=gen)
+    base.scales.fill_(2.0 ** -9)
+    whole = Kv8Cache(base.data.clone(), base.scales.clone())
+    kv8_append(whole, k, v, table, cu, start)
+    with pytest.raises(RuntimeError, match="201"):
+        _lib.status_for(dev).raise_if_set()
+    # in pieces of one block, a call each: the few-tokens kernel, which the definition test covers
+    pieces = Kv8Cache(base.data.clone(), base.scales.clone())
+    rows = [[0, new[0]], [new[0], new[0]], [new[0], new[0] + new[2]], [new[0] + new[2], tokens]]
+    starts, cus, tables = [], [0], []
+    ks, vs = [], []
+    for b in range(4):
+        pos, r = past[b], rows[b][0]
+        while r < rows[b][1]:
+            m = min(block - pos % block, rows[b][1] - r)
+            starts.append(pos % block)
+            tables.append(int(table[b, pos // block]) if (b, pos // block) != (0, 7) else -1)
+            cus.append(m)
+            pos, r = pos + m, r + m
+    cum = torch.tensor(cus).cumsum(0).to(torch.int32)
+    per_call = 8
+    tab = torch.tensor(tables, dtype=torch.int32, device=dev)[:, None]
+    st = torch.tensor(starts, dtype=torch.int32, device=dev)
+    for i in range(0, len(starts), per_call):
+        e = min(i + per_call, len(starts))
+        a, z = int(cum[i]), int(cum[e])
+        kv8_append(pieces, k[a:z], v[a:z], tab[i:e], (cum[i:e + 1] - a).to(dev), st[i:e])
+    with pytest.raises(RuntimeError, match="201"):
+        _lib.status_for(dev).raise_if_set()
+    assert torch.equal(whole.scales, pieces.scales)
+    assert torch.equal(whole.data.view(torch.uint8), pieces.data.view(torch.uint8))
+
+
+def test_negative_starts_of_late_requests_are_reported(dev):
+    from semblo_b200 import _lib
+    cache, k, v, table, cu, past = _case(dev, 13, 16, 1, 64, torch.bfloat16, [2] * 80, [0] * 80)
+    from semblo_b200.kv8_cache import kv8_append
+    past[70] = -5
+    kv8_append(cache, k, v, table, torch.tensor(cu, dtype=torch.int32, device=dev),
+               torch.tensor(past, dtype=torch.int32, device=dev))
+    with pytest.raises(RuntimeError, match="201"):
+        _lib.status_for(dev).raise_if_set()
+
+
 def test_token_by_token_grows_the_scale(dev):
     """One block filled token by token with rising magnitudes; a scale set by the caller (not a power of two) holds
     until a value needs more."""
