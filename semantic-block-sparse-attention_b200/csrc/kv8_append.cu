@@ -171,27 +171,45 @@ __device__ __forceinline__ float largest_of(const uint4 (&x)[NL]) {
   return fmaxf(t2.x, t2.y);
 }
 
-// The same without infinities and NaN: they saturate and stay, but do not set the scale of the others.
-template <typename T2, int NL>
-__device__ __forceinline__ float largest_finite_of(const uint4 (&x)[NL]) {
+// The rare cases read the input again, in loops of their own and out of line: unrolled beside the common ones
+// they filled the instruction cache (131072 tokens x 4 heads x 256: 166 us).
+// The largest magnitude without infinities and NaN, which saturate and stay but do not set the scale of others.
+template <typename T2>
+__device__ __noinline__ float largest_finite_of(const uint16_t* src, int64_t row_stride, int pieces, int col_log2, int tid,
+                                                int threads) {
   float f = 0.f;
-#pragma unroll
-  for (int i = 0; i < NL; ++i)
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const uint4& q = x[i];
-      const float2 v = widen<T2>(w == 0 ? q.x : w == 1 ? q.y : w == 2 ? q.z : q.w);
+#pragma unroll 1
+  for (int p = tid; p < pieces; p += threads) {
+    const uint4 x = __ldg(reinterpret_cast<const uint4*>(src + (p >> col_log2) * row_stride + (p & ((1 << col_log2) - 1)) * 8));
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = widen<T2>(w[i]);
       if (fabsf(v.x) <= 3.4e38f) f = fmaxf(f, fabsf(v.x));
       if (fabsf(v.y) <= 3.4e38f) f = fmaxf(f, fabsf(v.y));
     }
+  }
   return f;
+}
+
+// Codes under a scale that is not a power of two (set by the caller): divided as written.
+template <typename T2>
+__device__ __noinline__ void divide_rows(const uint16_t* src, int64_t row_stride, int pieces, int col_log2, uint2* dst,
+                                         float scale, int tid, int threads) {
+#pragma unroll 1
+  for (int p = tid; p < pieces; p += threads) {
+    const uint4 x = __ldg(reinterpret_cast<const uint4*>(src + (p >> col_log2) * row_stride + (p & ((1 << col_log2) - 1)) * 8));
+    const float2 a = widen<T2>(x.x), b = widen<T2>(x.y), c = widen<T2>(x.z), d = widen<T2>(x.w);
+    dst[p] = make_uint2(code4(make_float2(a.x / scale, a.y / scale), make_float2(b.x / scale, b.y / scale)),
+                        code4(make_float2(c.x / scale, c.y / scale), make_float2(d.x / scale, d.y / scale)));
+  }
 }
 
 // Scale, earlier rows and codes of one unit, by `threads` threads of which this is number `tid`; x are its
 // pieces tid, tid + threads, ... of the new rows and `largest` their largest magnitude over the unit.
 template <typename T2, int NL>
 __device__ __forceinline__ void write_unit(const AppendArgs& a, const Unit& u, int64_t cell, float before, float largest,
-                                           const uint4 (&x)[NL], int tid, int threads) {
+                                           const uint4 (&x)[NL], const uint16_t* src, int64_t row_stride, int tid,
+                                           int threads) {
   uint8_t* dst = a.data + (cell << a.block_log2) * a.head_dim;
   float scale = pow2(exponent_for(largest));
   if (u.off) {
@@ -218,24 +236,20 @@ __device__ __forceinline__ void write_unit(const AppendArgs& a, const Unit& u, i
   }
   if (tid == 0) a.scales[cell] = scale;
   const int pieces = u.m << a.col_log2;
-  const bool exact_inverse = (__float_as_uint(scale) & 0x7fffffu) == 0 && scale >= pow2(-126) && scale <= pow2(126);
-  const float inv = exact_inverse ? __int_as_float((254 << 23) - __float_as_int(scale)) : 0.f;
+  uint2* out = reinterpret_cast<uint2*>(dst) + (u.off << a.col_log2);
+  if ((__float_as_uint(scale) & 0x7fffffu) != 0 || !(scale >= pow2(-126) && scale <= pow2(126))) {
+    divide_rows<T2>(src, row_stride, pieces, a.col_log2, out, scale, tid, threads);
+    return;
+  }
+  const float inv = __int_as_float((254 << 23) - __float_as_int(scale));
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
     const int p = i * threads + tid;
     if (p >= pieces) break;
-    uint32_t out[2];
+    float2 f[4] = {widen<T2>(x[i].x), widen<T2>(x[i].y), widen<T2>(x[i].z), widen<T2>(x[i].w)};
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      float2 f0 = widen<T2>(w ? x[i].z : x[i].x), f1 = widen<T2>(w ? x[i].w : x[i].y);
-      if (exact_inverse) {
-        f0.x *= inv; f0.y *= inv; f1.x *= inv; f1.y *= inv;
-      } else {                                        // a scale set by the caller: divided as written
-        f0.x /= scale; f0.y /= scale; f1.x /= scale; f1.y /= scale;
-      }
-      out[w] = code4(f0, f1);
-    }
-    reinterpret_cast<uint2*>(dst)[(u.off << a.col_log2) + p] = make_uint2(out[0], out[1]);
+    for (int w = 0; w < 4; ++w) { f[w].x *= inv; f[w].y *= inv; }
+    out[p] = make_uint2(code4(f[0], f[1]), code4(f[2], f[3]));
   }
 }
 
@@ -265,8 +279,9 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs a) {
   const int64_t cell = ((int64_t)part * a.cache_blocks + u.page) * a.num_kv_heads + h;
   const float before = u.off ? a.scales[cell] : 0.f;
   float largest = block_max(largest_of<T2, NL>(x), slots);
-  if (!(largest <= 3.4e38f)) largest = block_max(largest_finite_of<T2, NL>(x), slots);
-  write_unit<T2, NL>(a, u, cell, before, largest, x, threadIdx.x, blockDim.x);
+  if (!(largest <= 3.4e38f))
+    largest = block_max(largest_finite_of<T2>(src, a.src_token[part], pieces, a.col_log2, threadIdx.x, blockDim.x), slots);
+  write_unit<T2, NL>(a, u, cell, before, largest, x, src, a.src_token[part], threadIdx.x, blockDim.x);
 }
 
 // A stream of cache blocks: GROUP threads take one (cache block, head, part) after the other, NL pieces a thread.
@@ -295,9 +310,12 @@ __global__ void __launch_bounds__(STREAM_THREADS, NL == 4 ? 2 : 1) kv8_stream_ke
     }
     return __uint_as_float(b);
   };
+  auto source = [&](const Unit& u, int h, int part) {
+    return static_cast<const uint16_t*>(a.src[part]) + u.row * a.src_token[part] + (int64_t)h * a.src_head[part];
+  };
   auto request = [&](const Unit& u, int h, int part) {        // the new rows of a unit on their way
     if (u.have && u.page >= 0) {
-      const uint16_t* src = static_cast<const uint16_t*>(a.src[part]) + u.row * a.src_token[part] + (int64_t)h * a.src_head[part];
+      const uint16_t* src = source(u, h, part);
       const int pieces = u.m << a.col_log2;
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
@@ -320,6 +338,8 @@ __global__ void __launch_bounds__(STREAM_THREADS, NL == 4 ? 2 : 1) kv8_stream_ke
   request(next, h, part);
   while (next.have) {
     const Unit u = next;
+    const uint16_t* src = source(u, h, part);
+    const int64_t row_stride = a.src_token[part];
     const int64_t cell = ((int64_t)part * a.cache_blocks + max(u.page, (int64_t)0)) * a.num_kv_heads + h;
     const float before = u.off && u.page >= 0 ? a.scales[cell] : 0.f;
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -337,8 +357,9 @@ __global__ void __launch_bounds__(STREAM_THREADS, NL == 4 ? 2 : 1) kv8_stream_ke
       if (tid == 0) atomicCAS(a.status, 0, sm100::STATUS_OVERFLOW);
       continue;
     }
-    if (!(largest <= 3.4e38f)) largest = group_max(largest_finite_of<T2, NL>(x));
-    write_unit<T2, NL>(a, u, cell, before, largest, x, tid, GROUP);
+    if (!(largest <= 3.4e38f))
+      largest = group_max(largest_finite_of<T2>(src, row_stride, u.m << a.col_log2, a.col_log2, tid, GROUP));
+    write_unit<T2, NL>(a, u, cell, before, largest, x, src, row_stride, tid, GROUP);
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
