@@ -204,14 +204,21 @@ struct TanhPoly {
   }
 };
 
-// What happens to a raw score: 0 scaled only, 1 capped, 2 biased by distance (and capped, if there is a cap).
-enum Mode { LINEAR = 0, CAPPED = 1, BIASED = 2 };
+// What happens to a raw score: 0 scaled only, 1 capped, 2 biased by distance (and capped, if there is a cap), 3
+// capped so low that no running maximum is needed.
+enum Mode { LINEAR = 0, CAPPED = 1, BIASED = 2, BOUNDED = 3 };
+
+// A cap bounds the scores, so with bf16 P (float's range) a fixed reference will do where 2^(score - reference)
+// stays between 2^-108 and 2^44: no maximum, no rescale of O, and the products P V stay inside float for |v| up to
+// 2^59 even over 2^24 keys.  That is caps up to 52.
+constexpr float BOUNDED_TOP = 44.f, BOUNDED_LOG2 = 76.f;
+__host__ __device__ inline float bounded_reference(float cap_log2) { return cap_log2 > BOUNDED_TOP ? cap_log2 - BOUNDED_TOP : 0.f; }
 
 // 32 raw scores in place -> what the exponential's scale multiplies.
 template <int MODE>
 __device__ __forceinline__ void transform32(uint32_t* x, const Args& a, float slope, int p, int key0) {
   if constexpr (MODE == LINEAR) return;
-  if (MODE == CAPPED || a.cap_log2 > 0.f) {
+  if (MODE == CAPPED || MODE == BOUNDED || a.cap_log2 > 0.f) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(tanh_exp(__uint_as_float(x[i]) * (a.score_scale * (1.f / TANH_ARG))));
   }
@@ -226,7 +233,7 @@ __device__ __forceinline__ void transform32(uint32_t* x, const Args& a, float sl
 
 // The factor that turns transformed scores into log2 units (positive: the maximum commutes with it).
 template <int MODE> __device__ __forceinline__ float scale_of(const Args& a) {
-  return MODE == LINEAR ? a.score_scale : MODE == CAPPED ? a.cap_log2 : 1.f;
+  return MODE == LINEAR ? a.score_scale : MODE == BIASED ? 1.f : a.cap_log2;
 }
 
 // Largest and smallest of 32 values (the smallest only where it is asked for).
@@ -244,6 +251,36 @@ __device__ __forceinline__ void range32(const uint32_t* x, float& most, float& l
   }
   most = fmaxf(t0, t1);
   if constexpr (LEAST) least = fminf(u0, u1);
+}
+
+// 32 raw scores in place -> arguments of the exponential under a fixed reference.  All lanes of a warp take part.
+__device__ __forceinline__ void bounded32(uint32_t* x, const Args& a, const TanhPoly& capped, bool all, uint32_t bits,
+                                          float neg_m) {
+  const f32x2 arg2 = join(a.score_scale, a.score_scale), neg2 = join(neg_m, neg_m);
+  uint32_t seen = 0;
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    float y0, y1;
+    split(mul2(join(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), arg2), y0, y1);
+    x[i] = __float_as_uint(y0);
+    x[i + 1] = __float_as_uint(y1);
+    seen |= x[i] | x[i + 1];
+  }
+  // every |y| < 2: the top bit of the exponent is clear in all of them
+  if (all && __all_sync(0xffffffffu, !(seen & 0x40000000u))) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      float e0, e1;
+      split(capped(join(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), neg2), e0, e1);
+      x[i] = __float_as_uint(e0);
+      x[i + 1] = __float_as_uint(e1);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      x[i] = __float_as_uint(fmaf(tanh_exp(__uint_as_float(x[i]) * (1.f / TANH_ARG)), a.cap_log2, neg_m));
+    if (!all) hide32(x, bits);
+  }
 }
 
 template <bool F16> __device__ __forceinline__ uint32_t pack_pair(float x, float y) {

@@ -238,7 +238,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     const float slope = a.slopes && valid ? a.slopes[head] * LOG2EF : 0.f;
     const float scale = scale_of<MODE>(a);
     const TanhPoly capped(a.cap_log2);
-    float m_ref = -INFINITY, l = 0.f;
+    float m_ref = MODE == BOUNDED ? bounded_reference(a.cap_log2) : -INFINITY, l = 0.f;
     bool ok = true;
     int count = 0;
     // this tile's walk: [0, gp), then [j0, j1)
@@ -252,7 +252,52 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       ok = mbar_wait_warp(bar(B_S + x), (uint32_t)(count & 1), abort_flag, a.status, STATUS_TIMEOUT_SOFTMAX);
       if (!ok) break;
       tc_fence_after();
-      constexpr int STEPS = MODE == LINEAR ? 1 : 2, CH = 4 / STEPS;       // chunks of 32 keys in a step
+      // P of chunk c (32 keys) of the tile to tensor memory: keys 2 i, 2 i + 1 share a column, P lies over logits that
+      // have been read.  After every second chunk a half is handed over
+      auto store = [&](int c, const uint32_t (&packed)[16]) {
+        tmem_st16(s_addr + c * 16, packed);
+        if (!(c & 1)) return;
+        // V's rows behind the document's end (another document's, or anything) are cleared: their P is 0, but 0 * NaN
+        // would not vanish.  Both tiles' warps may do it; the stage stays until both are multiplied
+        const int left = tile.lk - key0;
+        if (c == 1 && (warp & 3) == 0 && left < BN && (left & (PAGE - 1))) {
+          ok = mbar_wait_warp(bar(B_FULL + (2 * j + 1) % SLOTS), ((2 * j + 1) / SLOTS) & 1, abort_flag, a.status,
+                              STATUS_TIMEOUT_SOFTMAX);
+          if (ok) zero_rows<D, BN>(smem + C::KV_OFF + (2 * j + 1) % SLOTS * C::TILE, left, (left + PAGE - 1) / PAGE * PAGE);
+          fence_proxy_async_smem();
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_P + 2 * x + (c >> 1)));
+      };
+      constexpr int STEPS = MODE == BOUNDED ? 0 : MODE == LINEAR ? 1 : 2, CH = STEPS == 1 ? 4 : 2;   // chunks in a step
+      if constexpr (MODE == BOUNDED) {
+        // no maximum: chunk by chunk, the next one's scores on their way
+        const float neg_m = -bounded_reference(a.cap_log2);
+        uint32_t s[2][32];
+        tmem_ld32(s_addr, s[0]);
+        f32x2 sum0 = join(0.f, 0.f), sum1 = sum0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tmem_ld_wait();
+          if (c < 3) tmem_ld32(s_addr + (c + 1) * 32, s[(c + 1) & 1]);
+          const int lo = seen.lo - key0 - 32 * c, hi = seen.hi - key0 - 32 * c, pre = seen.pre - key0 - 32 * c;
+          const bool all = __all_sync(0xffffffffu, (lo <= 0 && hi >= 32) || pre >= 32);
+          bounded32(s[c & 1], a, capped, all, seen_bits(lo, hi, pre), neg_m);
+          uint32_t packed[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float e0 = fast_exp2(__uint_as_float(s[c & 1][2 * i])), e1 = fast_exp2(__uint_as_float(s[c & 1][2 * i + 1]));
+            packed[i] = pack_pair<F16>(e0, e1);
+            if (i & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
+          }
+          store(c, packed);
+        }
+        float s0, s1;
+        split(add2(sum0, sum1), s0, s1);
+        l += s0 + s1;
+      }
 #pragma unroll 1
       for (int step = 0; step < STEPS; ++step) {
         const int k0 = key0 + 64 * step;
@@ -328,24 +373,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
               packed[i] = pack_pair<F16>(e0, e1);
               if (i & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
             }
-            // keys 2 i, 2 i + 1 of the chunk share a column: P lies over logits that have been read
-            tmem_st16(s_addr + step * 32 + c * 16, packed);
-            if (c & 1) {
-              const int half = step + (c >> 1);
-              // V's rows behind the document's end (another document's, or anything) are cleared: their P is 0, but
-              // 0 * NaN would not vanish.  Both tiles' warps may do it; the stage stays until both are multiplied
-              const int left = tile.lk - key0;
-              if (half == 0 && (warp & 3) == 0 && left < BN && (left & (PAGE - 1))) {
-                ok = mbar_wait_warp(bar(B_FULL + (2 * j + 1) % SLOTS), ((2 * j + 1) / SLOTS) & 1, abort_flag, a.status,
-                                    STATUS_TIMEOUT_SOFTMAX);
-                if (ok) zero_rows<D, BN>(smem + C::KV_OFF + (2 * j + 1) % SLOTS * C::TILE, left, (left + PAGE - 1) / PAGE * PAGE);
-                fence_proxy_async_smem();
-              }
-              tmem_st_wait();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(bar(B_P + 2 * x + half));
-            }
+            store(2 * step + c, packed);
           }
         };
         if (MODE == CAPPED && poly) {
@@ -421,6 +449,7 @@ int launch_pair(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap&
 #define SEMBLO_PAIR(DD, FF, MM) \
   if (head_dim == DD && f16 == FF && mode == MM) return launch<DD, FF, MM>(mk, mv, mq, a, kv_heads, st);
   SEMBLO_PAIR(64, false, LINEAR) SEMBLO_PAIR(64, false, CAPPED) SEMBLO_PAIR(64, false, BIASED)
+  SEMBLO_PAIR(64, false, BOUNDED) SEMBLO_PAIR(128, false, BOUNDED)
   SEMBLO_PAIR(64, true, LINEAR) SEMBLO_PAIR(64, true, CAPPED) SEMBLO_PAIR(64, true, BIASED)
   SEMBLO_PAIR(128, false, LINEAR) SEMBLO_PAIR(128, false, CAPPED) SEMBLO_PAIR(128, false, BIASED)
   SEMBLO_PAIR(128, true, LINEAR) SEMBLO_PAIR(128, true, CAPPED) SEMBLO_PAIR(128, true, BIASED)

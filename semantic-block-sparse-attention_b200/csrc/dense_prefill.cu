@@ -191,7 +191,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     }
     const float scale = scale_of<MODE>(a);
     const TanhPoly capped(a.cap_log2);
-    float m_ref = -INFINITY, l_part = 0.f;
+    float m_ref = MODE == BOUNDED ? bounded_reference(a.cap_log2) : -INFINITY, l_part = 0.f;
     bool ok = true;
     float* mx = reinterpret_cast<float*>(smem + C::MX_OFF);
     for (int j = 0; j < keys.n; ++j) {
@@ -202,6 +202,27 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       const uint32_t s_addr = tmem_base + lane_addr + b * BN + hf * 32;
       const bool active = tile.lk > key0;                // the product wrote at least one page of this half
       uint32_t x[32];
+      if constexpr (MODE == BOUNDED) {
+        if (active) {
+          tmem_ld32(s_addr, x);
+          tmem_ld_wait();
+          const int lo = seen.lo - key0, hi = seen.hi - key0, pre = seen.pre - key0;
+          const bool all = __all_sync(0xffffffffu, (lo <= 0 && hi >= 32) || pre >= 32);
+          bounded32(x, a, capped, all, seen_bits(lo, hi, pre), -m_ref);
+          uint32_t packed[16];
+          f32x2 sum0 = join(0.f, 0.f), sum1 = sum0;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float e0 = fast_exp2(__uint_as_float(x[2 * i])), e1 = fast_exp2(__uint_as_float(x[2 * i + 1]));
+            packed[i] = pack_pair<F16>(e0, e1);
+            if (i & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
+          }
+          float s0, s1;
+          split(add2(sum0, sum1), s0, s1);
+          l_part += s0 + s1;
+          tmem_st16(s_addr, packed);
+        }
+      } else {
       float hm = -INFINITY, least = INFINITY;
       bool poly = MODE == CAPPED;                        // this half's tanh by polynomial, in the exponential's pass
       if (active) {
@@ -284,6 +305,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         l_part += s0 + s1;
         // P lies over this half's own logits; P V takes its 16-key slices from columns 0, 8, 32 and 40
         tmem_st16(s_addr, packed);
+      }
       }
       // V's rows behind the document's end (another document's, or anything) are cleared: their P is 0, but 0 * NaN
       // would not vanish.  S's barrier says that the stage has arrived
@@ -406,9 +428,10 @@ extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64
   }
   cudaStream_t st = (cudaStream_t)stream;
   const bool f16 = dtype == SEMBLO_F16;
-  const int mode = alibi_slopes ? BIASED : softcap > 0.f ? CAPPED : LINEAR;
+  const int mode = alibi_slopes ? BIASED : softcap > 0.f ? (!f16 && a.cap_log2 <= BOUNDED_LOG2 ? BOUNDED : CAPPED) : LINEAR;
   if (head_dim <= 128) return dense::launch_pair(mk, mv, mq, a, head_dim, f16, mode, num_kv_heads, st);
   if (mode == LINEAR) return f16 ? launch<256, true, LINEAR>(mk, mv, a, num_kv_heads, st) : launch<256, false, LINEAR>(mk, mv, a, num_kv_heads, st);
+  if (mode == BOUNDED) return launch<256, false, BOUNDED>(mk, mv, a, num_kv_heads, st);
   if (mode == CAPPED) return f16 ? launch<256, true, CAPPED>(mk, mv, a, num_kv_heads, st) : launch<256, false, CAPPED>(mk, mv, a, num_kv_heads, st);
   return f16 ? launch<256, true, BIASED>(mk, mv, a, num_kv_heads, st) : launch<256, false, BIASED>(mk, mv, a, num_kv_heads, st);
 }
