@@ -26,7 +26,7 @@ struct Args {
   int64_t tokens_q, tokens_k;
   int causal, window;
   int zero_tail;                  // write zeros to the rows behind the last document
-  float score_scale;              // raw product -> log2 units, or -> 4/3 of the capping tanh's argument
+  float score_scale;              // raw product -> log2 units, or -> 8/3 of the capping tanh's argument
   float cap_log2;                 // cap * log2(e)
   int* status;
 };
@@ -178,31 +178,46 @@ __device__ __forceinline__ float tanh_exp(float x) {
   return 1.f - __fdividef(2.f, 1.f + fast_exp2(x * (2.f * LOG2EF)));
 }
 
-// tanh(3/4 y) on (-2, 2) as y P(y^2), P of degree 7 fitted for the smallest largest error (3.4e-7; 5e-7 as
-// evaluated in 32 bits), on the multiply-add pipe: the exponentials of the softmax already fill the
-// special-function unit.  Scores beyond 1.5 caps are rare and take tanh_exp.
-constexpr float TANH_ARG = 4.f / 3.f, TANH_LIMIT = 2.f;
-__device__ __forceinline__ constexpr float tanh_coefficient(int i) {
-  const float c[8] = {0.74999702f, -0.140585884f, 0.0314894468f, -0.00693565886f,
-                      0.00137885404f, -0.000215864566f, 2.20087895e-05f, -1.04479068e-06f};
+// tanh(3/8 y) as y P(y^2) on the multiply-add pipe (the exponentials of the softmax fill the special-function
+// unit), P fitted for the smallest largest error: of degree 4 for |y| < 2 (2.5e-7 as evaluated in 32 bits), of
+// degree 7 for |y| < 4 (5e-7).  Scores beyond 1.5 caps are rare and take tanh_exp.
+constexpr float TANH_ARG = 8.f / 3.f, TANH_FAR = 4.f;
+__device__ __forceinline__ constexpr float near_coefficient(int i) {
+  const float c[5] = {0.374998957f, -0.0175727159f, 0.000980816782f, -5.13917694e-05f, 1.80655456e-06f};
   return c[i];
 }
-// factor * tanh(3/4 y) = y P(y^2) with the factor in the coefficients.
+__device__ __forceinline__ constexpr float far_coefficient(int i) {
+  const float c[8] = {0.37499851f, -0.0175732356f, 0.000984045211f, -5.41848349e-05f,
+                      2.69307429e-06f, -1.0540262e-07f, 2.68661982e-09f, -3.18844812e-11f};
+  return c[i];
+}
+// factor * tanh(3/8 y) = y P(y^2) with the factor in the N coefficients (5: near, 8: far).
+template <int N>
 struct TanhPoly {
-  f32x2 c[8];
+  f32x2 c[N];
   __device__ __forceinline__ explicit TanhPoly(float factor) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = join(factor * tanh_coefficient(i), factor * tanh_coefficient(i));
+    for (int i = 0; i < N; ++i) {
+      const float v = factor * (N == 5 ? near_coefficient(i) : far_coefficient(i));
+      c[i] = join(v, v);
+    }
   }
   // y P(y^2) + add
   __device__ __forceinline__ f32x2 operator()(f32x2 y, f32x2 add) const {
     const f32x2 u = mul2(y, y);
-    f32x2 r = c[7];
+    f32x2 r = c[N - 1];
 #pragma unroll
-    for (int i = 6; i >= 0; --i) r = fma2(r, u, c[i]);
+    for (int i = N - 2; i >= 0; --i) r = fma2(r, u, c[i]);
     return fma2(r, y, add);
   }
 };
+__device__ __forceinline__ float tanh_far(float y) {
+  const float u = y * y;
+  float r = far_coefficient(7);
+#pragma unroll
+  for (int i = 6; i >= 0; --i) r = fmaf(r, u, far_coefficient(i));
+  return r * y;
+}
 
 // What happens to a raw score: 0 scaled only, 1 capped, 2 biased by distance (and capped, if there is a cap), 3
 // capped so low that no running maximum is needed.
@@ -254,7 +269,7 @@ __device__ __forceinline__ void range32(const uint32_t* x, float& most, float& l
 }
 
 // 32 raw scores in place -> arguments of the exponential under a fixed reference.  All lanes of a warp take part.
-__device__ __forceinline__ void bounded32(uint32_t* x, const Args& a, const TanhPoly& capped, bool all, uint32_t bits,
+__device__ __forceinline__ void bounded32(uint32_t* x, const Args& a, const TanhPoly<5>& capped, bool all, uint32_t bits,
                                           float neg_m) {
   const f32x2 arg2 = join(a.score_scale, a.score_scale), neg2 = join(neg_m, neg_m);
   uint32_t seen = 0;
@@ -276,9 +291,17 @@ __device__ __forceinline__ void bounded32(uint32_t* x, const Args& a, const Tanh
       x[i + 1] = __float_as_uint(e1);
     }
   } else {
+    float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      x[i] = __float_as_uint(fmaf(tanh_exp(__uint_as_float(x[i]) * (1.f / TANH_ARG)), a.cap_log2, neg_m));
+    for (int i = 0; i < 32; i += 2) most = fmax3(most, fabsf(__uint_as_float(x[i])), fabsf(__uint_as_float(x[i + 1])));
+    if (__all_sync(0xffffffffu, most < TANH_FAR)) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(fmaf(tanh_far(__uint_as_float(x[i])), a.cap_log2, neg_m));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        x[i] = __float_as_uint(fmaf(tanh_exp(__uint_as_float(x[i]) * (1.f / TANH_ARG)), a.cap_log2, neg_m));
+    }
     if (!all) hide32(x, bits);
   }
 }

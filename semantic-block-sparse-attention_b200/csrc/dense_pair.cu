@@ -20,18 +20,27 @@ namespace {
 constexpr int BN = PAIR_BN;
 constexpr int PAGE = 16;
 
-template <int D>
+template <int D, int MODE>
 struct Cfg {
+  // threads per row.  With a running maximum one: two would have to meet for every tile and, with half the
+  // registers each, read the scores twice (16384 causal 1.4 times as long).  Under a fixed reference two pay where
+  // the softmax outweighs the products (8192 capped, windowed: D = 64 797 -> 666 us, D = 128 752 -> 780)
+  static constexpr int HALVES = MODE == BOUNDED && D == 64 ? 2 : 1;
+  static constexpr int WARPS = 8 * HALVES;                     // of the softmax; then the loading and the issuing warp
+  static constexpr int THREADS = (WARPS + 2) * 32;
   static constexpr int SLABS = D / 64;                         // 128-byte wide slabs of a 16-bit tile
   static constexpr int TILE = BN * D * 2;                      // a tile of Q, K or V
   static constexpr int SLOTS = D == 128 ? 5 : 8;
   static constexpr int Q_OFF = 0;
   static constexpr int KV_OFF = 2 * TILE;
-  static constexpr int BAR_OFF = KV_OFF + SLOTS * TILE;
+  static constexpr int SUM_OFF = KV_OFF + SLOTS * TILE;        // float [2 tiles][2 halves][128]
+  static constexpr int BAR_OFF = SUM_OFF + (HALVES == 2 ? 2048 : 0);
   static constexpr int TOTAL = BAR_OFF + 256;
   static constexpr int S_COL = 0;                              // + 128 x: S and P of tile x
   static constexpr int O_COL = 256;                            // + D x
   static constexpr int TMEM_COLS = 512;
+  // P of a half lies over logits that the half's own threads have read
+  static constexpr int P_HALF = HALVES == 2 ? 64 : 32;
 };
 
 enum { B_Q = 0, B_S = 1, B_P = 3, B_H = 7, B_O = 9, B_FULL = 11 };     // B_S + x, B_P + 2 x + half, B_H + x, B_O + x
@@ -73,11 +82,11 @@ struct Walk {
 };
 
 template <int D, bool F16, int MODE>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(Cfg<D, MODE>::THREADS, 1)
 dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                   const __grid_constant__ CUtensorMap tmap_v, const Args a) {
-  using C = Cfg<D>;
-  constexpr int SLOTS = C::SLOTS;
+  using C = Cfg<D, MODE>;
+  constexpr int SLOTS = C::SLOTS, HALVES = C::HALVES;
   constexpr int B_EMPTY = B_FULL + SLOTS;
   static_assert(8 * (B_EMPTY + SLOTS) + 8 <= 256, "barrier area");
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -93,7 +102,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   // barriers by the warp that loads, which need not wait for anybody with its first loads; tensor memory by the
   // warp that issues, while the others look for their tile
-  if (warp == 8 && lane == 0) {
+  if (warp == C::WARPS && lane == 0) {
     mbar_init(bar(B_Q), 1);
     for (int x = 0; x < 2; ++x) {
       mbar_init(bar(B_S + x), 1);
@@ -128,7 +137,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       tma_load_3d(smem_u32(smem + C::KV_OFF + s * C::TILE + sl * BN * 128), (i & 1) ? &tmap_v : &tmap_k, bar(B_FULL + s),
                   sl * 64, h, row);
   };
-  if (warp == 8 && lane == 0 && walk.n > 0) {
+  if (warp == C::WARPS && lane == 0 && walk.n > 0) {
     const int tiles = walk.any[1] ? 2 : 1;
     mbar_arrive_expect_tx(bar(B_Q), (uint32_t)(tiles * C::SLABS * qt * a.group * 128));
     for (int x = 0; x < tiles; ++x)
@@ -138,7 +147,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     load_kv(0);
     load_kv(1);
   }
-  if (warp == 9) {
+  if (warp == C::WARPS + 1) {
     tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
     tmem_relinquish();
   }
@@ -147,7 +156,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 8) {
+  if (warp == C::WARPS) {
     // ------------------------------------------------------------ producer: after Q, K(0), V(0): K(1), V(1), ...
     if (lane == 0) {
       for (int i = 2; i < 2 * walk.n; ++i) {
@@ -155,7 +164,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         load_kv(i);
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == C::WARPS + 1) {
     // ------------------------------------------------------------ UMMA issuer
     // UMMAs of one thread execute in order: S(j + 1) may overwrite the P that the P V before it reads.
     if (elect_one()) {
@@ -192,7 +201,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 #pragma unroll
           for (int kk = half * 4; kk < half * 4 + 4; ++kk)
             if (kk < pages)
-              umma_ts(tmem_base + C::O_COL + x * D, tmem_base + C::S_COL + x * 128 + kk * 8,
+              umma_ts(tmem_base + C::O_COL + x * D, tmem_base + C::S_COL + x * 128 + half * C::P_HALF + (kk & 3) * 8,
                       make_smem_desc(v_base + kk * PAGE * 128, BN * 128, 1024), idesc_pv, (done[x] > 0 || kk > 0) ? 1u : 0u);
           if (half == 0) umma_commit(bar(B_H + x));
         }
@@ -224,8 +233,8 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       }
     }
   } else {
-    // ------------------------------------------------------------ softmax + epilogue: thread = row
-    const int x = warp >> 2;
+    // ------------------------------------------------------------ softmax + epilogue: one or two threads per row
+    const int x = warp / (C::WARPS / 2), hf = HALVES == 2 ? (warp >> 2) & 1 : 0;
     const int row = threadIdx.x & 127;
     const int qi = row / a.group, hg = row - qi * a.group;
     const bool valid = qi < qt && x * qt + qi < tile.count;
@@ -233,11 +242,11 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     const Seen seen = valid ? seen_by(a, tile, p) : Seen{0, 0, 0};
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_addr + C::S_COL + x * 128;
-    const uint32_t o_addr = tmem_base + lane_addr + C::O_COL + x * D;
+    const uint32_t o_addr = tmem_base + lane_addr + C::O_COL + x * D + hf * (D / 2);
     const int head = h * a.group + hg;
     const float slope = a.slopes && valid ? a.slopes[head] * LOG2EF : 0.f;
     const float scale = scale_of<MODE>(a);
-    const TanhPoly capped(a.cap_log2);
+    const TanhPoly<MODE == BOUNDED ? 5 : 8> capped(a.cap_log2);
     float m_ref = MODE == BOUNDED ? bounded_reference(a.cap_log2) : -INFINITY, l = 0.f;
     bool ok = true;
     int count = 0;
@@ -255,12 +264,12 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       // P of chunk c (32 keys) of the tile to tensor memory: keys 2 i, 2 i + 1 share a column, P lies over logits that
       // have been read.  After every second chunk a half is handed over
       auto store = [&](int c, const uint32_t (&packed)[16]) {
-        tmem_st16(s_addr + c * 16, packed);
+        tmem_st16(s_addr + (c >> 1) * C::P_HALF + (c & 1) * 16, packed);
         if (!(c & 1)) return;
         // V's rows behind the document's end (another document's, or anything) are cleared: their P is 0, but 0 * NaN
         // would not vanish.  Both tiles' warps may do it; the stage stays until both are multiplied
         const int left = tile.lk - key0;
-        if (c == 1 && (warp & 3) == 0 && left < BN && (left & (PAGE - 1))) {
+        if (c >> 1 == (HALVES == 2 ? left >> 6 : 0) && (warp & 3) == 0 && left < BN && (left & (PAGE - 1))) {
           ok = mbar_wait_warp(bar(B_FULL + (2 * j + 1) % SLOTS), ((2 * j + 1) / SLOTS) & 1, abort_flag, a.status,
                               STATUS_TIMEOUT_SOFTMAX);
           if (ok) zero_rows<D, BN>(smem + C::KV_OFF + (2 * j + 1) % SLOTS * C::TILE, left, (left + PAGE - 1) / PAGE * PAGE);
@@ -273,24 +282,27 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       };
       constexpr int STEPS = MODE == BOUNDED ? 0 : MODE == LINEAR ? 1 : 2, CH = STEPS == 1 ? 4 : 2;   // chunks in a step
       if constexpr (MODE == BOUNDED) {
-        // no maximum: chunk by chunk, the next one's scores on their way
-        const float neg_m = -bounded_reference(a.cap_log2);
-        uint32_t s[2][32];
-        tmem_ld32(s_addr, s[0]);
+        // no maximum: chunk by chunk (with registers to spare the next one's scores on their way)
+        constexpr int CHUNKS = 4 / HALVES, BUFFERS = HALVES == 1 ? 2 : 1;
         f32x2 sum0 = join(0.f, 0.f), sum1 = sum0;
+        uint32_t held[BUFFERS][32];
+        if constexpr (BUFFERS == 2) tmem_ld32(s_addr, held[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int i = 0; i < CHUNKS; ++i) {
+          const int c = 2 * hf + i;
+          uint32_t (&s)[32] = held[i % BUFFERS];
+          if constexpr (BUFFERS == 1) tmem_ld32(s_addr + c * 32, s);
           tmem_ld_wait();
-          if (c < 3) tmem_ld32(s_addr + (c + 1) * 32, s[(c + 1) & 1]);
+          if (BUFFERS == 2 && i + 1 < CHUNKS) tmem_ld32(s_addr + (c + 1) * 32, held[(i + 1) % BUFFERS]);
           const int lo = seen.lo - key0 - 32 * c, hi = seen.hi - key0 - 32 * c, pre = seen.pre - key0 - 32 * c;
           const bool all = __all_sync(0xffffffffu, (lo <= 0 && hi >= 32) || pre >= 32);
-          bounded32(s[c & 1], a, capped, all, seen_bits(lo, hi, pre), neg_m);
+          bounded32(s, a, capped, all, seen_bits(lo, hi, pre), -m_ref);
           uint32_t packed[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float e0 = fast_exp2(__uint_as_float(s[c & 1][2 * i])), e1 = fast_exp2(__uint_as_float(s[c & 1][2 * i + 1]));
-            packed[i] = pack_pair<F16>(e0, e1);
-            if (i & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
+          for (int n = 0; n < 16; ++n) {
+            const float e0 = fast_exp2(__uint_as_float(s[2 * n])), e1 = fast_exp2(__uint_as_float(s[2 * n + 1]));
+            packed[n] = pack_pair<F16>(e0, e1);
+            if (n & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
           }
           store(c, packed);
         }
@@ -314,7 +326,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           for (int c = 0; c < CH; ++c) range32<MODE == CAPPED>(s[c], tmax, least);
         }
         if constexpr (MODE == CAPPED) {
-          poly = all && __all_sync(0xffffffffu, fmaxf(tmax, -least) * a.score_scale < TANH_LIMIT);
+          poly = all && __all_sync(0xffffffffu, fmaxf(tmax, -least) * a.score_scale < TANH_FAR);
           if (poly) tmax = tanh_exp(tmax * (a.score_scale * (1.f / TANH_ARG)));
         }
         if (MODE == BIASED || (MODE == CAPPED && !poly) || (MODE == LINEAR && !all)) {
@@ -391,14 +403,20 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
     if (ok) ok = mbar_wait_warp(bar(B_O + x), 0, abort_flag, a.status, STATUS_TIMEOUT_EPILOGUE);
     tc_fence_after();
+    if constexpr (HALVES == 2) {
+      float* sums = reinterpret_cast<float*>(smem + C::SUM_OFF) + x * 256;
+      sums[hf * 128 + row] = l;
+      asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");     // all of the tile's threads, whatever became of them
+      l += sums[(hf ^ 1) * 128 + row];
+    }
     if (ok && any) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int64_t at = (tile.token + x * qt + qi) * a.num_q_heads + head;
-      // through Q's shared memory (no product is in flight any more), 8 KB of it per warp
-      constexpr int PIECES = D / 8;
-      uint8_t* stage = smem + C::Q_OFF + warp * 32 * D * 2;
+      // through Q's shared memory (no product is in flight any more), a warp's own part of it
+      constexpr int PIECES = D / 8 / HALVES;
+      uint8_t* stage = smem + C::Q_OFF + warp * 32 * PIECES * 16;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
+      for (int c = 0; c < D / 32 / HALVES; ++c) {
         uint32_t o[32];
         if (count > 0) {
           tmem_ld32(o_addr + c * 32, o);
@@ -417,25 +435,25 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         const int q = rr / a.group;
         if (q < qt && x * qt + q < tile.count)
           reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) +
-                                   ((tile.token + x * qt + q) * a.num_q_heads + h * a.group + rr - q * a.group) * D)[piece] =
+                                   ((tile.token + x * qt + q) * a.num_q_heads + h * a.group + rr - q * a.group) * D + hf * (D / 2))[piece] =
               reinterpret_cast<const uint4*>(stage)[r * PIECES + (piece ^ (r & (PIECES - 1)))];
       }
-      if (valid && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m_ref + __log2f(l) - p_bias<F16>()) * LN2F;
+      if (valid && a.lse && hf == 0) a.lse[at] = l == 0.f ? -INFINITY : (m_ref + __log2f(l) - p_bias<F16>()) * LN2F;
     }
     tc_fence_before();
   }
   __syncthreads();
   if (*abort_flag) __nanosleep(50000);
-  if (warp == 9) tmem_dealloc(tmem_base, C::TMEM_COLS);
+  if (warp == C::WARPS + 1) tmem_dealloc(tmem_base, C::TMEM_COLS);
 }
 
 template <int D, bool F16, int MODE>
 int launch(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, const Args& a, int kv_heads, cudaStream_t st) {
-  using C = Cfg<D>;
+  using C = Cfg<D, MODE>;
   auto kern = dense_pair_kernel<D, F16, MODE>;
   SEMBLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TOTAL));
   dim3 grid((unsigned)(ceil_div(a.tokens_q, a.queries_per_tile) + a.docs), (unsigned)kv_heads);
-  kern<<<grid, 320, C::TOTAL, st>>>(mq, mk, mv, a);
+  kern<<<grid, C::THREADS, C::TOTAL, st>>>(mq, mk, mv, a);
   SEMBLO_LAUNCH_CHECK();
   return 0;
 }

@@ -190,7 +190,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       mbar_arrive(bar(B_QFULL));
     }
     const float scale = scale_of<MODE>(a);
-    const TanhPoly capped(a.cap_log2);
+    const TanhPoly<MODE == BOUNDED ? 5 : 8> capped(a.cap_log2);
     float m_ref = MODE == BOUNDED ? bounded_reference(a.cap_log2) : -INFINITY, l_part = 0.f;
     bool ok = true;
     float* mx = reinterpret_cast<float*>(smem + C::MX_OFF);
@@ -223,89 +223,89 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           tmem_st16(s_addr, packed);
         }
       } else {
-      float hm = -INFINITY, least = INFINITY;
-      bool poly = MODE == CAPPED;                        // this half's tanh by polynomial, in the exponential's pass
-      if (active) {
-        tmem_ld32(s_addr, x);
-        tmem_ld_wait();
-        const int lo = seen.lo - key0, hi = seen.hi - key0, pre = seen.pre - key0;
-        const bool all = __all_sync(0xffffffffu, (lo <= 0 && hi >= 32) || pre >= 32);
-        if constexpr (MODE == CAPPED) {
-          range32<true>(x, hm, least);
-          poly = all && __all_sync(0xffffffffu, fmaxf(hm, -least) * a.score_scale < TANH_LIMIT);
-          if (poly) hm = tanh_exp(hm * (a.score_scale * (1.f / TANH_ARG)));
-        }
-        if (!poly) {
-          transform32<MODE>(x, a, slope, p, key0);
-          if (!all) {
-            hide32(x, seen_bits(lo, hi, pre));
-          }
-          hm = -INFINITY;
-          range32<false>(x, hm, least);
-        }
-      }
-      float* slot = mx + b * 256;
-      slot[hf * 128 + row] = hm;
-      __syncwarp();                                      // one arrival per warp: the barrier counts warps
-      if (lane == 0) mbar_arrive(bar(B_PAIR + (warp & 3)));
-      ok = mbar_wait_warp(bar(B_PAIR + (warp & 3)), (uint32_t)(j & 1), abort_flag, a.status, STATUS_TIMEOUT_SOFTMAX);
-      if (!ok) break;
-      const float tmax = fmaxf(hm, slot[(hf ^ 1) * 128 + row]) * scale;
-      // lazy rescale: only when the running reference falls far behind
-      const bool need = m_ref != -INFINITY && tmax > m_ref + rescale_gap<F16>();
-      float alpha = 1.f;
-      if (need) {
-        alpha = fast_exp2(m_ref - tmax);
-        m_ref = tmax;
-        l_part *= alpha;
-      } else if (m_ref == -INFINITY) {
-        m_ref = tmax;
-      }
-      if (__any_sync(0xffffffffu, need)) {
-        // O must be quiescent: the previous tile's P V has to be complete
-        ok = mbar_wait_warp(bar(B_PVDONE + ((j - 1) & 1)), (uint32_t)(((j - 1) >> 1) & 1), abort_flag, a.status,
-                            STATUS_TIMEOUT_SOFTMAX);
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll 1
-        for (int c = 0; c < D / 64; ++c) {
-          uint32_t o[32];
-          const uint32_t addr = tmem_base + lane_addr + C::O_COL + hf * (D / 2) + c * 32;
-          tmem_ld32(addr, o);
+        float hm = -INFINITY, least = INFINITY;
+        bool poly = MODE == CAPPED;                        // this half's tanh by polynomial, in the exponential's pass
+        if (active) {
+          tmem_ld32(s_addr, x);
           tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_st32(addr, o);
-        }
-      }
-      if (active) {
-        const float neg_m = m_ref == -INFINITY ? 0.f : p_bias<F16>() - m_ref;
-        uint32_t packed[16];
-        f32x2 sum0 = join(0.f, 0.f), sum1 = sum0;
-        auto exponentials = [&](auto argument) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float e0, e1;
-            split(argument(join(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]))), e0, e1);
-            e0 = fast_exp2(e0);
-            e1 = fast_exp2(e1);
-            packed[i] = pack_pair<F16>(e0, e1);
-            if (i & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
+          const int lo = seen.lo - key0, hi = seen.hi - key0, pre = seen.pre - key0;
+          const bool all = __all_sync(0xffffffffu, (lo <= 0 && hi >= 32) || pre >= 32);
+          if constexpr (MODE == CAPPED) {
+            range32<true>(x, hm, least);
+            poly = all && __all_sync(0xffffffffu, fmaxf(hm, -least) * a.score_scale < TANH_FAR);
+            if (poly) hm = tanh_exp(hm * (a.score_scale * (1.f / TANH_ARG)));
           }
-        };
-        const f32x2 neg2 = join(neg_m, neg_m), scale2 = join(scale, scale);
-        if (MODE == CAPPED && poly) {
-          const f32x2 arg2 = join(a.score_scale, a.score_scale);
-          exponentials([&](f32x2 v) { return capped(mul2(v, arg2), neg2); });
-        } else {
-          exponentials([&](f32x2 v) { return fma2(v, scale2, neg2); });
+          if (!poly) {
+            transform32<MODE>(x, a, slope, p, key0);
+            if (!all) {
+              hide32(x, seen_bits(lo, hi, pre));
+            }
+            hm = -INFINITY;
+            range32<false>(x, hm, least);
+          }
         }
-        float s0, s1;
-        split(add2(sum0, sum1), s0, s1);
-        l_part += s0 + s1;
-        // P lies over this half's own logits; P V takes its 16-key slices from columns 0, 8, 32 and 40
-        tmem_st16(s_addr, packed);
-      }
+        float* slot = mx + b * 256;
+        slot[hf * 128 + row] = hm;
+        __syncwarp();                                      // one arrival per warp: the barrier counts warps
+        if (lane == 0) mbar_arrive(bar(B_PAIR + (warp & 3)));
+        ok = mbar_wait_warp(bar(B_PAIR + (warp & 3)), (uint32_t)(j & 1), abort_flag, a.status, STATUS_TIMEOUT_SOFTMAX);
+        if (!ok) break;
+        const float tmax = fmaxf(hm, slot[(hf ^ 1) * 128 + row]) * scale;
+        // lazy rescale: only when the running reference falls far behind
+        const bool need = m_ref != -INFINITY && tmax > m_ref + rescale_gap<F16>();
+        float alpha = 1.f;
+        if (need) {
+          alpha = fast_exp2(m_ref - tmax);
+          m_ref = tmax;
+          l_part *= alpha;
+        } else if (m_ref == -INFINITY) {
+          m_ref = tmax;
+        }
+        if (__any_sync(0xffffffffu, need)) {
+          // O must be quiescent: the previous tile's P V has to be complete
+          ok = mbar_wait_warp(bar(B_PVDONE + ((j - 1) & 1)), (uint32_t)(((j - 1) >> 1) & 1), abort_flag, a.status,
+                              STATUS_TIMEOUT_SOFTMAX);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 64; ++c) {
+            uint32_t o[32];
+            const uint32_t addr = tmem_base + lane_addr + C::O_COL + hf * (D / 2) + c * 32;
+            tmem_ld32(addr, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st32(addr, o);
+          }
+        }
+        if (active) {
+          const float neg_m = m_ref == -INFINITY ? 0.f : p_bias<F16>() - m_ref;
+          uint32_t packed[16];
+          f32x2 sum0 = join(0.f, 0.f), sum1 = sum0;
+          auto exponentials = [&](auto argument) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float e0, e1;
+              split(argument(join(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]))), e0, e1);
+              e0 = fast_exp2(e0);
+              e1 = fast_exp2(e1);
+              packed[i] = pack_pair<F16>(e0, e1);
+              if (i & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
+            }
+          };
+          const f32x2 neg2 = join(neg_m, neg_m), scale2 = join(scale, scale);
+          if (MODE == CAPPED && poly) {
+            const f32x2 arg2 = join(a.score_scale, a.score_scale);
+            exponentials([&](f32x2 v) { return capped(mul2(v, arg2), neg2); });
+          } else {
+            exponentials([&](f32x2 v) { return fma2(v, scale2, neg2); });
+          }
+          float s0, s1;
+          split(add2(sum0, sum1), s0, s1);
+          l_part += s0 + s1;
+          // P lies over this half's own logits; P V takes its 16-key slices from columns 0, 8, 32 and 40
+          tmem_st16(s_addr, packed);
+        }
       }
       // V's rows behind the document's end (another document's, or anything) are cleared: their P is 0, but 0 * NaN
       // would not vanish.  S's barrier says that the stage has arrived
