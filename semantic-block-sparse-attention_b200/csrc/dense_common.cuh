@@ -95,6 +95,68 @@ __device__ __forceinline__ Tile find_tile(const Args& a, int want) {
   return t;
 }
 
+// The same for more documents than a warp looks at in one step: all threads of the block, a run of documents
+// each.  Two barriers, which every thread has to reach.
+template <int THREADS>
+__device__ __forceinline__ Tile find_tile_block(const Args& a, int want) {
+  __shared__ int totals[THREADS / 32];
+  __shared__ Tile found;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qt = a.queries_per_tile;
+  const int per = (a.docs + THREADS - 1) / THREADS;
+  const int d0 = min((int)threadIdx.x * per, a.docs), d1 = min(d0 + per, a.docs);
+  auto start_of = [&](int d) { return min(max((int64_t)a.cu_q[d], (int64_t)0), a.tokens_q); };
+  auto end_of = [&](int d, int64_t from) { return min(max((int64_t)a.cu_q[d + 1], from), a.tokens_q); };
+  int mine = 0;
+  for (int d = d0; d < d1; ++d) {
+    const int64_t c0 = start_of(d);
+    mine += (int)((end_of(d, c0) - c0 + qt - 1) / qt);
+  }
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) totals[warp] = upto;
+  __syncthreads();
+  int before = upto - mine, all = 0;
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += totals[w];
+    all += totals[w];
+  }
+  if (want >= all) {
+    Tile t{};
+    t.doc = -1;
+    t.first = want - all;
+    return t;                                      // the same answer in every thread
+  }
+  if (want >= before && want < before + mine) {
+    int rest = want - before, d = d0;
+    int64_t c0 = 0, c1 = 0;
+    int tiles = 0;
+    for (;; ++d) {
+      c0 = start_of(d);
+      c1 = end_of(d, c0);
+      tiles = (int)((c1 - c0 + qt - 1) / qt);
+      if (rest < tiles) break;
+      rest -= tiles;
+    }
+    Tile t;
+    t.doc = d;
+    t.first = (tiles - 1 - rest) * qt;
+    t.count = (int)min((int64_t)qt, c1 - c0 - t.first);
+    t.token = c0 + t.first;
+    t.k0 = (int)min(max((int64_t)a.cu_k[d], (int64_t)0), a.tokens_k);
+    t.lk = (int)min(max((int64_t)a.cu_k[d + 1], (int64_t)t.k0), a.tokens_k) - t.k0;
+    t.pos = t.lk - (int)(c1 - c0) + t.first;
+    t.prefix = a.prefix ? min(max(a.prefix[d], 0), t.lk) : 0;
+    found = t;
+  }
+  __syncthreads();
+  return found;
+}
+constexpr int WARP_DOCS = 64;                      // up to here every warp searches for itself
+
 // Rows behind the last document, as zeros with a log-sum-exp of -inf: the spare blocks share them by tiles.
 template <int D>
 __device__ __forceinline__ void zero_tail(const Args& a, int nth, int kv_head, int threads) {
@@ -224,9 +286,9 @@ __device__ __forceinline__ float tanh_far(float y) {
 enum Mode { LINEAR = 0, CAPPED = 1, BIASED = 2, BOUNDED = 3 };
 
 // A cap bounds the scores, so with bf16 P (float's range) a fixed reference will do where 2^(score - reference)
-// stays between 2^-108 and 2^44: no maximum, no rescale of O, and the products P V stay inside float for |v| up to
-// 2^59 even over 2^24 keys.  That is caps up to 52.
-constexpr float BOUNDED_TOP = 44.f, BOUNDED_LOG2 = 76.f;
+// stays between 2^-92 and 2^60: no maximum, no rescale of O, and the products P V stay inside float for |v| from
+// 2^-34 (rows whose scores are all at the lower end) to 2^43 (over 2^24 keys).  That is caps up to 52.
+constexpr float BOUNDED_TOP = 60.f, BOUNDED_LOG2 = 76.f;
 __host__ __device__ inline float bounded_reference(float cap_log2) { return cap_log2 > BOUNDED_TOP ? cap_log2 - BOUNDED_TOP : 0.f; }
 
 // 32 raw scores in place -> what the exponential's scale multiplies.

@@ -123,7 +123,8 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     tma_prefetch_desc(&tmap_v);
   }
   __syncwarp();
-  const Tile tile = find_tile(a, blockIdx.x);      // the same answer in every warp
+  // the same answer in every warp
+  const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, blockIdx.x) : find_tile_block<C::THREADS>(a, blockIdx.x);
   if (tile.doc < 0) {
     if (a.zero_tail) zero_tail<D>(a, tile.first, h, blockDim.x);
     return;

@@ -58,7 +58,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     if (threadIdx.x == 0) atomicCAS(a.status, 0, STATUS_SMEM_ALIGN);
     return;
   }
-  const Tile tile = find_tile(a, blockIdx.x);
+  const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, blockIdx.x) : find_tile_block<320>(a, blockIdx.x);
   if (tile.doc < 0) {
     if (a.zero_tail) zero_tail<D>(a, tile.first, h, blockDim.x);
     return;

@@ -147,6 +147,59 @@ __device__ __forceinline__ Unit find_unit(const AppendArgs& a, int64_t want, Cur
   return u;                              // behind the last one
 }
 
+// The same for a call with many requests: all threads of the block, a run of requests each.
+__device__ __forceinline__ Unit find_unit_block(const AppendArgs& a, int64_t want, uint32_t* slots) {
+  __shared__ Unit found;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int per = (a.batch + blockDim.x - 1) / blockDim.x;
+  const int b0 = min((int)threadIdx.x * per, a.batch), b1 = min(b0 + per, a.batch);
+  struct Run { int64_t row; int n, start, blocks; };
+  auto run_of = [&](int b) {
+    Run r{a.cu[b], 0, a.start[b], 0};
+    r.n = r.row < 0 ? 0 : (int)max((int64_t)0, min((int64_t)a.cu[b + 1], a.tokens) - r.row);
+    if (r.n > 0 && r.start < 0) {
+      atomicCAS(a.status, 0, sm100::STATUS_OVERFLOW);
+      r.n = 0;
+    }
+    if (r.n > 0) r.blocks = (int)(((int64_t)r.start + r.n - 1) >> a.block_log2) - (r.start >> a.block_log2) + 1;
+    return r;
+  };
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) mine += run_of(b).blocks;
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += t;
+  }
+  if (lane == 31) slots[warp] = upto;
+  if (threadIdx.x == 0) found.have = false;
+  __syncthreads();
+  int64_t rest = want - (upto - mine);
+  for (int w = 0; w < warp; ++w) rest -= slots[w];
+  if (rest >= 0 && rest < mine) {
+    int b = b0;
+    Run r = run_of(b);
+    while (rest >= r.blocks) {
+      rest -= r.blocks;
+      r = run_of(++b);
+    }
+    const int block = 1 << a.block_log2, slot = (r.start >> a.block_log2) + (int)rest;
+    Unit u;
+    u.have = true;
+    u.off = rest == 0 ? r.start & (block - 1) : 0;
+    const int64_t pos0 = ((int64_t)slot << a.block_log2) + u.off;
+    u.m = (int)min((int64_t)(block - u.off), (int64_t)r.start + r.n - pos0);
+    u.row = r.row + pos0 - r.start;
+    u.page = slot < a.table_len ? a.table[(int64_t)b * a.table_stride + slot] : -1;
+    if (u.page >= a.cache_blocks) u.page = -1;
+    found = u;
+  }
+  __syncthreads();
+  return found;
+}
+constexpr int WARP_REQUESTS = 64;        // up to here every warp searches for itself
+
 // 2^e * 256 <= largest < 2^e * 512 with 448 as the limit: the exponent of the scale a block needs.
 __device__ __forceinline__ int exponent_for(float largest) {
   const uint32_t bits = __float_as_uint(largest);
@@ -259,7 +312,7 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs a) {
   __shared__ uint32_t slots[16];
   const int h = blockIdx.y, part = blockIdx.z;
   Cursor cursor{0, 0};
-  const Unit u = find_unit(a, blockIdx.x, cursor);
+  const Unit u = a.batch <= WARP_REQUESTS ? find_unit(a, blockIdx.x, cursor) : find_unit_block(a, blockIdx.x, slots);
   if (!u.have) return;                                // the grid covers the largest possible number of blocks
   const uint16_t* src = static_cast<const uint16_t*>(a.src[part]) + u.row * a.src_token[part] + (int64_t)h * a.src_head[part];
   // ---- the new rows into registers, their largest magnitude

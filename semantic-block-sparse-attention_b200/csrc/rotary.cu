@@ -6,7 +6,7 @@
 //
 // with (x1, x2) = (x_i, x_{i + R/2}) in the half layout and (x_2i, x_2i+1) in the interleaved one;
 // dimensions from R on are copied.  Frequencies are doubles and the angle is reduced to a fraction of a
-// turn in double: a float product is off by half a radian at position 1e6 * f = 1, which no later step
+// turn in double: at position 1e6 and f = 1 a float product is off by up to 0.03 radians, which no later step
 // can repair.  sincospi of the reduced fraction is then as accurate as a float can be.
 //
 // Bound: HBM, one read and one write of every element.  A cos/sin costs ~50 instructions and serves all

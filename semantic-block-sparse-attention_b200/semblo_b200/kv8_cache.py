@@ -120,6 +120,7 @@ def _mask_arguments(window, softcap, prefix_lens, alibi_slopes, batch: int, head
     window = int(window or 0)
     if window < 0:
         raise ValueError(f"the window must not be negative (got {window}; 0 is none)")
+    window = min(window, 1 << 30)            # beyond every position, and inside the kernels' arithmetic
     softcap = float(softcap or 0.0)
     if not 0.0 <= softcap < float("inf"):
         raise ValueError(f"the soft cap must be finite and not negative (got {softcap}; 0 is none)")
@@ -140,7 +141,7 @@ def kv8_decode_attention(q: torch.Tensor, cache: Kv8Cache, block_table: torch.Te
                          sm_scale: float, softcap: float | None = None, window: int = 0,
                          prefix_lens: torch.Tensor | None = None, alibi_slopes: torch.Tensor | None = None,
                          out: torch.Tensor | None = None, return_logsumexp: bool = False) -> PagedSparseAttentionResult:
-    """Attention of the last tokens of each request over the 8-bit cache.
+    """Attention of the last tokens of each request (up to 4096 of them) over the 8-bit cache.
 
     ``q`` [B, n, Hq, D] (bf16 or fp16; 1 to 16 queries per request): query i of request b stands at position
     p = lengths[b] - n + i and sees key j < lengths[b] if j <= p (and p - j < ``window``, where one is given) or

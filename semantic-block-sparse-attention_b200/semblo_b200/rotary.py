@@ -123,6 +123,8 @@ def _check_output(name: str, y: torch.Tensor, x: torch.Tensor) -> tuple:
     strides = _check_rows(name, y, x.shape[0], x.shape[2], x.dtype, x.device)
     if y.shape != x.shape:
         raise ValueError(f"{name} must have the shape of its input")
+    if any(n > 1 and s == 0 for n, s in zip(y.shape, strides)):
+        raise ValueError(f"{name} must not repeat memory")
     if _overlaps(x, y) and (x.data_ptr() != y.data_ptr() or x.stride() != y.stride()):
         raise ValueError(f"{name} overlaps its input without being it")
     return strides

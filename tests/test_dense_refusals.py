@@ -114,6 +114,7 @@ def test_rotary_refusals(hostside):
     no(ValueError, q, None, pos, freq, k_out=k)
     buf = torch.zeros(5, 2, 64)
     no(ValueError, buf[:4], None, pos, freq, q_out=buf[1:])
+    no(ValueError, q, None, pos, freq, q_out=torch.zeros(1, 2, 64).expand(4, 2, 64))
     no(RuntimeError, q.clone().requires_grad_(), k, pos, freq)
     with pytest.raises(ValueError):
         rotary.RotaryFrequencies(torch.zeros(4))

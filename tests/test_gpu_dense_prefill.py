@@ -247,3 +247,29 @@ def test_window_matches_the_chunk_kernel(dev):
     # both are within eps of sum |p v| (P) and eps / 2 of the value (output) of the formula
     eps = 2.0 ** -7
     assert bool(((got.output.double() - out.double()).abs() <= (2 * want[2] + want[0].abs()) * eps).all())
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+def test_very_many_documents_and_huge_windows(dev, dim):
+    """More documents than threads in a block, empty ones among them, and a window beyond every position."""
+    lens = [(i * 5) % 4 for i in range(1500)]
+    q, k, v, _ = _inputs(dev, 11, lens, lens, 4, 1, dim, torch.bfloat16)
+    pad = torch.randn(100, 4, dim, device=dev).to(torch.bfloat16)
+    kw = dict(sm_scale=0.1, window=(1 << 40) + 3)
+    got = _call(torch.cat([q, pad]), k, v, lens, lens, **kw)
+    assert bool((got.output[len(q):] == 0).all()) and bool((got.logsumexp[len(q):] == -math.inf).all())
+    plain = _call(q, k, v, lens, lens, sm_scale=0.1)
+    assert torch.equal(got.output[:len(q)], plain.output)
+    _check(plain, _formula(q, k, v, lens, lens, sm_scale=0.1), 3)
+
+
+def test_scores_at_the_lower_end_of_the_cap(dev):
+    """Every score of a row close to -cap, small values: the fixed reference must not run out of range."""
+    for cap in (50.0, 52.0):
+        lens = [300]
+        q, k, v, _ = _inputs(dev, 12, lens, lens, 2, 1, 128, torch.bfloat16)
+        q[...], k[...] = 4.0, -4.0
+        q[::2] *= -1                                             # and every other row close to +cap
+        v *= 2.0 ** -20
+        kw = dict(sm_scale=1.0, softcap=cap)
+        _check(_call(q, k, v, lens, lens, **kw), _formula(q, k, v, lens, lens, **kw), 300)

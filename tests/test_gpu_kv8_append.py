@@ -273,3 +273,10 @@ def test_cache_past_32_bits(dev):
     got = cache.data.view(torch.uint8)[:, [blocks - 1, blocks - 3]]
     assert torch.equal(got, small.data.view(torch.uint8))
     assert torch.equal(cache.scales[:, [blocks - 1, blocks - 3]], small.scales)
+
+
+def test_a_large_batch_of_single_tokens(dev):
+    """More requests than threads in a block, some of them without a token."""
+    new = [(i % 7 != 3) + 0 for i in range(700)]
+    past = [(i * 29) % 64 for i in range(700)]
+    _run_and_compare(*_case(dev, 14, 32, 1, 64, torch.bfloat16, new, past), 32)
