@@ -69,7 +69,7 @@ def dense_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *
         raise ValueError(f"sm_scale must be positive (got {sm_scale})")
     given = out is not None
     if not given:
-        out = torch.empty((tokens_q, hq, dim), dtype=dtype, device=device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != dtype or out.device != device or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("out must be contiguous, 16-byte aligned and have the shape, type and device of q")
     lse = None

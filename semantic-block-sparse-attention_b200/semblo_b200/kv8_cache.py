@@ -173,7 +173,7 @@ def kv8_decode_attention(q: torch.Tensor, cache: Kv8Cache, block_table: torch.Te
     if not q.is_contiguous() or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
     if out is None:
-        out = torch.empty((batch, queries, hq, dim), dtype=dtype, device=device)
+        out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
         raise ValueError("out must be contiguous and have the shape, type and device of q")
     lse = torch.empty((batch, queries, hq), dtype=torch.float32, device=device) if return_logsumexp else None

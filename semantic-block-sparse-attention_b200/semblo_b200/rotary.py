@@ -158,7 +158,7 @@ def apply_rotary(q_pre: torch.Tensor, k_pre: torch.Tensor | None, positions: tor
         raise ValueError(f"the positions ({positions.device}) and frequencies ({inv_freq.device}) must be on the "
                          f"device of q_pre ({device})")
     if q_out is None:
-        q_out, qos = torch.empty((tokens, hq, dim), dtype=dtype, device=device), (hq * dim, dim)
+        q_out, qos = torch.empty_like(q_pre, memory_format=torch.contiguous_format), (hq * dim, dim)
     else:
         qos = _check_output("q_out", q_out, q_pre)
     hkv, k_args = 0, (None, 0, 0, None, 0, 0, 0)
@@ -169,7 +169,7 @@ def apply_rotary(q_pre: torch.Tensor, k_pre: torch.Tensor | None, positions: tor
         ks = _check_rows("k_pre", k_pre, tokens, dim, dtype, device)
         hkv = k_pre.shape[1]
         if k_out is None:
-            k_out, kos = torch.empty((tokens, hkv, dim), dtype=dtype, device=device), (hkv * dim, dim)
+            k_out, kos = torch.empty_like(k_pre, memory_format=torch.contiguous_format), (hkv * dim, dim)
         else:
             kos = _check_output("k_out", k_out, k_pre)
         if hkv:
