@@ -207,9 +207,10 @@ int launch(RotaryArgs& a, bool interleaved, cudaStream_t st) {
   const int most_tokens = std::max(1, 1024 / std::max(1, a.rotary_dim / 2));          // 2 x 8 KB of cos/sin
   int tb = 1, lanes = std::min(rows, a.heads);
   double best = 0;
+  const int sms = semblo::sm_count();
   for (int l = 1; l <= std::min(rows, a.heads); ++l) {
     const int t = std::min(rows / l, most_tokens);
-    if (a.tokens < (int64_t)t * 2 * semblo::sm_count()) continue;
+    if (a.tokens < (int64_t)t * 2 * sms) continue;
     const int64_t slots = ceil_div(ceil_div(a.heads, l), AHEAD) * AHEAD;
     const double used = (double)t * a.heads / ((double)rows * slots);
     if (used >= best) { best = used; tb = t; lanes = l; }
@@ -220,7 +221,7 @@ int launch(RotaryArgs& a, bool interleaved, cudaStream_t st) {
   // many more blocks than fit at once, each with a handful of tiles: with one resident wave the blocks step
   // through memory in lockstep (131072 tokens x 20 heads x 256: 398 us at 64 per multiprocessor, 415 at 16, 500
   // at 3; 8192 x 40 x 128: 30.8, 30.9 and 30.3)
-  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(a.tokens, tb), (int64_t)semblo::sm_count() * 64);
+  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(a.tokens, tb), (int64_t)sms * 64);
   if (interleaved) rotary_kernel<T, NP, true><<<grid, THREADS, smem, st>>>(a);
   else rotary_kernel<T, NP, false><<<grid, THREADS, smem, st>>>(a);
   SEMBLO_LAUNCH_CHECK();

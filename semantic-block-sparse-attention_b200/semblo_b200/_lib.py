@@ -143,6 +143,17 @@ def refuse_gradients(*tensors: torch.Tensor | None) -> None:
                                    "or on tensors that require none")
 
 
+def overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory from the first to the last element of ``a`` meets that of ``b``."""
+    def span(t):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 def raw_stream(index: int) -> int:
     """The current stream of device ``index`` as the C entries take it."""
     return torch._C._cuda_getCurrentRawStream(index)

@@ -10,8 +10,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import check, device_scope, dtype_code, lib, raw_stream, refuse_gradients, require_cuda
-from .kv8_cache import HEAD_DIMS, _mask_arguments, _per_request, _token_rows
+from ._lib import check, device_scope, dtype_code, lib, overlaps, raw_stream, refuse_gradients, require_cuda
+from .kv8_cache import HEAD_DIMS, _mask_arguments, _per_request, _row_arguments
 from .paged_attention import PagedSparseAttentionResult
 
 MAX_GROUP = 128              # query heads per KV head
@@ -31,9 +31,9 @@ def dense_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *
     Scores are q . k sm_scale, then ``softcap`` tanh(score / softcap), then minus alibi_slopes[h] |p - j|.  A row that
     sees nothing gives 0 and a log-sum-exp of -inf.  Rows behind the last document are left
     as they were in a given ``out``, and are 0 without one; their log-sum-exp is -inf.  Keys behind a document's end are never
-    used, whatever they hold; K and V inside a document have to be finite."""
+    used, whatever they hold; K and V inside a document have to be finite.  ``out`` must not overlap an input."""
     require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k, prefix_lens, alibi_slopes, out)
-    refuse_gradients(q, k, v)
+    refuse_gradients(q, k, v, out)
     if q.ndim != 3 or k.ndim != 3 or v.shape != k.shape:
         raise ValueError("q must have shape [Tq, Hq, D], k and v [Tk, Hkv, D]")
     tokens_q, hq, dim = q.shape
@@ -64,7 +64,7 @@ def dense_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *
     window, softcap, prefix_lens, alibi_slopes = _mask_arguments(window, softcap, prefix_lens, alibi_slopes, docs, hq, device)
     if not causal and (window or prefix_lens is not None):
         raise ValueError("a window or a prefix needs the causal mask")
-    q, k, v = _token_rows(q), _token_rows(k), _token_rows(v)
+    (q, *q_rows), (k, *k_rows), (v, *v_rows) = _row_arguments(q), _row_arguments(k), _row_arguments(v)
     if not float(sm_scale) > 0.0:
         raise ValueError(f"sm_scale must be positive (got {sm_scale})")
     given = out is not None
@@ -72,15 +72,16 @@ def dense_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != dtype or out.device != device or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("out must be contiguous, 16-byte aligned and have the shape, type and device of q")
+    elif any(overlaps(out, x) for x in (q, k, v)):
+        raise ValueError("out must not overlap q, k or v")
     lse = None
     if return_logsumexp:
-        lse = torch.empty((tokens_q, hq), dtype=torch.float32, device=device)
+        lse = q.new_empty((tokens_q, hq), dtype=torch.float32)
         if given:
             lse.fill_(float("-inf"))
     with device_scope(device):
         check(lib().semblo_dense_prefill(
-            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-            v.stride(1), tokens_q, tokens_k, hq, hkv, dim, dtype_code(dtype, "prefill"), cu_q.data_ptr(), cu_k.data_ptr(),
+            *q_rows, *k_rows, *v_rows, tokens_q, tokens_k, hq, hkv, dim, dtype_code(dtype, "prefill"), cu_q.data_ptr(), cu_k.data_ptr(),
             docs, bool(causal), window, None if prefix_lens is None else prefix_lens.data_ptr(), sm_scale, softcap,
             None if alibi_slopes is None else alibi_slopes.data_ptr(), out.data_ptr(), not given,
             None if lse is None else lse.data_ptr(), _lib.status_for(device).word.data_ptr(), raw_stream(device.index)))

@@ -11,7 +11,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import check, device_scope, dtype_code, lib, raw_stream, refuse_gradients, require_cuda, require_same_device
+from ._lib import (check, device_scope, dtype_code, lib, overlaps, raw_stream, refuse_gradients, require_cuda,
+                   require_same_device)
 from .paged_attention import PagedSparseAttentionResult
 
 BLOCK_SIZES = (16, 32, 64, 128, 256)
@@ -66,15 +67,25 @@ def _block_table(table: torch.Tensor, batch: int) -> torch.Tensor:
 def _per_request(name: str, x: torch.Tensor, n: int) -> torch.Tensor:
     if x.shape != (n,) or x.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be {n} int32 or int64 values (got {x.dtype} {tuple(x.shape)})")
-    return (x if x.dtype == torch.int32 else x.to(torch.int32)).contiguous()
+    if x.dtype != torch.int32:
+        x = x.to(torch.int32)
+    return x if x.is_contiguous() else x.contiguous()
 
 
 def _token_rows(x: torch.Tensor) -> torch.Tensor:
     """x [T, H, D] as the kernels read it: contiguous heads of a 16-byte aligned start and step."""
+    return _row_arguments(x)[0]
+
+
+def _row_arguments(x: torch.Tensor) -> tuple:
+    """(the rows as the kernels read them, their address, token stride, head stride)"""
     s0, s1, s2 = x.stride()
-    if s2 == 1 and x.data_ptr() % 16 == 0 and s0 % 8 == 0 and s1 % 8 == 0 and s0 > 0 and s1 > 0:
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
+    address = x.data_ptr()
+    if s2 != 1 or (address | 2 * s0 | 2 * s1) & 15 or s0 <= 0 or s1 <= 0:
+        x = x.clone(memory_format=torch.contiguous_format)
+        address = x.data_ptr()
+        s0, s1, _ = x.stride()
+    return x, address, s0, s1
 
 
 def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -102,14 +113,15 @@ def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, block_table: t
     require_same_device(cache.data, k, v, block_table, cu_seqlens, start_positions)
     table = _block_table(block_table, batch)
     cu, start = _per_request("cu_seqlens", cu_seqlens, batch + 1), _per_request("start_positions", start_positions, batch)
-    k, v = _token_rows(k), _token_rows(v)
-    with device_scope(k.device):
+    (k, *k_rows), (v, *v_rows) = _row_arguments(k), _row_arguments(v)
+    device = k.device
+    with device_scope(device):
         check(lib().semblo_kv8_append(
-            k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2], shape[0],
+            *k_rows, *v_rows, shape[0],
             dtype_code(k.dtype, "append"), cache.data.data_ptr(), cache.scales.data_ptr(), cache.num_blocks,
             cache.block_size, cache.num_kv_heads, cache.head_dim, table.data_ptr(), table.stride(0), table.shape[1],
-            cu.data_ptr(), start.data_ptr(), batch, _lib.status_for(k.device).word.data_ptr(),
-            raw_stream(k.device.index)))
+            cu.data_ptr(), start.data_ptr(), batch, _lib.status_for(device).word.data_ptr(),
+            raw_stream(device.index)))
 
 
 MAX_QUERIES = 16
@@ -147,10 +159,11 @@ def kv8_decode_attention(q: torch.Tensor, cache: Kv8Cache, block_table: torch.Te
     p = lengths[b] - n + i and sees key j < lengths[b] if j <= p (and p - j < ``window``, where one is given) or
     j < prefix_lens[b].  Scores are q . k sm_scale, then ``softcap`` tanh(score / softcap), then minus
     alibi_slopes[h] |p - j|.  A row that sees nothing (a length of 0, a position below 0) gives 0 and a log-sum-exp
-    of -inf.  The result [B, n, Hq, D] has the type of ``q``; log-sum-exps are natural, fp32 [B, n, Hq].  Table
+    of -inf.  The result [B, n, Hq, D] (``out``, apart from the
+    inputs, where it is given) has the type of ``q``; log-sum-exps are natural, fp32 [B, n, Hq].  Table
     entries outside the pool are taken as absent and set status 201, as does a length beyond the table."""
     require_cuda(q, cache.data, block_table, lengths, prefix_lens, alibi_slopes, out)
-    refuse_gradients(q)
+    refuse_gradients(q, out)
     if q.ndim != 4:
         raise ValueError("q must have shape [B, n, Hq, D]")
     batch, queries, hq, dim = q.shape
@@ -176,7 +189,9 @@ def kv8_decode_attention(q: torch.Tensor, cache: Kv8Cache, block_table: torch.Te
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
         raise ValueError("out must be contiguous and have the shape, type and device of q")
-    lse = torch.empty((batch, queries, hq), dtype=torch.float32, device=device) if return_logsumexp else None
+    elif overlaps(out, q) or overlaps(out, cache.data):
+        raise ValueError("out must not overlap q or the cache")
+    lse = q.new_empty((batch, queries, hq), dtype=torch.float32) if return_logsumexp else None
     width = table.shape[1]
     with device_scope(device):
         nbytes = lib().semblo_kv8_decode_workspace_bytes(batch, queries, hq, cache.num_kv_heads, dim, cache.block_size,
@@ -184,7 +199,7 @@ def kv8_decode_attention(q: torch.Tensor, cache: Kv8Cache, block_table: torch.Te
         if nbytes < 0:
             check(int(nbytes))
         # made for this call: a recorded graph keeps its own, and calls on two streams do not share one
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        workspace = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         check(lib().semblo_kv8_decode(
             q.data_ptr(), dtype_code(dtype, "decode"), batch, queries, hq, cache.num_kv_heads, dim,
             cache.data.data_ptr(), cache.scales.data_ptr(), cache.num_blocks, cache.block_size, table.data_ptr(),

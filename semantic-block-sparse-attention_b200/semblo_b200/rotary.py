@@ -12,7 +12,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import check, device_scope, dtype_code, lib, raw_stream, refuse_gradients, require_cuda
+from ._lib import check, device_scope, dtype_code, lib, overlaps, raw_stream, refuse_gradients, require_cuda
 
 _SCALING_KEYS = {"linear": {"factor"}, "ntk": {"factor"},
                  "yarn": {"factor", "original_max_position", "beta_fast", "beta_slow", "attention_factor"},
@@ -109,23 +109,13 @@ def _check_rows(name: str, x: torch.Tensor, tokens: int, dim: int, dtype, device
     return strides
 
 
-def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
-    def span(t):
-        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
-
-
 def _check_output(name: str, y: torch.Tensor, x: torch.Tensor) -> tuple:
     strides = _check_rows(name, y, x.shape[0], x.shape[2], x.dtype, x.device)
     if y.shape != x.shape:
         raise ValueError(f"{name} must have the shape of its input")
     if any(n > 1 and s == 0 for n, s in zip(y.shape, strides)):
         raise ValueError(f"{name} must not repeat memory")
-    if _overlaps(x, y) and (x.data_ptr() != y.data_ptr() or x.stride() != y.stride()):
+    if overlaps(x, y) and (x.data_ptr() != y.data_ptr() or x.stride() != y.stride()):
         raise ValueError(f"{name} overlaps its input without being it")
     return strides
 
@@ -141,7 +131,7 @@ def apply_rotary(q_pre: torch.Tensor, k_pre: torch.Tensor | None, positions: tor
     with ``interleaved``; the others are copied.  ``inverse`` rotates back (the transpose).  ``q_out`` / ``k_out``
     receive the result; either may be its input itself (in place).  Angles are formed in 64 bits."""
     require_cuda(q_pre, k_pre, positions, q_out, k_out)
-    refuse_gradients(q_pre, k_pre)
+    refuse_gradients(q_pre, k_pre, q_out, k_out)
     if q_pre.ndim != 3:
         raise ValueError("q_pre must have shape [T, Hq, D]")
     tokens, hq, dim = q_pre.shape

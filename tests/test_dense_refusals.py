@@ -188,6 +188,9 @@ def test_decode_refusals(hostside):
     no(ValueError, alibi_slopes=torch.zeros(4, dtype=torch.float64))
     no(ValueError, out=torch.zeros(3, 1, 4, 64))
     no(ValueError, out=torch.zeros(3, 1, 64, 4, dtype=torch.bfloat16).transpose(2, 3))
+    no(ValueError, out=q)
+    no(ValueError, out=cache.data.view(torch.bfloat16).view(-1)[:768].view(3, 1, 4, 64))
+    no(RuntimeError, out=torch.zeros_like(q).requires_grad_())
     no(RuntimeError, q=q.clone().requires_grad_())
 
 
@@ -227,6 +230,11 @@ def test_dense_prefill_refusals(hostside):
     no(ValueError, alibi_slopes=torch.zeros(2))
     no(ValueError, out=torch.zeros(5, 4, 64))
     no(ValueError, out=torch.zeros(6, 4, 64, dtype=torch.float16)[:5, :, ::1].transpose(0, 1))
+    no(ValueError, out=q)
+    big = torch.zeros(20, 2, 64, dtype=torch.float16)
+    no(ValueError, k=big[:7], v=big[12:19], out=big[2:12].view(5, 4, 64))
+    no(ValueError, k=big[:7], v=big[12:19], out=big[9:19].view(5, 4, 64))
+    no(RuntimeError, out=torch.zeros_like(q).requires_grad_())
     no(RuntimeError, k=k.clone().requires_grad_())
 
 
