@@ -24,8 +24,9 @@
 //
 // Work is split evenly whatever the lengths: the 16-key groups of all (request, KV head, row tile) segments
 // form one line, every block takes an equal piece of it, writes the segments that lie inside its piece and
-// leaves partials of those that do not; a second launch (a programmatic dependent) merges them.  Where no
-// segment can be longer than 64 groups, a block takes one segment and there is nothing to merge.
+// leaves partials of those that do not; a second launch (a programmatic dependent) merges them.  Where the
+// lengths turn out short, blocks take whole segments, and where the table allows no segment of more than 64
+// groups, there is no second launch.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -137,13 +138,14 @@ __device__ __forceinline__ Span span_of(const DecodeArgs& a, int b) {
 
 template <int D, int NT>
 struct Cfg {
-  static constexpr int STAGES = D == 256 ? 3 : D == 128 ? 3 : 4;
+  static constexpr int STAGES = D == 256 ? 3 : D == 128 ? (NT > 2 ? 4 : 3) : 4;
   static constexpr int KV_BYTES = GROUP * D;                    // K or V of a group
   static constexpr int RING = STAGES * 2 * KV_BYTES;            // per warp
   static constexpr int KC = D / 32;                             // 16-byte pieces of K per lane
   static constexpr int VI = D == 256 ? 2 : 1;                   // pieces of V per lane and key (16 bytes, 8 for D = 64)
   static constexpr int KSTEPS = D / 16;
   static constexpr int ROWS = 8 * NT;
+  static constexpr int PER_SM = D == 256 || NT > 2 || (D == 128 && NT == 2) ? 1 : 2;     // resident blocks
   static constexpr bool Q_SMEM = D * NT > 256;                  // the query's fragments do not fit in registers
   static constexpr int ACC = KSTEPS * NT * 4;                   // accumulators of O^T per lane
   static constexpr int RECORD = ACC * 32 + 3 * ROWS;            // floats: O fragments, then m, M, l of each row
@@ -151,39 +153,52 @@ struct Cfg {
   static constexpr int ML_OFF = META_OFF + WARPS * STAGES * 8;  // float [3][WARPS][ROWS]
   static constexpr int FAC_OFF = ML_OFF + 3 * WARPS * ROWS * 4; // float [WARPS][ROWS] factors, [3][ROWS] totals
   static constexpr int Q_OFF = FAC_OFF + (WARPS + 3) * ROWS * 4;
-  static constexpr int SUM_OFF = Q_OFF + (Q_SMEM ? KSTEPS * NT * 32 * 8 : 0);   // int [batch + 1], then [WARPS]
+  static constexpr int SUM_OFF = Q_OFF + (Q_SMEM ? KSTEPS * NT * 32 * 8 : 0);   // int [batch + 1], then [2 WARPS + 1]
   static_assert(ACC * 32 * 4 <= RING, "a warp's O must fit its ring");
 };
 
-// Inclusive sums of groups * segments-per-request over the batch into sums[1 ...]; sums[0] = 0.
-__device__ __forceinline__ void line_sums(const DecodeArgs& a, int segs, int* sums, int* scratch) {
+// Inclusive sums of groups * segments-per-request over the batch into sums[1 ...]; sums[0] = 0.  Returns the most
+// groups of a segment.
+__device__ __forceinline__ int line_sums(const DecodeArgs& a, int segs, int* sums, int* scratch) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  int carry = 0;
+  int carry = 0, longest = 0;
   for (int b0 = 0; b0 < a.batch; b0 += blockDim.x) {
     const int b = b0 + threadIdx.x;
-    int v = b < a.batch ? span_of(a, b).groups * segs : 0;
+    const int groups = b < a.batch ? span_of(a, b).groups : 0;
+    longest = max(longest, groups);
+    int v = groups * segs;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int t = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += t;
     }
-    if (lane == 31) scratch[warp] = v;
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (lane == 31) { scratch[warp] = v; scratch[warps + warp] = longest; }
     __syncthreads();
     int before = carry;
     for (int w = 0; w < warps; ++w) {
       const int t = scratch[w];
       if (w < warp) before += t;
       carry += t;
+      longest = max(longest, scratch[warps + w]);
     }
     if (b < a.batch) sums[b + 1] = before + v;
     __syncthreads();
   }
   if (threadIdx.x == 0) sums[0] = 0;
   __syncthreads();
+  return longest;
 }
 
 __device__ __forceinline__ int quota_of(int total, int blocks) {
   return max(WARPS, (total + blocks - 1) / blocks);
+}
+
+// Whether a block takes whole segments: where the rounds that this needs cost less than even pieces with their
+// merge, which is worth DIRECT_GROUPS of them.  Tables are as wide as the longest request may grow, so that what
+// the launch is sized for says little about the lengths in it.
+__device__ __forceinline__ bool takes_whole(int segments, int longest, int quota, int blocks) {
+  return (int64_t)((segments + blocks - 1) / blocks) * longest <= quota + DIRECT_GROUPS;
 }
 
 // Element e of a record in fragment order -> row of the tile and dimension.
@@ -197,24 +212,20 @@ __device__ __forceinline__ void element_of(int e, int& row, int& dim) {
   else dim = 16 * g + (x & 15) + 128 * (x >> 4);
 }
 
-__device__ __forceinline__ void store_value(const DecodeArgs& a, int64_t at, float v) {
-  if (a.q_f16) static_cast<__half*>(a.out)[at] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
+// Row of the output [B, n, Hq] of row `row` (query, head of the group) of KV head h.
+__device__ __forceinline__ int64_t output_row(const DecodeArgs& a, int b, int h, int row) {
+  const int qi = row / a.group;
+  return ((int64_t)b * a.queries + qi) * a.num_q_heads + h * a.group + row - qi * a.group;
 }
 
-// One output value (and, with dimension 0, the row's log-sum-exp) from the sum of P' codes and the references.
-template <int D>
-__device__ __forceinline__ void finish(const DecodeArgs& a, int b, int h, int row, int dim, float acc, float m, float mv,
-                                       float l) {
-  const int qi = row / a.group;
-  const int64_t at = ((int64_t)b * a.queries + qi) * a.num_q_heads + h * a.group + row - qi * a.group;
-  store_value(a, at * D + dim, l == 0.f ? 0.f : acc * (sm100::fast_exp2(mv - m - P_BIAS) / l));
-  if (dim == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2;
+// From the sum of P' codes to the output, by the references.
+__device__ __forceinline__ float finish_factor(float m, float mv, float l) {
+  return sm100::fast_exp2(mv - m - P_BIAS) / l;
 }
 
 // ---------------------------------------------------------------- attention
 template <int D, int NT, bool CAP>
-__global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_decode_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__(THREADS, Cfg<D, NT>::PER_SM) kv8_decode_kernel(const DecodeArgs a) {
   using C = Cfg<D, NT>;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -229,26 +240,29 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
   const uint32_t ring_u32 = sm100::smem_u32(ring), meta_u32 = sm100::smem_u32(meta);
   const int segs = a.num_kv_heads * a.row_tiles;
 
-  int pos, end, quota = 0;
-  if (a.direct) {
-    pos = 0; end = 1;
-  } else {
-    line_sums(a, segs, sums, scratch);
-    const int total = sums[a.batch];
-    quota = quota_of(total, gridDim.x);
-    pos = (int)min((int64_t)total, (int64_t)blockIdx.x * quota);
-    end = min(total, pos + quota);
+  // positions are segments where blocks take whole ones, groups on the line otherwise
+  int pos = blockIdx.x, end = a.batch * segs;
+  int* const whole = scratch + 2 * WARPS;                           // read again for every segment: no register through its loop
+  if (!a.direct) {
+    const int longest = line_sums(a, segs, sums, scratch), total = sums[a.batch], quota = quota_of(total, gridDim.x);
+    const bool w = takes_whole(end, longest, quota, gridDim.x);
+    if (threadIdx.x == 0) *whole = w;
+    __syncthreads();
+    if (!w) {
+      pos = (int)min((int64_t)total, (int64_t)blockIdx.x * quota);
+      end = min(total, pos + quota);
+    }
   }
 
   while (pos < end) {
     // ---- the segment at pos
     int b, seg, i0, i1;
     Span sp;
-    if (a.direct) {
-      b = blockIdx.x / segs; seg = blockIdx.x - b * segs;
+    if (a.direct || *whole) {
+      b = pos / segs; seg = pos - b * segs;
       sp = span_of(a, b);
       i0 = 0; i1 = sp.groups;
-      pos = end;
+      pos += gridDim.x;
     } else {
       int lo = 0, hi = a.batch;                                 // the last request that starts at or before pos
       while (hi - lo > 1) {
@@ -265,6 +279,22 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
     }
     const int h = seg / a.row_tiles, row0 = (seg - h * a.row_tiles) * C::ROWS;
     if (a.lengths[b] > sp.length && threadIdx.x == 0) atomicCAS(a.status, 0, sm100::STATUS_OVERFLOW);
+
+    // ---- the query's rows, on their way while the first groups are looked up
+    uint2 raw[NT][C::KSTEPS];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = row0 + nt * 8 + g;
+      const bool have = r < a.rows;
+      const int qi = have ? r / a.group : 0;
+      const int64_t qrow = ((int64_t)b * a.queries + qi) * a.num_q_heads + h * a.group + (have ? r - qi * a.group : 0);
+#pragma unroll
+      for (int s = 0; s < C::KSTEPS; ++s) {
+        raw[nt][s] = make_uint2(0u, 0u);
+        if (have) raw[nt][s] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.q) + qrow * D +
+                                                                    64 * (s >> 2) + 16 * t + 4 * (s & 3)));
+      }
+    }
 
     // ---- pipeline over this warp's groups
     const int count = max(0, (i1 - i0 - warp + WARPS - 1) / WARPS);
@@ -340,11 +370,6 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
     float slope[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = row0 + nt * 8 + g;
-      const bool have = r < a.rows;
-      const int qi = have ? r / a.group : 0;
-      const int64_t qrow = ((int64_t)b * a.queries + qi) * a.num_q_heads + h * a.group + (have ? r - qi * a.group : 0);
-      uint2 raw[C::KSTEPS];
       float top = 0.f;
       auto pair = [&](uint32_t w) -> float2 {
         if (a.q_f16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
@@ -352,10 +377,7 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
       };
 #pragma unroll
       for (int s = 0; s < C::KSTEPS; ++s) {
-        raw[s] = make_uint2(0u, 0u);
-        if (have) raw[s] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.q) + qrow * D + 64 * (s >> 2) +
-                                                                16 * t + 4 * (s & 3)));
-        const float2 x = pair(raw[s].x), y = pair(raw[s].y);
+        const float2 x = pair(raw[nt][s].x), y = pair(raw[nt][s].y);
         top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -366,7 +388,7 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
       const float down = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
       for (int s = 0; s < C::KSTEPS; ++s) {
-        const float2 x = pair(raw[s].x), y = pair(raw[s].y);
+        const float2 x = pair(raw[nt][s].x), y = pair(raw[nt][s].y);
         const uint2 f = make_uint2(half2_bits(x.x * down, x.y * down), half2_bits(y.x * down, y.y * down));
         if constexpr (C::Q_SMEM) {
           if (warp == 0) q_frag[(s * NT + nt) * 32 + lane] = f;
@@ -585,17 +607,42 @@ __global__ void __launch_bounds__(THREADS, (D == 256 || NT == 2) ? 1 : 2) kv8_de
     __syncthreads();
     const bool complete = i0 == 0 && i1 == sp.groups;
     float* record = complete ? nullptr : a.partial + ((int64_t)blockIdx.x * 2 + (i0 == 0 ? 1 : 0)) * C::RECORD;
-    for (int e = threadIdx.x; e < C::ACC * 32; e += THREADS) {
+    // a thread takes 8 consecutive dimensions of a row: values c and c + 2 of a lane's four fragments
+    constexpr int QUADS = C::KSTEPS / 4;
+    for (int i = threadIdx.x; i < NT * QUADS * 64; i += THREADS) {
+      const int e0 = (i >> 6) * 512 + (i & 63);
       int r, dim;
-      element_of<D, NT>(e, r, dim);
-      float acc = 0.f;
+      element_of<D, NT>(e0, r, dim);
+      float acc[8];
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w)
-        acc += reinterpret_cast<const float*>(smem + w * C::RING)[e] * factors[w * C::ROWS + r];
+      for (int x = 0; x < 8; ++x) acc[x] = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float f = factors[w * C::ROWS + r];
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          acc[x] += reinterpret_cast<const float*>(smem + w * C::RING)[e0 + (x >> 1) * 128 + (x & 1) * 64] * f;
+      }
       if (!complete) {
-        record[e] = acc;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) record[e0 + (x >> 1) * 128 + (x & 1) * 64] = acc[x];
       } else if (row0 + r < a.rows) {
-        finish<D>(a, b, h, row0 + r, dim, acc, totals[r], totals[C::ROWS + r], totals[2 * C::ROWS + r]);
+        const float lt = totals[2 * C::ROWS + r], f = finish_factor(totals[r], totals[C::ROWS + r], lt);
+        const int64_t at = output_row(a, b, h, row0 + r);
+        uint4 o8;
+        uint32_t* const words = reinterpret_cast<uint32_t*>(&o8);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float lo = lt == 0.f ? 0.f : acc[2 * x] * f, hi = lt == 0.f ? 0.f : acc[2 * x + 1] * f;
+          if (a.q_f16) {
+            words[x] = half2_bits(lo, hi);
+          } else {
+            const __nv_bfloat162 y = __floats2bfloat162_rn(lo, hi);
+            words[x] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+        }
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at * D + dim) = o8;
+        if (dim == 0 && a.lse) a.lse[at] = lt == 0.f ? -INFINITY : (totals[r] + __log2f(lt)) * LN2;
       }
     }
     if (!complete && threadIdx.x < 3 * C::ROWS) record[C::ACC * 32 + threadIdx.x] = totals[threadIdx.x];
@@ -616,13 +663,14 @@ __global__ void __launch_bounds__(THREADS) kv8_merge_kernel(const DecodeArgs a, 
   int* scratch = sums + a.batch + 1;
   const int segs = a.num_kv_heads * a.row_tiles;
   const int b = blockIdx.x / segs, seg = blockIdx.x - b * segs;
-  line_sums(a, segs, sums, scratch);
+  const int longest = line_sums(a, segs, sums, scratch);
   const Span sp = span_of(a, b);
   const int quota = quota_of(sums[a.batch], blocks);
   const int s0 = sums[b] + seg * sp.groups, s1 = s0 + sp.groups;
   const int c0 = s0 / quota, c1 = sp.groups ? (s1 - 1) / quota : c0;
   sm100::pdl_wait();                                  // every block waits: this launch must not end before the other
-  if (sp.groups > 0 && c0 == c1) return;              // one block had it whole
+  // one block had it whole
+  if ((sp.groups > 0 && c0 == c1) || takes_whole(a.batch * segs, longest, quota, blocks)) return;
   const int parts = sp.groups ? c1 - c0 + 1 : 0;
   // the block where the segment starts left it in its slot 1, the others in their slot 0
   auto record = [&](int i) { return a.partial + ((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * C::RECORD; };
@@ -657,7 +705,12 @@ __global__ void __launch_bounds__(THREADS) kv8_merge_kernel(const DecodeArgs a, 
   float acc = 0.f;
 #pragma unroll 8
   for (int i = 0; i < parts; ++i) acc += record(i)[e] * factors[i * C::ROWS + r];
-  finish<D>(a, b, h, row0 + r, dim, acc, totals[r], totals[C::ROWS + r], totals[2 * C::ROWS + r]);
+  const float lt = totals[2 * C::ROWS + r];
+  const float value = lt == 0.f ? 0.f : acc * finish_factor(totals[r], totals[C::ROWS + r], lt);
+  const int64_t at = output_row(a, b, h, row0 + r);
+  if (a.q_f16) static_cast<__half*>(a.out)[at * D + dim] = __float2half_rn(value);
+  else static_cast<__nv_bfloat16*>(a.out)[at * D + dim] = __float2bfloat16_rn(value);
+  if (dim == 0 && a.lse) a.lse[at] = lt == 0.f ? -INFINITY : (totals[r] + __log2f(lt)) * LN2;
 }
 
 struct Plan {
@@ -670,10 +723,9 @@ Plan plan_for(int64_t segments, int64_t longest) {
   using C = Cfg<D, NT>;
   Plan p;
   p.direct = longest <= DIRECT_GROUPS;
-  const int64_t per_sm = (D == 256 || NT == 2) ? 1 : 2;
   // no more blocks than there can be pieces of WARPS groups
   p.blocks = (int)(p.direct ? segments
-                            : std::min<int64_t>(semblo::sm_count() * per_sm, ceil_div(segments * longest, WARPS)));
+                            : std::min<int64_t>((int64_t)semblo::sm_count() * C::PER_SM, ceil_div(segments * longest, WARPS)));
   p.bytes = p.direct ? 0 : (int64_t)p.blocks * 2 * C::RECORD * 4;
   return p;
 }
@@ -687,7 +739,7 @@ int64_t longest_segment(int queries, int window, int table_len, int block_size, 
 template <int D, int NT, bool CAP>
 int launch(DecodeArgs& a, const Plan& plan, cudaStream_t st) {
   using C = Cfg<D, NT>;
-  const int sums = (a.batch + 1 + WARPS) * 4;
+  const int sums = (a.batch + 2 + 2 * WARPS) * 4;
   const int smem = C::SUM_OFF + sums;
   auto kern = kv8_decode_kernel<D, NT, CAP>;
   SEMBLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
@@ -721,9 +773,11 @@ int check_shape(int batch, int queries, int num_q_heads, int num_kv_heads, int h
   SEMBLO_REQUIRE(batch >= 0 && batch <= 4096, "at most 4096 requests (got %d)", batch);
   SEMBLO_REQUIRE(table_len >= 0 && window >= 0, "negative table length or window");
   *rows = queries * (num_q_heads / num_kv_heads);
-  *nt = *rows <= 8 ? 1 : 2;
-  *tiles = (int)ceil_div(*rows, 8 * *nt);
-  const int64_t groups = ceil_div((int64_t)table_len * block_size, 16);
+  // the widest tiles whose O stays in registers (the cache is read and widened once per tile), as narrow as
+  // that number of tiles allows
+  *tiles = (int)ceil_div(*rows, head_dim == 256 ? 16 : 32);
+  *nt = (int)ceil_div(ceil_div(*rows, *tiles), 8);
+  const int64_t groups = std::max<int64_t>(1, ceil_div((int64_t)table_len * block_size, 16));
   SEMBLO_REQUIRE(groups * batch * num_kv_heads * *tiles < ((int64_t)1 << 31), "batch x context is too large for one call");
   return 0;
 }
@@ -731,6 +785,7 @@ int check_shape(int batch, int queries, int num_q_heads, int num_kv_heads, int h
 Plan plan_of(int head_dim, int nt, int64_t segments, int64_t longest) {
 #define SEMBLO_PLAN(DD, NN) if (head_dim == DD && nt == NN) return plan_for<DD, NN>(segments, longest);
   SEMBLO_PLAN(64, 1) SEMBLO_PLAN(64, 2) SEMBLO_PLAN(128, 1) SEMBLO_PLAN(128, 2) SEMBLO_PLAN(256, 1)
+  SEMBLO_PLAN(64, 3) SEMBLO_PLAN(64, 4) SEMBLO_PLAN(128, 3) SEMBLO_PLAN(128, 4)
 #undef SEMBLO_PLAN
   return plan_for<256, 2>(segments, longest);
 }
@@ -763,8 +818,8 @@ extern "C" int semblo_kv8_decode(const void* q, int dtype, int batch, int querie
   SEMBLO_REQUIRE(softcap >= 0.f, "the soft cap must not be negative");
   if (batch == 0) return 0;
   SEMBLO_REQUIRE(q && cache && scales && block_table && lengths && out && status, "null pointer");
-  SEMBLO_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache)) & 15) == 0,
-                 "q and the cache must be 16-byte aligned");
+  SEMBLO_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
+                 "q, the cache and out must be 16-byte aligned");
   const Plan plan = plan_of(head_dim, nt, (int64_t)batch * num_kv_heads * tiles,
                             longest_segment(queries, window, table_len, block_size, prefix_lens != nullptr));
   if (plan.bytes > workspace_bytes || (plan.bytes && !workspace))
@@ -789,7 +844,7 @@ extern "C" int semblo_kv8_decode(const void* q, int dtype, int batch, int querie
   if (head_dim == DD && nt == NN)                                                                 \
     return cap ? launch<DD, NN, true>(a, plan, st) : launch<DD, NN, false>(a, plan, st);
   SEMBLO_DECODE(64, 1) SEMBLO_DECODE(64, 2) SEMBLO_DECODE(128, 1) SEMBLO_DECODE(128, 2) SEMBLO_DECODE(256, 1)
-  SEMBLO_DECODE(256, 2)
+  SEMBLO_DECODE(256, 2) SEMBLO_DECODE(64, 3) SEMBLO_DECODE(64, 4) SEMBLO_DECODE(128, 3) SEMBLO_DECODE(128, 4)
 #undef SEMBLO_DECODE
   return semblo::fail(semblo::SEMBLO_EINVAL, "unreachable");
 }

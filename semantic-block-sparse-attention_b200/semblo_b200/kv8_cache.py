@@ -187,8 +187,8 @@ def kv8_decode_attention(q: torch.Tensor, cache: Kv8Cache, block_table: torch.Te
         q = q.clone(memory_format=torch.contiguous_format)
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
-        raise ValueError("out must be contiguous and have the shape, type and device of q")
+    elif out.shape != q.shape or out.dtype != dtype or out.device != device or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError("out must be contiguous, 16-byte aligned and have the shape, type and device of q")
     elif overlaps(out, q) or overlaps(out, cache.data):
         raise ValueError("out must not overlap q or the cache")
     lse = q.new_empty((batch, queries, hq), dtype=torch.float32) if return_logsumexp else None

@@ -189,6 +189,7 @@ def test_decode_refusals(hostside):
     no(ValueError, out=torch.zeros(3, 1, 4, 64))
     no(ValueError, out=torch.zeros(3, 1, 64, 4, dtype=torch.bfloat16).transpose(2, 3))
     no(ValueError, out=q)
+    no(ValueError, out=torch.zeros(769, dtype=torch.bfloat16)[1:].view(3, 1, 4, 64))
     no(ValueError, out=cache.data.view(torch.bfloat16).view(-1)[:768].view(3, 1, 4, 64))
     no(RuntimeError, out=torch.zeros_like(q).requires_grad_())
     no(RuntimeError, q=q.clone().requires_grad_())
