@@ -652,14 +652,21 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NT>::PER_SM) kv8_decode_kernel
 }
 
 // ---------------------------------------------------------------- segments that more than one block worked on
-// blockIdx.x: segment; blockIdx.y: 256 of its record's elements.
+// blockIdx: segment; of its fragments of 16 dimensions every gridDim.y-th; 8 of its rows.  The 8 warps take the
+// parts in turn, a lane 4 of a fragment's 128 values; the first of them are on their way while the references and
+// sums of all parts become a factor each.  One thread per value with the parts one after the other took 16 us
+// for 524288 keys x 4 heads x 256 (of 186 in all), this takes 6.
+constexpr int MERGE_AHEAD = 4;
+
 template <int D, int NT>
 __global__ void __launch_bounds__(THREADS) kv8_merge_kernel(const DecodeArgs a, int blocks) {
   using C = Cfg<D, NT>;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* factors = reinterpret_cast<float*>(smem);              // [blocks][ROWS]
-  float* totals = factors + blocks * C::ROWS;                   // [3][ROWS]
-  int* sums = reinterpret_cast<int*>(totals + 3 * C::ROWS);
+  float4* slots = reinterpret_cast<float4*>(smem);              // [WARPS][32]
+  float* most = reinterpret_cast<float*>(slots + WARPS * 32);   // [2][WARPS][8]
+  float* sum_l = most + 2 * WARPS * 8;                          // [WARPS][8]
+  float* state = sum_l + WARPS * 8;                             // [3][blocks][8]: m, M (then the factor), l of each part
+  int* sums = reinterpret_cast<int*>(state + 3 * blocks * 8);
   int* scratch = sums + a.batch + 1;
   const int segs = a.num_kv_heads * a.row_tiles;
   const int b = blockIdx.x / segs, seg = blockIdx.x - b * segs;
@@ -674,43 +681,95 @@ __global__ void __launch_bounds__(THREADS) kv8_merge_kernel(const DecodeArgs a, 
   const int parts = sp.groups ? c1 - c0 + 1 : 0;
   // the block where the segment starts left it in its slot 1, the others in their slot 0
   auto record = [&](int i) { return a.partial + ((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * C::RECORD; };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int r = warp; r < C::ROWS; r += WARPS) {
-    float mt = -INFINITY, mvt = -INFINITY, lt = 0.f;
-    for (int i = lane; i < parts; i += 32) {
-      const float* x = record(i) + C::ACC * 32;
-      mt = fmaxf(mt, x[r]);
-      mvt = fmaxf(mvt, x[C::ROWS + r]);
-    }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nt = blockIdx.z;
+  auto values = [&](int j, int i) {
+    return __ldcg(reinterpret_cast<const float4*>(record(i) + (nt * C::KSTEPS + j) * 128) + lane);
+  };
+  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 ahead[MERGE_AHEAD];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
-      mvt = fmaxf(mvt, __shfl_xor_sync(0xffffffffu, mvt, o));
-    }
-    for (int i = lane; i < parts; i += 32) {
-      const float* x = record(i) + C::ACC * 32;
-      lt += x[2 * C::ROWS + r] * ratio2(x[r], mt);
-      factors[i * C::ROWS + r] = ratio2(x[C::ROWS + r], mvt);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) lt += __shfl_xor_sync(0xffffffffu, lt, o);
-    if (lane == 0) { totals[r] = mt; totals[C::ROWS + r] = mvt; totals[2 * C::ROWS + r] = lt; }
+  for (int x = 0; x < MERGE_AHEAD; ++x) ahead[x] = warp + x * WARPS < parts ? values(blockIdx.y, warp + x * WARPS) : zero;
+
+  // ---- a factor for each part and row; thread: row tid & 7, parts tid / 8, + 32, ...
+  const int row = threadIdx.x & 7;
+  float* const state_m = state, * const state_mv = state + blocks * 8, * const state_l = state + 2 * blocks * 8;
+  float mt = -INFINITY, mvt = -INFINITY;
+  for (int i = threadIdx.x >> 3; i < parts; i += THREADS / 8) {
+    const float* x = record(i) + C::ACC * 32 + nt * 8 + row;
+    const float m = __ldcg(x), mv = __ldcg(x + C::ROWS), l = __ldcg(x + 2 * C::ROWS);
+    state_m[i * 8 + row] = m; state_mv[i * 8 + row] = mv; state_l[i * 8 + row] = l;
+    mt = fmaxf(mt, m);
+    mvt = fmaxf(mvt, mv);
   }
+#pragma unroll
+  for (int o = 8; o < 32; o <<= 1) {
+    mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
+    mvt = fmaxf(mvt, __shfl_xor_sync(0xffffffffu, mvt, o));
+  }
+  if (lane < 8) { most[warp * 8 + lane] = mt; most[(WARPS + warp) * 8 + lane] = mvt; }
   __syncthreads();
-  const int h = seg / a.row_tiles, row0 = (seg - h * a.row_tiles) * C::ROWS;
-  const int e = blockIdx.y * THREADS + threadIdx.x;
-  int r, dim;
-  element_of<D, NT>(e, r, dim);
-  if (row0 + r >= a.rows) return;
-  float acc = 0.f;
-#pragma unroll 8
-  for (int i = 0; i < parts; ++i) acc += record(i)[e] * factors[i * C::ROWS + r];
-  const float lt = totals[2 * C::ROWS + r];
-  const float value = lt == 0.f ? 0.f : acc * finish_factor(totals[r], totals[C::ROWS + r], lt);
-  const int64_t at = output_row(a, b, h, row0 + r);
-  if (a.q_f16) static_cast<__half*>(a.out)[at * D + dim] = __float2half_rn(value);
-  else static_cast<__nv_bfloat16*>(a.out)[at * D + dim] = __float2bfloat16_rn(value);
-  if (dim == 0 && a.lse) a.lse[at] = lt == 0.f ? -INFINITY : (totals[r] + __log2f(lt)) * LN2;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    mt = fmaxf(mt, most[w * 8 + row]);
+    mvt = fmaxf(mvt, most[(WARPS + w) * 8 + row]);
+  }
+  float lt = 0.f;
+  for (int i = threadIdx.x >> 3; i < parts; i += THREADS / 8) {
+    lt += state_l[i * 8 + row] * ratio2(state_m[i * 8 + row], mt);
+    state_mv[i * 8 + row] = ratio2(state_mv[i * 8 + row], mvt);
+  }
+#pragma unroll
+  for (int o = 8; o < 32; o <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, o);
+  if (lane < 8) sum_l[warp * 8 + lane] = lt;
+  __syncthreads();
+  lt = 0.f;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) lt += sum_l[w * 8 + row];
+
+  // ---- the values: of fragment lane 4 (lane & 7) + k, accumulator lane >> 3, that is of row 2 k + (lane >> 3 & 1)
+  const int h = seg / a.row_tiles, out_row = (seg - h * a.row_tiles) * C::ROWS + nt * 8 + row;
+  for (int j = blockIdx.y; j < C::KSTEPS; j += gridDim.y) {
+    float4 acc = zero;
+    auto add = [&](const float4& v, int i) {
+      const float* f = state_mv + i * 8 + (lane >> 3 & 1);
+      acc.x += v.x * f[0]; acc.y += v.y * f[2]; acc.z += v.z * f[4]; acc.w += v.w * f[6];
+    };
+#pragma unroll
+    for (int x = 0; x < MERGE_AHEAD; ++x)
+      if (warp + x * WARPS < parts) add(ahead[x], warp + x * WARPS);
+#pragma unroll 4
+    for (int i = warp + MERGE_AHEAD * WARPS; i < parts; i += WARPS) add(values(j, i), i);
+    const int next = j + gridDim.y;
+    if (next < C::KSTEPS) {
+#pragma unroll
+      for (int x = 0; x < MERGE_AHEAD; ++x) if (warp + x * WARPS < parts) ahead[x] = values(next, warp + x * WARPS);
+    }
+    slots[warp * 32 + lane] = acc;
+    __syncthreads();
+    // thread: row tid & 7, dimensions of fragment row tid / 8: accumulators row & 1 and that + 2
+    if (threadIdx.x < 64 && out_row < a.rows) {
+      const int g = threadIdx.x >> 3;
+      const float* at0 = reinterpret_cast<const float*>(slots) + (row & 1) * 32 + g * 4 + (row >> 1);
+      float lo = 0.f, hi = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) { lo += at0[w * 128]; hi += at0[w * 128 + 64]; }
+      const float f = finish_factor(mt, mvt, lt);
+      lo = lt == 0.f ? 0.f : lo * f;
+      hi = lt == 0.f ? 0.f : hi * f;
+      const int dim = D == 64 ? 8 * g + 2 * j : 16 * g + 2 * (j & 7) + 128 * (j >> 3);
+      const int64_t at = output_row(a, b, h, out_row);
+      uint32_t word;
+      if (a.q_f16) {
+        word = half2_bits(lo, hi);
+      } else {
+        const __nv_bfloat162 y = __floats2bfloat162_rn(lo, hi);
+        word = *reinterpret_cast<const uint32_t*>(&y);
+      }
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at * D + dim) = word;
+      if (dim == 0 && a.lse) a.lse[at] = lt == 0.f ? -INFINITY : (mt + __log2f(lt)) * LN2;
+    }
+    __syncthreads();
+  }
 }
 
 struct Plan {
@@ -748,9 +807,14 @@ int launch(DecodeArgs& a, const Plan& plan, cudaStream_t st) {
   SEMBLO_LAUNCH_CHECK();
   if (plan.direct) return 0;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(a.batch * a.num_kv_heads * a.row_tiles), C::ACC * 32 / THREADS);
+  // a block per fragment of 16 dimensions while there are few segments to merge
+  const int segments = a.batch * a.num_kv_heads * a.row_tiles;
+  const int slices = std::max(1, std::min(C::KSTEPS, 8 * semblo::sm_count() / (segments * NT)));
+  cfg.gridDim = dim3((unsigned)segments, (unsigned)slices, NT);
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = sums + (plan.blocks + 3) * C::ROWS * 4;
+  cfg.dynamicSmemBytes = WARPS * 32 * 16 + (3 * WARPS + 3 * plan.blocks) * 8 * 4 + sums;
+  SEMBLO_CUDA(cudaFuncSetAttribute(kv8_merge_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)cfg.dynamicSmemBytes));
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -822,6 +886,7 @@ extern "C" int semblo_kv8_decode(const void* q, int dtype, int batch, int querie
                  "q, the cache and out must be 16-byte aligned");
   const Plan plan = plan_of(head_dim, nt, (int64_t)batch * num_kv_heads * tiles,
                             longest_segment(queries, window, table_len, block_size, prefix_lens != nullptr));
+  SEMBLO_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "the workspace must be 16-byte aligned");
   if (plan.bytes > workspace_bytes || (plan.bytes && !workspace))
     return semblo::fail(semblo::SEMBLO_ENOSPC, "workspace of %lld bytes needed, %lld given", (long long)plan.bytes,
                         (long long)workspace_bytes);

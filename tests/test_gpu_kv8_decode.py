@@ -149,6 +149,29 @@ def test_many_requests_and_long_rows(dev):
     assert torch.equal(first.output, again.output) and torch.equal(first.logsumexp, again.logsumexp)
 
 
+@pytest.mark.parametrize("long", [40, 300, 1100, 5000])
+@pytest.mark.parametrize("queries,group", [(1, 4), (3, 8), (4, 8)])
+def test_short_requests_in_a_wide_table(dev, long, queries, group):
+    # a table for 6400 keys; what is in it decides whether blocks take whole segments or even pieces
+    lens = [3, 0, 17, long, 1, 64, 5]
+    for dim in (64, 128):
+        cache, table, gen = _pool(dev, 31, lens, 64, 2, dim, width=100)
+        q = torch.randn(len(lens), queries, 2 * group, dim, device=dev, generator=gen).to(torch.bfloat16)
+        want = _formula(q, cache, table, lens, dim ** -0.5, None, 0, None, None)
+        _check(_call(q, cache, table, lens, sm_scale=dim ** -0.5), want, max(lens))
+
+
+def test_the_most_requests_in_a_wide_table(dev):
+    lens = [i % 3 for i in range(4096)]
+    lens[17], lens[4000] = 1500, 700
+    cache, table, gen = _pool(dev, 32, lens, 16, 1, 64, width=100)
+    q = torch.randn(len(lens), 1, 2, 64, device=dev, generator=gen).to(torch.float16)
+    some = [0, 1, 2, 17, 18, 3999, 4000, 4095]
+    want = _formula(q[some], cache, table[some], [lens[i] for i in some], 0.125, 30.0, 0, None, None)
+    got = _call(q, cache, table, lens, sm_scale=0.125, softcap=30.0)
+    _check(type(got)(got.output[some], got.logsumexp[some]), want, max(lens))
+
+
 @pytest.mark.parametrize("dim", [128, 256])
 def test_scales_of_every_size(dev, dim):
     """V in blocks of very different magnitude, K scales that are not powers of two, peaked scores."""
