@@ -1,12 +1,13 @@
 // Attention of packed prompts for head dimensions 64 and 128 (the mathematics is in dense_prefill.cu).
 //
-// One block owns two tiles of 128 rows (queries x the heads of a KV head) that take turns: while the tensor core
+// Two tiles of 128 rows (queries x the heads of a KV head) take turns on a multiprocessor: while the tensor core
 // works on one tile (P V of a key tile, then S of the next), a warpgroup runs the softmax of the other, one
 // thread per row.  At D = 128 the two S buffers and the two O accumulators are all of
-// tensor memory; P lies over the S it came from.  Q, K and V are in shared memory (64 KB of Q and a ring of
+// tensor memory; P lies over the S it came from.  Q, K and V are in shared memory (Q and a ring of
 // K, V tiles by TMA).  P is handed over in halves, so that P V starts when half the exponentials are done.
-// Where scores are capped or biased, a half is a step of the running maximum of its own: the 128 scores of a
-// whole row, the polynomial's coefficients and its chains do not fit in registers together.
+// The two tiles belong to one block, which loads K and V once for both, or to two blocks (one_tile() below).
+// Where scores are capped or biased or two blocks share the registers, a half is a step of the running maximum of
+// its own: the 128 scores of a whole row, the polynomial's coefficients and its chains do not fit together.
 #include <algorithm>
 
 #include "dense_pair.h"
@@ -20,43 +21,44 @@ namespace {
 constexpr int BN = PAIR_BN;
 constexpr int PAGE = 16;
 
-template <int D, int MODE>
+template <int D, int MODE, int TILES>
 struct Cfg {
   // threads per row.  With a running maximum one: two would have to meet for every tile and, with half the
   // registers each, read the scores twice (16384 causal 1.4 times as long).  Under a fixed reference two pay where
   // the softmax outweighs the products (8192 capped, windowed: D = 64 797 -> 666 us, D = 128 752 -> 780)
   static constexpr int HALVES = MODE == BOUNDED && D == 64 ? 2 : 1;
-  static constexpr int WARPS = 8 * HALVES;                     // of the softmax; then the loading and the issuing warp
+  static constexpr int WARPS = 4 * TILES * HALVES;               // of the softmax; then the loading and the issuing warp
   static constexpr int THREADS = (WARPS + 2) * 32;
   static constexpr int SLABS = D / 64;                         // 128-byte wide slabs of a 16-bit tile
   static constexpr int TILE = BN * D * 2;                      // a tile of Q, K or V
-  static constexpr int SLOTS = D == 128 ? 5 : 8;
+  static constexpr int SLOTS = D == 128 ? (TILES == 2 ? 5 : 2) : TILES == 2 ? 8 : 5;
   static constexpr int Q_OFF = 0;
-  static constexpr int KV_OFF = 2 * TILE;
+  static constexpr int KV_OFF = TILES * TILE;
   static constexpr int SUM_OFF = KV_OFF + SLOTS * TILE;        // float [2 tiles][2 halves][128]
   static constexpr int BAR_OFF = SUM_OFF + (HALVES == 2 ? 2048 : 0);
   static constexpr int TOTAL = BAR_OFF + 256;
   static constexpr int S_COL = 0;                              // + 128 x: S and P of tile x
-  static constexpr int O_COL = 256;                            // + D x
-  static constexpr int TMEM_COLS = 512;
+  static constexpr int O_COL = 128 * TILES;                    // + D x
+  static constexpr int TMEM_COLS = 256 * TILES;
   // P of a half lies over logits that the half's own threads have read
   static constexpr int P_HALF = HALVES == 2 ? 64 : 32;
 };
 
 enum { B_Q = 0, B_S = 1, B_P = 3, B_H = 7, B_O = 9, B_FULL = 11 };     // B_S + x, B_P + 2 x + half, B_H + x, B_O + x
 
-// Which key tiles the block walks over and which of its two row tiles sees each.
+// Which key tiles the block walks over and which of its row tiles sees each.
+template <int TILES>
 struct Walk {
   int gp, first, n;                       // prefix tiles, first tile of the main part, tiles in all
-  int glo[2], end[2];
-  bool any[2];
+  int glo[TILES], end[TILES];
+  bool any[TILES];
   __device__ __forceinline__ Walk(const Args& a, const Tile& t) {
-    const int qt = a.queries_per_tile >> 1;
+    const int qt = a.queries_per_tile / TILES;
     int last = 0;
     first = 1 << 30;
     gp = 0;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < TILES; ++x) {
       Tile s = t;
       s.pos += x * qt;
       s.count = min(qt, t.count - x * qt);
@@ -81,17 +83,17 @@ struct Walk {
   }
 };
 
-template <int D, bool F16, int MODE>
-__global__ void __launch_bounds__(Cfg<D, MODE>::THREADS, 1)
+template <int D, bool F16, int MODE, int TILES>
+__global__ void __launch_bounds__(Cfg<D, MODE, TILES>::THREADS, 3 - TILES)
 dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                   const __grid_constant__ CUtensorMap tmap_v, const Args a) {
-  using C = Cfg<D, MODE>;
+  using C = Cfg<D, MODE, TILES>;
   constexpr int SLOTS = C::SLOTS, HALVES = C::HALVES;
   constexpr int B_EMPTY = B_FULL + SLOTS;
   static_assert(8 * (B_EMPTY + SLOTS) + 8 <= 256, "barrier area");
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.y;
+  const int want = blockIdx.x / a.num_kv_heads, h = blockIdx.x - want * a.num_kv_heads;
   if (smem_u32(smem) & 1023u) {                    // the swizzled tiles need 1024-byte alignment
     if (threadIdx.x == 0) atomicCAS(a.status, 0, STATUS_SMEM_ALIGN);
     return;
@@ -124,13 +126,13 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   }
   __syncwarp();
   // the same answer in every warp
-  const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, blockIdx.x) : find_tile_block<C::THREADS>(a, blockIdx.x);
+  const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, want) : find_tile_block<C::THREADS>(a, want);
   if (tile.doc < 0) {
     if (a.zero_tail) zero_tail<D>(a, tile.first, h, blockDim.x);
     return;
   }
-  const Walk walk(a, tile);
-  const int qt = a.queries_per_tile >> 1;
+  const Walk<TILES> walk(a, tile);
+  const int qt = a.queries_per_tile / TILES;
   auto load_kv = [&](int i) {                      // K(i / 2) or V(i / 2) into its slot, which is free
     const int s = i % SLOTS, row = tile.k0 + walk.tile(i >> 1) * BN;
     mbar_arrive_expect_tx(bar(B_FULL + s), (uint32_t)C::TILE);
@@ -139,7 +141,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                   sl * 64, h, row);
   };
   if (warp == C::WARPS && lane == 0 && walk.n > 0) {
-    const int tiles = walk.any[1] ? 2 : 1;
+    const int tiles = walk.any[TILES - 1] ? TILES : 1;
     mbar_arrive_expect_tx(bar(B_Q), (uint32_t)(tiles * C::SLABS * qt * a.group * 128));
     for (int x = 0; x < tiles; ++x)
       for (int sl = 0; sl < C::SLABS; ++sl)
@@ -210,7 +212,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       };
       if (ok && n > 0 && wait_slot(0)) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int x = 0; x < TILES; ++x)
           if (walk.sees(x, 0)) issue_s(x, 0);
         umma_commit(bar(B_EMPTY));
       }
@@ -218,13 +220,13 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         if (!wait_slot(2 * j + 1)) break;
         const bool more = j + 1 < n;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+        for (int x = 0; x < TILES; ++x) {
           if (ok && walk.sees(x, j)) issue_pv(x, j);
-          if (x == 1 && ok) umma_commit(bar(B_EMPTY + (2 * j + 1) % SLOTS));
+          if (x == TILES - 1 && ok) umma_commit(bar(B_EMPTY + (2 * j + 1) % SLOTS));
           if (more && ok) {
             if (x == 0) wait_slot(2 * j + 2);
             if (ok && walk.sees(x, j + 1)) issue_s(x, j + 1);
-            if (x == 1 && ok) umma_commit(bar(B_EMPTY + (2 * j + 2) % SLOTS));
+            if (x == TILES - 1 && ok) umma_commit(bar(B_EMPTY + (2 * j + 2) % SLOTS));
           }
         }
       }
@@ -235,7 +237,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
   } else {
     // ------------------------------------------------------------ softmax + epilogue: one or two threads per row
-    const int x = warp / (C::WARPS / 2), hf = HALVES == 2 ? (warp >> 2) & 1 : 0;
+    const int x = TILES == 2 ? warp / (C::WARPS / 2) : 0, hf = HALVES == 2 ? (warp >> 2) & 1 : 0;
     const int row = threadIdx.x & 127;
     const int qi = row / a.group, hg = row - qi * a.group;
     const bool valid = qi < qt && x * qt + qi < tile.count;
@@ -252,8 +254,9 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     bool ok = true;
     int count = 0;
     // this tile's walk: [0, gp), then [j0, j1)
-    const bool any = x ? walk.any[1] : walk.any[0];
-    const int glo = x ? walk.glo[1] : walk.glo[0], gend = x ? walk.end[1] : walk.end[0];
+    constexpr int LAST = TILES - 1;
+    const bool any = x ? walk.any[LAST] : walk.any[0];
+    const int glo = x ? walk.glo[LAST] : walk.glo[0], gend = x ? walk.end[LAST] : walk.end[0];
     const int gp = any ? walk.gp : 0;
     const int j0 = any && gend > glo ? walk.gp + glo - walk.first : gp;
     const int j1 = any && gend > glo ? j0 + gend - glo : gp;
@@ -281,7 +284,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_P + 2 * x + (c >> 1)));
       };
-      constexpr int STEPS = MODE == BOUNDED ? 0 : MODE == LINEAR ? 1 : 2, CH = STEPS == 1 ? 4 : 2;   // chunks in a step
+      constexpr int STEPS = MODE == BOUNDED ? 0 : MODE == LINEAR && TILES == 2 ? 1 : 2, CH = STEPS == 1 ? 4 : 2;   // chunks in a step
       if constexpr (MODE == BOUNDED) {
         // no maximum: chunk by chunk (with registers to spare the next one's scores on their way)
         constexpr int CHUNKS = 4 / HALVES, BUFFERS = HALVES == 1 ? 2 : 1;
@@ -448,15 +451,30 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   if (warp == C::WARPS + 1) tmem_dealloc(tmem_base, C::TMEM_COLS);
 }
 
-template <int D, bool F16, int MODE>
-int launch(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, const Args& a, int kv_heads, cudaStream_t st) {
-  using C = Cfg<D, MODE>;
-  auto kern = dense_pair_kernel<D, F16, MODE>;
+template <int D, bool F16, int MODE, int TILES>
+int launch(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, Args a, cudaStream_t st) {
+  using C = Cfg<D, MODE, TILES>;
+  auto kern = dense_pair_kernel<D, F16, MODE, TILES>;
   SEMBLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TOTAL));
-  dim3 grid((unsigned)(ceil_div(a.tokens_q, a.queries_per_tile) + a.docs), (unsigned)kv_heads);
+  a.queries_per_tile = TILES * (128 / a.group);
+  const unsigned grid = (unsigned)((ceil_div(a.tokens_q, a.queries_per_tile) + a.docs) * a.num_kv_heads);
   kern<<<grid, C::THREADS, C::TOTAL, st>>>(mq, mk, mv, a);
   SEMBLO_LAUNCH_CHECK();
   return 0;
+}
+
+// One row tile per block, two blocks per multiprocessor, instead of two tiles that take turns in one block: twice
+// the loads of K and V, but a block's beginning and end (about 6 us without products) overlap the other block's
+// work.  us, 32 heads over 8, two tiles against one: 64 tokens x 128 10.6 : 7.6; 64 documents in 8192 tokens 108 :
+// 79, 16 of them 126 : 113, 8 of them 190 : 188, one 508 : 559; a window of 512 in 16384 271 : 232; at head
+// dimension 64 with 16 documents 104 : 100, with 8 166 : 174.  Where the softmax weighs most (a bias by
+// distance; a cap in fp16) one tile is no slower at any length: biased, 16384 tokens x 128 3457 : 3057 us; capped,
+// fp16, 8 heads over 2 x 64 830 : 822.
+bool one_tile(const Args& a, int head_dim, int mode) {
+  if (mode == BIASED || mode == CAPPED) return true;
+  int64_t reach = a.tokens_k / std::max(1, a.docs);
+  if (a.window > 0) reach = std::min<int64_t>(reach, a.window + BN);
+  return reach <= (head_dim == 128 ? 1024 : 640);
 }
 
 }  // namespace
@@ -464,9 +482,14 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, 
 namespace dense {
 
 int launch_pair(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, const Args& a, int head_dim,
-                bool f16, int mode, int kv_heads, cudaStream_t st) {
-#define SEMBLO_PAIR(DD, FF, MM) \
-  if (head_dim == DD && f16 == FF && mode == MM) return launch<DD, FF, MM>(mk, mv, mq, a, kv_heads, st);
+                bool f16, int mode, cudaStream_t st) {
+  const bool single = one_tile(a, head_dim, mode);
+#define SEMBLO_PAIR(DD, FF, MM)                                                          \
+  if (head_dim == DD && f16 == FF && mode == MM) {                                       \
+    if constexpr (MM == LINEAR || MM == BOUNDED)                                         \
+      if (!single) return launch<DD, FF, MM, 2>(mk, mv, mq, a, st);                      \
+    return launch<DD, FF, MM, 1>(mk, mv, mq, a, st);                                     \
+  }
   SEMBLO_PAIR(64, false, LINEAR) SEMBLO_PAIR(64, false, CAPPED) SEMBLO_PAIR(64, false, BIASED)
   SEMBLO_PAIR(64, false, BOUNDED) SEMBLO_PAIR(128, false, BOUNDED)
   SEMBLO_PAIR(64, true, LINEAR) SEMBLO_PAIR(64, true, CAPPED) SEMBLO_PAIR(64, true, BIASED)

@@ -6,8 +6,8 @@ namespace dense {
 
 constexpr int PAIR_BN = 128;             // keys per tile: the box of the K and V maps
 
-// mq: box {64, group, 128 / group}; mk, mv: box {64, 1, PAIR_BN}; a.queries_per_tile: 2 (128 / group).
+// mq: box {64, group, 128 / group}; mk, mv: box {64, 1, PAIR_BN}.
 int launch_pair(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, const Args& a, int head_dim,
-                bool f16, int mode, int kv_heads, cudaStream_t st);
+                bool f16, int mode, cudaStream_t st);
 
 }  // namespace dense

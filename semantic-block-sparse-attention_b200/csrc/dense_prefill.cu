@@ -53,12 +53,12 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   static_assert(8 * (B_KVEMPTY + STAGES) <= 256, "barrier area");
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.y;
+  const int want = blockIdx.x / a.num_kv_heads, h = blockIdx.x - want * a.num_kv_heads;
   if (smem_u32(smem) & 1023u) {                    // the swizzled tiles need 1024-byte alignment
     if (threadIdx.x == 0) atomicCAS(a.status, 0, STATUS_SMEM_ALIGN);
     return;
   }
-  const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, blockIdx.x) : find_tile_block<320>(a, blockIdx.x);
+  const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, want) : find_tile_block<320>(a, want);
   if (tile.doc < 0) {
     if (a.zero_tail) zero_tail<D>(a, tile.first, h, blockDim.x);
     return;
@@ -356,11 +356,11 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
 }
 
 template <int D, bool F16, int MODE>
-int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int kv_heads, cudaStream_t st) {
+int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, cudaStream_t st) {
   using C = Cfg<D>;
   auto kern = dense_prefill_kernel<D, F16, MODE>;
   SEMBLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TOTAL));
-  dim3 grid((unsigned)(ceil_div(a.tokens_q, a.queries_per_tile) + a.docs), (unsigned)kv_heads);
+  const unsigned grid = (unsigned)((ceil_div(a.tokens_q, a.queries_per_tile) + a.docs) * a.num_kv_heads);
   kern<<<grid, 320, C::TOTAL, st>>>(mk, mv, a);
   SEMBLO_LAUNCH_CHECK();
   return 0;
@@ -382,10 +382,11 @@ extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64
                  "query heads must be a multiple of the KV heads");
   const int group = num_q_heads / num_kv_heads;
   SEMBLO_REQUIRE(group <= 128, "at most 128 query heads per KV head (got %d)", group);
-  SEMBLO_REQUIRE(num_kv_heads <= 65535, "too many KV heads");
   SEMBLO_REQUIRE(dtype == SEMBLO_BF16 || dtype == SEMBLO_F16, "prompts are bf16 or fp16 (got dtype code %d)", dtype);
   SEMBLO_REQUIRE(tokens_q >= 0 && tokens_k >= 0 && documents >= 0, "negative token or document count");
   SEMBLO_REQUIRE(tokens_q < ((int64_t)1 << 30) && tokens_k < ((int64_t)1 << 30) && documents < (1 << 30), "too many tokens");
+  SEMBLO_REQUIRE((ceil_div(tokens_q, std::max(1, 128 / group)) + documents) * num_kv_heads < ((int64_t)1 << 31),
+                 "tokens x KV heads is too large for one call");
   SEMBLO_REQUIRE(window >= 0 && softcap >= 0.f, "negative window or soft cap");
   SEMBLO_REQUIRE(sm_scale > 0.f, "the score scale must be positive");
   SEMBLO_REQUIRE(causal || (window == 0 && prefix_lens == nullptr), "a window or a prefix needs the causal mask");
@@ -400,7 +401,8 @@ extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64
   a.out = out; a.lse = lse;
   a.cu_q = cu_seqlens_q; a.cu_k = cu_seqlens_k; a.prefix = prefix_lens; a.slopes = alibi_slopes;
   a.docs = documents; a.group = group; a.num_q_heads = num_q_heads;
-  a.queries_per_tile = (head_dim <= 128 ? 2 : 1) * (128 / group);
+  a.queries_per_tile = 128 / group;                // D = 256; launch_pair chooses its own
+  a.num_kv_heads = num_kv_heads;
   a.tokens_q = tokens_q; a.tokens_k = tokens_k;
   a.causal = causal; a.window = window; a.zero_tail = zero_tail;
   a.score_scale = softcap > 0.f ? sm_scale / softcap * TANH_ARG : sm_scale * LOG2EF;
@@ -429,9 +431,9 @@ extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64
   cudaStream_t st = (cudaStream_t)stream;
   const bool f16 = dtype == SEMBLO_F16;
   const int mode = alibi_slopes ? BIASED : softcap > 0.f ? (!f16 && a.cap_log2 <= BOUNDED_LOG2 ? BOUNDED : CAPPED) : LINEAR;
-  if (head_dim <= 128) return dense::launch_pair(mk, mv, mq, a, head_dim, f16, mode, num_kv_heads, st);
-  if (mode == LINEAR) return f16 ? launch<256, true, LINEAR>(mk, mv, a, num_kv_heads, st) : launch<256, false, LINEAR>(mk, mv, a, num_kv_heads, st);
-  if (mode == BOUNDED) return launch<256, false, BOUNDED>(mk, mv, a, num_kv_heads, st);
-  if (mode == CAPPED) return f16 ? launch<256, true, CAPPED>(mk, mv, a, num_kv_heads, st) : launch<256, false, CAPPED>(mk, mv, a, num_kv_heads, st);
-  return f16 ? launch<256, true, BIASED>(mk, mv, a, num_kv_heads, st) : launch<256, false, BIASED>(mk, mv, a, num_kv_heads, st);
+  if (head_dim <= 128) return dense::launch_pair(mk, mv, mq, a, head_dim, f16, mode, st);
+  if (mode == LINEAR) return f16 ? launch<256, true, LINEAR>(mk, mv, a, st) : launch<256, false, LINEAR>(mk, mv, a, st);
+  if (mode == BOUNDED) return launch<256, false, BOUNDED>(mk, mv, a, st);
+  if (mode == CAPPED) return f16 ? launch<256, true, CAPPED>(mk, mv, a, st) : launch<256, false, CAPPED>(mk, mv, a, st);
+  return f16 ? launch<256, true, BIASED>(mk, mv, a, st) : launch<256, false, BIASED>(mk, mv, a, st);
 }
