@@ -300,13 +300,35 @@ enum Mode { LINEAR = 0, CAPPED = 1, BIASED = 2, BOUNDED = 3 };
 constexpr float BOUNDED_TOP = 60.f, BOUNDED_LOG2 = 76.f;
 __host__ __device__ inline float bounded_reference(float cap_log2) { return cap_log2 > BOUNDED_TOP ? cap_log2 - BOUNDED_TOP : 0.f; }
 
-// 32 raw scores in place -> what the exponential's scale multiplies.
+// 32 raw scores in place -> what the exponential's scale multiplies.  All lanes of a warp take part.
 template <int MODE>
 __device__ __forceinline__ void transform32(uint32_t* x, const Args& a, float slope, int p, int key0) {
   if constexpr (MODE == LINEAR) return;
   if (MODE == CAPPED || MODE == BOUNDED || a.cap_log2 > 0.f) {
+    const f32x2 arg2 = join(a.score_scale, a.score_scale);
+    float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(tanh_exp(__uint_as_float(x[i]) * (a.score_scale * (1.f / TANH_ARG))));
+    for (int i = 0; i < 32; i += 2) {
+      float y0, y1;
+      split(mul2(join(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), arg2), y0, y1);
+      most = fmax3(most, fabsf(y0), fabsf(y1));
+      x[i] = __float_as_uint(y0);
+      x[i + 1] = __float_as_uint(y1);
+    }
+    if (__all_sync(0xffffffffu, most < TANH_FAR)) {
+      const TanhPoly<8> poly(1.f);
+      const f32x2 zero2 = join(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        float y0, y1;
+        split(poly(join(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), zero2), y0, y1);
+        x[i] = __float_as_uint(y0);
+        x[i + 1] = __float_as_uint(y1);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(tanh_exp(__uint_as_float(x[i]) * (1.f / TANH_ARG)));
+    }
   }
   if constexpr (MODE == BIASED) {
     const float scale = a.cap_log2 > 0.f ? a.cap_log2 : a.score_scale;
