@@ -375,16 +375,20 @@ int semblo_kv8_decode(const void* q, int dtype, int batch, int queries, int num_
  * j < prefix_lens[d] (NULL: none); causal = 0: every key of its document.  softcap > 0: scores become
  * softcap tanh(score / softcap); alibi_slopes [Hq] fp32 (NULL: none): minus slope |p - j|.  lse [tokens_q,
  * Hq] natural log, may be NULL; a row that sees nothing: 0 and -inf.  zero_tail: rows behind the last
- * document become 0 and -inf, otherwise they are not written.  The reference leaves dense requests to the
- * engine's stock attention (semblo/vllm_plugin/model.py:1169-1269). */
+ * document become 0 and -inf, otherwise they are not written.  The workspace needs no initialisation; its size
+ * is 0 unless there are few queries for the number of keys (their pieces are joined in it).  The reference
+ * leaves dense requests to the engine's stock attention (semblo/vllm_plugin/model.py:1169-1269). */
+int64_t semblo_dense_prefill_workspace_bytes(int64_t tokens_q, int64_t tokens_k, int num_q_heads,
+                                             int num_kv_heads, int head_dim, int documents, int causal,
+                                             int window, int has_prefix);
 int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                          int64_t k_token_stride, int64_t k_head_stride, const void* v,
                          int64_t v_token_stride, int64_t v_head_stride, int64_t tokens_q, int64_t tokens_k,
                          int num_q_heads, int num_kv_heads, int head_dim, int dtype,
                          const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int documents, int causal,
                          int window, const int32_t* prefix_lens, float sm_scale, float softcap,
-                         const float* alibi_slopes, void* out, int zero_tail, float* lse, int32_t* status,
-                         void* stream);
+                         const float* alibi_slopes, void* out, int zero_tail, float* lse, void* workspace,
+                         int64_t workspace_bytes, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -29,6 +29,8 @@ struct Args {
   float score_scale;              // raw product -> log2 units, or -> 8/3 of the capping tanh's argument
   float cap_log2;                 // cap * log2(e)
   int* status;
+  int splits;                     // pieces that a tile's keys may be cut into, a block each
+  float* partial;                 // with splits > 1: [tile][KV head][splits][record_floats(D)]
 };
 
 // The block's share: queries [q0, q0 + nq) of a document (token of query 0: tok0), keys k0 ... of length lk.
@@ -211,7 +213,7 @@ __device__ __forceinline__ void hide32(uint32_t* x, uint32_t bits) {
 // The key tiles of BN rows that any row of the block's tile sees: [0, gp) then [glo, ...), n in all.
 template <int BN>
 struct KeyTiles {
-  int gp, glo, n;
+  int gp, glo, n, base = 0;
   __device__ __forceinline__ KeyTiles(const Args& a, const Tile& t) {
     const Seen lo = seen_by(a, t, t.pos), hi = seen_by(a, t, t.pos + t.count - 1);
     gp = (lo.pre + BN - 1) / BN;
@@ -219,7 +221,27 @@ struct KeyTiles {
     glo = min(max(gp, lo.lo / BN), end);
     n = gp + end - glo;
   }
-  __device__ __forceinline__ int at(int j) const { return (j < gp ? j : j - gp + glo) * BN; }
+  __device__ __forceinline__ int at(int j) const { j += base; return (j < gp ? j : j - gp + glo) * BN; }
+};
+
+// ---- keys cut into pieces, where there are too few tiles for the multiprocessors.  A piece has SPLIT_KEYS keys at
+// least; its block leaves O, the reference and the sum of each of its 128 rows, and a second launch joins them.
+constexpr int SPLIT_KEYS = 512;
+__host__ __device__ constexpr int record_floats(int d) { return 128 * (d + 2); }       // O [128][D], m [128], l [128]
+__device__ __forceinline__ int pieces_of(const Args& a, int n, int bn) { return min(a.splits, max(1, n / (SPLIT_KEYS / bn))); }
+
+// The block's share of the grid: tile number `want` of KV head h, piece `split`.
+struct Share {
+  int want, h, split;
+  __device__ __forceinline__ Share(const Args& a, int splits) {
+    const int unit = splits > 1 ? blockIdx.x / splits : blockIdx.x;
+    split = blockIdx.x - unit * splits;
+    want = unit / a.num_kv_heads;
+    h = unit - want * a.num_kv_heads;
+  }
+  __device__ __forceinline__ float* record(const Args& a, int d, int s) const {
+    return a.partial + (((int64_t)want * a.num_kv_heads + h) * a.splits + s) * record_floats(d);
+  }
 };
 
 // ---- two floats in a 64-bit register: one instruction for both
@@ -445,6 +467,59 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int from, int to) {
   for (int i = lane; i < (to - from) * 8 * (D / 64); i += 32) {
     const int slab = i / ((to - from) * 8), r = i % ((to - from) * 8);
     reinterpret_cast<uint4*>(tile + slab * BN * 128 + (from + r / 8) * 128)[r % 8] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// 32 accumulators of a lane's row from tensor memory to its partial.  Warp-collective; `keep`: the row exists.
+__device__ __forceinline__ void store_partial(uint32_t tmem, float* to, bool keep) {
+  uint32_t o[32];
+  tmem_ld32(tmem, o);
+  tmem_ld_wait();
+  if (keep) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      reinterpret_cast<uint4*>(to)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+  }
+}
+
+// Joins the pieces of a tile: blockIdx.x is its share without a split; 8 dimensions of a row per thread.
+template <int D, int BN, bool F16>
+__global__ void __launch_bounds__(256) join_pieces_kernel(const Args a) {
+  const Share share(a, 1);
+  const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, share.want) : find_tile_block<256>(a, share.want);
+  pdl_wait();                                        // every block waits: this launch must not end before the other
+  if (tile.doc < 0) return;
+  const KeyTiles<BN> keys(a, tile);
+  const int pieces = pieces_of(a, keys.n, BN);
+  if (pieces == 1) return;
+  const float* first = share.record(a, D, 0);
+  constexpr int CH = D / 8;
+  for (int i = blockIdx.y * 256 + threadIdx.x; i < tile.count * a.group * CH; i += gridDim.y * 256) {
+    const int r = i / CH, c = i - r * CH;
+    float m = -INFINITY;
+    for (int s = 0; s < pieces; ++s) m = fmaxf(m, __ldcg(first + s * record_floats(D) + 128 * D + r));
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < pieces; ++s) {
+      const float* record = first + s * record_floats(D);
+      const float ms = __ldcg(record + 128 * D + r), f = ms == m ? 1.f : fast_exp2(ms - m);
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(record + r * D + c * 8));
+      const float4 y = __ldcg(reinterpret_cast<const float4*>(record + r * D + c * 8) + 1);
+      l += f * __ldcg(record + 128 * D + 128 + r);
+      acc[0] += f * x.x; acc[1] += f * x.y; acc[2] += f * x.z; acc[3] += f * x.w;
+      acc[4] += f * y.x; acc[5] += f * y.y; acc[6] += f * y.z; acc[7] += f * y.w;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int q = r / a.group;
+    const int64_t at = (tile.token + q) * a.num_q_heads + share.h * a.group + r - q * a.group;
+    uint4 w;
+    w.x = pack_pair<F16>(acc[0] * inv, acc[1] * inv);
+    w.y = pack_pair<F16>(acc[2] * inv, acc[3] * inv);
+    w.z = pack_pair<F16>(acc[4] * inv, acc[5] * inv);
+    w.w = pack_pair<F16>(acc[6] * inv, acc[7] * inv);
+    if (l == 0.f) w = make_uint4(0u, 0u, 0u, 0u);
+    reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at * D)[c] = w;
+    if (a.lse && c == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l) - p_bias<F16>()) * LN2F;
   }
 }
 

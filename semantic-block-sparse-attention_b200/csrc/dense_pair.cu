@@ -50,6 +50,7 @@ enum { B_Q = 0, B_S = 1, B_P = 3, B_H = 7, B_O = 9, B_FULL = 11 };     // B_S + 
 template <int TILES>
 struct Walk {
   int gp, first, n;                       // prefix tiles, first tile of the main part, tiles in all
+  int base = 0;                           // first of the block's, where the keys are cut into pieces (one row tile)
   int glo[TILES], end[TILES];
   bool any[TILES];
   __device__ __forceinline__ Walk(const Args& a, const Tile& t) {
@@ -76,8 +77,12 @@ struct Walk {
     }
     n = gp + max(0, last - first);
   }
-  __device__ __forceinline__ int tile(int j) const { return j < gp ? j : j - gp + first; }
+  __device__ __forceinline__ int tile(int j) const {
+    if (TILES == 1) j += base;
+    return j < gp ? j : j - gp + first;
+  }
   __device__ __forceinline__ bool sees(int x, int j) const {
+    if (TILES == 1) return j < n;
     const int i = tile(j);
     return any[x] && j < n && (j < gp || (i >= glo[x] && i < end[x]));
   }
@@ -93,7 +98,8 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   static_assert(8 * (B_EMPTY + SLOTS) + 8 <= 256, "barrier area");
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int want = blockIdx.x / a.num_kv_heads, h = blockIdx.x - want * a.num_kv_heads;
+  const Share share(a, a.splits);
+  const int h = share.h;
   if (smem_u32(smem) & 1023u) {                    // the swizzled tiles need 1024-byte alignment
     if (threadIdx.x == 0) atomicCAS(a.status, 0, STATUS_SMEM_ALIGN);
     return;
@@ -126,12 +132,19 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   }
   __syncwarp();
   // the same answer in every warp
-  const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, want) : find_tile_block<C::THREADS>(a, want);
+  const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, share.want) : find_tile_block<C::THREADS>(a, share.want);
   if (tile.doc < 0) {
-    if (a.zero_tail) zero_tail<D>(a, tile.first, h, blockDim.x);
+    if (a.zero_tail && share.split == 0) zero_tail<D>(a, tile.first, h, blockDim.x);
     return;
   }
-  const Walk<TILES> walk(a, tile);
+  Walk<TILES> walk(a, tile);
+  int pieces = 1;
+  if constexpr (TILES == 1) {
+    pieces = pieces_of(a, walk.n, BN);
+    if (share.split >= pieces) return;
+    walk.base = (int)((int64_t)walk.n * share.split / pieces);
+    walk.n = (int)((int64_t)walk.n * (share.split + 1) / pieces) - walk.base;
+  }
   const int qt = a.queries_per_tile / TILES;
   auto load_kv = [&](int i) {                      // K(i / 2) or V(i / 2) into its slot, which is free
     const int s = i % SLOTS, row = tile.k0 + walk.tile(i >> 1) * BN;
@@ -257,9 +270,9 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     constexpr int LAST = TILES - 1;
     const bool any = x ? walk.any[LAST] : walk.any[0];
     const int glo = x ? walk.glo[LAST] : walk.glo[0], gend = x ? walk.end[LAST] : walk.end[0];
-    const int gp = any ? walk.gp : 0;
-    const int j0 = any && gend > glo ? walk.gp + glo - walk.first : gp;
-    const int j1 = any && gend > glo ? j0 + gend - glo : gp;
+    const int gp = TILES == 2 && any ? walk.gp : 0;
+    const int j0 = TILES == 2 && any && gend > glo ? walk.gp + glo - walk.first : gp;
+    const int j1 = TILES == 1 ? walk.n : any && gend > glo ? j0 + gend - glo : gp;
     for (int j = gp > 0 ? 0 : j0; j < gp || (j >= j0 && j < j1); j = j + 1 == gp ? j0 : j + 1) {
       const int key0 = walk.tile(j) * BN;
       ok = mbar_wait_warp(bar(B_S + x), (uint32_t)(count & 1), abort_flag, a.status, STATUS_TIMEOUT_SOFTMAX);
@@ -413,7 +426,17 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");     // all of the tile's threads, whatever became of them
       l += sums[(hf ^ 1) * 128 + row];
     }
-    if (ok && any) {
+    if (TILES == 1 && pieces > 1) {
+      if (ok) {
+        float* record = share.record(a, D, share.split);
+#pragma unroll 1
+        for (int c = 0; c < D / 32 / HALVES; ++c) store_partial(o_addr + c * 32, record + row * D + hf * (D / 2) + c * 32, valid);
+        if (valid && hf == 0) {
+          record[128 * D + row] = m_ref;
+          record[128 * D + 128 + row] = l;
+        }
+      }
+    } else if (ok && any) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int64_t at = (tile.token + x * qt + qi) * a.num_q_heads + head;
       // through Q's shared memory (no product is in flight any more), a warp's own part of it
@@ -457,7 +480,7 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, 
   auto kern = dense_pair_kernel<D, F16, MODE, TILES>;
   SEMBLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TOTAL));
   a.queries_per_tile = TILES * (128 / a.group);
-  const unsigned grid = (unsigned)((ceil_div(a.tokens_q, a.queries_per_tile) + a.docs) * a.num_kv_heads);
+  const unsigned grid = (unsigned)((ceil_div(a.tokens_q, a.queries_per_tile) + a.docs) * a.num_kv_heads * a.splits);
   kern<<<grid, C::THREADS, C::TOTAL, st>>>(mq, mk, mv, a);
   SEMBLO_LAUNCH_CHECK();
   return 0;
@@ -471,7 +494,7 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, 
 // distance; a cap in fp16) one tile is no slower at any length: biased, 16384 tokens x 128 3457 : 3057 us; capped,
 // fp16, 8 heads over 2 x 64 830 : 822.
 bool one_tile(const Args& a, int head_dim, int mode) {
-  if (mode == BIASED || mode == CAPPED) return true;
+  if (mode == BIASED || mode == CAPPED || a.splits > 1) return true;
   int64_t reach = a.tokens_k / std::max(1, a.docs);
   if (a.window > 0) reach = std::min<int64_t>(reach, a.window + BN);
   return reach <= (head_dim == 128 ? 1024 : 640);

@@ -53,17 +53,22 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   static_assert(8 * (B_KVEMPTY + STAGES) <= 256, "barrier area");
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int want = blockIdx.x / a.num_kv_heads, h = blockIdx.x - want * a.num_kv_heads;
+  const Share share(a, a.splits);
+  const int h = share.h;
   if (smem_u32(smem) & 1023u) {                    // the swizzled tiles need 1024-byte alignment
     if (threadIdx.x == 0) atomicCAS(a.status, 0, STATUS_SMEM_ALIGN);
     return;
   }
-  const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, want) : find_tile_block<320>(a, want);
+  const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, share.want) : find_tile_block<320>(a, share.want);
   if (tile.doc < 0) {
-    if (a.zero_tail) zero_tail<D>(a, tile.first, h, blockDim.x);
+    if (a.zero_tail && share.split == 0) zero_tail<D>(a, tile.first, h, blockDim.x);
     return;
   }
-  const KeyTiles<BN> keys(a, tile);
+  KeyTiles<BN> keys(a, tile);
+  const int pieces = pieces_of(a, keys.n, BN);
+  if (share.split >= pieces) return;
+  keys.base = (int)((int64_t)keys.n * share.split / pieces);
+  keys.n = (int)((int64_t)keys.n * (share.split + 1) / pieces) - keys.base;
 
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::SLOT_OFF);
@@ -325,7 +330,17 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     xchg[hf * 128 + row] = l_part;
     mbar_arrive(bar(B_EPI));
     if (ok) ok = mbar_wait_warp(bar(B_EPI), 0, abort_flag, a.status, STATUS_TIMEOUT_EPILOGUE);
-    if (ok) {
+    if (ok && pieces > 1) {
+      const float l = l_part + xchg[(hf ^ 1) * 128 + row];
+      float* record = share.record(a, D, share.split);
+#pragma unroll 1
+      for (int c = 0; c < D / 64; ++c)
+        store_partial(tmem_base + lane_addr + C::O_COL + hf * (D / 2) + c * 32, record + row * D + hf * (D / 2) + c * 32, valid);
+      if (valid && hf == 0) {
+        record[128 * D + row] = m_ref;
+        record[128 * D + 128 + row] = l;
+      }
+    } else if (ok) {
       const float l = l_part + xchg[(hf ^ 1) * 128 + row];
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int64_t at = (tile.token + qi) * a.num_q_heads + head;
@@ -360,13 +375,80 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, cudaStre
   using C = Cfg<D>;
   auto kern = dense_prefill_kernel<D, F16, MODE>;
   SEMBLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TOTAL));
-  const unsigned grid = (unsigned)((ceil_div(a.tokens_q, a.queries_per_tile) + a.docs) * a.num_kv_heads);
+  const unsigned grid = (unsigned)((ceil_div(a.tokens_q, a.queries_per_tile) + a.docs) * a.num_kv_heads * a.splits);
   kern<<<grid, 320, C::TOTAL, st>>>(mk, mv, a);
   SEMBLO_LAUNCH_CHECK();
   return 0;
 }
 
+template <int D, int BN_, bool F16>
+int join_pieces(const Args& a, cudaStream_t st) {
+  const int64_t units = (ceil_div(a.tokens_q, a.queries_per_tile) + a.docs) * a.num_kv_heads;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)units, (unsigned)std::max<int64_t>(1, std::min<int64_t>(D / 16, 4 * semblo::sm_count() / units)));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  SEMBLO_CUDA(cudaLaunchKernelEx(&cfg, join_pieces_kernel<D, BN_, F16>, a));
+  return 0;
+}
+
+// Into how many pieces a tile's keys may be cut: as many as bring the longest tile down to what each multiprocessor
+// would get of an even share (causal tiles differ, so that is up to twice the free room).  A tile's mean number of
+// keys is what a document has less half its queries.  us without and with: 16 tokens x 32 heads over 8 x 128 behind
+// 8192 others 139 : 25, 128 behind 30000 463 : 95, 512 behind 30000 469 : 278, 8192 tokens x 4 heads over 1 136 : 106;
+// 1024 tokens x 8 heads over 2 20 : 24, so two short pieces are not worth the second launch.
+int splits_for(int64_t tokens_q, int64_t tokens_k, int group, int num_kv_heads, int head_dim, int documents, int causal,
+               int window, bool prefix) {
+  if (documents == 0) return 1;
+  const int64_t qt = 128 / group, tiles = (tokens_q + documents * (qt - 1)) / qt;      // no more than these have queries
+  const int64_t slots = (int64_t)semblo::sm_count() * (head_dim == 256 ? 1 : 2);
+  int64_t keys = tokens_k / documents;
+  if (window > 0 && !prefix) keys = std::min<int64_t>(keys, window + qt);
+  // the longest tile's keys over the mean of all
+  const double skew = causal && tokens_q < tokens_k ? 2.0 * tokens_k / (2.0 * tokens_k - tokens_q) : causal ? 2.0 : 1.0;
+  if (keys < 1.5 * SPLIT_KEYS * skew) return 1;
+  const int64_t room = (int64_t)(skew * slots / std::max<int64_t>(1, tiles * num_kv_heads));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({room, keys / SPLIT_KEYS, 32}));
+}
+
+int64_t split_bytes(int64_t tokens_q, int group, int num_kv_heads, int head_dim, int documents, int splits) {
+  if (splits == 1) return 0;
+  return (ceil_div(tokens_q, 128 / group) + documents) * num_kv_heads * splits * record_floats(head_dim) * 4;
+}
+
+int check_shape(int64_t tokens_q, int64_t tokens_k, int num_q_heads, int num_kv_heads, int head_dim, int documents,
+                int causal, int window, bool prefix) {
+  SEMBLO_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, "head_dim must be 64, 128 or 256 (got %d)",
+                 head_dim);
+  SEMBLO_REQUIRE(num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0,
+                 "query heads must be a multiple of the KV heads");
+  const int group = num_q_heads / num_kv_heads;
+  SEMBLO_REQUIRE(group <= 128, "at most 128 query heads per KV head (got %d)", group);
+  SEMBLO_REQUIRE(tokens_q >= 0 && tokens_k >= 0 && documents >= 0, "negative token or document count");
+  SEMBLO_REQUIRE(tokens_q < ((int64_t)1 << 30) && tokens_k < ((int64_t)1 << 30) && documents < (1 << 30), "too many tokens");
+  SEMBLO_REQUIRE((ceil_div(tokens_q, 128 / group) + documents) * num_kv_heads < ((int64_t)1 << 31),
+                 "tokens x KV heads is too large for one call");
+  SEMBLO_REQUIRE(window >= 0, "negative window");
+  SEMBLO_REQUIRE(causal || (window == 0 && !prefix), "a window or a prefix needs the causal mask");
+  return 0;
+}
+
 }  // namespace
+
+extern "C" int64_t semblo_dense_prefill_workspace_bytes(int64_t tokens_q, int64_t tokens_k, int num_q_heads,
+                                                        int num_kv_heads, int head_dim, int documents, int causal,
+                                                        int window, int has_prefix) {
+  const int rc = check_shape(tokens_q, tokens_k, num_q_heads, num_kv_heads, head_dim, documents, causal, window, has_prefix);
+  if (rc) return rc;
+  const int group = num_q_heads / num_kv_heads;
+  return split_bytes(tokens_q, group, num_kv_heads, head_dim, documents,
+                     splits_for(tokens_q, tokens_k, group, num_kv_heads, head_dim, documents, causal, window, has_prefix));
+}
 
 extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                                     int64_t k_token_stride, int64_t k_head_stride, const void* v,
@@ -375,21 +457,14 @@ extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64
                                     const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int documents,
                                     int causal, int window, const int32_t* prefix_lens, float sm_scale,
                                     float softcap, const float* alibi_slopes, void* out, int zero_tail, float* lse,
-                                    int32_t* status, void* stream) {
-  SEMBLO_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, "head_dim must be 64, 128 or 256 (got %d)",
-                 head_dim);
-  SEMBLO_REQUIRE(num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0,
-                 "query heads must be a multiple of the KV heads");
+                                    void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+  const int rc0 = check_shape(tokens_q, tokens_k, num_q_heads, num_kv_heads, head_dim, documents, causal, window,
+                              prefix_lens != nullptr);
+  if (rc0) return rc0;
   const int group = num_q_heads / num_kv_heads;
-  SEMBLO_REQUIRE(group <= 128, "at most 128 query heads per KV head (got %d)", group);
   SEMBLO_REQUIRE(dtype == SEMBLO_BF16 || dtype == SEMBLO_F16, "prompts are bf16 or fp16 (got dtype code %d)", dtype);
-  SEMBLO_REQUIRE(tokens_q >= 0 && tokens_k >= 0 && documents >= 0, "negative token or document count");
-  SEMBLO_REQUIRE(tokens_q < ((int64_t)1 << 30) && tokens_k < ((int64_t)1 << 30) && documents < (1 << 30), "too many tokens");
-  SEMBLO_REQUIRE((ceil_div(tokens_q, std::max(1, 128 / group)) + documents) * num_kv_heads < ((int64_t)1 << 31),
-                 "tokens x KV heads is too large for one call");
-  SEMBLO_REQUIRE(window >= 0 && softcap >= 0.f, "negative window or soft cap");
+  SEMBLO_REQUIRE(softcap >= 0.f, "the soft cap must not be negative");
   SEMBLO_REQUIRE(sm_scale > 0.f, "the score scale must be positive");
-  SEMBLO_REQUIRE(causal || (window == 0 && prefix_lens == nullptr), "a window or a prefix needs the causal mask");
   if (tokens_q == 0 || (documents == 0 && !zero_tail)) return 0;
   SEMBLO_REQUIRE(q && out && status && cu_seqlens_q && cu_seqlens_k && (tokens_k == 0 || (k && v)), "null pointer");
   SEMBLO_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
@@ -408,6 +483,13 @@ extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64
   a.score_scale = softcap > 0.f ? sm_scale / softcap * TANH_ARG : sm_scale * LOG2EF;
   a.cap_log2 = softcap * LOG2EF;
   a.status = status;
+  a.splits = splits_for(tokens_q, tokens_k, group, num_kv_heads, head_dim, documents, causal, window, prefix_lens != nullptr);
+  a.partial = (float*)workspace;
+  const int64_t bytes = split_bytes(tokens_q, group, num_kv_heads, head_dim, documents, a.splits);
+  SEMBLO_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "the workspace must be 16-byte aligned");
+  if (bytes > workspace_bytes || (bytes && !workspace))
+    return semblo::fail(semblo::SEMBLO_ENOSPC, "workspace of %lld bytes needed, %lld given", (long long)bytes,
+                        (long long)workspace_bytes);
   // no keys at all: the maps are not read, but have to describe something
   CUtensorMap mk, mv;
   const uint64_t dims[3] = {(uint64_t)head_dim, (uint64_t)num_kv_heads, (uint64_t)std::max<int64_t>(tokens_k, 1)};
@@ -431,9 +513,13 @@ extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64
   cudaStream_t st = (cudaStream_t)stream;
   const bool f16 = dtype == SEMBLO_F16;
   const int mode = alibi_slopes ? BIASED : softcap > 0.f ? (!f16 && a.cap_log2 <= BOUNDED_LOG2 ? BOUNDED : CAPPED) : LINEAR;
-  if (head_dim <= 128) return dense::launch_pair(mk, mv, mq, a, head_dim, f16, mode, st);
-  if (mode == LINEAR) return f16 ? launch<256, true, LINEAR>(mk, mv, a, st) : launch<256, false, LINEAR>(mk, mv, a, st);
-  if (mode == BOUNDED) return launch<256, false, BOUNDED>(mk, mv, a, st);
-  if (mode == CAPPED) return f16 ? launch<256, true, CAPPED>(mk, mv, a, st) : launch<256, false, CAPPED>(mk, mv, a, st);
-  return f16 ? launch<256, true, BIASED>(mk, mv, a, st) : launch<256, false, BIASED>(mk, mv, a, st);
+  if (head_dim <= 128) rc = dense::launch_pair(mk, mv, mq, a, head_dim, f16, mode, st);
+  else if (mode == LINEAR) rc = f16 ? launch<256, true, LINEAR>(mk, mv, a, st) : launch<256, false, LINEAR>(mk, mv, a, st);
+  else if (mode == BOUNDED) rc = launch<256, false, BOUNDED>(mk, mv, a, st);
+  else if (mode == CAPPED) rc = f16 ? launch<256, true, CAPPED>(mk, mv, a, st) : launch<256, false, CAPPED>(mk, mv, a, st);
+  else rc = f16 ? launch<256, true, BIASED>(mk, mv, a, st) : launch<256, false, BIASED>(mk, mv, a, st);
+  if (rc || a.splits == 1) return rc;
+  if (head_dim == 64) return f16 ? join_pieces<64, PAIR_BN, true>(a, st) : join_pieces<64, PAIR_BN, false>(a, st);
+  if (head_dim == 128) return f16 ? join_pieces<128, PAIR_BN, true>(a, st) : join_pieces<128, PAIR_BN, false>(a, st);
+  return f16 ? join_pieces<256, BN, true>(a, st) : join_pieces<256, BN, false>(a, st);
 }

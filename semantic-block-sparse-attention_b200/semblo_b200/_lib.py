@@ -76,7 +76,8 @@ _SIGNATURES = {
     "semblo_kv8_append": (c_int, [c_void_p, c_int64, c_int64] * 2 + [c_int64, c_int, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     "semblo_kv8_decode_workspace_bytes": (c_int64, [c_int] * 9),
     "semblo_kv8_decode": (c_int, [c_void_p] + [c_int] * 6 + [c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_float, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
-    "semblo_dense_prefill": (c_int, [c_void_p, c_int64, c_int64] * 3 + [c_int64, c_int64] + [c_int] * 4 + [c_void_p, c_void_p] + [c_int] * 3 + [c_void_p, c_float, c_float, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    "semblo_dense_prefill_workspace_bytes": (c_int64, [c_int64, c_int64] + [c_int] * 7),
+    "semblo_dense_prefill": (c_int, [c_void_p, c_int64, c_int64] * 3 + [c_int64, c_int64] + [c_int] * 4 + [c_void_p, c_void_p] + [c_int] * 3 + [c_void_p, c_float, c_float, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
     "semblo_merge_attention_states": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
 }
 

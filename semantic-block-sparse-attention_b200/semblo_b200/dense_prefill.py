@@ -80,9 +80,16 @@ def dense_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *
         if given:
             lse.fill_(float("-inf"))
     with device_scope(device):
+        nbytes = lib().semblo_dense_prefill_workspace_bytes(tokens_q, tokens_k, hq, hkv, dim, docs, bool(causal), window,
+                                                            prefix_lens is not None)
+        if nbytes < 0:
+            check(int(nbytes))
+        # made for this call: a recorded graph keeps its own, and calls on two streams do not share one
+        workspace = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         check(lib().semblo_dense_prefill(
-            *q_rows, *k_rows, *v_rows, tokens_q, tokens_k, hq, hkv, dim, dtype_code(dtype, "prefill"), cu_q.data_ptr(), cu_k.data_ptr(),
-            docs, bool(causal), window, None if prefix_lens is None else prefix_lens.data_ptr(), sm_scale, softcap,
+            *q_rows, *k_rows, *v_rows, tokens_q, tokens_k, hq, hkv, dim, dtype_code(dtype, "prefill"), cu_q.data_ptr(),
+            cu_k.data_ptr(), docs, bool(causal), window, None if prefix_lens is None else prefix_lens.data_ptr(), sm_scale, softcap,
             None if alibi_slopes is None else alibi_slopes.data_ptr(), out.data_ptr(), not given,
-            None if lse is None else lse.data_ptr(), _lib.status_for(device).word.data_ptr(), raw_stream(device.index)))
+            None if lse is None else lse.data_ptr(), None if workspace is None else workspace.data_ptr(), nbytes,
+            _lib.status_for(device).word.data_ptr(), raw_stream(device.index)))
     return PagedSparseAttentionResult(out, lse)

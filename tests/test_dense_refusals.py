@@ -290,11 +290,17 @@ def test_c_entries_refuse():
     assert lib.semblo_kv8_decode_workspace_bytes(1, 1, 3, 2, 64, 16, 4096, 0, 0) == -1
 
     def prefill(q=p, k=p, v=p, tq=4, tk=4, hq=2, hkv=1, dim=64, dtype=0, cu=p, docs=1, causal=1, window=0, prefix=None,
-                sm=0.1, cap=0.0, out=p, stride=64, status=p):
+                sm=0.1, cap=0.0, out=p, stride=64, status=p, room=0):
         return lib.semblo_dense_prefill(q, stride, 64, k, 64, 64, v, 64, 64, tq, tk, hq, hkv, dim, dtype, cu, cu, docs, causal,
-                                        window, prefix, sm, cap, None, out, 0, None, status, None)
+                                        window, prefix, sm, cap, None, out, 0, None, p, room, status, None)
 
     assert prefill(tq=0) == 0 and prefill(docs=0) == 0
+    sizes = lib.semblo_dense_prefill_workspace_bytes
+    assert sizes(4, 4, 2, 1, 64, 1, 1, 0, 0) == 0 and sizes(100000, 100000, 32, 8, 64, 1, 1, 0, 0) == 0
+    need = sizes(4, 4096, 2, 1, 64, 1, 1, 0, 0)                  # a few queries over many keys
+    assert need > 0 and sizes(4, 4096, 2, 1, 64, 1, 1, 100, 0) == 0
+    assert prefill(tk=4096, room=need - 1) == -3
+    assert sizes(4, 4096, 3, 2, 64, 1, 1, 0, 0) == -1
     for kw in (dict(dim=80), dict(hq=3, hkv=2), dict(hq=129), dict(dtype=1), dict(tq=-1), dict(window=-1), dict(cap=-1.0),
                dict(sm=0.0), dict(causal=0, window=4), dict(causal=0, prefix=p), dict(q=None), dict(k=None), dict(out=None),
                dict(cu=None), dict(status=None), dict(q=ctypes.c_void_p(264)), dict(stride=60)):

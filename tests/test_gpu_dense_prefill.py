@@ -104,6 +104,44 @@ def _call(q, k, v, q_lens, k_lens, prefix=None, slopes=None, **kw):
                                    return_logsumexp=True, **kw)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("options", ["plain", "full", "cap", "window", "all"])
+def test_few_queries_over_many_keys(dev, dim, dtype, options):
+    # enough keys per document for several pieces; documents of one piece and of none among them
+    q_lens, k_lens = [5, 0, 33, 200, 1], [4100, 900, 1537, 1800, 3]
+    q, k, v, gen = _inputs(dev, dim, q_lens, k_lens, 6, 2, dim, dtype)
+    kw = {"sm_scale": dim ** -0.5}
+    if options == "full":
+        kw["causal"] = False
+    if options in ("cap", "all"):
+        kw["softcap"] = 20.0
+    if options in ("window", "all"):
+        kw["window"] = 1500
+        kw["prefix"] = torch.tensor([700, 3, 0, 40, 2], device=dev)
+    if options == "all":
+        kw["slopes"] = torch.rand(6, device=dev, generator=gen) * 0.1
+    want = _formula(q, k, v, q_lens, k_lens, **kw)
+    got = _call(q, k, v, q_lens, k_lens, **kw)
+    _check(got, want, max(k_lens))
+    again = _call(q, k, v, q_lens, k_lens, **kw)
+    assert torch.equal(got.output, again.output) and torch.equal(got.logsumexp, again.logsumexp)
+
+
+def test_pieces_leave_the_tail_alone(dev):
+    from semblo_b200.dense_prefill import dense_prefill_attention
+    q, k, v, _ = _inputs(dev, 3, [50], [3000], 2, 1, 128, torch.bfloat16)
+    cu_q, cu_k = torch.tensor([0, 7], device=dev), torch.tensor([0, 2500], device=dev)
+    k[2500:], v[2500:] = math.nan, math.inf
+    out = torch.full_like(q, 9.0)
+    got = dense_prefill_attention(q, k, v, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, sm_scale=0.1, out=out, return_logsumexp=True)
+    want = _formula(q[:7], k[:2500], v[:2500], [7], [2500], sm_scale=0.1)
+    _check(type(got)(out[:7], got.logsumexp[:7]), want, 2500)
+    assert bool((out[7:] == 9).all()) and bool((got.logsumexp[7:] == -math.inf).all())
+    fresh = dense_prefill_attention(q, k, v, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, sm_scale=0.1, return_logsumexp=True)
+    assert torch.equal(fresh.output[:7], out[:7]) and bool((fresh.output[7:] == 0).all())
+
+
 Q_LENS = [1, 0, 63, 64, 65, 300, 17, 5, 130]
 K_LENS = [1, 7, 63, 200, 65, 300, 529, 3, 0]          # more keys than queries, fewer, and none
 
