@@ -201,16 +201,16 @@ template <typename T, int NP>
 int launch(RotaryArgs& a, bool interleaved, cudaStream_t st) {
   a.rot_cols = a.rotary_dim / (2 * NP);
   a.cols = a.rot_cols + (int)ceil_div(a.head_dim - a.rotary_dim, 2 * NP);
-  // a block's threads are tokens x head lanes x columns: the split that leaves the fewest of them idle.  While
-  // there are fewer tokens than two blocks per multiprocessor would take, one token per block and every thread
+  // a block's threads are tokens x head lanes x columns: the split that leaves the fewest of them idle, with no more
+  // tokens than leave two blocks for every multiprocessor
   const int rows = THREADS / a.cols;
-  const int most_tokens = std::max(1, 1024 / std::max(1, a.rotary_dim / 2));          // 2 x 8 KB of cos/sin
+  const int sms = semblo::sm_count();
+  const int most_tokens = (int)std::min<int64_t>(std::max(1, 1024 / std::max(1, a.rotary_dim / 2)),   // 2 x 8 KB of cos/sin
+                                                 std::max<int64_t>(1, a.tokens / (2 * sms)));
   int tb = 1, lanes = std::min(rows, a.heads);
   double best = 0;
-  const int sms = semblo::sm_count();
   for (int l = 1; l <= std::min(rows, a.heads); ++l) {
     const int t = std::min(rows / l, most_tokens);
-    if (a.tokens < (int64_t)t * 2 * sms) continue;
     const int64_t slots = ceil_div(ceil_div(a.heads, l), AHEAD) * AHEAD;
     const double used = (double)t * a.heads / ((double)rows * slots);
     if (used >= best) { best = used; tb = t; lanes = l; }
