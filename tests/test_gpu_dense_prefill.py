@@ -128,6 +128,45 @@ def test_few_queries_over_many_keys(dev, dim, dtype, options):
     assert torch.equal(got.output, again.output) and torch.equal(got.logsumexp, again.logsumexp)
 
 
+@pytest.mark.parametrize("dim", [64, 256])
+def test_pieces_of_many_documents(dev, dim):
+    # more documents than a warp looks over, each with a few queries over many keys
+    q_lens, k_lens = [i % 3 for i in range(70)], [1100 + 37 * (i % 20) for i in range(70)]
+    q, k, v, _ = _inputs(dev, 4, q_lens, k_lens, 1, 1, dim, torch.bfloat16)
+    want = _formula(q, k, v, q_lens, k_lens, sm_scale=dim ** -0.5)
+    _check(_call(q, k, v, q_lens, k_lens, sm_scale=dim ** -0.5), want, max(k_lens))
+
+
+def test_pieces_on_two_streams_and_in_graphs(dev):
+    from semblo_b200.dense_prefill import dense_prefill_attention
+    inputs = [_inputs(dev, 40 + i, [20], [4000], 8, 2, 128, torch.float16)[:3] for i in range(2)]
+    cu_q, cu_k = torch.tensor([0, 20], dtype=torch.int32, device=dev), torch.tensor([0, 4000], dtype=torch.int32, device=dev)
+
+    def call(i):
+        q, k, v = inputs[i]
+        return dense_prefill_attention(q, k, v, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, sm_scale=0.1).output
+
+    want = [call(0), call(1)]
+    streams, graphs, outs = [torch.cuda.Stream(), torch.cuda.Stream()], [], [None, None]
+    torch.cuda.synchronize()
+    for i, stream in enumerate(streams):
+        with torch.cuda.stream(stream):
+            for _ in range(5):
+                outs[i] = call(i)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            outs[i] = call(i)
+    for i, stream in enumerate(streams):                       # replayed side by side: each graph has its own workspace
+        with torch.cuda.stream(stream):
+            for _ in range(5):
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
 def test_pieces_leave_the_tail_alone(dev):
     from semblo_b200.dense_prefill import dense_prefill_attention
     q, k, v, _ = _inputs(dev, 3, [50], [3000], 2, 1, 128, torch.bfloat16)
