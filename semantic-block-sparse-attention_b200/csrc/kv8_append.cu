@@ -14,9 +14,9 @@
 // Bound: HBM, 2 bytes read and 1 written per value.  The maximum is needed before the first code, so a
 // thread holds its share of the block in registers between the two steps and the input is read once.  A few
 // tokens of each request take a warp per head (kv8_token_kernel), more of them one thread block per cache block
-// and head (kv8_append_kernel); a prompt's blocks are a stream
-// (kv8_stream_kernel): while a group of threads works on one block from registers, the next one's rows travel
-// into shared memory (131072 tokens x 4 heads x 256: 166 us without that overlap).
+// and head (kv8_append_kernel); a prompt's blocks are a stream (kv8_stream_kernel): while a group of threads works
+// on one block from registers, the next one's rows travel into shared memory.  131072 tokens x 4 heads x 256:
+// 126 us, 6.4 TB/s; 163 us block by block, and no less as a stream while the rare cases were unrolled in the loop.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

@@ -16,7 +16,9 @@
 //     bytes are its elements of four k-steps.  The same freedom over the rows of O^T = V^T P^T turns 16
 //     consecutive bytes of four keys into eight A fragments with two byte permutes per four values;
 //   * P^T is S^T's accumulator transposed by movmatrix; heads are the n dimension of both products, so that
-//     up to 8 rows (queries x heads of a KV head) cost one n-tile, up to 16 two.
+//     8 rows (queries x heads of a KV head) cost one n-tile.  A row tile has up to four of them (two at D = 256, where
+//     O fills the registers): 80 x 3071 keys x 8 heads x 64 with 24 rows each 166 us in tiles of 16, 104 in one of 24.
+//     There the latency of the products and the softmax between them bounds it, not HBM.
 // V's scale changes from block to block, so P carries it: P' = 2^(s + log2 scale - M + 11) in fp16 with its own
 // running reference M next to the softmax's m (a block of large values with little weight must not push the
 // others under fp16's range).  Both move only when a score passes them by 2^4: P' stays below 2^15, and what
