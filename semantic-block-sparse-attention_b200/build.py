@@ -16,7 +16,7 @@ CSRC = HERE / "csrc"
 LIB = HERE / "libsemblo_b200.so"
 SOURCES = ["host_common.cu", "index_build.cu", "select.cu", "prefill.cu", "prefill_sparse.cu", "decode.cu",
            "rotary.cu", "kv8_append.cu", "kv8_decode.cu", "dense_prefill.cu",
-           "dense_pair.cu"]
+           "dense_narrow.cu"]
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
          "--expt-relaxed-constexpr", "--extended-lambda", "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
 

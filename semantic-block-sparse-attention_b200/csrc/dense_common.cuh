@@ -117,10 +117,12 @@ __device__ __forceinline__ Tile find_tile(const Args& a, int want) {
 
 // For more documents, in their order (and a document's last tiles first): all threads of the block, a run of documents
 // each.  Two barriers, which every thread has to reach.
+constexpr int FIND_BYTES = 128;                    // of shared memory
 template <int THREADS>
-__device__ __forceinline__ Tile find_tile_block(const Args& a, int want) {
-  __shared__ int totals[THREADS / 32];
-  __shared__ Tile found;
+__device__ __forceinline__ Tile find_tile_block(const Args& a, int want, void* scratch) {
+  static_assert(sizeof(Tile) % 8 == 0 && sizeof(Tile) + THREADS / 8 <= FIND_BYTES, "scratch");
+  Tile& found = *static_cast<Tile*>(scratch);
+  int* totals = reinterpret_cast<int*>(&found + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qt = a.queries_per_tile;
   const int per = (a.docs + THREADS - 1) / THREADS;
   const int d0 = min((int)threadIdx.x * per, a.docs), d1 = min(d0 + per, a.docs);
@@ -485,8 +487,9 @@ __device__ __forceinline__ void store_partial(uint32_t tmem, float* to, bool kee
 // Joins the pieces of a tile: blockIdx.x is its share without a split; 8 dimensions of a row per thread.
 template <int D, int BN, bool F16>
 __global__ void __launch_bounds__(256) join_pieces_kernel(const Args a) {
+  __shared__ __align__(8) uint8_t scratch[FIND_BYTES];
   const Share share(a, 1);
-  const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, share.want) : find_tile_block<256>(a, share.want);
+  const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, share.want) : find_tile_block<256>(a, share.want, scratch);
   pdl_wait();                                        // every block waits: this launch must not end before the other
   if (tile.doc < 0) return;
   const KeyTiles<BN> keys(a, tile);

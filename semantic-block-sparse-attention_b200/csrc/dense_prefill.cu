@@ -13,7 +13,7 @@
 
 #include "../../include/semblo_b200.h"
 #include "dense_common.cuh"
-#include "dense_pair.h"
+#include "dense_narrow.h"
 #include "host_common.h"
 
 using namespace dense;
@@ -34,7 +34,8 @@ struct Cfg {
   static constexpr int MX_OFF = EPI_OFF + 1024;               // float [2][2][128]: half-row maxima
   static constexpr int BAR_OFF = MX_OFF + 2048;
   static constexpr int SLOT_OFF = BAR_OFF + 256;
-  static constexpr int TOTAL = SLOT_OFF + 64;
+  static constexpr int FIND_OFF = SLOT_OFF + 64;              // of the search among many documents
+  static constexpr int TOTAL = FIND_OFF + FIND_BYTES;
   static constexpr int O_COL = 2 * BN;                        // S/P buffers, then O, then Q
   static constexpr int Q_COL = O_COL + D;
   static constexpr int TMEM_COLS = Q_COL + D / 2 <= 256 ? 256 : 512;
@@ -59,7 +60,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     if (threadIdx.x == 0) atomicCAS(a.status, 0, STATUS_SMEM_ALIGN);
     return;
   }
-  const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, share.want) : find_tile_block<320>(a, share.want);
+  const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, share.want) : find_tile_block<320>(a, share.want, smem + C::FIND_OFF);
   if (tile.doc < 0) {
     if (a.zero_tail && share.split == 0) zero_tail<D>(a, tile.first, h, blockDim.x);
     return;
@@ -476,7 +477,7 @@ extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64
   a.out = out; a.lse = lse;
   a.cu_q = cu_seqlens_q; a.cu_k = cu_seqlens_k; a.prefix = prefix_lens; a.slopes = alibi_slopes;
   a.docs = documents; a.group = group; a.num_q_heads = num_q_heads;
-  a.queries_per_tile = 128 / group;                // D = 256; launch_pair chooses its own
+  a.queries_per_tile = 128 / group;
   a.num_kv_heads = num_kv_heads;
   a.tokens_q = tokens_q; a.tokens_k = tokens_k;
   a.causal = causal; a.window = window; a.zero_tail = zero_tail;
@@ -495,7 +496,7 @@ extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64
   const uint64_t dims[3] = {(uint64_t)head_dim, (uint64_t)num_kv_heads, (uint64_t)std::max<int64_t>(tokens_k, 1)};
   const uint64_t sk[2] = {(uint64_t)k_head_stride * 2, (uint64_t)k_token_stride * 2};
   const uint64_t sv[2] = {(uint64_t)v_head_stride * 2, (uint64_t)v_token_stride * 2};
-  const int bn = head_dim <= 128 ? PAIR_BN : BN;
+  const int bn = head_dim <= 128 ? NARROW_BN : BN;
   const uint32_t box[3] = {64, 1, (uint32_t)bn};
   const uint64_t dense_stride[2] = {(uint64_t)head_dim * 2, (uint64_t)head_dim * num_kv_heads * 2};
   int rc = semblo::make_tensor_map_bf16(&mk, tokens_k ? k : q, 3, dims, tokens_k ? sk : dense_stride, box);
@@ -513,13 +514,13 @@ extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64
   cudaStream_t st = (cudaStream_t)stream;
   const bool f16 = dtype == SEMBLO_F16;
   const int mode = alibi_slopes ? BIASED : softcap > 0.f ? (!f16 && a.cap_log2 <= BOUNDED_LOG2 ? BOUNDED : CAPPED) : LINEAR;
-  if (head_dim <= 128) rc = dense::launch_pair(mk, mv, mq, a, head_dim, f16, mode, st);
+  if (head_dim <= 128) rc = dense::launch_narrow(mk, mv, mq, a, head_dim, f16, mode, st);
   else if (mode == LINEAR) rc = f16 ? launch<256, true, LINEAR>(mk, mv, a, st) : launch<256, false, LINEAR>(mk, mv, a, st);
   else if (mode == BOUNDED) rc = launch<256, false, BOUNDED>(mk, mv, a, st);
   else if (mode == CAPPED) rc = f16 ? launch<256, true, CAPPED>(mk, mv, a, st) : launch<256, false, CAPPED>(mk, mv, a, st);
   else rc = f16 ? launch<256, true, BIASED>(mk, mv, a, st) : launch<256, false, BIASED>(mk, mv, a, st);
   if (rc || a.splits == 1) return rc;
-  if (head_dim == 64) return f16 ? join_pieces<64, PAIR_BN, true>(a, st) : join_pieces<64, PAIR_BN, false>(a, st);
-  if (head_dim == 128) return f16 ? join_pieces<128, PAIR_BN, true>(a, st) : join_pieces<128, PAIR_BN, false>(a, st);
+  if (head_dim == 64) return f16 ? join_pieces<64, NARROW_BN, true>(a, st) : join_pieces<64, NARROW_BN, false>(a, st);
+  if (head_dim == 128) return f16 ? join_pieces<128, NARROW_BN, true>(a, st) : join_pieces<128, NARROW_BN, false>(a, st);
   return f16 ? join_pieces<256, BN, true>(a, st) : join_pieces<256, BN, false>(a, st);
 }
