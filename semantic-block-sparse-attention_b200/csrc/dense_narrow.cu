@@ -168,12 +168,14 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       if (ok) umma_commit(bar(B_O));
     }
   } else {
-    // ------------------------------------------------------------ softmax + epilogue: one or two threads per row
+    // ------------------------------------------------------------ softmax + epilogue: one thread per row
     const int row = threadIdx.x & 127;
     const int qi = row / a.group, hg = row - qi * a.group;
     const bool valid = qi < tile.count;
-    const int p = tile.pos + qi;
-    const Seen seen = valid ? seen_by(a, tile, p) : Seen{0, 0, 0};
+    // a row that no query has counts as the last query's, so that its warp need not mask more than that
+    const int p = tile.pos + min(qi, tile.count - 1);
+    const Seen seen = seen_by(a, tile, p);
+    const bool idle = warp * 32 >= tile.count * a.group;     // no row of this warp has a query
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_addr + C::S_COL;
     const uint32_t o_addr = tmem_base + lane_addr + C::O_COL;
@@ -187,6 +189,10 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       const int key0 = keys.at(j), b = j & 1;
       ok = mbar_wait_warp(bar(B_S + b), (uint32_t)((j >> 1) & 1), abort_flag, a.status, STATUS_TIMEOUT_SOFTMAX);
       if (!ok) break;
+      if (idle) {                                  // whatever P is
+        if (lane == 0) mbar_arrive(bar(B_P + b));
+        continue;
+      }
       tc_fence_after();
       const uint32_t s_buf = s_addr + b * BN;
       if constexpr (MODE == BOUNDED) {

@@ -173,8 +173,10 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     const int row = threadIdx.x & 127;
     const int qi = row / a.group, hg = row - qi * a.group;
     const bool valid = qi < tile.count;
-    const int p = tile.pos + qi;
-    const Seen seen = valid ? seen_by(a, tile, p) : Seen{0, 0, 0};
+    // a row that no query has counts as the last query's, so that its warp need not mask more than that
+    const int p = tile.pos + min(qi, tile.count - 1);
+    const Seen seen = seen_by(a, tile, p);
+    const bool idle = (warp & 3) * 32 >= tile.count * a.group;     // no row of this warp has a query
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
     const int head = h * a.group + hg;
     const float slope = a.slopes && valid ? a.slopes[head] * LOG2EF : 0.f;
@@ -204,6 +206,10 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       const int b = j & 1, key0 = keys.at(j) + 32 * hf;
       ok = mbar_wait_warp(bar(B_SFULL + b), (uint32_t)((j >> 1) & 1), abort_flag, a.status, STATUS_TIMEOUT_SOFTMAX);
       if (!ok) break;
+      if (idle) {                                  // whatever P is
+        if (lane == 0) mbar_arrive(bar(B_PFULL + b));
+        continue;
+      }
       tc_fence_after();
       const uint32_t s_addr = tmem_base + lane_addr + b * BN + hf * 32;
       const bool active = tile.lk > key0;                // the product wrote at least one page of this half
