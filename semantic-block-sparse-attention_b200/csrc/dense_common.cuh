@@ -29,7 +29,7 @@ struct Args {
   float score_scale;              // raw product -> log2 units, or -> 8/3 of the capping tanh's argument
   float cap_log2;                 // cap * log2(e)
   int* status;
-  int splits;                     // pieces that a tile's keys may be cut into, a block each
+  int splits, piece_keys;         // pieces that a tile's keys may be cut into, a block each, and their least size
   float* partial;                 // with splits > 1: [tile][KV head][splits][record_floats(D)]
 };
 
@@ -226,11 +226,10 @@ struct KeyTiles {
   __device__ __forceinline__ int at(int j) const { j += base; return (j < gp ? j : j - gp + glo) * BN; }
 };
 
-// ---- keys cut into pieces, where there are too few tiles for the multiprocessors.  A piece has SPLIT_KEYS keys at
-// least; its block leaves O, the reference and the sum of each of its 128 rows, and a second launch joins them.
-constexpr int SPLIT_KEYS = 512;
+// ---- keys cut into pieces, where there are too few tiles for the multiprocessors.  A piece's block leaves O, the
+// reference and the sum of each of its 128 rows, and a second launch joins them.
 __host__ __device__ constexpr int record_floats(int d) { return 128 * (d + 2); }       // O [128][D], m [128], l [128]
-__device__ __forceinline__ int pieces_of(const Args& a, int n, int bn) { return min(a.splits, max(1, n / (SPLIT_KEYS / bn))); }
+__device__ __forceinline__ int pieces_of(const Args& a, int n, int bn) { return min(a.splits, max(1, n * bn / a.piece_keys)); }
 
 // The block's share of the grid: tile number `want` of KV head h, piece `split`.
 struct Share {

@@ -404,23 +404,28 @@ int join_pieces(const Args& a, cudaStream_t st) {
   return 0;
 }
 
-// Into how many pieces a tile's keys may be cut: as many as bring the longest tile down to what each multiprocessor
-// would get of an even share (causal tiles differ, so that is up to twice the free room).  A tile's mean number of
-// keys is what a document has less half its queries.  us without and with: 16 tokens x 32 heads over 8 x 128 behind
-// 8192 others 139 : 25, 128 behind 30000 463 : 95, 512 behind 30000 469 : 278, 8192 tokens x 4 heads over 1 136 : 106;
-// 1024 tokens x 8 heads over 2 20 : 24, so two short pieces are not worth the second launch.
-int splits_for(int64_t tokens_q, int64_t tokens_k, int group, int num_kv_heads, int head_dim, int documents, int causal,
-               int window, bool prefix) {
-  if (documents == 0) return 1;
+// Into how many pieces a tile's keys may be cut, and the least keys of a piece.  Pieces of 512 keys: as many as bring
+// the longest tile down to what each multiprocessor would get of an even share (causal tiles differ, so that is up to
+// twice the free room).  A tile's mean number of keys is what a document has less half its queries.  Where even half
+// the blocks that fit are not there, pieces of 256: the join, which reads every piece, is small then.  us without
+// and with, D = 128: 16 tokens x 32 heads over 8 behind 8192 others 139 -> 22, 128 behind 30000 463 -> 71, 512 behind
+// 30000 469 -> 242, 8192 tokens x 4 heads over 1 136 -> 105, 11 tokens of 2 documents behind 1250 20 -> 13 (in pieces
+// of 512: 20); 1024 tokens x 8 heads over 2 20 -> 24, so a tile of few keys is not cut.
+struct Split { int pieces, keys; };
+Split split_for(int64_t tokens_q, int64_t tokens_k, int group, int num_kv_heads, int head_dim, int documents, int causal,
+                int window, bool prefix) {
+  if (documents == 0 || tokens_q == 0) return {1, 512};
   const int64_t qt = 128 / group, tiles = (tokens_q + documents * (qt - 1)) / qt;      // no more than these have queries
-  const int64_t slots = (int64_t)semblo::sm_count() * (head_dim == 256 ? 1 : 2);
+  const int64_t slots = (int64_t)semblo::sm_count() * (head_dim == 256 ? 1 : 2), units = tiles * num_kv_heads;
   int64_t keys = tokens_k / documents;
   if (window > 0 && !prefix) keys = std::min<int64_t>(keys, window + qt);
   // the longest tile's keys over the mean of all
   const double skew = causal && tokens_q < tokens_k ? 2.0 * tokens_k / (2.0 * tokens_k - tokens_q) : causal ? 2.0 : 1.0;
-  if (keys < 1.5 * SPLIT_KEYS * skew) return 1;
-  const int64_t room = (int64_t)(skew * slots / std::max<int64_t>(1, tiles * num_kv_heads));
-  return (int)std::max<int64_t>(1, std::min<int64_t>({room, keys / SPLIT_KEYS, 32}));
+  int64_t large = keys < 768 * skew ? 1 : std::min<int64_t>((int64_t)(skew * slots / units), keys / 512);
+  int64_t small = keys < 512 * skew ? 1 : std::min(slots / (2 * units), keys / 256);
+  large = std::min<int64_t>(std::max<int64_t>(large, 1), 32);
+  small = std::min<int64_t>(small, 32);
+  return small > large ? Split{(int)small, 256} : Split{(int)large, 512};
 }
 
 int64_t split_bytes(int64_t tokens_q, int group, int num_kv_heads, int head_dim, int documents, int splits) {
@@ -454,7 +459,7 @@ extern "C" int64_t semblo_dense_prefill_workspace_bytes(int64_t tokens_q, int64_
   if (rc) return rc;
   const int group = num_q_heads / num_kv_heads;
   return split_bytes(tokens_q, group, num_kv_heads, head_dim, documents,
-                     splits_for(tokens_q, tokens_k, group, num_kv_heads, head_dim, documents, causal, window, has_prefix));
+                     split_for(tokens_q, tokens_k, group, num_kv_heads, head_dim, documents, causal, window, has_prefix).pieces);
 }
 
 extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
@@ -490,7 +495,9 @@ extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64
   a.score_scale = softcap > 0.f ? sm_scale / softcap * TANH_ARG : sm_scale * LOG2EF;
   a.cap_log2 = softcap * LOG2EF;
   a.status = status;
-  a.splits = splits_for(tokens_q, tokens_k, group, num_kv_heads, head_dim, documents, causal, window, prefix_lens != nullptr);
+  const Split split = split_for(tokens_q, tokens_k, group, num_kv_heads, head_dim, documents, causal, window, prefix_lens != nullptr);
+  a.splits = split.pieces;
+  a.piece_keys = split.keys;
   a.partial = (float*)workspace;
   const int64_t bytes = split_bytes(tokens_q, group, num_kv_heads, head_dim, documents, a.splits);
   SEMBLO_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "the workspace must be 16-byte aligned");
