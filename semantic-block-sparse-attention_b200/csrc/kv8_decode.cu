@@ -27,8 +27,8 @@
 // Work is split evenly whatever the lengths: the 16-key groups of all (request, KV head, row tile) segments
 // form one line, every block takes an equal piece of it, writes the segments that lie inside its piece and
 // leaves partials of those that do not; a second launch (a programmatic dependent) merges them.  Where the
-// lengths turn out short, blocks take whole segments, and where the table allows no segment of more than 64
-// groups, there is no second launch.
+// lengths turn out short, blocks take whole segments, and where the table allows no segment of more than
+// 8 groups per warp of a block, there is no second launch.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -42,10 +42,8 @@ using semblo::ceil_div;
 
 namespace {
 
-constexpr int WARPS = 8;
-constexpr int THREADS = WARPS * 32;
 constexpr int GROUP = 16;                 // keys per step of a warp
-constexpr int DIRECT_GROUPS = 64;         // longest segment that one block takes whole
+constexpr int DIRECT_STEPS = 8;           // steps of a block's warps that one block takes for a whole segment
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr float GAP = 4.f;                // log2 units by which a score may pass a reference
@@ -141,13 +139,17 @@ __device__ __forceinline__ Span span_of(const DecodeArgs& a, int b) {
 template <int D, int NT>
 struct Cfg {
   static constexpr int STAGES = D == 256 ? 3 : D == 128 ? (NT > 2 ? 4 : 3) : 4;
+  // two blocks per multiprocessor, of fewer warps where their registers are many (and the ring is large)
+  static constexpr int WARPS = D == 256 || NT > 2 || (D == 128 && NT == 2) ? 4 : 8;
+  static constexpr int THREADS = WARPS * 32;
+  static constexpr int PER_SM = 2;
+  static constexpr int DIRECT = DIRECT_STEPS * WARPS;           // groups
   static constexpr int KV_BYTES = GROUP * D;                    // K or V of a group
   static constexpr int RING = STAGES * 2 * KV_BYTES;            // per warp
   static constexpr int KC = D / 32;                             // 16-byte pieces of K per lane
   static constexpr int VI = D == 256 ? 2 : 1;                   // pieces of V per lane and key (16 bytes, 8 for D = 64)
   static constexpr int KSTEPS = D / 16;
   static constexpr int ROWS = 8 * NT;
-  static constexpr int PER_SM = D == 256 || NT > 2 || (D == 128 && NT == 2) ? 1 : 2;     // resident blocks
   static constexpr bool Q_SMEM = D * NT > 256;                  // the query's fragments do not fit in registers
   static constexpr int ACC = KSTEPS * NT * 4;                   // accumulators of O^T per lane
   static constexpr int RECORD = ACC * 32 + 3 * ROWS;            // floats: O fragments, then m, M, l of each row
@@ -192,15 +194,16 @@ __device__ __forceinline__ int line_sums(const DecodeArgs& a, int segs, int* sum
   return longest;
 }
 
-__device__ __forceinline__ int quota_of(int total, int blocks) {
-  return max(WARPS, (total + blocks - 1) / blocks);
+// Groups of a block's piece: no fewer than give each of its warps one.
+__device__ __forceinline__ int quota_of(int total, int blocks, int warps) {
+  return max(warps, (total + blocks - 1) / blocks);
 }
 
 // Whether a block takes whole segments: where the rounds that this needs cost less than even pieces with their
-// merge, which is worth DIRECT_GROUPS of them.  Tables are as wide as the longest request may grow, so that what
+// merge, which is worth `direct` groups.  Tables are as wide as the longest request may grow, so that what
 // the launch is sized for says little about the lengths in it.
-__device__ __forceinline__ bool takes_whole(int segments, int longest, int quota, int blocks) {
-  return (int64_t)((segments + blocks - 1) / blocks) * longest <= quota + DIRECT_GROUPS;
+__device__ __forceinline__ bool takes_whole(int segments, int longest, int quota, int blocks, int direct) {
+  return (int64_t)((segments + blocks - 1) / blocks) * longest <= quota + direct;
 }
 
 // Element e of a record in fragment order -> row of the tile and dimension.
@@ -227,8 +230,9 @@ __device__ __forceinline__ float finish_factor(float m, float mv, float l) {
 
 // ---------------------------------------------------------------- attention
 template <int D, int NT, bool CAP>
-__global__ void __launch_bounds__(THREADS, Cfg<D, NT>::PER_SM) kv8_decode_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__((Cfg<D, NT>::THREADS), (Cfg<D, NT>::PER_SM)) kv8_decode_kernel(const DecodeArgs a) {
   using C = Cfg<D, NT>;
+  constexpr int WARPS = C::WARPS, THREADS = C::THREADS;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   int* sums = reinterpret_cast<int*>(smem + C::SUM_OFF);
@@ -246,8 +250,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NT>::PER_SM) kv8_decode_kernel
   int pos = blockIdx.x, end = a.batch * segs;
   int* const whole = scratch + 2 * WARPS;                           // read again for every segment: no register through its loop
   if (!a.direct) {
-    const int longest = line_sums(a, segs, sums, scratch), total = sums[a.batch], quota = quota_of(total, gridDim.x);
-    const bool w = takes_whole(end, longest, quota, gridDim.x);
+    const int longest = line_sums(a, segs, sums, scratch), total = sums[a.batch], quota = quota_of(total, gridDim.x, WARPS);
+    const bool w = takes_whole(end, longest, quota, gridDim.x, C::DIRECT);
     if (threadIdx.x == 0) *whole = w;
     __syncthreads();
     if (!w) {
@@ -658,28 +662,28 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NT>::PER_SM) kv8_decode_kernel
 // parts in turn, a lane 4 of a fragment's 128 values; the first of them are on their way while the references and
 // sums of all parts become a factor each.  One thread per value with the parts one after the other took 16 us
 // for 524288 keys x 4 heads x 256 (of 186 in all), this takes 6.
-constexpr int MERGE_AHEAD = 4;
+constexpr int MERGE_AHEAD = 4, MERGE_WARPS = 8, MERGE_THREADS = MERGE_WARPS * 32;
 
 template <int D, int NT>
-__global__ void __launch_bounds__(THREADS) kv8_merge_kernel(const DecodeArgs a, int blocks) {
+__global__ void __launch_bounds__(MERGE_THREADS) kv8_merge_kernel(const DecodeArgs a, int blocks) {
   using C = Cfg<D, NT>;
   extern __shared__ __align__(16) uint8_t smem[];
-  float4* slots = reinterpret_cast<float4*>(smem);              // [WARPS][32]
-  float* most = reinterpret_cast<float*>(slots + WARPS * 32);   // [2][WARPS][8]
-  float* sum_l = most + 2 * WARPS * 8;                          // [WARPS][8]
-  float* state = sum_l + WARPS * 8;                             // [3][blocks][8]: m, M (then the factor), l of each part
+  float4* slots = reinterpret_cast<float4*>(smem);              // [MERGE_WARPS][32]
+  float* most = reinterpret_cast<float*>(slots + MERGE_WARPS * 32);   // [2][MERGE_WARPS][8]
+  float* sum_l = most + 2 * MERGE_WARPS * 8;                          // [MERGE_WARPS][8]
+  float* state = sum_l + MERGE_WARPS * 8;                             // [3][blocks][8]: m, M (then the factor), l of each part
   int* sums = reinterpret_cast<int*>(state + 3 * blocks * 8);
   int* scratch = sums + a.batch + 1;
   const int segs = a.num_kv_heads * a.row_tiles;
   const int b = blockIdx.x / segs, seg = blockIdx.x - b * segs;
   const int longest = line_sums(a, segs, sums, scratch);
   const Span sp = span_of(a, b);
-  const int quota = quota_of(sums[a.batch], blocks);
+  const int quota = quota_of(sums[a.batch], blocks, C::WARPS);
   const int s0 = sums[b] + seg * sp.groups, s1 = s0 + sp.groups;
   const int c0 = s0 / quota, c1 = sp.groups ? (s1 - 1) / quota : c0;
   sm100::pdl_wait();                                  // every block waits: this launch must not end before the other
   // one block had it whole
-  if ((sp.groups > 0 && c0 == c1) || takes_whole(a.batch * segs, longest, quota, blocks)) return;
+  if ((sp.groups > 0 && c0 == c1) || takes_whole(a.batch * segs, longest, quota, blocks, C::DIRECT)) return;
   const int parts = sp.groups ? c1 - c0 + 1 : 0;
   // the block where the segment starts left it in its slot 1, the others in their slot 0
   auto record = [&](int i) { return a.partial + ((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * C::RECORD; };
@@ -690,13 +694,13 @@ __global__ void __launch_bounds__(THREADS) kv8_merge_kernel(const DecodeArgs a, 
   const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
   float4 ahead[MERGE_AHEAD];
 #pragma unroll
-  for (int x = 0; x < MERGE_AHEAD; ++x) ahead[x] = warp + x * WARPS < parts ? values(blockIdx.y, warp + x * WARPS) : zero;
+  for (int x = 0; x < MERGE_AHEAD; ++x) ahead[x] = warp + x * MERGE_WARPS < parts ? values(blockIdx.y, warp + x * MERGE_WARPS) : zero;
 
   // ---- a factor for each part and row; thread: row tid & 7, parts tid / 8, + 32, ...
   const int row = threadIdx.x & 7;
   float* const state_m = state, * const state_mv = state + blocks * 8, * const state_l = state + 2 * blocks * 8;
   float mt = -INFINITY, mvt = -INFINITY;
-  for (int i = threadIdx.x >> 3; i < parts; i += THREADS / 8) {
+  for (int i = threadIdx.x >> 3; i < parts; i += MERGE_THREADS / 8) {
     const float* x = record(i) + C::ACC * 32 + nt * 8 + row;
     const float m = __ldcg(x), mv = __ldcg(x + C::ROWS), l = __ldcg(x + 2 * C::ROWS);
     state_m[i * 8 + row] = m; state_mv[i * 8 + row] = mv; state_l[i * 8 + row] = l;
@@ -708,15 +712,15 @@ __global__ void __launch_bounds__(THREADS) kv8_merge_kernel(const DecodeArgs a, 
     mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
     mvt = fmaxf(mvt, __shfl_xor_sync(0xffffffffu, mvt, o));
   }
-  if (lane < 8) { most[warp * 8 + lane] = mt; most[(WARPS + warp) * 8 + lane] = mvt; }
+  if (lane < 8) { most[warp * 8 + lane] = mt; most[(MERGE_WARPS + warp) * 8 + lane] = mvt; }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
+  for (int w = 0; w < MERGE_WARPS; ++w) {
     mt = fmaxf(mt, most[w * 8 + row]);
-    mvt = fmaxf(mvt, most[(WARPS + w) * 8 + row]);
+    mvt = fmaxf(mvt, most[(MERGE_WARPS + w) * 8 + row]);
   }
   float lt = 0.f;
-  for (int i = threadIdx.x >> 3; i < parts; i += THREADS / 8) {
+  for (int i = threadIdx.x >> 3; i < parts; i += MERGE_THREADS / 8) {
     lt += state_l[i * 8 + row] * ratio2(state_m[i * 8 + row], mt);
     state_mv[i * 8 + row] = ratio2(state_mv[i * 8 + row], mvt);
   }
@@ -726,7 +730,7 @@ __global__ void __launch_bounds__(THREADS) kv8_merge_kernel(const DecodeArgs a, 
   __syncthreads();
   lt = 0.f;
 #pragma unroll
-  for (int w = 0; w < WARPS; ++w) lt += sum_l[w * 8 + row];
+  for (int w = 0; w < MERGE_WARPS; ++w) lt += sum_l[w * 8 + row];
 
   // ---- the values: of fragment lane 4 (lane & 7) + k, accumulator lane >> 3, that is of row 2 k + (lane >> 3 & 1)
   const int h = seg / a.row_tiles, out_row = (seg - h * a.row_tiles) * C::ROWS + nt * 8 + row;
@@ -738,13 +742,13 @@ __global__ void __launch_bounds__(THREADS) kv8_merge_kernel(const DecodeArgs a, 
     };
 #pragma unroll
     for (int x = 0; x < MERGE_AHEAD; ++x)
-      if (warp + x * WARPS < parts) add(ahead[x], warp + x * WARPS);
+      if (warp + x * MERGE_WARPS < parts) add(ahead[x], warp + x * MERGE_WARPS);
 #pragma unroll 4
-    for (int i = warp + MERGE_AHEAD * WARPS; i < parts; i += WARPS) add(values(j, i), i);
+    for (int i = warp + MERGE_AHEAD * MERGE_WARPS; i < parts; i += MERGE_WARPS) add(values(j, i), i);
     const int next = j + gridDim.y;
     if (next < C::KSTEPS) {
 #pragma unroll
-      for (int x = 0; x < MERGE_AHEAD; ++x) if (warp + x * WARPS < parts) ahead[x] = values(next, warp + x * WARPS);
+      for (int x = 0; x < MERGE_AHEAD; ++x) if (warp + x * MERGE_WARPS < parts) ahead[x] = values(next, warp + x * MERGE_WARPS);
     }
     slots[warp * 32 + lane] = acc;
     __syncthreads();
@@ -754,7 +758,7 @@ __global__ void __launch_bounds__(THREADS) kv8_merge_kernel(const DecodeArgs a, 
       const float* at0 = reinterpret_cast<const float*>(slots) + (row & 1) * 32 + g * 4 + (row >> 1);
       float lo = 0.f, hi = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) { lo += at0[w * 128]; hi += at0[w * 128 + 64]; }
+      for (int w = 0; w < MERGE_WARPS; ++w) { lo += at0[w * 128]; hi += at0[w * 128 + 64]; }
       const float f = finish_factor(mt, mvt, lt);
       lo = lt == 0.f ? 0.f : lo * f;
       hi = lt == 0.f ? 0.f : hi * f;
@@ -783,10 +787,10 @@ template <int D, int NT>
 Plan plan_for(int64_t segments, int64_t longest) {
   using C = Cfg<D, NT>;
   Plan p;
-  p.direct = longest <= DIRECT_GROUPS;
-  // no more blocks than there can be pieces of WARPS groups
+  p.direct = longest <= C::DIRECT;
+  // no more blocks than there can be pieces
   p.blocks = (int)(p.direct ? segments
-                            : std::min<int64_t>((int64_t)semblo::sm_count() * C::PER_SM, ceil_div(segments * longest, WARPS)));
+                            : std::min<int64_t>((int64_t)semblo::sm_count() * C::PER_SM, ceil_div(segments * longest, C::WARPS)));
   p.bytes = p.direct ? 0 : (int64_t)p.blocks * 2 * C::RECORD * 4;
   return p;
 }
@@ -800,12 +804,12 @@ int64_t longest_segment(int queries, int window, int table_len, int block_size, 
 template <int D, int NT, bool CAP>
 int launch(DecodeArgs& a, const Plan& plan, cudaStream_t st) {
   using C = Cfg<D, NT>;
-  const int sums = (a.batch + 2 + 2 * WARPS) * 4;
+  const int sums = (a.batch + 2 + 2 * std::max(C::WARPS, MERGE_WARPS)) * 4;
   const int smem = C::SUM_OFF + sums;
   auto kern = kv8_decode_kernel<D, NT, CAP>;
   SEMBLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   a.direct = plan.direct;
-  kern<<<plan.blocks, THREADS, smem, st>>>(a);
+  kern<<<plan.blocks, C::THREADS, smem, st>>>(a);
   SEMBLO_LAUNCH_CHECK();
   if (plan.direct) return 0;
   cudaLaunchConfig_t cfg{};
@@ -813,8 +817,8 @@ int launch(DecodeArgs& a, const Plan& plan, cudaStream_t st) {
   const int segments = a.batch * a.num_kv_heads * a.row_tiles;
   const int slices = std::max(1, std::min(C::KSTEPS, 8 * semblo::sm_count() / (segments * NT)));
   cfg.gridDim = dim3((unsigned)segments, (unsigned)slices, NT);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = WARPS * 32 * 16 + (3 * WARPS + 3 * plan.blocks) * 8 * 4 + sums;
+  cfg.blockDim = dim3(MERGE_THREADS);
+  cfg.dynamicSmemBytes = MERGE_WARPS * 32 * 16 + (3 * MERGE_WARPS + 3 * plan.blocks) * 8 * 4 + sums;
   SEMBLO_CUDA(cudaFuncSetAttribute(kv8_merge_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    (int)cfg.dynamicSmemBytes));
   cfg.stream = st;
