@@ -17,7 +17,8 @@
 //     consecutive bytes of four keys into eight A fragments with two byte permutes per four values;
 //   * P^T is S^T's accumulator transposed by movmatrix; heads are the n dimension of both products, so that
 //     8 rows (queries x heads of a KV head) cost one n-tile.  A row tile has up to four of them (two at D = 256, where
-//     O fills the registers): 80 x 3071 keys x 8 heads x 64 with 24 rows each 166 us in tiles of 16, 104 in one of 24.
+//     O fills the registers): 80 x 3071 keys x 8 heads x 64 with 24 rows each 166 us in tiles of 16, 104 in one of 24
+//     (90 in two blocks of four warps per multiprocessor instead of one of eight).
 //     There the latency of the products and the softmax between them bounds it, not HBM.
 // V's scale changes from block to block, so P carries it: P' = 2^(s + log2 scale - M + 11) in fp16 with its own
 // running reference M next to the softmax's m (a block of large values with little weight must not push the
