@@ -228,7 +228,7 @@ struct KeyTiles {
 
 // ---- keys cut into pieces, where there are too few tiles for the multiprocessors.  A piece's block leaves O, the
 // reference and the sum of each of its 128 rows, and a second launch joins them.
-__host__ __device__ constexpr int record_floats(int d) { return 128 * (d + 2); }       // O [128][D], m [128], l [128]
+__host__ __device__ constexpr int record_floats(int d) { return 128 * (d + 3); }       // O [128][D], m, l, lr [128]
 __device__ __forceinline__ int pieces_of(const Args& a, int n, int bn) { return min(a.splits, max(1, n * bn / a.piece_keys)); }
 
 // The block's share of the grid: tile number `want` of KV head h, piece `split`.
@@ -448,6 +448,30 @@ __host__ __device__ constexpr uint32_t idesc_of(int m, int n, bool b_mn_major) {
   return F16 ? d & ~((1u << 7) | (1u << 10)) : d;
 }
 
+// A row's sum of P, twice where P is bf16: as computed, for the log-sum-exp, and as rounded, which divides O.  So the
+// weights sum to 1 as the products see them: a row that sees one key gives its V whatever the reference is, and
+// dominant weights lose nothing.  fp16's rounding is an eighth of bf16's and is left.
+template <bool F16>
+struct RowSum {
+  f32x2 exact[2], rounded[2];
+  __device__ __forceinline__ RowSum() {
+    exact[0] = exact[1] = rounded[0] = rounded[1] = join(0.f, 0.f);
+  }
+  __device__ __forceinline__ void add(int i, float e0, float e1, uint32_t packed) {
+    exact[i & 1] = add2(exact[i & 1], join(e0, e1));
+    if constexpr (!F16)
+      rounded[i & 1] = add2(rounded[i & 1], join(__uint_as_float(packed << 16), __uint_as_float(packed & 0xffff0000u)));
+  }
+  __device__ __forceinline__ void into(float& l, float& lr) const {
+    float x, y;
+    split(add2(exact[0], exact[1]), x, y);
+    l += x + y;
+    if constexpr (F16) { lr = l; return; }
+    split(add2(rounded[0], rounded[1]), x, y);
+    lr += x + y;
+  }
+};
+
 // A warp's share of the output: each lane holds 32 values of its row (16-byte pieces piece0 ... + 3 as packed
 // words) and has put them into `stage` (32 rows of PIECES 16-byte pieces, permuted so that neither side
 // collides); this writes `rows` rows of it, PIECES lanes to a row, so that whole lines leave at once.
@@ -500,7 +524,7 @@ __global__ void __launch_bounds__(256) join_pieces_kernel(const Args a) {
     const int r = i / CH, c = i - r * CH;
     float m = -INFINITY;
     for (int s = 0; s < pieces; ++s) m = fmaxf(m, __ldcg(first + s * record_floats(D) + 128 * D + r));
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f, lr = 0.f;
 #pragma unroll 4
     for (int s = 0; s < pieces; ++s) {
       const float* record = first + s * record_floats(D);
@@ -508,10 +532,11 @@ __global__ void __launch_bounds__(256) join_pieces_kernel(const Args a) {
       const float4 x = __ldcg(reinterpret_cast<const float4*>(record + r * D + c * 8));
       const float4 y = __ldcg(reinterpret_cast<const float4*>(record + r * D + c * 8) + 1);
       l += f * __ldcg(record + 128 * D + 128 + r);
+      lr += f * __ldcg(record + 128 * D + 256 + r);
       acc[0] += f * x.x; acc[1] += f * x.y; acc[2] += f * x.z; acc[3] += f * x.w;
       acc[4] += f * y.x; acc[5] += f * y.y; acc[6] += f * y.z; acc[7] += f * y.w;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = lr == 0.f ? 0.f : 1.f / lr;
     const int q = r / a.group;
     const int64_t at = (tile.token + q) * a.num_q_heads + share.h * a.group + r - q * a.group;
     uint4 w;
@@ -519,7 +544,7 @@ __global__ void __launch_bounds__(256) join_pieces_kernel(const Args a) {
     w.y = pack_pair<F16>(acc[2] * inv, acc[3] * inv);
     w.z = pack_pair<F16>(acc[4] * inv, acc[5] * inv);
     w.w = pack_pair<F16>(acc[6] * inv, acc[7] * inv);
-    if (l == 0.f) w = make_uint4(0u, 0u, 0u, 0u);
+    if (lr == 0.f) w = make_uint4(0u, 0u, 0u, 0u);
     reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at * D)[c] = w;
     if (a.lse && c == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l) - p_bias<F16>()) * LN2F;
   }

@@ -183,7 +183,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     const float slope = a.slopes && valid ? a.slopes[head] * LOG2EF : 0.f;
     const float scale = scale_of<MODE>(a);
     const TanhPoly<MODE == BOUNDED ? 5 : 8> capped(a.cap_log2);
-    float m_ref = MODE == BOUNDED ? bounded_reference(a.cap_log2) : -INFINITY, l = 0.f;
+    float m_ref = MODE == BOUNDED ? bounded_reference(a.cap_log2) : -INFINITY, l = 0.f, lr = 0.f;
     bool ok = true;
     for (int j = 0; j < keys.n; ++j) {
       const int key0 = keys.at(j), b = j & 1;
@@ -197,7 +197,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       const uint32_t s_buf = s_addr + b * BN;
       if constexpr (MODE == BOUNDED) {
         // no maximum: 32 keys, with the next ones' scores on their way
-        f32x2 sum0 = join(0.f, 0.f), sum1 = sum0;
+        RowSum<F16> sum;
         uint32_t held[2][32];
         tmem_ld32(s_buf, held[0]);
 #pragma unroll
@@ -213,13 +213,11 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           for (int n = 0; n < 16; ++n) {
             const float e0 = fast_exp2(__uint_as_float(s[2 * n])), e1 = fast_exp2(__uint_as_float(s[2 * n + 1]));
             packed[n] = pack_pair<F16>(e0, e1);
-            if (n & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
+            sum.add(n, e0, e1, packed[n]);
           }
           tmem_st16(s_buf + c * 16, packed);
         }
-        float s0, s1;
-        split(add2(sum0, sum1), s0, s1);
-        l += s0 + s1;
+        sum.into(l, lr);
       } else {
         constexpr int CH = 2;
         uint32_t s[CH][32];
@@ -257,6 +255,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           alpha = fast_exp2(m_ref - tmax);
           m_ref = tmax;
           l *= alpha;
+          lr *= alpha;
         } else if (m_ref == -INFINITY) {
           m_ref = tmax;
         }
@@ -278,7 +277,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         }
         const float neg_m = m_ref == -INFINITY ? 0.f : p_bias<F16>() - m_ref;
         const f32x2 scale2 = join(scale, scale), neg2 = join(neg_m, neg_m);
-        f32x2 sum0 = join(0.f, 0.f), sum1 = sum0;
+        RowSum<F16> sum;
         auto exponentials = [&](auto argument) {
 #pragma unroll
           for (int c = 0; c < CH; ++c) {
@@ -290,7 +289,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
               e0 = fast_exp2(e0);
               e1 = fast_exp2(e1);
               packed[i] = pack_pair<F16>(e0, e1);
-              if (i & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
+              sum.add(i, e0, e1, packed[i]);
             }
             tmem_st16(s_buf + c * 16, packed);
           }
@@ -301,9 +300,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         } else {
           exponentials([&](f32x2 v) { return fma2(v, scale2, neg2); });
         }
-        float s0, s1;
-        split(add2(sum0, sum1), s0, s1);
-        l += s0 + s1;
+        sum.into(l, lr);
       }
       // V's rows behind the document's end (another document's, or anything) are cleared: their P is 0, but 0 * NaN
       // would not vanish
@@ -329,9 +326,10 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       if (valid) {
         record[128 * D + row] = m_ref;
         record[128 * D + 128 + row] = l;
+        record[128 * D + 256 + row] = lr;
       }
     } else if (ok) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = lr == 0.f ? 0.f : 1.f / lr;
       const int64_t at = (tile.token + qi) * a.num_q_heads + head;
       // through Q's shared memory (no product is in flight any more), a warp's own part of it
       constexpr int PIECES = D / 8;
@@ -346,7 +344,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          w[i] = l == 0.f ? 0u : pack_pair<F16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+          w[i] = lr == 0.f ? 0u : pack_pair<F16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
         stage_pieces<PIECES>(stage, c * 4, w);
       }
       __syncwarp();

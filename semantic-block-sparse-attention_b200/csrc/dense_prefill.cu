@@ -30,8 +30,8 @@ struct Cfg {
   static constexpr int KV_BYTES = BN * D * 2;
   static constexpr int K_OFF = 0;
   static constexpr int V_OFF = K_OFF + STAGES * KV_BYTES;
-  static constexpr int EPI_OFF = V_OFF + STAGES * KV_BYTES;   // float [2][128]
-  static constexpr int MX_OFF = EPI_OFF + 1024;               // float [2][2][128]: half-row maxima
+  static constexpr int EPI_OFF = V_OFF + STAGES * KV_BYTES;   // float [2][2][128]
+  static constexpr int MX_OFF = EPI_OFF + 2048;               // float [2][2][128]: half-row maxima
   static constexpr int BAR_OFF = MX_OFF + 2048;
   static constexpr int SLOT_OFF = BAR_OFF + 256;
   static constexpr int FIND_OFF = SLOT_OFF + 64;              // of the search among many documents
@@ -199,7 +199,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     }
     const float scale = scale_of<MODE>(a);
     const TanhPoly<MODE == BOUNDED ? 5 : 8> capped(a.cap_log2);
-    float m_ref = MODE == BOUNDED ? bounded_reference(a.cap_log2) : -INFINITY, l_part = 0.f;
+    float m_ref = MODE == BOUNDED ? bounded_reference(a.cap_log2) : -INFINITY, l_part = 0.f, lr_part = 0.f;
     bool ok = true;
     float* mx = reinterpret_cast<float*>(smem + C::MX_OFF);
     for (int j = 0; j < keys.n; ++j) {
@@ -222,16 +222,14 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           const bool all = __all_sync(0xffffffffu, (lo <= 0 && hi >= 32) || pre >= 32);
           bounded32(x, a, capped, all, seen_bits(lo, hi, pre), -m_ref);
           uint32_t packed[16];
-          f32x2 sum0 = join(0.f, 0.f), sum1 = sum0;
+          RowSum<F16> sum;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float e0 = fast_exp2(__uint_as_float(x[2 * i])), e1 = fast_exp2(__uint_as_float(x[2 * i + 1]));
             packed[i] = pack_pair<F16>(e0, e1);
-            if (i & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
+            sum.add(i, e0, e1, packed[i]);
           }
-          float s0, s1;
-          split(add2(sum0, sum1), s0, s1);
-          l_part += s0 + s1;
+          sum.into(l_part, lr_part);
           tmem_st16(s_addr, packed);
         }
       } else {
@@ -270,6 +268,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           alpha = fast_exp2(m_ref - tmax);
           m_ref = tmax;
           l_part *= alpha;
+          lr_part *= alpha;
         } else if (m_ref == -INFINITY) {
           m_ref = tmax;
         }
@@ -293,7 +292,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         if (active) {
           const float neg_m = m_ref == -INFINITY ? 0.f : p_bias<F16>() - m_ref;
           uint32_t packed[16];
-          f32x2 sum0 = join(0.f, 0.f), sum1 = sum0;
+          RowSum<F16> sum;
           auto exponentials = [&](auto argument) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -302,7 +301,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
               e0 = fast_exp2(e0);
               e1 = fast_exp2(e1);
               packed[i] = pack_pair<F16>(e0, e1);
-              if (i & 1) sum1 = add2(sum1, join(e0, e1)); else sum0 = add2(sum0, join(e0, e1));
+              sum.add(i, e0, e1, packed[i]);
             }
           };
           const f32x2 neg2 = join(neg_m, neg_m), scale2 = join(scale, scale);
@@ -312,9 +311,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           } else {
             exponentials([&](f32x2 v) { return fma2(v, scale2, neg2); });
           }
-          float s0, s1;
-          split(add2(sum0, sum1), s0, s1);
-          l_part += s0 + s1;
+          sum.into(l_part, lr_part);
           // P lies over this half's own logits; P V takes its 16-key slices from columns 0, 8, 32 and 40
           tmem_st16(s_addr, packed);
         }
@@ -335,10 +332,11 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     tc_fence_after();
     float* xchg = reinterpret_cast<float*>(smem + C::EPI_OFF);
     xchg[hf * 128 + row] = l_part;
+    xchg[256 + hf * 128 + row] = lr_part;
     mbar_arrive(bar(B_EPI));
     if (ok) ok = mbar_wait_warp(bar(B_EPI), 0, abort_flag, a.status, STATUS_TIMEOUT_EPILOGUE);
     if (ok && pieces > 1) {
-      const float l = l_part + xchg[(hf ^ 1) * 128 + row];
+      const float l = l_part + xchg[(hf ^ 1) * 128 + row], lr = lr_part + xchg[256 + (hf ^ 1) * 128 + row];
       float* record = share.record(a, D, share.split);
 #pragma unroll 1
       for (int c = 0; c < D / 64; ++c)
@@ -346,10 +344,11 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       if (valid && hf == 0) {
         record[128 * D + row] = m_ref;
         record[128 * D + 128 + row] = l;
+        record[128 * D + 256 + row] = lr;
       }
     } else if (ok) {
-      const float l = l_part + xchg[(hf ^ 1) * 128 + row];
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float l = l_part + xchg[(hf ^ 1) * 128 + row], lr = lr_part + xchg[256 + (hf ^ 1) * 128 + row];
+      const float inv = lr == 0.f ? 0.f : 1.f / lr;
       const int64_t at = (tile.token + qi) * a.num_q_heads + head;
       uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at * D + hf * (D / 2));
 #pragma unroll 1
@@ -363,7 +362,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            w[i] = l == 0.f ? 0u : pack_pair<F16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+            w[i] = lr == 0.f ? 0u : pack_pair<F16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
 #pragma unroll
           for (int i = 0; i < 4; ++i) dst[c * 4 + i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
         }
