@@ -215,6 +215,23 @@ def test_long_documents(dev, window, dim):
         _check(_call(q, k, v, lens, lens, sm_scale=0.1, **kw), want, 1500)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("softcap", [0.0, 20.0, 50.0, 80.0])
+def test_a_row_that_sees_one_key_gives_its_value(dev, dim, dtype, softcap):
+    # its weight is p / p with p a 16-bit number: p v is exact in 32 bits (22 bits at most), the reciprocal and the product
+    # are off by 2^-23 together, and the rounding to 16 bits returns v.  In fp16 p is the power of two that the reference
+    # stands for, and the sum as computed differs from it by the score's rounding, |s| 2^-23 < 2^-14 at most
+    lens = [1] * 40
+    q, k, v, _ = _inputs(dev, dim, lens, lens, 6, 2, dim, dtype, scale=6.0)
+    got = _call(q, k, v, lens, lens, sm_scale=dim ** -0.5, softcap=softcap)
+    assert torch.equal(got.output, v.repeat_interleave(3, 1))
+    long = [300]
+    q, k, v, _ = _inputs(dev, dim + 1, long, long, 6, 2, dim, dtype, scale=6.0)
+    got = _call(q, k, v, long, long, sm_scale=dim ** -0.5, softcap=softcap, window=1)
+    assert torch.equal(got.output, v.repeat_interleave(3, 1))
+
+
 def test_rising_scores_rescale(dev):
     """Scores that climb along the keys by far more than the range of a lazy rescale, and large caps."""
     lens = [640]
