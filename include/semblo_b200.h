@@ -356,8 +356,9 @@ int semblo_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stri
  * j < prefix_lens[b] (NULL: none).  softcap > 0: scores become softcap tanh(score / softcap); alibi_slopes
  * [Hq] fp32 (NULL: none): minus slope |p - j|.  lse [batch, queries, Hq] natural log, -inf for a row that
  * sees nothing (its output is 0), may be NULL.  The workspace needs no initialisation; its size is 0 where
- * every request's keys fit one block's share.  Status 201: a table entry outside the pool (its keys are
- * taken as absent) or a length beyond the table. */
+ * every request's keys fit one block's share.  q, cache, out and the workspace are 16-byte aligned; out does
+ * not overlap an input.  Status 201: a table entry outside the pool (its keys are taken as absent) or a
+ * length beyond the table. */
 int64_t semblo_kv8_decode_workspace_bytes(int batch, int queries, int num_q_heads, int num_kv_heads,
                                           int head_dim, int block_size, int table_len, int window,
                                           int has_prefix);
@@ -376,8 +377,9 @@ int semblo_kv8_decode(const void* q, int dtype, int batch, int queries, int num_
  * softcap tanh(score / softcap); alibi_slopes [Hq] fp32 (NULL: none): minus slope |p - j|.  lse [tokens_q,
  * Hq] natural log, may be NULL; a row that sees nothing: 0 and -inf.  zero_tail: rows behind the last
  * document become 0 and -inf, otherwise they are not written.  The workspace needs no initialisation; its size
- * is 0 unless there are few queries for the number of keys (their pieces are joined in it).  The reference
- * leaves dense requests to the engine's stock attention (semblo/vllm_plugin/model.py:1169-1269). */
+ * is 0 unless there are few queries for the number of keys (their pieces are joined in it).  q, k, v, out and the
+ * workspace are 16-byte aligned; out does not overlap an input.  The reference leaves dense requests to the
+ * engine's stock attention (semblo/vllm_plugin/model.py:1169-1269). */
 int64_t semblo_dense_prefill_workspace_bytes(int64_t tokens_q, int64_t tokens_k, int num_q_heads,
                                              int num_kv_heads, int head_dim, int documents, int causal,
                                              int window, int has_prefix);

@@ -327,7 +327,7 @@ __host__ __device__ inline float bounded_reference(float cap_log2) { return cap_
 template <int MODE>
 __device__ __forceinline__ void transform32(uint32_t* x, const Args& a, float slope, int p, int key0) {
   if constexpr (MODE == LINEAR) return;
-  if (MODE == CAPPED || MODE == BOUNDED || a.cap_log2 > 0.f) {
+  if (MODE == CAPPED || a.cap_log2 > 0.f) {
     const f32x2 arg2 = join(a.score_scale, a.score_scale);
     float most = 0.f;
 #pragma unroll

@@ -26,7 +26,7 @@ constexpr int PAGE = 16;
 
 template <int D>
 struct Cfg {
-  static constexpr int STAGES = D >= 256 ? 3 : 6;
+  static constexpr int STAGES = 3;
   static constexpr int KV_BYTES = BN * D * 2;
   static constexpr int K_OFF = 0;
   static constexpr int V_OFF = K_OFF + STAGES * KV_BYTES;
@@ -38,7 +38,7 @@ struct Cfg {
   static constexpr int TOTAL = FIND_OFF + FIND_BYTES;
   static constexpr int O_COL = 2 * BN;                        // S/P buffers, then O, then Q
   static constexpr int Q_COL = O_COL + D;
-  static constexpr int TMEM_COLS = Q_COL + D / 2 <= 256 ? 256 : 512;
+  static constexpr int TMEM_COLS = 512;
   static_assert(Q_COL + D / 2 <= 512, "tensor memory budget");
 };
 
