@@ -61,6 +61,8 @@ class SembloAttention(nn.Module):
         if attention_window and not serves_dense_only:
             raise RuntimeError("a local window is served in dense layers only (uses_sparse_attention=False with "
                                "dense_cache_bits=8)")
+        if uses_sparse_attention:
+            self._refuse_dense_requests_under_a_recorded_step(runtime_config)
         if int(runtime_config.index_dim) > int(self.head_dim):
             raise RuntimeError("the kernels route in a space of the head dimension: index_dim must not exceed "
                                "head_dim (the identity map, a loaded square map, or a map into fewer dimensions, "
@@ -384,6 +386,15 @@ class SembloAttention(nn.Module):
         return output.flatten(-2, -1)
 
     # ---- dense requests and layers -------------------------------------------------------
+    @staticmethod
+    def _refuse_dense_requests_under_a_recorded_step(cfg: SembloVllmConfig) -> None:
+        """The recorded decode step replays the arena's kernels, whatever the request is: one whose prompt went to the
+        8-bit cache would attend over an arena that never saw it."""
+        if cfg.dense_cache_bits and cfg.engage_above_tokens > 0 and _arena.full_graph_decode_enabled():
+            raise RuntimeError("SEMBLO_FULL_GRAPH_DECODE=1 records the sparse decode step, so that every request has to "
+                               "engage the index: dense_cache_bits=8 then needs engage_above_tokens=0 (got "
+                               f"{cfg.engage_above_tokens})")
+
     def _dense_attention(self, positions, q_post, k_post, v_states, output) -> None:
         """Exact attention: a prompt over its own K/V, a generated token over the layer's 8-bit cache, which both
         write.  A layer that shares another layer's K/V reads what that layer left."""
@@ -431,6 +442,7 @@ class SembloAttention(nn.Module):
                                                       engage_above_tokens=self.runtime_config.engage_above_tokens)
             self._dense_attention(positions, q_post, k_post, v_states, output)
             return
+        self._refuse_dense_requests_under_a_recorded_step(self.runtime_config)
         if _arena.full_graph_decode_enabled() and positions.numel() == 1:
             self._full_graph_decode_step(positions, q_post, k_post, v_states, q_pre, output, k_pre=k_pre)
             return
