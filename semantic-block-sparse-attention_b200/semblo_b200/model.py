@@ -87,6 +87,8 @@ class SembloAttention(nn.Module):
         self._decode_buffers_cache = None
         if not hasattr(self, "is_kv_shared_layer"):
             self.is_kv_shared_layer = False
+        if self.is_kv_shared_layer and runtime_config.dense_cache_bits:
+            runtime_state.register_dense_sharer(self.source_layer_idx, self.layer_idx)
         if self.builds_product_index:
             # the routing map of this layer's keys and of the queries of every layer that reads its index:
             # the identity until a map is loaded into ``semblo_key_router.weight``
@@ -422,12 +424,13 @@ class SembloAttention(nn.Module):
             if int(positions[0].item()) != 0:
                 raise RuntimeError("the full prompt of a dense request must arrive in one call")
             if self.is_kv_shared_layer:
-                if self.source_layer_idx not in state.dense_prompt_kv:
+                shared = state.shared_dense_prompt(self.source_layer_idx, self.layer_idx)
+                if shared is None:
                     raise RuntimeError(f"layer {self.layer_idx} shares the K/V of layer {self.source_layer_idx}, which "
                                        "has not seen this prompt")
-                k, v = state.dense_prompt_kv[self.source_layer_idx]
+                k, v = shared
             else:
-                state.dense_prompt_kv[self.source_layer_idx] = (k, v)
+                state.keep_dense_prompt(self.source_layer_idx, k, v)
             dense_prefill_attention(q, k, v, cu_seqlens_q=starts, sm_scale=self.scaling,
                                     softcap=self.attention_logits_soft_cap, window=self.attention_window, out=out)
         _lib.status_for(device).poll()

@@ -289,7 +289,8 @@ class SembloRuntimeState:
         self.step_suffix_key = None
         self.step_suffix_tiles = None
         self.step_recorded_key = None
-        self.dense_prompt_kv: dict = {}          # of the running prompt, by source layer (for layers that share it)
+        self.dense_prompt_kv: dict = {}          # of the running prompt, by source layer: K, V, the layers yet to read them
+        self.dense_sharers: dict = {}            # source layer -> the layers that read its K/V
 
     # ---- 8-bit cache of the dense requests and layers ------------------------------------------
     def dense_cache(self, layer_idx: int, *, num_kv_heads: int, head_dim: int, device):
@@ -303,6 +304,25 @@ class SembloRuntimeState:
             held = (signature, Kv8Cache.allocate(blocks, DENSE_BLOCK, num_kv_heads, head_dim, device), table)
             self.index_buffers[key] = held
         return held[1], held[2]
+
+    def register_dense_sharer(self, source_layer_idx: int, layer_idx: int) -> None:
+        self.dense_sharers.setdefault(int(source_layer_idx), set()).add(int(layer_idx))
+
+    def keep_dense_prompt(self, source_layer_idx: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """A prompt's 16-bit K/V, for as long as a layer that shares them has not run."""
+        readers = self.dense_sharers.get(int(source_layer_idx))
+        if readers:
+            self.dense_prompt_kv[int(source_layer_idx)] = (k, v, set(readers))
+
+    def shared_dense_prompt(self, source_layer_idx: int, layer_idx: int):
+        """(K, V) that the source layer left for ``layer_idx`` in this prompt, or None; the last reader drops them."""
+        held = self.dense_prompt_kv.get(int(source_layer_idx))
+        if held is None or int(layer_idx) not in held[2]:
+            return None
+        held[2].discard(int(layer_idx))
+        if not held[2]:
+            del self.dense_prompt_kv[int(source_layer_idx)]
+        return held[0], held[1]
 
     # ---- the layers' own store of generated K/V (state.py:1239-1284 of the reference) ----------
     def ensure_suffix_store(self, layer_idx, *, prompt_length, max_model_len, num_kv_heads, head_dim, dtype,
@@ -385,6 +405,9 @@ class SembloRuntimeState:
     def reset(self) -> None:
         self.dense_request = False
         self.source_indexes.clear()
+        # what an earlier request left; layers in front of the one that begins a prompt have already run for this one
+        for source in [s for s in self.dense_prompt_kv if self.reset_layer_idx is None or s >= int(self.reset_layer_idx)]:
+            del self.dense_prompt_kv[source]
         self.prompt_epoch += 1
 
     def maybe_begin_prompt(self, layer_idx: int, positions: torch.Tensor, engage_above_tokens: int = 0) -> None:

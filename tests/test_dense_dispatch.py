@@ -66,3 +66,64 @@ def test_the_variable_set_after_the_layer_was_made(monkeypatch):
         with pytest.raises(RuntimeError, match="engage_above_tokens"):
             layer.attention_forward(positions, None, q, None, None, None, None, q)
     assert taken == ["dense", "dense"]
+
+
+@pytest.fixture
+def operators(monkeypatch):
+    """The operators replaced: what each call was given, in order."""
+    from semblo_b200 import model
+    calls = []
+    monkeypatch.delenv("SEMBLO_FULL_GRAPH_DECODE", raising=False)
+    monkeypatch.setattr(model, "kv8_append", lambda cache, k, v, table, cu, start: calls.append(("append", k)))
+    monkeypatch.setattr(model, "dense_prefill_attention", lambda q, k, v, **kw: calls.append(("prompt", k)))
+    monkeypatch.setattr(model, "kv8_decode_attention", lambda q, cache, *a, **kw: calls.append(("decode", cache)))
+    monkeypatch.setattr(model._lib, "status_for", lambda device: SimpleNamespace(poll=lambda: None))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(model.SembloAttention, "_windows_ahead_enabled", lambda *a: True)
+    monkeypatch.setattr(model.SembloAttention, "_prompt_with_windows_ahead", lambda *a: calls.append(("sparse", None)))
+    return calls
+
+
+def _run(layer, positions):
+    n = positions.numel()
+    q = torch.zeros(n, HQ * DIM)
+    kv = None if layer.is_kv_shared_layer else torch.zeros(n, HKV * DIM)
+    layer.attention_forward(positions, None, q, kv, kv, None, None, q)
+
+
+def test_a_prompt_that_no_layer_shares_is_not_kept(operators):
+    state = _state()
+    dense, sparse = _layer(state, 0, sparse=False), _layer(state, 1)
+    for layer in (dense, sparse):
+        _run(layer, torch.arange(40))
+    assert [c[0] for c in operators] == ["append", "prompt"] * 2 and not state.dense_prompt_kv
+
+
+def test_a_shared_prompt_is_kept_until_its_last_reader(operators):
+    """Layer 0 runs before the layer that begins the prompt, layer 1 begins it."""
+    state = _state()
+    layers = [_layer(state, 0, sparse=False), _layer(state, 1), _layer(state, 2, source=0, sparse=False),
+              _layer(state, 3, source=1), _layer(state, 4, source=1)]
+    for _ in range(2):
+        held = []
+        for layer in layers:
+            _run(layer, torch.arange(40))
+            held.append(sorted(state.dense_prompt_kv))
+        assert held == [[0], [0, 1], [1], [1], []]
+        assert operators[4][1] is operators[1][1] and operators[5][1] is operators[3][1] and operators[6][1] is operators[3][1]
+        operators.clear()
+
+
+@pytest.mark.parametrize("sparse", [True, False])
+def test_a_shared_prompt_does_not_outlive_its_request(operators, sparse):
+    """A request that ends before the reader ran, then one whose source layer takes the sparse path."""
+    state = _state()
+    source, reader = _layer(state, 1), _layer(state, 2, source=1, sparse=sparse)
+    _run(source, torch.arange(40))
+    _run(source, torch.arange(200))
+    assert operators[-1][0] == "sparse" and not state.dense_prompt_kv
+    if not sparse:
+        operators.clear()
+        with pytest.raises(RuntimeError):
+            _run(reader, torch.arange(200))
+        assert not operators
