@@ -403,6 +403,9 @@ class SembloAttention(nn.Module):
         state = self.runtime_state
         device = q_post.device
         tokens = positions.numel()
+        if self.is_kv_shared_layer and not state.dense_request and self.source_layer_idx in state.source_modules:
+            raise RuntimeError(f"layer {self.layer_idx} shares the K/V of layer {self.source_layer_idx}, which serves this "
+                               "request on the sparse path: its 8-bit cache does not hold the request")
         q = q_post.view(tokens, self.num_heads, self.head_dim)
         out = output.view(tokens, self.num_heads, self.head_dim)
         cache, table = state.dense_cache(self.source_layer_idx, num_kv_heads=self.num_kv_heads, head_dim=self.head_dim,

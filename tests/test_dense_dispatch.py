@@ -127,3 +127,20 @@ def test_a_shared_prompt_does_not_outlive_its_request(operators, sparse):
         with pytest.raises(RuntimeError):
             _run(reader, torch.arange(200))
         assert not operators
+
+
+def test_a_dense_layer_does_not_read_what_its_sparse_source_did_not_write(operators):
+    """A request on the sparse path leaves nothing in its source layer's 8-bit cache: what is there is another's."""
+    state = _state()
+    source, reader = _layer(state, 1), _layer(state, 2, source=1, sparse=False)
+    for layer in (source, reader):                                             # a short request fills the cache
+        _run(layer, torch.arange(40))
+    for layer in (source, reader):
+        _run(layer, torch.tensor([40]))
+    assert [c[0] for c in operators] == ["append", "prompt", "prompt", "append", "decode", "decode"]
+    _run(source, torch.arange(200))
+    operators.clear()
+    for positions in (torch.arange(200), torch.tensor([200])):
+        with pytest.raises(RuntimeError, match="sparse path"):
+            _run(reader, positions)
+    assert not operators
