@@ -412,6 +412,8 @@ class SembloAttention(nn.Module):
                                          device=device)
         if not self.is_kv_shared_layer and (k_post is None or v_states is None):
             raise RuntimeError("physical layers must produce K/V")
+        if tokens > 1 and int(positions[0].item()) != 0:               # before anything is written
+            raise RuntimeError("the full prompt of a dense request must arrive in one call")
         first = positions[:1].to(torch.int32)
         starts = torch.arange(0, 2 * tokens, tokens, dtype=torch.int32, device=device)           # 0, tokens
         if not self.is_kv_shared_layer:
@@ -424,8 +426,6 @@ class SembloAttention(nn.Module):
                                  sm_scale=self.scaling, softcap=self.attention_logits_soft_cap,
                                  window=self.attention_window, out=out.view(1, 1, self.num_heads, self.head_dim))
         else:
-            if int(positions[0].item()) != 0:
-                raise RuntimeError("the full prompt of a dense request must arrive in one call")
             if self.is_kv_shared_layer:
                 shared = state.shared_dense_prompt(self.source_layer_idx, self.layer_idx)
                 if shared is None:

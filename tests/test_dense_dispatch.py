@@ -144,3 +144,17 @@ def test_a_dense_layer_does_not_read_what_its_sparse_source_did_not_write(operat
         with pytest.raises(RuntimeError, match="sparse path"):
             _run(reader, positions)
     assert not operators
+
+
+def test_a_refused_piece_of_a_prompt_writes_nothing(operators):
+    layer = _layer(_state(), 0, sparse=False)
+    with pytest.raises(RuntimeError, match="one call"):
+        _run(layer, torch.arange(8, 48))
+    assert not operators
+
+
+def test_a_reader_without_its_source_writes_nothing(operators):
+    layer = _layer(_state(), 2, source=1, sparse=False)
+    with pytest.raises(RuntimeError, match="has not seen"):
+        _run(layer, torch.arange(40))
+    assert not operators
