@@ -802,13 +802,20 @@ int64_t longest_segment(int queries, int window, int table_len, int block_size, 
   return ceil_div(keys, GROUP);
 }
 
+// Shared memory of the line's sums, and of the merge.
+constexpr int MAX_BATCH = 4096;
+template <int D, int NT> constexpr int sum_bytes(int batch) { return (batch + 2 + 2 * std::max(Cfg<D, NT>::WARPS, MERGE_WARPS)) * 4; }
+constexpr int merge_bytes(int blocks, int sums) { return MERGE_WARPS * 32 * 16 + (3 * MERGE_WARPS + 3 * blocks) * 8 * 4 + sums; }
+
 template <int D, int NT, bool CAP>
 int launch(DecodeArgs& a, const Plan& plan, cudaStream_t st) {
   using C = Cfg<D, NT>;
-  const int sums = (a.batch + 2 + 2 * std::max(C::WARPS, MERGE_WARPS)) * 4;
-  const int smem = C::SUM_OFF + sums;
+  const int sums = sum_bytes<D, NT>(a.batch);
   auto kern = kv8_decode_kernel<D, NT, CAP>;
-  SEMBLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // the limits are a kernel's, not a launch's: set to the same value by every call, since another thread may be between
+  // its own two lines
+  SEMBLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SUM_OFF + sum_bytes<D, NT>(MAX_BATCH)));
+  const int smem = C::SUM_OFF + sums;
   a.direct = plan.direct;
   kern<<<plan.blocks, C::THREADS, smem, st>>>(a);
   SEMBLO_LAUNCH_CHECK();
@@ -819,9 +826,9 @@ int launch(DecodeArgs& a, const Plan& plan, cudaStream_t st) {
   const int slices = std::max(1, std::min(C::KSTEPS, 8 * semblo::sm_count() / (segments * NT)));
   cfg.gridDim = dim3((unsigned)segments, (unsigned)slices, NT);
   cfg.blockDim = dim3(MERGE_THREADS);
-  cfg.dynamicSmemBytes = MERGE_WARPS * 32 * 16 + (3 * MERGE_WARPS + 3 * plan.blocks) * 8 * 4 + sums;
+  cfg.dynamicSmemBytes = merge_bytes(plan.blocks, sums);
   SEMBLO_CUDA(cudaFuncSetAttribute(kv8_merge_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   (int)cfg.dynamicSmemBytes));
+                                   merge_bytes(semblo::sm_count() * C::PER_SM, sum_bytes<D, NT>(MAX_BATCH))));
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -841,7 +848,7 @@ int check_shape(int batch, int queries, int num_q_heads, int num_kv_heads, int h
   SEMBLO_REQUIRE(block_size >= 16 && block_size <= 256 && (block_size & (block_size - 1)) == 0,
                  "block_size must be 16, 32, 64, 128 or 256 (got %d)", block_size);
   SEMBLO_REQUIRE(queries >= 1 && queries <= 16, "1 to 16 queries per request (got %d)", queries);
-  SEMBLO_REQUIRE(batch >= 0 && batch <= 4096, "at most 4096 requests (got %d)", batch);
+  SEMBLO_REQUIRE(batch >= 0 && batch <= MAX_BATCH, "at most %d requests (got %d)", MAX_BATCH, batch);
   SEMBLO_REQUIRE(table_len >= 0 && window >= 0, "negative table length or window");
   *rows = queries * (num_q_heads / num_kv_heads);
   // the widest tiles whose O stays in registers (the cache is read and widened once per tile), as narrow as

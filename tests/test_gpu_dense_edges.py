@@ -1,0 +1,66 @@
+"""The dense-request operators where their range ends: calls from two threads, scales that lie far apart, the ends of a
+16-bit type's exponent, caps far above the scores, the angle's last bits."""
+from __future__ import annotations
+
+import math
+import threading
+
+import pytest
+import torch
+
+import test_gpu_dense_prefill as prompt_ref
+import test_gpu_kv8_append as append_ref
+import test_gpu_kv8_decode as decode_ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    from semblo_b200 import _lib
+    _lib.lib()
+    return torch.device("cuda:0")
+
+
+# ---- calls from two threads
+
+def test_decode_of_two_batch_sizes_from_several_threads(dev):
+    """The launch's shared memory grows with the batch: one thread's small call must not take the limit away from
+    another's large one.  The C entry, which a thread is in without the interpreter's lock most of the time."""
+    from semblo_b200 import _lib
+    lib, status = _lib.lib(), _lib.status_for(dev).word
+    cache, table, gen = decode_ref._pool(dev, 1, [900, 40], 16, 1, 64, width=100)
+    jobs = []
+    for lens in ([900], [(i * 7) % 40 for i in range(4095)] + [900]):
+        n = len(lens)
+        q = torch.randn(n, 1, 2, 64, device=dev, generator=gen).to(torch.bfloat16)
+        rows = table[torch.tensor([1] * (n - 1) + [0], device=dev)].contiguous()
+        lengths = torch.tensor(lens, dtype=torch.int32, device=dev)
+        nbytes = lib.semblo_kv8_decode_workspace_bytes(n, 1, 2, 1, 64, 16, 100, 0, 0)
+        assert nbytes > 0
+        want = decode_ref._call(q, cache, rows, lens, sm_scale=0.125).output
+        for _ in range(3):
+            out, stream = torch.empty_like(q), torch.cuda.Stream()
+            room = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            args = (q.data_ptr(), 0, n, 1, 2, 1, 64, cache.data.data_ptr(), cache.scales.data_ptr(), cache.num_blocks, 16,
+                    rows.data_ptr(), 100, 100, lengths.data_ptr(), None, 0, 0.125, 0.0, None, out.data_ptr(), None,
+                    room.data_ptr(), nbytes, status.data_ptr(), stream.cuda_stream)
+            jobs.append((args, out, want, (q, rows, lengths, room, stream)))
+    torch.cuda.synchronize()
+    codes, start = [], threading.Barrier(len(jobs))
+
+    def loop(args):
+        start.wait()
+        codes.append([lib.semblo_kv8_decode(*args) for _ in range(1000)])
+
+    threads = [threading.Thread(target=loop, args=(job[0],)) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert len(codes) == len(jobs) and sum(c != 0 for run in codes for c in run) == 0
+    for _, out, want, _held in jobs:
+        assert torch.equal(out, want)
