@@ -319,7 +319,8 @@ constexpr int TOKEN_THREADS = 256, TOKEN_HEADS = 256;
 template <typename T2>
 __global__ void __launch_bounds__(TOKEN_THREADS) kv8_token_kernel(const AppendArgs a) {
   __shared__ uint32_t slots[TOKEN_THREADS / 32];
-  __shared__ float grown[TOKEN_HEADS];               // old / new scale of a head whose scale grew, else 0
+  __shared__ float grown[TOKEN_HEADS];               // old / new scale of a head whose scale grew (it may round to 0), else KEPT
+  constexpr float KEPT = 2.f;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = blockIdx.z;
   Cursor cursor{0, 0};
   const Unit u = a.batch <= WARP_REQUESTS ? find_unit(a, blockIdx.x, cursor) : find_unit_block(a, blockIdx.x, slots);
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS) kv8_token_kernel(const AppendAr
     if (!(largest <= 3.4e38f))
       largest = __uint_as_float(__reduce_max_sync(
           0xffffffffu, __float_as_uint(largest_finite_of<T2>(src, row_stride, pieces, a.col_log2, lane, 32))));
-    float scale = pow2(exponent_for(largest)), ratio = 0.f;
+    float scale = pow2(exponent_for(largest)), ratio = KEPT;
     if (u.off) {
       if (before >= scale) scale = before;
       else ratio = before / scale;
@@ -374,7 +375,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS) kv8_token_kernel(const AppendAr
   if (u.off == 0) return;
   __syncthreads();
   for (int h = 0; h < a.num_kv_heads; ++h)
-    if (grown[h] != 0.f)
+    if (grown[h] != KEPT)
       recode_rows(a.data + ((cell0 + h) << a.block_log2) * a.head_dim, u.off << (a.col_log2 - 1), grown[h], threadIdx.x,
                   TOKEN_THREADS);
 }

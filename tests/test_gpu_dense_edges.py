@@ -64,3 +64,26 @@ def test_decode_of_two_batch_sizes_from_several_threads(dev):
     assert len(codes) == len(jobs) and sum(c != 0 for run in codes for c in run) == 0
     for _, out, want, _held in jobs:
         assert torch.equal(out, want)
+
+
+# ---- the append's scales
+
+@pytest.mark.parametrize("stored", [2.0 ** -100, 0.0])
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [16, 1, 0, 30]])
+def test_a_scale_that_grows_beyond_what_a_ratio_holds(dev, stored, new):
+    """Rows stored near 2^-94, then tokens near 2^60: the ratio of the scales is 0 in 32 bits, and so are the earlier rows
+    under the new scale.  One token per request, and whole blocks; more heads than a block has warps."""
+    cache, k, v, table, cu, past = append_ref._case(dev, 21, 16, 12, 64, torch.bfloat16, new, [5, 15, 16, 7])
+    cache.scales.fill_(stored)
+    k, v = ((x.float() * 2.0 ** 60).to(torch.bfloat16) for x in (k, v))
+    append_ref._run_and_compare(cache, k, v, table, cu, past, 16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_special_values_in_single_tokens(dev, dtype):
+    """Infinities, NaN and zeros in calls of one token per request, in blocks that start and that are continued."""
+    cache, k, v, table, cu, past = append_ref._case(dev, 22, 32, 10, 128, dtype, [1] * 6, [0, 5, 31, 32, 64, 9])
+    k[0, 0, 3], k[1, 9, 0], v[2, 4, 127], v[3, 8, 64] = math.inf, -math.inf, math.nan, math.inf
+    k[4], v[5] = 0.0, math.inf                                      # nothing but zeros, nothing finite
+    v[1, 2] = math.nan
+    append_ref._run_and_compare(cache, k, v, table, cu, past, 32)
