@@ -11,7 +11,9 @@
 //     it will need itself reached 4.7 TB/s, in memory order 6.2.  The 16-byte pieces are permuted inside their
 //     128-byte lines so that the fragments are read back without bank conflicts;
 //   * e4m3 becomes fp16 by the hardware's pair conversion and is exact there, as is the query after a power
-//     of two per row is taken out, so the products S^T = K Q^T of m16n8k16 are exact up to the fp32 sums.
+//     of two per row is taken out (bf16 elements down to 2^-16 of the row's largest, fp16 ones down to 2^-13; fp16 ends at
+//     2^-24, so that a smaller one is off by 2^-24 of the largest at most, a 32-bit sum's own rounding).  The products
+//     S^T = K Q^T of m16n8k16 are exact up to that and the fp32 sums.
 //     The order of the 16 values inside a k-step is free as long as K and Q agree: a lane's 16 consecutive
 //     bytes are its elements of four k-steps.  The same freedom over the rows of O^T = V^T P^T turns 16
 //     consecutive bytes of four keys into eight A fragments with two byte permutes per four values;
@@ -391,7 +393,7 @@ __global__ void __launch_bounds__((Cfg<D, NT>::THREADS), (Cfg<D, NT>::PER_SM)) k
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       int e = (int)(__float_as_uint(top) >> 23) - 126;          // top < 2^e
       if (e == 129 || top == 0.f) e = 0;                        // infinities pass as they are
-      e = max(e, -100);
+      e = min(max(e, -120), 126);                               // 2^e and 2^-e are normal numbers, as is sm_scale 2^e
       const float down = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
       for (int s = 0; s < C::KSTEPS; ++s) {

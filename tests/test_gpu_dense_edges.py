@@ -87,3 +87,26 @@ def test_special_values_in_single_tokens(dev, dtype):
     k[4], v[5] = 0.0, math.inf                                      # nothing but zeros, nothing finite
     v[1, 2] = math.nan
     append_ref._run_and_compare(cache, k, v, table, cu, past, 32)
+
+
+# ---- queries at the ends of bf16
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("exponent", [125, 124, -113, -118, -122])
+@pytest.mark.parametrize("softcap", [0.0, 5.0])
+def test_queries_of_every_exponent(dev, dim, exponent, softcap):
+    """Queries up to 2^128 and down to 2^-125 over K scales that bring the scores back to a few units."""
+    lens = [200, 33, 1]
+    cache, table, gen = decode_ref._pool(dev, 41 + dim, lens, 32, 2, dim)
+    if exponent > 0:                                                # codes of a few units: scales below 2^-126 are not needed
+        cache.data.copy_((cache.data.float() / 32).to(torch.float8_e4m3fn))
+        cache.scales[0] = 2.0 ** (-exponent - 1)
+    else:
+        cache.scales[0] = 2.0 ** (-exponent - 6)
+    q = torch.randn(3, 1, 8, dim, device=dev, generator=gen).clamp(-3.9, 3.9)
+    q = (q.double() * 2.0 ** exponent).to(torch.bfloat16)
+    q[0, 0, 0, 0], q[1, 0, 3, 5] = 3.9 * 2.0 ** exponent, -3.0 * 2.0 ** exponent
+    assert bool(q.isfinite().all()) and float(q.double().abs().max()) > 1.9 * 2.0 ** (exponent + 1)
+    kw = dict(sm_scale=dim ** -0.5, softcap=softcap)
+    want = decode_ref._formula(q, cache, table, lens, kw["sm_scale"], softcap, 0, None, None)
+    decode_ref._check(decode_ref._call(q, cache, table, lens, **kw), want, 200)
