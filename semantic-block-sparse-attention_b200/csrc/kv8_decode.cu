@@ -481,15 +481,25 @@ __global__ void __launch_bounds__((Cfg<D, NT>::THREADS), (Cfg<D, NT>::PER_SM)) k
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float x = s[nt][c] * (ks * coef[nt][c & 1]);
-          if constexpr (CAP) {
-            // tanh(x) = 1 - 2 / (1 + e^2x): exact at both ends, absolute error a few 2^-24
-            const float ex = sm100::fast_exp2(x * (2.f * LOG2E));
-            x = a.softcap * LOG2E * (1.f - __fdividef(2.f, 1.f + ex));
-          }
-          s[nt][c] = x;
+        for (int c = 0; c < 4; ++c) s[nt][c] *= ks * coef[nt][c & 1];
+      if constexpr (CAP) {
+        // a value's form depends on the value alone; the vote leaves out the second one where no value takes it
+        float most = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) most = fmaxf(most, sm100::fmax3(fmaxf(fabsf(s[nt][0]), fabsf(s[nt][1])), fabsf(s[nt][2]), fabsf(s[nt][3])));
+        const float cap = a.softcap * LOG2E;
+        if (__all_sync(0xffffffffu, most < sm100::TANH_NEAR)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[nt][c] = cap * sm100::tanh_near(s[nt][c]);
+        } else {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[nt][c] = cap * sm100::tanh_any(s[nt][c]);
         }
+      }
       const bool all_seen = key0 + GROUP - 1 <= sp.first &&
                             (a.window == 0 || key0 >= sp.first + a.queries - a.window || key0 + GROUP <= sp.prefix) &&
                             key0 + GROUP <= sp.length;

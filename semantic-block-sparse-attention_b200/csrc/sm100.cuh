@@ -295,6 +295,22 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
+// tanh by its odd polynomial for |x| < 3/4 and by 1 - 2 / (1 + e^2x) above: relative errors of 1.1e-7 (own fit of the smallest
+// largest relative error, as evaluated in 32 bits) and of a few 2^-23.  Near 0 the second form keeps its absolute error.
+constexpr float TANH_NEAR = 0.75f;
+__device__ __forceinline__ float tanh_near(float x) {
+  const float u = x * x;
+  float r = fmaf(u, -0.00476949057f, 0.0196649134f);
+  r = fmaf(r, u, -0.0533902571f);
+  r = fmaf(r, u, 0.133265212f);
+  r = fmaf(r, u, -0.333330691f);
+  return fmaf(x * u, r, x);
+}
+__device__ __forceinline__ float tanh_any(float x) {
+  const float far = 1.f - __fdividef(2.f, 1.f + fast_exp2(x * 2.8853900817779268f));      // 2 log2 e
+  return fabsf(x) < TANH_NEAR ? tanh_near(x) : far;
+}
+
 // Byte offset of element (row, 16-byte chunk) inside a [rows][128 B] tile stored with
 // the 128-byte swizzle (what TMA writes and UMMA reads): chunk ^= row % 8.
 __device__ __forceinline__ uint32_t swz128(uint32_t row, uint32_t chunk) {

@@ -110,3 +110,35 @@ def test_queries_of_every_exponent(dev, dim, exponent, softcap):
     kw = dict(sm_scale=dim ** -0.5, softcap=softcap)
     want = decode_ref._formula(q, cache, table, lens, kw["sm_scale"], softcap, 0, None, None)
     decode_ref._check(decode_ref._call(q, cache, table, lens, **kw), want, 200)
+
+
+# ---- caps far above the scores
+
+def _uncapped(want, cap, scores=40.0):
+    """What is allowed where |score| stays below ``scores``: cap tanh(s / cap) is s but for s^3 / (3 cap^2), and its error
+    is relative to the score (2^-17), not to the cap."""
+    out, lse, mag, off = want
+    assert scores < cap
+    return out, lse, mag, off + scores ** 3 / (3 * cap * cap) + scores * 2.0 ** -17
+
+
+@pytest.mark.parametrize("cap", [3.0e3, 1.0e5, 1.0e7, 1.0e30])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_decode_under_a_cap_far_above_its_scores(dev, dim, cap):
+    lens = [700, 45]
+    cache, table, gen = decode_ref._pool(dev, 51 + dim, lens, 64, 2, dim)
+    q = torch.randn(2, 2, 8, dim, device=dev, generator=gen).to(torch.bfloat16)
+    want = decode_ref._formula(q, cache, table, lens, dim ** -0.5, 0.0, 0, None, None)
+    decode_ref._check(decode_ref._call(q, cache, table, lens, sm_scale=dim ** -0.5, softcap=cap), _uncapped(want, cap), 700)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_decode_of_a_capped_head_beside_heads_far_below_the_cap(dev, dim):
+    """One head's scores reach the cap; the others' are as accurate as without that head."""
+    cap, sm, lens = 1.0e6, dim ** -0.5, [300]
+    cache, table, gen = decode_ref._pool(dev, 61 + dim, lens, 64, 1, dim)
+    q = torch.randn(1, 1, 8, dim, device=dev, generator=gen).to(torch.bfloat16)
+    want = decode_ref._formula(q[:, :, 1:], cache, table, lens, sm, 0.0, 0, None, None)
+    q[:, :, 0] *= 2.0 ** 21
+    got = decode_ref._call(q, cache, table, lens, sm_scale=sm, softcap=cap)
+    decode_ref._check(type(got)(got.output[:, :, 1:], got.logsumexp[:, :, 1:]), _uncapped(want, cap), 300)
