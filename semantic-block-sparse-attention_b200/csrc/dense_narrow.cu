@@ -182,6 +182,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     const int head = h * a.group + hg;
     const float slope = a.slopes && valid ? a.slopes[head] * LOG2EF : 0.f;
     const float scale = scale_of<MODE>(a);
+    const Vote vote(valid);
     const TanhPoly<MODE == BOUNDED ? 5 : 8> capped(a.cap_log2);
     float m_ref = MODE == BOUNDED ? bounded_reference(a.cap_log2) : -INFINITY, l = 0.f, lr = 0.f;
     bool ok = true;
@@ -207,7 +208,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           if (c == 0) tmem_ld32(s_buf + 32, held[1]);
           const int lo = seen.lo - key0 - 32 * c, hi = seen.hi - key0 - 32 * c, pre = seen.pre - key0 - 32 * c;
           const bool all = __all_sync(0xffffffffu, (lo <= 0 && hi >= 32) || pre >= 32);
-          bounded32(s, a, capped, all, seen_bits(lo, hi, pre), -m_ref);
+          bounded32(s, a, capped, all, seen_bits(lo, hi, pre), -m_ref, vote);
           uint32_t packed[16];
 #pragma unroll
           for (int n = 0; n < 16; ++n) {
@@ -233,17 +234,16 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           for (int c = 0; c < CH; ++c) range32<MODE == CAPPED>(s[c], tmax, least);
         }
         if constexpr (MODE == CAPPED) {
-          poly = all && __all_sync(0xffffffffu, fmaxf(tmax, -least) * a.score_scale < TANH_FAR);
+          poly = all && __all_sync(0xffffffffu, fmaxf(tmax, -least) * a.score_scale < vote.far);
           if (poly) tmax = tanh_exp(tmax * (a.score_scale * (1.f / TANH_ARG)));
         }
         if (MODE == BIASED || (MODE == CAPPED && !poly) || (MODE == LINEAR && !all)) {
           tmax = -INFINITY;
 #pragma unroll
           for (int c = 0; c < CH; ++c) {
-            transform32<MODE>(s[c], a, slope, p, key0 + 32 * c);
-            if (!all) {
-              hide32(s[c], seen_bits(lo - 32 * c, hi - 32 * c, pre - 32 * c));
-            }
+            const uint32_t bits = seen_bits(lo - 32 * c, hi - 32 * c, pre - 32 * c);
+            transform32<MODE>(s[c], a, slope, p, key0 + 32 * c, all, bits, vote);
+            if (!all) hide32(s[c], bits);
             range32<false>(s[c], tmax, least);
           }
         }

@@ -198,6 +198,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       mbar_arrive(bar(B_QFULL));
     }
     const float scale = scale_of<MODE>(a);
+    const Vote vote(valid);
     const TanhPoly<MODE == BOUNDED ? 5 : 8> capped(a.cap_log2);
     float m_ref = MODE == BOUNDED ? bounded_reference(a.cap_log2) : -INFINITY, l_part = 0.f, lr_part = 0.f;
     bool ok = true;
@@ -220,7 +221,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           tmem_ld_wait();
           const int lo = seen.lo - key0, hi = seen.hi - key0, pre = seen.pre - key0;
           const bool all = __all_sync(0xffffffffu, (lo <= 0 && hi >= 32) || pre >= 32);
-          bounded32(x, a, capped, all, seen_bits(lo, hi, pre), -m_ref);
+          bounded32(x, a, capped, all, seen_bits(lo, hi, pre), -m_ref, vote);
           uint32_t packed[16];
           RowSum<F16> sum;
 #pragma unroll
@@ -242,14 +243,13 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           const bool all = __all_sync(0xffffffffu, (lo <= 0 && hi >= 32) || pre >= 32);
           if constexpr (MODE == CAPPED) {
             range32<true>(x, hm, least);
-            poly = all && __all_sync(0xffffffffu, fmaxf(hm, -least) * a.score_scale < TANH_FAR);
+            poly = all && __all_sync(0xffffffffu, fmaxf(hm, -least) * a.score_scale < vote.far);
             if (poly) hm = tanh_exp(hm * (a.score_scale * (1.f / TANH_ARG)));
           }
           if (!poly) {
-            transform32<MODE>(x, a, slope, p, key0);
-            if (!all) {
-              hide32(x, seen_bits(lo, hi, pre));
-            }
+            const uint32_t bits = seen_bits(lo, hi, pre);
+            transform32<MODE>(x, a, slope, p, key0, all, bits, vote);
+            if (!all) hide32(x, bits);
             hm = -INFINITY;
             range32<false>(x, hm, least);
           }

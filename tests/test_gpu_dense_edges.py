@@ -142,3 +142,27 @@ def test_decode_of_a_capped_head_beside_heads_far_below_the_cap(dev, dim):
     q[:, :, 0] *= 2.0 ** 21
     got = decode_ref._call(q, cache, table, lens, sm_scale=sm, softcap=cap)
     decode_ref._check(type(got)(got.output[:, :, 1:], got.logsumexp[:, :, 1:]), _uncapped(want, cap), 300)
+
+
+# ---- what decides a tanh's form
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("dtype,softcap,biased", [(torch.bfloat16, 20.0, False), (torch.float16, 20.0, False),
+                                                  (torch.bfloat16, 80.0, False), (torch.bfloat16, 20.0, True)])
+def test_a_document_keeps_its_bits_whatever_is_beside_it(dev, dim, dtype, softcap, biased):
+    """The rows and keys that share a document's tiles without being its own: the next document's, of any size, NaN, none
+    at all, and what an earlier launch left."""
+    heads, lens = 6, [50, 75]
+    q, k, v, gen = prompt_ref._inputs(dev, 81 + dim, lens, lens, heads, 2, dim, dtype, scale=6.0)
+    slopes = torch.rand(heads, device=dev, generator=gen) if biased else None
+    kw = dict(sm_scale=dim ** -0.5, softcap=softcap, slopes=slopes)
+    alone = [prompt_ref._call(q[:50], k[:50], v[:50], [50], [50], **kw)]
+    for factor in (0.0, 1.0, 2.0 ** 9, math.nan):
+        q2, k2 = q.clone(), k.clone()
+        q2[50:], k2[50:] = q[50:] * factor, k[50:] * factor
+        # a launch whose scores are far from these ones, for the tensor memory that it leaves behind
+        prompt_ref._call(torch.full_like(q, 200.0), torch.full_like(k, 200.0), v, lens, lens, sm_scale=1.0)
+        got = prompt_ref._call(q2, k2, v, lens, lens, **kw)
+        alone.append(type(got)(got.output[:50], got.logsumexp[:50]))
+    for got in alone[1:]:
+        assert torch.equal(got.logsumexp, alone[0].logsumexp) and torch.equal(got.output, alone[0].output)
