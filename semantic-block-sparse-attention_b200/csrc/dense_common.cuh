@@ -275,14 +275,15 @@ __device__ __forceinline__ float fmin3(float a, float b, float c) {
   return d;
 }
 
-// tanh(x) = 1 - 2 / (1 + e^2x): exact at both ends, absolute error a few 2^-24; two special-function operations.
+// tanh(x) = 1 - 2 / (1 + e^2x): exact at both ends, absolute error a few 2^-24; two special-function operations.  For caps up
+// to 52 that is enough; under higher ones tanh_any keeps small scores relative beside a row that reaches the cap.
 __device__ __forceinline__ float tanh_exp(float x) {
   return 1.f - __fdividef(2.f, 1.f + fast_exp2(x * (2.f * LOG2EF)));
 }
 
 // tanh(3/8 y) as y P(y^2) on the multiply-add pipe (the exponentials of the softmax fill the special-function
 // unit), P fitted for the smallest largest error: of degree 4 for |y| < 2 (2.5e-7 as evaluated in 32 bits), of
-// degree 7 for |y| < 4 (5e-7).  Scores beyond 1.5 caps are rare and take tanh_exp.
+// degree 7 for |y| < 4 (5e-7; near 0 relative to y, 4e-6).  Scores beyond 1.5 caps are rare and take an exponential.
 constexpr float TANH_ARG = 8.f / 3.f, TANH_FAR = 4.f;
 __device__ __forceinline__ constexpr float near_coefficient(int i) {
   const float c[5] = {0.374998957f, -0.0175727159f, 0.000980816782f, -5.13917694e-05f, 1.80655456e-06f};
@@ -368,7 +369,7 @@ __device__ __forceinline__ void transform32(uint32_t* x, const Args& a, float sl
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(tanh_exp(__uint_as_float(x[i]) * (1.f / TANH_ARG)));
+      for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(tanh_any(__uint_as_float(x[i]) * (1.f / TANH_ARG)));
     }
   }
   if constexpr (MODE == BIASED) {

@@ -235,7 +235,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         }
         if constexpr (MODE == CAPPED) {
           poly = all && __all_sync(0xffffffffu, fmaxf(tmax, -least) * a.score_scale < vote.far);
-          if (poly) tmax = tanh_exp(tmax * (a.score_scale * (1.f / TANH_ARG)));
+          if (poly) tmax = tanh_any(tmax * (a.score_scale * (1.f / TANH_ARG)));
         }
         if (MODE == BIASED || (MODE == CAPPED && !poly) || (MODE == LINEAR && !all)) {
           tmax = -INFINITY;

@@ -244,7 +244,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           if constexpr (MODE == CAPPED) {
             range32<true>(x, hm, least);
             poly = all && __all_sync(0xffffffffu, fmaxf(hm, -least) * a.score_scale < vote.far);
-            if (poly) hm = tanh_exp(hm * (a.score_scale * (1.f / TANH_ARG)));
+            if (poly) hm = tanh_any(hm * (a.score_scale * (1.f / TANH_ARG)));
           }
           if (!poly) {
             const uint32_t bits = seen_bits(lo, hi, pre);

@@ -166,3 +166,31 @@ def test_a_document_keeps_its_bits_whatever_is_beside_it(dev, dim, dtype, softca
         alone.append(type(got)(got.output[:50], got.logsumexp[:50]))
     for got in alone[1:]:
         assert torch.equal(got.logsumexp, alone[0].logsumexp) and torch.equal(got.output, alone[0].output)
+
+
+# ---- caps far above a prompt's scores
+
+@pytest.mark.parametrize("cap", [3.0e3, 1.0e5, 1.0e7, 1.0e30])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("biased", [False, True])
+def test_prompt_under_a_cap_far_above_its_scores(dev, dim, cap, biased):
+    lens = [200, 45]
+    q, k, v, gen = prompt_ref._inputs(dev, 51 + dim, lens, lens, 4, 2, dim, torch.bfloat16, scale=1.0)
+    kw = dict(sm_scale=dim ** -0.5, slopes=torch.rand(4, device=dev, generator=gen) if biased else None)
+    want = prompt_ref._formula(q, k, v, lens, lens, **kw)
+    prompt_ref._check(prompt_ref._call(q, k, v, lens, lens, softcap=cap, **kw), _uncapped(want, cap), 200)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_prompt_of_a_capped_head_beside_heads_far_below_the_cap(dev, dim, dtype):
+    cap, lens = 1.0e6, [300]
+    q, k, v, _ = prompt_ref._inputs(dev, 61 + dim, lens, lens, 8, 1, dim, dtype, scale=1.0)
+    kw = dict(sm_scale=dim ** -0.5)
+    if dtype == torch.float16:                                      # its largest value holds the scores back: a smaller query
+        q *= 2.0 ** -10
+        kw = dict(sm_scale=dim ** -0.5 * 2.0 ** 10)
+    want = prompt_ref._formula(q[:, 1:], k, v, lens, lens, **kw)
+    q[:, 0] *= 2.0 ** 21
+    got = prompt_ref._call(q, k, v, lens, lens, softcap=cap, **kw)
+    prompt_ref._check(type(got)(got.output[:, 1:], got.logsumexp[:, 1:]), _uncapped(want, cap), 300)
