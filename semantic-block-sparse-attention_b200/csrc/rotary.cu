@@ -7,7 +7,8 @@
 // with (x1, x2) = (x_i, x_{i + R/2}) in the half layout and (x_2i, x_2i+1) in the interleaved one;
 // dimensions from R on are copied.  Frequencies are doubles and the angle is reduced to a fraction of a
 // turn in double: at position 1e6 and f = 1 a float product is off by up to 0.03 radians, which no later step
-// can repair.  sincospi of the reduced fraction is then as accurate as a float can be.
+// can repair.  sincospi takes the fraction rounded to a float (off by up to 2^-25 of a half turn, 1e-7 radians); the rest of
+// it turns the result once more, to first order (its square is below 2^-46).
 //
 // Bound: HBM, one read and one write of every element.  A cos/sin costs ~50 instructions and serves all
 // heads of a token, so a block walks over tiles of whole tokens and keeps two of everything: while a thread
@@ -149,8 +150,11 @@ __global__ void __launch_bounds__(THREADS, NP * sizeof(T) > 16 ? 2 : 3) rotary_k
                                  : (double)static_cast<const int32_t*>(a.positions)[token0 + t];
       double turns = pos * a.inv_freq[p] * 0.15915494309189535;      // 1 / (2 pi)
       turns -= rint(turns);
-      float sn, cs;
-      sincospif((float)(2.0 * turns), &sn, &cs);
+      const double half_turns = 2.0 * turns;
+      const float whole = (float)half_turns, rest = (float)((half_turns - whole) * 3.14159265358979324);
+      float s0, c0;
+      sincospif(whole, &s0, &c0);
+      const float cs = fmaf(-s0, rest, c0), sn = fmaf(c0, rest, s0);
       buf[t * pairs + (p % NP) * a.rot_cols + p / NP] = make_float2(cs * a.scale, sn * a.scale * a.sin_sign);
     }
   };

@@ -194,3 +194,28 @@ def test_prompt_of_a_capped_head_beside_heads_far_below_the_cap(dev, dim, dtype)
     q[:, 0] *= 2.0 ** 21
     got = prompt_ref._call(q, k, v, lens, lens, softcap=cap, **kw)
     prompt_ref._check(type(got)(got.output[:, 1:], got.logsumexp[:, 1:]), _uncapped(want, cap), 300)
+
+
+# ---- the rotation's angle
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,rotary", [(128, 128), (66, 34)])
+def test_cos_and_sin_to_their_last_bits(dev, interleaved, dim, rotary):
+    """Rows (1, 0): the rotated pair is (cos, sin) itself.  The angle is reduced in 64 bits (three roundings of 2^-53 of its
+    turns); cos and sin of a turn's fraction, 1 ulp of the result each, and one rounding of their correction: 2^-22 of the
+    value, nothing relative to 1."""
+    from semblo_b200.rotary import apply_rotary, rotary_frequencies
+    tokens = 4096
+    x = torch.zeros(tokens, 1, dim, device=dev)
+    first = slice(0, rotary, 2) if interleaved else slice(0, rotary // 2)
+    second = slice(1, rotary, 2) if interleaved else slice(rotary // 2, rotary)
+    x[..., first] = 1.0
+    pos = torch.arange(tokens, device=dev) * 251 + 5
+    freq = rotary_frequencies(rotary, 500000.0, device=dev)
+    y, _ = apply_rotary(x, None, pos, freq, interleaved=interleaved)
+    angle = pos.double()[:, None] * freq.inv_freq
+    slack = angle * 2.0 ** -51 + 2.0 ** -44                         # the angle in 64 bits, here and there; second order
+    for part, want in ((first, angle.cos()), (second, angle.sin())):
+        err = (y[:, 0, part].double() - want).abs()
+        bound = want.abs() * 2.0 ** -22 + slack
+        assert bool((err <= bound).all()), float((err / bound).max())
