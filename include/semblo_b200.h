@@ -376,7 +376,7 @@ int semblo_kv8_decode(const void* q, int dtype, int batch, int queries, int num_
  * j < prefix_lens[d] (NULL: none); causal = 0: every key of its document.  softcap > 0: scores become
  * softcap tanh(score / softcap); alibi_slopes [Hq] fp32 (NULL: none): minus slope |p - j|.  lse [tokens_q,
  * Hq] natural log, may be NULL; a row that sees nothing: 0 and -inf.  zero_tail: rows behind the last
- * document become 0 and -inf, otherwise they are not written.  The workspace needs no initialisation; its size
+ * document and in front of the first become 0 and -inf, otherwise they are not written.  The workspace needs no initialisation; its size
  * is 0 unless there are few queries for the number of keys (their pieces are joined in it).  q, k, v, out and the
  * workspace are 16-byte aligned; out does not overlap an input.  The reference leaves dense requests to the
  * engine's stock attention (semblo/vllm_plugin/model.py:1169-1269). */

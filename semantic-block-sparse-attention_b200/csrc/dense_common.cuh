@@ -25,7 +25,7 @@ struct Args {
   int queries_per_tile, num_kv_heads;
   int64_t tokens_q, tokens_k;
   int causal, window;
-  int zero_tail;                  // write zeros to the rows behind the last document
+  int zero_tail;                  // write zeros to the rows that no document has
   float score_scale;              // raw product -> log2 units, or -> 8/3 of the capping tanh's argument
   float cap_log2;                 // cap * log2(e)
   int* status;
@@ -178,16 +178,18 @@ __device__ __forceinline__ Tile find_tile_block(const Args& a, int want, void* s
   return found;
 }
 
-// Rows behind the last document, as zeros with a log-sum-exp of -inf: the spare blocks share them by tiles.
+// Rows that no document has, those behind the last one and then those in front of the first, as zeros with a log-sum-exp
+// of -inf: the spare blocks share them by tiles (there are enough: a grid of T / qt + docs tiles has at least the rest's).
 template <int D>
-__device__ __forceinline__ void zero_tail(const Args& a, int nth, int kv_head, int threads) {
-  const int64_t last = min(max((int64_t)a.cu_q[a.docs], (int64_t)0), a.tokens_q);
-  const int64_t t0 = last + (int64_t)nth * a.queries_per_tile;
-  const int64_t t1 = min(a.tokens_q, t0 + a.queries_per_tile);
+__device__ __forceinline__ void zero_rest(const Args& a, int nth, int kv_head, int threads) {
+  const int64_t front = min(max((int64_t)a.cu_q[0], (int64_t)0), a.tokens_q);
+  const int64_t last = min(max((int64_t)a.cu_q[a.docs], front), a.tokens_q);
+  const int64_t behind = a.tokens_q - last;
+  const int64_t r0 = (int64_t)nth * a.queries_per_tile, r1 = min(behind + front, r0 + a.queries_per_tile);
   constexpr int CH = D / 8;
-  for (int64_t i = threadIdx.x; i < (t1 - t0) * a.group * CH; i += threads) {
-    const int64_t row = i / CH;
-    const int64_t at = (t0 + row / a.group) * a.num_q_heads + kv_head * a.group + row % a.group;
+  for (int64_t i = threadIdx.x; i < (r1 - r0) * a.group * CH; i += threads) {
+    const int64_t row = i / CH, r = r0 + row / a.group;
+    const int64_t at = (r < behind ? last + r : r - behind) * a.num_q_heads + kv_head * a.group + row % a.group;
     reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at * D)[i % CH] = make_uint4(0u, 0u, 0u, 0u);
     if (a.lse && i % CH == 0) a.lse[at] = -INFINITY;
   }

@@ -86,7 +86,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   // the same answer in every warp
   const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, share.want) : find_tile_block<C::THREADS>(a, share.want, smem + C::FIND_OFF);
   if (tile.doc < 0) {
-    if (a.zero_tail && share.split == 0) zero_tail<D>(a, tile.first, h, blockDim.x);
+    if (a.zero_tail && share.split == 0) zero_rest<D>(a, tile.first, h, blockDim.x);
     return;
   }
   KeyTiles<BN> keys(a, tile);

@@ -62,7 +62,7 @@ dense_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   }
   const Tile tile = a.docs <= WARP_DOCS ? find_tile(a, share.want) : find_tile_block<320>(a, share.want, smem + C::FIND_OFF);
   if (tile.doc < 0) {
-    if (a.zero_tail && share.split == 0) zero_tail<D>(a, tile.first, h, blockDim.x);
+    if (a.zero_tail && share.split == 0) zero_rest<D>(a, tile.first, h, blockDim.x);
     return;
   }
   KeyTiles<BN> keys(a, tile);

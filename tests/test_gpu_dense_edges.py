@@ -219,3 +219,28 @@ def test_cos_and_sin_to_their_last_bits(dev, interleaved, dim, rotary):
         err = (y[:, 0, part].double() - want).abs()
         bound = want.abs() * 2.0 ** -22 + slack
         assert bool((err <= bound).all()), float((err / bound).max())
+
+
+# ---- rows that no document has
+
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("front,tail", [(7, 0), (300, 41), (63, 65)])
+def test_rows_in_front_of_the_first_document(dev, dim, front, tail):
+    """As behind the last one: 0 and -inf in a fresh result, untouched in a given one."""
+    from semblo_b200.dense_prefill import dense_prefill_attention
+    lens = [20, 75]
+    q, k, v, _ = prompt_ref._inputs(dev, 71, [front] + lens + [tail], [front] + lens + [tail], 4, 2, dim, torch.bfloat16)
+    cu = torch.tensor([front, front + 20, front + 95], dtype=torch.int32, device=dev)
+    inside = slice(front, front + 95)
+    want = prompt_ref._formula(q[inside], k[inside], v[inside], lens, lens, sm_scale=0.1)
+    junk = torch.full((1 << 22,), 3.0, device=dev)                  # freed: what a fresh buffer would show
+    del junk
+    got = dense_prefill_attention(q, k, v, cu_seqlens_q=cu, sm_scale=0.1, return_logsumexp=True)
+    prompt_ref._check(type(got)(got.output[inside], got.logsumexp[inside]), want, 75)
+    outside = torch.ones(len(q), dtype=torch.bool, device=dev)
+    outside[inside] = False
+    assert bool((got.output[outside] == 0).all()) and bool((got.logsumexp[outside] == -math.inf).all())
+    out = torch.full_like(q, 7.0)
+    given = dense_prefill_attention(q, k, v, cu_seqlens_q=cu, sm_scale=0.1, out=out, return_logsumexp=True)
+    assert torch.equal(out[inside], got.output[inside]) and bool((out[outside] == 7).all())
+    assert bool((given.logsumexp[outside] == -math.inf).all())
