@@ -341,8 +341,8 @@ int semblo_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, 
  * positions start_positions[b] ... and go through block_table [batch, table_len] (row stride
  * table_stride).  A block's scale is the smallest power of two in [2^-100, 2^120] that holds its largest
  * finite magnitude within 448; a continued block keeps a sufficient scale, otherwise its earlier rows are
- * re-rounded to the new one.  Status 201: a block outside the pool or the table, or a negative start (that
- * block is skipped).  No reference counterpart. */
+ * re-rounded to the new one.  k and v do not overlap the cache or the scales.  Status 201: a block outside
+ * the pool or the table, or a negative start (that block is skipped).  No reference counterpart. */
 int semblo_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
                       int64_t v_token_stride, int64_t v_head_stride, int64_t tokens, int dtype, void* cache,
                       float* scales, int64_t cache_blocks, int block_size, int num_kv_heads, int head_dim,

@@ -564,6 +564,17 @@ extern "C" int semblo_kv8_append(const void* k, int64_t k_token_stride, int64_t 
   SEMBLO_REQUIRE(((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) == 0,
                  "strides of k and v must be multiples of 8 elements");
   SEMBLO_REQUIRE(tokens < ((int64_t)1 << 31), "too many tokens");
+  // blocks write while others still read: the rows lie apart from the codes and the scales
+  const uintptr_t codes0 = reinterpret_cast<uintptr_t>(cache), scales0 = reinterpret_cast<uintptr_t>(scales);
+  const int64_t cells = 2 * cache_blocks * num_kv_heads;
+  auto apart = [&](const void* rows, int64_t token_stride, int64_t head_stride) {
+    const uintptr_t r0 = reinterpret_cast<uintptr_t>(rows);
+    const uintptr_t r1 = r0 + 2 * ((tokens - 1) * token_stride + (num_kv_heads - 1) * head_stride + head_dim);
+    return (r1 <= codes0 || r0 >= codes0 + (uintptr_t)(cells * block_size * head_dim)) &&
+           (r1 <= scales0 || r0 >= scales0 + (uintptr_t)(cells * 4));
+  };
+  SEMBLO_REQUIRE(apart(k, k_token_stride, k_head_stride) && apart(v, v_token_stride, v_head_stride),
+                 "k and v must not overlap the cache or its scales");
   AppendArgs a{};
   a.src[0] = k; a.src[1] = v;
   a.src_token[0] = k_token_stride; a.src_head[0] = k_head_stride;

@@ -97,7 +97,8 @@ def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, block_table: t
     smallest power-of-two scale that holds its largest finite magnitude; one that is continued keeps its scale
     unless a new value needs a larger one, and then the rows already there follow.  Infinities saturate, NaN stay
     NaN.  Rows of ``k`` / ``v`` behind the last request and rows of a block behind the last token are left as they
-    are.  Two requests of one call must not share a block they write.  A table entry outside the pool, a position
+    are.  Two requests of one call must not share a block they write, and ``k`` and
+    ``v`` must lie apart from the cache.  A table entry outside the pool, a position
     outside the table or a negative start sets status 201, and what it names is not written."""
     require_cuda(cache.data, k, v, block_table, cu_seqlens, start_positions)
     refuse_gradients(k, v)

@@ -3,13 +3,15 @@ one fused buffer.  Without a device, against the elements counted one by one."""
 from __future__ import annotations
 
 import contextlib
+import ctypes
 import itertools
 import random
+from types import SimpleNamespace
 
 import pytest
 import torch
 
-from test_dense_refusals import hostside                             # noqa: F401 (the fixture)
+from test_dense_refusals import _lib, hostside                       # noqa: F401 (the fixture)
 
 
 def _elements(x):
@@ -95,3 +97,38 @@ def test_rotary_outputs(hostside, monkeypatch):                      # noqa: F81
     reaches(q_out=other[:, :8], k_out=other[:, 8:10])
     reaches(q_out=other[:, :8], k_out=qkv[:, 10:])                   # the value heads' place
     reaches()
+
+
+def test_append_over_its_cache():
+    """k and v apart from the codes and the scales, by addresses (nothing is read: the calls are refused)."""
+    lib = _lib()
+    blocks, block, heads, dim, tokens = 4, 16, 2, 64, 3
+    cache, scales, codes = 1 << 20, 1 << 24, 2 * blocks * block * heads * dim
+    rows = ((tokens - 1) * heads * dim + (heads - 1) * dim + dim) * 2
+
+    def append(k=1 << 28, v=1 << 29, cache=cache, scales=scales, dtype=0):
+        p = ctypes.c_void_p
+        return lib.semblo_kv8_append(p(k), heads * dim, dim, p(v), heads * dim, dim, tokens, dtype, p(cache), p(scales), blocks,
+                                     block, heads, dim, p(1 << 30), 1, 1, p(1 << 31), p(1 << 32), 1, p(1 << 33), None)
+
+    for kw in (dict(k=cache), dict(v=cache + codes - 16), dict(k=cache - rows + 16), dict(v=scales),
+               dict(k=scales + 2 * blocks * heads * 4 - 16), dict(v=scales - rows + 16)):
+        assert append(**kw) == -1 and b"overlap" in lib.semblo_last_error(), kw
+    # apart by nothing: the type is looked at next, and one is refused there, so that nothing is launched
+    for kw in (dict(k=cache + codes), dict(v=cache - rows), dict(k=scales - rows), dict(v=scales + 2 * blocks * heads * 4)):
+        assert append(**kw, dtype=1) == -1 and b"dtype" in lib.semblo_last_error(), kw
+
+
+def test_append_to_a_cache_made_of_its_input(hostside, monkeypatch):   # noqa: F811
+    """The same through the Python entry: a pool that was cut from the buffer of the keys."""
+    _, kv8 = hostside
+    buf = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
+    cache = kv8.Kv8Cache(buf.view(torch.uint8).view(torch.float8_e4m3fn).view(-1)[:2 * 4 * 2 * 16 * 64].view(2, 4, 2, 16, 64),
+                         torch.ones(2, 4, 2))
+    x = buf[0, :3]
+    monkeypatch.setattr(kv8, "device_scope", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(kv8, "raw_stream", lambda index: None)
+    monkeypatch.setattr(kv8._lib, "status_for", lambda device: SimpleNamespace(word=torch.zeros(1, dtype=torch.int32)))
+    monkeypatch.setattr(kv8, "lib", _lib)
+    with pytest.raises(ValueError, match="overlap"):
+        kv8.kv8_append(cache, x, x, torch.zeros(1, 2, dtype=torch.int32), torch.tensor([0, 3]), torch.tensor([0]))
