@@ -353,8 +353,8 @@ int semblo_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stri
 /* Attention of the last `queries` (1 to 16) tokens of each request over the 8-bit paged cache: q, out
  * [batch, queries, Hq, D] bf16 or fp16 (contiguous), D 64, 128 or 256; query i of request b is at position
  * lengths[b] - queries + i and sees key j < lengths[b] when (j <= p and (window == 0 or p - j < window)) or
- * j < prefix_lens[b] (NULL: none).  softcap > 0: scores become softcap tanh(score / softcap); alibi_slopes
- * [Hq] fp32 (NULL: none): minus slope |p - j|.  lse [batch, queries, Hq] natural log, -inf for a row that
+ * j < prefix_lens[b] (NULL: none).  softcap in [2^-100, 2^100] (0: none): scores become softcap tanh(score
+ * / softcap); alibi_slopes [Hq] fp32 (NULL: none): minus slope |p - j|.  lse [batch, queries, Hq] natural log, -inf for a row that
  * sees nothing (its output is 0), may be NULL.  The workspace needs no initialisation; its size is 0 where
  * every request's keys fit one block's share.  q, cache, out and the workspace are 16-byte aligned; out does
  * not overlap an input.  Status 201: a table entry outside the pool (its keys are taken as absent) or a
@@ -373,11 +373,11 @@ int semblo_kv8_decode(const void* q, int dtype, int batch, int queries, int num_
  * contiguous, the others with strides in elements, multiples of 8), D 64, 128 or 256, up to 128 query heads
  * per KV head.  Document d: queries cu_seqlens_q[d] ..., keys cu_seqlens_k[d] ... (device, non-decreasing);
  * query i is at p = Lk - Lq + i and sees key j when (j <= p and (window == 0 or p - j < window)) or
- * j < prefix_lens[d] (NULL: none); causal = 0: every key of its document.  softcap > 0: scores become
- * softcap tanh(score / softcap); alibi_slopes [Hq] fp32 (NULL: none): minus slope |p - j|.  lse [tokens_q,
+ * j < prefix_lens[d] (NULL: none); causal = 0: every key of its document.  softcap in [2^-100, 2^100] (0:
+ * none): scores become softcap tanh(score / softcap); alibi_slopes [Hq] fp32 (NULL: none): minus slope |p - j|.  lse [tokens_q,
  * Hq] natural log, may be NULL; a row that sees nothing: 0 and -inf.  zero_tail: rows behind the last
- * document and in front of the first become 0 and -inf, otherwise they are not written.  The workspace needs no initialisation; its size
- * is 0 unless there are few queries for the number of keys (their pieces are joined in it).  q, k, v, out and the
+ * document and in front of the first become 0 and -inf, otherwise they are not written.  The workspace
+ * needs no initialisation; its size is 0 unless there are few queries for the number of keys (their pieces are joined in it).  q, k, v, out and the
  * workspace are 16-byte aligned; out does not overlap an input.  The reference leaves dense requests to the
  * engine's stock attention (semblo/vllm_plugin/model.py:1169-1269). */
 int64_t semblo_dense_prefill_workspace_bytes(int64_t tokens_q, int64_t tokens_k, int num_q_heads,

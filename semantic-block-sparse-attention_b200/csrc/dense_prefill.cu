@@ -474,7 +474,7 @@ extern "C" int semblo_dense_prefill(const void* q, int64_t q_token_stride, int64
   if (rc0) return rc0;
   const int group = num_q_heads / num_kv_heads;
   SEMBLO_REQUIRE(dtype == SEMBLO_BF16 || dtype == SEMBLO_F16, "prompts are bf16 or fp16 (got dtype code %d)", dtype);
-  SEMBLO_REQUIRE(softcap >= 0.f, "the soft cap must not be negative");
+  SEMBLO_REQUIRE(semblo::cap_in_range(softcap), "the soft cap must be 0 or lie in [2^-100, 2^100] (got %g)", (double)softcap);
   SEMBLO_REQUIRE(sm_scale > 0.f, "the score scale must be positive");
   if (tokens_q == 0 || (documents == 0 && !zero_tail)) return 0;
   SEMBLO_REQUIRE(q && out && status && cu_seqlens_q && cu_seqlens_k && (tokens_k == 0 || (k && v)), "null pointer");

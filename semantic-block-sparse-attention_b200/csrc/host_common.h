@@ -57,6 +57,9 @@ int make_tensor_map_bf16(CUtensorMap* map, const void* base, int rank, const uin
 // Multiprocessors of the current device (148 if the query fails): persistent grids are sized by it.
 int sm_count();
 
+// A cap on scores is 0 (none) or within this: neither it nor what divides a score by it leaves 32 bits.
+inline bool cap_in_range(float cap) { return cap == 0.f || (cap >= 0x1p-100f && cap <= 0x1p100f); }
+
 __host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace semblo

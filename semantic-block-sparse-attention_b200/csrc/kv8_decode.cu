@@ -905,7 +905,7 @@ extern "C" int semblo_kv8_decode(const void* q, int dtype, int batch, int querie
                              &rows, &nt, &tiles);
   if (rc) return rc;
   SEMBLO_REQUIRE(dtype == SEMBLO_BF16 || dtype == SEMBLO_F16, "queries are bf16 or fp16 (got dtype code %d)", dtype);
-  SEMBLO_REQUIRE(softcap >= 0.f, "the soft cap must not be negative");
+  SEMBLO_REQUIRE(semblo::cap_in_range(softcap), "the soft cap must be 0 or lie in [2^-100, 2^100] (got %g)", (double)softcap);
   if (batch == 0) return 0;
   SEMBLO_REQUIRE(q && cache && scales && block_table && lengths && out && status, "null pointer");
   SEMBLO_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,

@@ -126,6 +126,7 @@ def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, block_table: t
 
 
 MAX_QUERIES = 16
+MIN_CAP, MAX_CAP = 2.0 ** -100, 2.0 ** 100       # so that neither the cap nor what divides a score by it leaves 32 bits
 
 
 def _mask_arguments(window, softcap, prefix_lens, alibi_slopes, batch: int, heads: int, device):
@@ -135,8 +136,8 @@ def _mask_arguments(window, softcap, prefix_lens, alibi_slopes, batch: int, head
         raise ValueError(f"the window must not be negative (got {window}; 0 is none)")
     window = min(window, 1 << 30)            # beyond every position, and inside the kernels' arithmetic
     softcap = float(softcap or 0.0)
-    if not 0.0 <= softcap < float("inf"):
-        raise ValueError(f"the soft cap must be finite and not negative (got {softcap}; 0 is none)")
+    if softcap != 0.0 and not MIN_CAP <= softcap <= MAX_CAP:
+        raise ValueError(f"the soft cap must lie in [2^-100, 2^100] (got {softcap}; 0 is none)")
     if prefix_lens is not None:
         prefix_lens = _per_request("prefix_lens", prefix_lens, batch)
         if prefix_lens.device != device:
