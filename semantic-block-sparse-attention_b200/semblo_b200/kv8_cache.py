@@ -56,10 +56,19 @@ class Kv8Cache:
         return out[0], out[1]
 
 
+def _narrowed(x: torch.Tensor) -> torch.Tensor:
+    """64-bit values as the kernels' 32-bit ones: those that do not fit stay out of every range."""
+    return x.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
+
+
 def _block_table(table: torch.Tensor, batch: int) -> torch.Tensor:
     if table.ndim != 2 or int(table.shape[0]) != batch:
         raise ValueError(f"the block table must have shape [{batch}, blocks per request] (got {tuple(table.shape)})")
-    if table.dtype != torch.int32:
+    if table.dtype == torch.int64:
+        table = _narrowed(table)
+    elif table.dtype != torch.int32:
+        if table.dtype not in (torch.int16, torch.int8, torch.uint8):
+            raise ValueError(f"the block table must be whole numbers (got {table.dtype})")
         table = table.to(torch.int32)
     return table if table.stride(1) == 1 or table.shape[1] <= 1 else table.contiguous()
 
@@ -68,7 +77,7 @@ def _per_request(name: str, x: torch.Tensor, n: int) -> torch.Tensor:
     if x.shape != (n,) or x.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be {n} int32 or int64 values (got {x.dtype} {tuple(x.shape)})")
     if x.dtype != torch.int32:
-        x = x.to(torch.int32)
+        x = _narrowed(x)
     return x if x.is_contiguous() else x.contiguous()
 
 

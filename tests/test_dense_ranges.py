@@ -38,3 +38,29 @@ def test_caps_beyond_the_kernels_range(cap):
                                  None) == -1 and b"cap" in lib.semblo_last_error()
     assert lib.semblo_dense_prefill(p, 64, 64, p, 64, 64, p, 64, 64, 4, 4, 2, 1, 64, 0, p, p, 1, 1, 0, None, 0.1, cap, None, p,
                                     0, None, p, 0, p, None) == -1 and b"cap" in lib.semblo_last_error()
+
+
+FAR = [(1 << 32) + 1, 1 << 40, -(1 << 33) + 2, (1 << 31), -(1 << 31) - 1]
+
+
+def _clamped(x):
+    return [max(-(1 << 31), min((1 << 31) - 1, v)) for v in x]
+
+
+def test_64_bit_values_stay_out_of_range(hostside):                  # noqa: F811
+    """A table entry, length or position that does not fit 32 bits must not become another one that does."""
+    _, kv8 = hostside
+    x = torch.tensor(FAR + [0, 7, -1])
+    assert kv8._per_request("lengths", x, len(x)).tolist() == _clamped(x.tolist())
+    table = kv8._block_table(x[None], 1)
+    assert table.dtype == torch.int32 and table[0].tolist() == _clamped(x.tolist())
+    kept = torch.zeros(3, dtype=torch.int32)
+    assert kv8._per_request("lengths", kept, 3) is kept
+
+
+def test_tables_of_other_types(hostside):                            # noqa: F811
+    _, kv8 = hostside
+    for dtype in (torch.float32, torch.bool, torch.bfloat16):
+        with pytest.raises(ValueError, match="block table"):
+            kv8._block_table(torch.zeros(1, 2, dtype=dtype), 1)
+    assert kv8._block_table(torch.tensor([[3, -1]], dtype=torch.int16), 1).tolist() == [[3, -1]]
