@@ -409,7 +409,9 @@ int join_pieces(const Args& a, cudaStream_t st) {
 // the blocks that fit are not there, pieces of 256: the join, which reads every piece, is small then.  us without
 // and with, D = 128: 16 tokens x 32 heads over 8 behind 8192 others 139 -> 22, 128 behind 30000 463 -> 71, 512 behind
 // 30000 469 -> 242, 8192 tokens x 4 heads over 1 136 -> 105, 11 tokens of 2 documents behind 1250 20 -> 13 (in pieces
-// of 512: 20); 1024 tokens x 8 heads over 2 20 -> 24, so a tile of few keys is not cut.
+// of 512: 20).  1024 tokens x 8 heads over 2 20 -> 24, so a tile of few keys is not cut: the mean tile (the longest is
+// `skew` of it) has to have 1.5 large pieces, 768 keys, or 2 small ones, 512, since with fewer the second launch and the
+// partials cost what the cut saves.
 struct Split { int pieces, keys; };
 Split split_for(int64_t tokens_q, int64_t tokens_k, int group, int num_kv_heads, int head_dim, int documents, int causal,
                 int window, bool prefix) {

@@ -29,9 +29,14 @@ def dense_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *
     same).  Its queries are its last positions: query i stands at p = Lk - Lq + i and sees key j if j <= p (and
     p - j < ``window``, where one is given) or j < prefix_lens[d]; without ``causal`` every key of the document.
     Scores are q . k sm_scale, then ``softcap`` tanh(score / softcap), then minus alibi_slopes[h] |p - j|.  A row that
-    sees nothing gives 0 and a log-sum-exp of -inf.  Rows behind the last document and in
-    front of the first are left as they were in a given ``out``, and are 0 without one; their log-sum-exp is -inf.  Keys behind a document's end are never
-    used, whatever they hold; K and V inside a document have to be finite.  ``out`` must not overlap an input."""
+    sees nothing gives 0 and a log-sum-exp of -inf.  Rows behind the last document and in front of the first are left as
+    they were in a given ``out``, and are 0 without one; their log-sum-exp is -inf.  ``out`` must not overlap an input.
+
+    Keys behind a document's end are never used, whatever they hold; K and V inside a document have to be finite.  (In
+    bf16 under a cap up to 52 the weights run from 2^-92 to 2^60 before they are divided: V beyond 2^43 overflows there,
+    and V below 2^-34 loses bits in rows whose scores are all at -cap.)  What is packed beside a document does not change
+    its result, unless the call's number of tokens cuts its keys into other pieces: then the weights are rounded to 16
+    bits against other references."""
     require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k, prefix_lens, alibi_slopes, out)
     refuse_gradients(q, k, v, out)
     if q.ndim != 3 or k.ndim != 3 or v.shape != k.shape:

@@ -170,7 +170,8 @@ def kv8_decode_attention(q: torch.Tensor, cache: Kv8Cache, block_table: torch.Te
     p = lengths[b] - n + i and sees key j < lengths[b] if j <= p (and p - j < ``window``, where one is given) or
     j < prefix_lens[b].  Scores are q . k sm_scale, then ``softcap`` tanh(score / softcap), then minus
     alibi_slopes[h] |p - j|.  A row that sees nothing (a length of 0, a position below 0) gives 0 and a log-sum-exp
-    of -inf.  The result [B, n, Hq, D] (``out``, apart from the
+    of -inf.  Keys that no query of a request sees may hold anything; a NaN in the V of a key that one of them sees
+    reaches all of them.  The result [B, n, Hq, D] (``out``, apart from the
     inputs, where it is given) has the type of ``q``; log-sum-exps are natural, fp32 [B, n, Hq].  Table
     entries outside the pool are taken as absent and set status 201, as does a length beyond the table."""
     require_cuda(q, cache.data, block_table, lengths, prefix_lens, alibi_slopes, out)
