@@ -326,8 +326,9 @@ int semblo_merge_attention_states(const void* out_a, const float* lse_a, const v
  * elements) with the first rotary_dim dimensions of token t turned by positions[t] * inv_freq[i]
  * (inv_freq [rotary_dim / 2], double), cos and sin times attention_scale; pair i is (i, i + R/2), or
  * (2i, 2i + 1) with interleaved; inverse turns back.  The other dimensions are copied.  An output may be
- * its input (same pointer and strides).  k may be NULL.  The reference receives both tensors from the
- * engine (semblo/vllm_plugin/model.py:1130-1167). */
+ * its input (same pointer and strides); otherwise no element of it is an element of an input or of the other
+ * output.  Strides are not negative.  k may be NULL.  The reference receives both tensors from the engine
+ * (semblo/vllm_plugin/model.py:1130-1167). */
 int semblo_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
                   int64_t qo_token_stride, int64_t qo_head_stride, int num_q_heads, const void* k,
                   int64_t k_token_stride, int64_t k_head_stride, void* k_out, int64_t ko_token_stride,

@@ -249,6 +249,66 @@ int dispatch(RotaryArgs& a, bool interleaved, cudaStream_t st) {
   return launch<T, 1>(a, interleaved, st);
 }
 
+// ---------------------------------------------------------------- which rows share memory
+// The dimensions of [tokens, heads, head_dim] that move, widest step first, in bytes.
+struct Steps {
+  int n = 0;
+  bool still = false;             // a dimension of several indices does not move
+  int64_t count[3], step[3];
+  void add(int64_t c, int64_t s) {
+    if (c <= 1) return;
+    if (s == 0) { still = true; return; }
+    int i = n++;
+    for (; i > 0 && step[i - 1] < s; --i) { count[i] = count[i - 1]; step[i] = step[i - 1]; }
+    count[i] = c;
+    step[i] = s;
+  }
+  int64_t extent(int from, int64_t size) const {
+    int64_t e = size;
+    for (int i = from; i < n; ++i) e += (count[i] - 1) * step[i];
+    return e;
+  }
+};
+
+struct Rows {
+  const char* at;
+  Steps steps;
+  Rows(const void* p, int64_t tokens, int64_t token_stride, int heads, int64_t head_stride, int head_dim, int size)
+      : at(static_cast<const char*>(p)) {
+    steps.add(tokens, token_stride * size);
+    steps.add(heads, head_stride * size);
+    steps.add(head_dim, size);
+  }
+};
+
+// Whether elements of a, from dimension ia on, and of b, `offset` bytes on, meet.  Slices of one fused buffer, whose
+// spans overlap, are told apart; rows that reach into each other count as meeting.
+bool meet(int64_t offset, const Steps& a, int ia, const Steps& b, int ib, int64_t size) {
+  if (offset >= a.extent(ia, size) || -offset >= b.extent(ib, size)) return false;
+  if (ia == a.n && ib == b.n) return true;
+  const int64_t step = std::max(ia < a.n ? a.step[ia] : 0, ib < b.n ? b.step[ib] : 0);
+  int64_t na = 1, nb = 1;
+  if (ia < a.n && a.step[ia] == step) na = a.count[ia++];
+  if (ib < b.n && b.step[ib] == step) nb = b.count[ib++];
+  const int64_t ea = a.extent(ia, size), eb = b.extent(ib, size);
+  if (ea > step || eb > step) return true;
+  // row i of a starts at i steps, row j of b at offset + j steps: they meet for -eb < offset + (j - i) steps < ea only,
+  // which is at most three values of j - i
+  auto below = [&](int64_t x) { return x >= 0 ? x / step : -((-x + step - 1) / step); };
+  const int64_t last = std::min(nb - 1, below(ea - offset - 1));
+  for (int64_t k = std::max(1 - na, below(-eb - offset) + 1); k <= last; ++k)
+    if (meet(offset + k * step, a, ia, b, ib, size)) return true;
+  return false;
+}
+bool meet(const Rows& a, const Rows& b, int64_t size) { return meet(b.at - a.at, a.steps, 0, b.steps, 0, size); }
+
+bool repeats(const Rows& a, int64_t size) {
+  if (a.steps.still) return true;
+  for (int i = 0; i < a.steps.n; ++i)
+    if (a.steps.extent(i + 1, size) > a.steps.step[i]) return true;
+  return false;
+}
+
 }  // namespace
 
 extern "C" int semblo_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
@@ -267,6 +327,25 @@ extern "C" int semblo_rotary(const void* q, int64_t q_token_stride, int64_t q_he
   SEMBLO_REQUIRE(q != nullptr && q_out != nullptr && positions != nullptr, "q, q_out and positions are required");
   SEMBLO_REQUIRE(rotary_dim == 0 || inv_freq != nullptr, "inv_freq is required");
   SEMBLO_REQUIRE(tokens < (int64_t)1 << 31, "too many tokens");
+  SEMBLO_REQUIRE(std::min({q_token_stride, q_head_stride, qo_token_stride, qo_head_stride}) >= 0 &&
+                     (!k || std::min({k_token_stride, k_head_stride, ko_token_stride, ko_head_stride}) >= 0),
+                 "strides must not be negative");
+  // one launch turns query and key heads in any order
+  const int size = dtype == SEMBLO_F32 ? 4 : 2;
+  const Rows qi(q, tokens, q_token_stride, num_q_heads, q_head_stride, head_dim, size);
+  const Rows qo(q_out, tokens, qo_token_stride, num_q_heads, qo_head_stride, head_dim, size);
+  SEMBLO_REQUIRE(!repeats(qo, size), "q_out must not repeat memory");
+  SEMBLO_REQUIRE((q == q_out && q_token_stride == qo_token_stride && q_head_stride == qo_head_stride) || !meet(qi, qo, size),
+                 "q_out overlaps its input without being it");
+  if (k && num_kv_heads) {
+    const Rows ki(k, tokens, k_token_stride, num_kv_heads, k_head_stride, head_dim, size);
+    const Rows ko(k_out, tokens, ko_token_stride, num_kv_heads, ko_head_stride, head_dim, size);
+    SEMBLO_REQUIRE(!repeats(ko, size), "k_out must not repeat memory");
+    SEMBLO_REQUIRE((k == k_out && k_token_stride == ko_token_stride && k_head_stride == ko_head_stride) || !meet(ki, ko, size),
+                   "k_out overlaps its input without being it");
+    SEMBLO_REQUIRE(!meet(qo, ki, size) && !meet(ko, qi, size) && !meet(qo, ko, size),
+                   "q_out and k_out must not overlap each other or the other's input");
+  }
   RotaryArgs a{};
   a.q_in = q; a.q_out = q_out; a.k_in = k; a.k_out = k_out;
   a.q_in_token = q_token_stride; a.q_in_head = q_head_stride;

@@ -155,49 +155,6 @@ def overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
-def _steps(t: torch.Tensor) -> list:
-    """(count, bytes) of the dimensions that move, widest first."""
-    size = t.element_size()
-    return sorted(((n, s * size) for n, s in zip(t.shape, t.stride()) if n > 1 and s), key=lambda d: -d[1])
-
-
-def _extent(steps: list, size: int) -> int:
-    return sum((n - 1) * s for n, s in steps) + size
-
-
-def _meet(offset: int, a: list, b: list, size: int) -> bool:
-    ea, eb = _extent(a, size), _extent(b, size)
-    if offset >= ea or -offset >= eb:
-        return False
-    if not a and not b:
-        return True
-    step = max(d[0][1] for d in (a, b) if d)
-    na, a = (a[0][0], a[1:]) if a and a[0][1] == step else (1, a)
-    nb, b = (b[0][0], b[1:]) if b and b[0][1] == step else (1, b)
-    ea, eb = _extent(a, size), _extent(b, size)
-    if ea > step or eb > step:
-        return True                              # rows that reach into each other: not told apart
-    # row i of a starts at i steps, row j of b at offset + j steps: they meet for -eb < offset + (j - i) steps < ea only
-    first, last = max(1 - na, (-eb - offset) // step + 1), min(nb - 1, (ea - offset - 1) // step)
-    return any(_meet(offset + k * step, a, b, size) for k in range(first, last + 1))
-
-
-def shares_elements(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two tensors of one type have an element's memory in common, by their strides: slices of one fused buffer do
-    not, although their spans overlap.  Layouts whose rows do not nest count as sharing where their spans meet."""
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-    return _meet(b.data_ptr() - a.data_ptr(), _steps(a), _steps(b), a.element_size())
-
-
-def repeats_elements(t: torch.Tensor) -> bool:
-    """Whether two indices of ``t`` may be the same memory."""
-    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
-        return True
-    steps, size = _steps(t), t.element_size()
-    return t.numel() > 0 and any(_extent(steps[i + 1:], size) > steps[i][1] for i in range(len(steps)))
-
-
 def raw_stream(index: int) -> int:
     """The current stream of device ``index`` as the C entries take it."""
     return torch._C._cuda_getCurrentRawStream(index)

@@ -12,7 +12,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import check, device_scope, dtype_code, lib, raw_stream, refuse_gradients, repeats_elements, require_cuda, shares_elements
+from ._lib import check, device_scope, dtype_code, lib, overlaps, raw_stream, refuse_gradients, require_cuda
 
 _SCALING_KEYS = {"linear": {"factor"}, "ntk": {"factor"},
                  "yarn": {"factor", "original_max_position", "beta_fast", "beta_slow", "attention_factor"},
@@ -113,17 +113,11 @@ def _check_output(name: str, y: torch.Tensor, x: torch.Tensor) -> tuple:
     strides = _check_rows(name, y, x.shape[0], x.shape[2], x.dtype, x.device)
     if y.shape != x.shape:
         raise ValueError(f"{name} must have the shape of its input")
-    if repeats_elements(y):
+    if any(n > 1 and s == 0 for n, s in zip(y.shape, strides)):
         raise ValueError(f"{name} must not repeat memory")
-    if (x.data_ptr() != y.data_ptr() or x.stride() != y.stride()) and shares_elements(x, y):
+    if (x.data_ptr() != y.data_ptr() or x.stride() != strides) and overlaps(x, y):
         raise ValueError(f"{name} overlaps its input without being it")
     return strides
-
-
-def _check_apart(name: str, y: torch.Tensor, other_name: str, other: torch.Tensor) -> None:
-    """One launch turns query and key heads, in any order."""
-    if shares_elements(y, other):
-        raise ValueError(f"{name} must not overlap {other_name}")
 
 
 def apply_rotary(q_pre: torch.Tensor, k_pre: torch.Tensor | None, positions: torch.Tensor,
@@ -136,7 +130,7 @@ def apply_rotary(q_pre: torch.Tensor, k_pre: torch.Tensor | None, positions: tor
     The first ``frequencies.rotary_dim`` dimensions are rotated: pair i is (x_i, x_{i + R/2}), or (x_2i, x_2i+1)
     with ``interleaved``; the others are copied.  ``inverse`` rotates back (the transpose).  ``q_out`` / ``k_out``
     receive the result; either may be its input itself (in place), and must not share an element with the other
-    input or output (slices of one fused buffer do not).  Angles are formed in 64 bits."""
+    input or output (slices of one fused buffer do not; the C entry looks at strides).  Angles are formed in 64 bits."""
     require_cuda(q_pre, k_pre, positions, q_out, k_out)
     refuse_gradients(q_pre, k_pre, q_out, k_out)
     if q_pre.ndim != 3:
@@ -154,8 +148,7 @@ def apply_rotary(q_pre: torch.Tensor, k_pre: torch.Tensor | None, positions: tor
     if positions.device != device or inv_freq.device != device:
         raise ValueError(f"the positions ({positions.device}) and frequencies ({inv_freq.device}) must be on the "
                          f"device of q_pre ({device})")
-    q_given, k_given = q_out is not None, k_out is not None
-    if not q_given:
+    if q_out is None:
         q_out, qos = torch.empty_like(q_pre, memory_format=torch.contiguous_format), (hq * dim, dim)
     else:
         qos = _check_output("q_out", q_out, q_pre)
@@ -166,15 +159,10 @@ def apply_rotary(q_pre: torch.Tensor, k_pre: torch.Tensor | None, positions: tor
     else:
         ks = _check_rows("k_pre", k_pre, tokens, dim, dtype, device)
         hkv = k_pre.shape[1]
-        if q_given:
-            _check_apart("q_out", q_out, "k_pre", k_pre)
-        if not k_given:
+        if k_out is None:
             k_out, kos = torch.empty_like(k_pre, memory_format=torch.contiguous_format), (hkv * dim, dim)
         else:
             kos = _check_output("k_out", k_out, k_pre)
-            _check_apart("k_out", k_out, "q_pre", q_pre)
-            if q_given:
-                _check_apart("q_out", q_out, "k_out", k_out)
         if hkv:
             k_args = (k_pre.data_ptr(), ks[0], ks[1], k_out.data_ptr(), kos[0], kos[1], hkv)
     if not positions.is_contiguous():

@@ -22,9 +22,10 @@ def _elements(x):
 
 
 def _views(rng):
-    """Views of one buffer as layers make them: head slices, token ranges, heads first, every other head or token."""
+    """Two views [T, heads, D] of one buffer as layers make them: head slices, token ranges, heads first, every other head
+    or token."""
     t, h, d = rng.choice([1, 2, 5]), rng.choice([4, 6]), rng.choice([2, 3])
-    flat = torch.zeros(2 * t * h * d + 7)
+    flat = torch.zeros(2 * t * h * d + 7, dtype=torch.bfloat16)
     out = []
     for _ in range(2):
         off = rng.choice([0, 0, d, 1, h * d, t * h * d])
@@ -42,61 +43,92 @@ def _views(rng):
         else:
             x = x[rng.randrange(min(t, 2))::2]
         out.append(x)
-    return out
+    tokens = min(len(x) for x in out)
+    return [x[:tokens] for x in out]
+
+
+NO_TYPE = 9            # looked at after the overlaps and refused, so that nothing is ever launched
+
+
+def _rotary(q, q_out, k, k_out):
+    """The C entry's answer: b"dtype" where it found nothing to say about the memory."""
+    lib, far = _lib(), ctypes.c_void_p(1 << 50)
+    rows = lambda x: (x.data_ptr(), x.stride(0), x.stride(1))
+    keys = (None, 0, 0, None, 0, 0, 0) if k is None else (*rows(k), *rows(k_out), k.shape[1])
+    assert lib.semblo_rotary(*rows(q), *rows(q_out), q.shape[1], *keys, q.shape[0], q.shape[2], 2, NO_TYPE, far, 1, far, 1.0, 0,
+                             0, None) == -1
+    return lib.semblo_last_error()
+
+
+def _fresh(x):
+    return torch.zeros_like(x, memory_format=torch.contiguous_format)
+
+
+def _shares(a, b):
+    """a as the queries' output, b as the keys' input; and the other way round."""
+    said = [b"overlap" in _rotary(_fresh(a), a, b, _fresh(b)), b"overlap" in _rotary(_fresh(b), b, a, _fresh(a)),
+            b"overlap" in _rotary(a, _fresh(a), _fresh(b), b), b"overlap" in _rotary(_fresh(a), a, _fresh(b), b)]
+    assert len(set(said)) == 1
+    return said[0]
 
 
 def test_shared_elements():
-    from semblo_b200._lib import shares_elements
     rng, told = random.Random(1), 0
-    for _ in range(3000):
+    for _ in range(1500):
         a, b = _views(rng)
         shared = bool(_elements(a) & _elements(b))
-        assert shares_elements(a, b) or not shared
-        assert shares_elements(a, b) == shares_elements(b, a)
-        told += not shared and not shares_elements(a, b)
-    assert told > 500                                                # and disjoint views are told apart
+        found = _shares(a, b)
+        assert found or not shared
+        told += not shared and not found
+    assert told > 200                                                # and disjoint views are told apart
     # the layouts that layers have, told apart exactly
-    qkv = torch.zeros(7, 12, 16)
-    q, k, v = qkv[:, :8], qkv[:, 8:10], qkv[:, 10:]
-    assert not shares_elements(q, k) and not shares_elements(k, v) and shares_elements(q, qkv[:, 7:9])
-    grouped = torch.zeros(7, 2, 6, 16)                               # per KV head: its queries, K and V
-    assert not shares_elements(grouped[:, :, 4], grouped[:, :, 5]) and not shares_elements(grouped[:, :, 0], grouped[:, :, 5])
-    first = torch.zeros(12, 7, 16).transpose(0, 1)                   # heads first
-    assert not shares_elements(first[:, :8], first[:, 8:10]) and shares_elements(first[:, :8], first[:, 7:])
-    assert not shares_elements(qkv[:0], qkv) and shares_elements(qkv[:1].expand(7, 12, 16), qkv[:1])
-    assert not shares_elements(qkv[:3], qkv[3:]) and shares_elements(qkv[:4], qkv[3:])
+    qkv = torch.zeros(7, 12, 16, dtype=torch.bfloat16)
+    assert not _shares(qkv[:, :8], qkv[:, 8:10]) and not _shares(qkv[:, 8:10], qkv[:, 10:]) and _shares(qkv[:, :8], qkv[:, 7:9])
+    grouped = torch.zeros(7, 2, 6, 16, dtype=torch.bfloat16)         # per KV head: its queries, K and V
+    assert not _shares(grouped[:, :, 4], grouped[:, :, 5]) and not _shares(grouped[:, :, 0], grouped[:, :, 5])
+    first = torch.zeros(12, 7, 16, dtype=torch.bfloat16).transpose(0, 1)                   # heads first
+    assert not _shares(first[:, :8], first[:, 8:10]) and _shares(first[:, :8], first[:, 7:])
+    assert not _shares(qkv[:3], qkv[3:6]) and _shares(qkv[:4], qkv[3:7])
+
+
+def test_outputs_in_place_over_their_input_and_over_themselves():
+    qkv, pool = torch.zeros(4, 12, 64, dtype=torch.bfloat16), torch.zeros(4000, dtype=torch.bfloat16)
+    q, k = qkv[:, :8], qkv[:, 8:10]
+    assert b"dtype" in _rotary(q, q, k, k) and b"dtype" in _rotary(q, q, None, None)
+    assert b"dtype" in _rotary(q, q, k, _fresh(k)) and b"dtype" in _rotary(q, _fresh(q), k, k)
+    assert b"overlap" in _rotary(q, qkv[:, 1:9], None, None) and b"overlap" in _rotary(k, qkv[:, 9:11], None, None)
+    assert b"overlap" in _rotary(q, q, k, qkv[:, 7:9]) and b"overlap" in _rotary(q, qkv[:, 2:10], k, k)
+    for strides in ((64, 64, 1), (512, 32, 1), (0, 64, 1), (256, 64, 1)):
+        said = _rotary(_fresh(q), pool.as_strided((4, 8, 64), strides), None, None)
+        assert b"repeat" in said, strides
+    lib, p = _lib(), ctypes.c_void_p(1 << 40)
+    assert lib.semblo_rotary(p, -64, 64, p, 64, 64, 2, None, 0, 0, None, 0, 0, 0, 4, 64, 2, NO_TYPE, p, 1, p, 1.0, 0, 0, None) == -1
+    assert b"negative" in lib.semblo_last_error()
 
 
 def test_rotary_outputs(hostside, monkeypatch):                      # noqa: F811
+    """The same through the Python entry, which hands the library a type that it refuses."""
     rotary, _ = hostside
-    monkeypatch.setattr(rotary, "device_scope", lambda device: contextlib.nullcontext())
     freq, pos = rotary.rotary_frequencies(64, device="cpu"), torch.arange(4)
-    qkv = torch.zeros(4, 12, 64)
+    monkeypatch.setattr(rotary, "device_scope", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(rotary, "raw_stream", lambda index: None)
+    monkeypatch.setattr(rotary, "dtype_code", lambda *_: NO_TYPE)
+    monkeypatch.setattr(rotary, "lib", _lib)
+    qkv = torch.zeros(4, 12, 64, dtype=torch.bfloat16)
     q, k = qkv[:, :8], qkv[:, 8:10]
-    other = torch.zeros(4, 12, 64)
+    other = torch.zeros(4, 12, 64, dtype=torch.bfloat16)
 
-    def no(**kw):
-        with pytest.raises(ValueError, match="overlap|repeat"):
+    def says(what, **kw):
+        with pytest.raises(ValueError, match=what):
             rotary.apply_rotary(q, k, pos, freq, **kw)
 
-    def reaches(**kw):                                               # accepted: the library is asked for
-        with pytest.raises(AssertionError, match="not refused"):
-            rotary.apply_rotary(q, k, pos, freq, **kw)
-
-    no(q_out=qkv[:, 2:10])                                           # over the keys
-    no(q_out=qkv[:, 1:9])
-    no(k_out=q[:, :2])
-    no(k_out=qkv[:, 7:9])
-    no(q_out=other[:, :8], k_out=other[:, 7:9])                      # over each other
-    no(q_out=other[:, :8], k_out=other[:, :2])
-    no(q_out=torch.zeros(4000).as_strided((4, 8, 64), (64, 64, 1)))  # rows over rows of their own
-    no(q_out=torch.zeros(4000).as_strided((4, 8, 64), (512, 32, 1)))
-    reaches(q_out=q, k_out=k)                                        # in place, in the fused buffer
-    reaches(q_out=q)
-    reaches(k_out=k)
-    reaches(q_out=other[:, :8], k_out=other[:, 8:10])
-    reaches(q_out=other[:, :8], k_out=qkv[:, 10:])                   # the value heads' place
-    reaches()
+    says("overlap", q_out=qkv[:, 2:10])                              # over the keys
+    says("overlap", k_out=q[:, :2])
+    says("overlap", q_out=other[:, :8], k_out=other[:, 7:9])         # over each other
+    says("overlap", q_out=other[:, :8], k_out=other[:, :2])
+    says("repeat", q_out=torch.zeros(4000, dtype=torch.bfloat16).as_strided((4, 8, 64), (64, 64, 1)))
+    for kw in (dict(q_out=q, k_out=k), dict(q_out=q), dict(k_out=k), dict(q_out=other[:, :8], k_out=other[:, 8:10]), {}):
+        says("dtype", **kw)
 
 
 def test_append_over_its_cache():

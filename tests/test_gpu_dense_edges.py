@@ -244,3 +244,20 @@ def test_rows_in_front_of_the_first_document(dev, dim, front, tail):
     given = dense_prefill_attention(q, k, v, cu_seqlens_q=cu, sm_scale=0.1, out=out, return_logsumexp=True)
     assert torch.equal(out[inside], got.output[inside]) and bool((out[outside] == 7).all())
     assert bool((given.logsumexp[outside] == -math.inf).all())
+
+
+# ---- outputs in the buffer of the inputs
+
+def test_rotary_in_the_buffer_of_its_inputs(dev):
+    """Queries and keys turned in place in one fused buffer, and into another one's slices: the bytes of separate calls, and
+    nothing else touched."""
+    from semblo_b200.rotary import apply_rotary, rotary_frequencies
+    qkv = torch.randn(300, 12, 128, device=dev).to(torch.bfloat16)
+    held, pos = qkv.clone(), torch.arange(300, device=dev)
+    freq = rotary_frequencies(128, device=dev)
+    want = apply_rotary(qkv[:, :8], qkv[:, 8:10], pos, freq)
+    other = torch.full_like(qkv, 3.0)
+    apply_rotary(qkv[:, :8], qkv[:, 8:10], pos, freq, q_out=other[:, :8], k_out=other[:, 8:10])
+    apply_rotary(qkv[:, :8], qkv[:, 8:10], pos, freq, q_out=qkv[:, :8], k_out=qkv[:, 8:10])
+    for got, rest in ((qkv, held[:, 10:]), (other, torch.full_like(held[:, 10:], 3.0))):
+        assert torch.equal(got[:, :8], want[0]) and torch.equal(got[:, 8:10], want[1]) and torch.equal(got[:, 10:], rest)
