@@ -300,6 +300,9 @@ class SembloRuntimeState:
         key, signature = ("dense", int(layer_idx)), (blocks, num_kv_heads, head_dim, torch.device(device))
         held = self.index_buffers.get(key)
         if held is None or held[0] != signature:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"layer {layer_idx} has no 8-bit cache yet: run a prompt or a step before one is recorded "
+                                   "(made in a recording, every replay would empty it)")
             table = torch.arange(blocks, dtype=torch.int32, device=device).view(1, -1)
             held = (signature, Kv8Cache.allocate(blocks, DENSE_BLOCK, num_kv_heads, head_dim, device), table)
             self.index_buffers[key] = held

@@ -158,3 +158,19 @@ def test_a_reader_without_its_source_writes_nothing(operators):
     with pytest.raises(RuntimeError, match="has not seen"):
         _run(layer, torch.arange(40))
     assert not operators
+
+
+def test_the_cache_is_not_made_while_a_step_is_recorded(operators, monkeypatch):
+    """Its memory and its first fill would become part of the recording: every replay would empty it."""
+    state = _state()
+    layer = _layer(state, 0, sparse=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before"):
+        _run(layer, torch.tensor([3]))
+    assert not operators and not state.index_buffers
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    _run(layer, torch.arange(40))
+    operators.clear()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    _run(layer, torch.tensor([40]))
+    assert [c[0] for c in operators] == ["append", "decode"]
