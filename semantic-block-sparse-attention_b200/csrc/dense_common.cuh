@@ -428,23 +428,31 @@ __device__ __forceinline__ void bounded32(uint32_t* x, const Args& a, const Tanh
     }
   };
   // every |y| < 2: the top bit of the exponent is clear in all of them.  Where that fails, perhaps by unseen ones only, it
-  // is looked at again without them; cleared in front of the first vote they cost every tile 4 %, here 3 % where scores
-  // beyond 3/4 of the cap are common (8192 tokens x 32 heads over 8 x 128 capped at 20: 847 -> 888 us, at 50 670 and 670)
+  // is looked at again without them, in code of its own: cleared in front of the first vote they cost every tile 4 %, in
+  // front of a shared second one 5 % where scores beyond 3/4 of the cap are common, here 2 % (8192 tokens x 32 heads over
+  // 8 x 128 capped at 20: 846 us with the unseen ones in the vote, 891, 860; capped at 50: 670 each way)
   if (__all_sync(0xffffffffu, !(seen & vote.near))) {
     all_by(capped);
   } else {
-    if (!all) clear32(x, bits);
-    float most = 0.f;
+    auto beyond = [&](bool masked) {
+      float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) most = fmax3(most, fabsf(__uint_as_float(x[i])), fabsf(__uint_as_float(x[i + 1])));
-    if (__all_sync(0xffffffffu, most < vote.near_most)) {
-      all_by(capped);
-    } else if (__all_sync(0xffffffffu, most < vote.far)) {
-      all_by(TanhPoly<8>(a.cap_log2));
+      for (int i = 0; i < 32; i += 2) most = fmax3(most, fabsf(__uint_as_float(x[i])), fabsf(__uint_as_float(x[i + 1])));
+      if (masked && __all_sync(0xffffffffu, most < vote.near_most)) {
+        all_by(capped);
+      } else if (__all_sync(0xffffffffu, most < vote.far)) {
+        all_by(TanhPoly<8>(a.cap_log2));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          x[i] = __float_as_uint(fmaf(tanh_exp(__uint_as_float(x[i]) * (1.f / TANH_ARG)), a.cap_log2, neg_m));
+      }
+    };
+    if (all) {
+      beyond(false);
     } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        x[i] = __float_as_uint(fmaf(tanh_exp(__uint_as_float(x[i]) * (1.f / TANH_ARG)), a.cap_log2, neg_m));
+      clear32(x, bits);
+      beyond(true);
     }
   }
   if (!all) hide32(x, bits);
